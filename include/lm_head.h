@@ -1,4 +1,5 @@
-/* lm_head.h: the C ABI of the LM head's pick on MI355X (gfx950), in libdense_reader.so beside dense_reader.h.
+/* lm_head.h: the C ABI of the LM head's pick and of its losses on MI355X (gfx950), in libdense_reader.so beside
+ * dense_reader.h.
  *
  * An LM head run as dense_reader matmuls with top-k records (dr_matmul's dr_topk, bf16 keys) leaves, per row, the
  * best candidates of every 32-column tile of the vocabulary. These entry points turn the records into token ids on the
@@ -44,6 +45,62 @@ int dr_head_pick(const void* records, int n_records, int rows, int k, int top, i
  * ids_out (or NULL): row 0's token also into ids_out[0]. */
 int dr_head_pick_records(const void* records, int n_records, int rows, int k, int64_t vocab, const void* token_map,
                          void* out, void* ids_out, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The losses. A head [vocab][dim] bf16 (one row a token, as dr_head_pick reads it) against rows x [rows][dim] bf16:
+ * z = x . head^T, float32 sums, never in memory as a whole. Per row, with lse = log(sum over v < valid of exp(z[v] / T)):
+ *   tokens (vals NULL, k 1, T 1): loss = lse - z[id];
+ *   a teacher's best k logits (vals): over the entries held, q = softmax(vals / T),
+ *     loss = sum q (log q - z[id] / T + lse), the divergence of the row's softmax at temperature T from the teacher's
+ *     over its entries. An id that comes twice counts twice.
+ * An entry is held when its id lies in 0 .. valid - 1 and (teacher) its value is not -inf. A row with no entry held is
+ * left out: loss, lse, logits and dx 0, nothing into dhead, whatever x, g or vals hold there.
+ *
+ * Gradients of sum over rows of g[row] * loss[row]: dz[v] = g / T (p[v] - sum of q over entries of id v), p = exp(z / T -
+ * lse); dx = dz . head, dhead = dz^T . x (rows valid .. vocab - 1 zeros). z is computed again, piece by piece of the
+ * vocabulary; dz is rounded to bf16 (scaled by the largest |g| of the rows that count, which the float32 sums get back),
+ * the sums are float32, dx and dhead rounded once.
+ *
+ * No counterpart in the reference, which has no training: the head and the teacher's records are its
+ * lm_head_topk/head_pick.py:43-52 and dense_reader/linear.py:747-768.
+ */
+#define DR_LOSS_MAX_K 64
+
+/* what a call computes */
+#define DR_LOSS_FORWARD 1  /* loss, lse, logits */
+#define DR_LOSS_BACKWARD 2 /* dx, dhead, from lse and logits (a forward call's, of the same inputs) */
+
+typedef struct dr_head_loss {
+    const void* x;        /* [rows][ldx] bf16, 16-byte aligned, ldx a multiple of 8 */
+    int64_t ldx;
+    const void* head;     /* [vocab][ld_head] bf16, 16-byte aligned, ld_head a multiple of 8 */
+    int64_t ld_head;
+    int32_t rows, dim;    /* dim a multiple of 8 */
+    int32_t vocab, valid; /* 1 <= valid <= vocab: the head's rows that take part */
+    const void* ids;      /* [rows][ld_ids] int32, or int64 (ids64) */
+    int64_t ld_ids;
+    int32_t ids64;
+    int32_t k;            /* entries a row, 1 .. DR_LOSS_MAX_K */
+    const float* vals;    /* [rows][ld_vals] the teacher's logits, or NULL: tokens (k 1) */
+    int64_t ld_vals;
+    float temperature;    /* T > 0, finite (tokens: 1) */
+    float* loss;          /* [rows] */
+    float* lse;           /* [rows] */
+    float* logits;        /* [rows][k]: z at the entries (0 where none is held) */
+    const float* g;       /* [rows], or NULL: ones */
+    void* dx;             /* [rows][ld_dx] bf16, 8-byte aligned, ld_dx a multiple of 4, or NULL */
+    int64_t ld_dx;
+    void* dhead;          /* [vocab][ld_dhead] bf16, 8-byte aligned, ld_dhead a multiple of 4, or NULL */
+    int64_t ld_dhead;
+    void* workspace;      /* dr_head_loss_workspace_bytes, 256-byte aligned; its contents mean nothing between calls */
+    int64_t workspace_bytes;
+    void* stream;
+} dr_head_loss;
+
+/* Bytes of workspace the call needs (what: DR_LOSS_FORWARD, DR_LOSS_BACKWARD or both), -1 if it is invalid. */
+int64_t dr_head_loss_workspace_bytes(const dr_head_loss* a, int what);
+
+/* Enqueues the call on the stream: nothing is allocated, kept or waited for, so it can be captured. */
+int dr_head_loss_run(const dr_head_loss* a, int what);
 
 #ifdef __cplusplus
 }

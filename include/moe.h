@@ -109,6 +109,41 @@ int dr_moe_route(const dr_route* route);
  * boundary between them. */
 int dr_moe_route_gate_up(const dr_launch* launch, const dr_moe* moe, const dr_route* route);
 
+/* The router's balance loss of batches of rows (a batch: a sequence, or all of a step's tokens), each expert's count and
+ * the gradient of the logits. Per batch, over its rows t that count:
+ *   p[t] = softmax of the logits (kind 0; a row with none above -inf: 0), or their sigmoids over the sigmoids' sum (kind 1);
+ *   counts[e] = the rows' slots that chose e (an id >= experts chooses none), f[e] = experts * counts[e] / sum of counts;
+ *   loss = sum over e of f[e] * mean over t of p[t][e]  (1 where all are chosen alike; 0 where no row counts);
+ *   dlogits = g times its gradient, the counts taken as constants (as the choice has none).
+ * No counterpart in the reference, which has no training: logits and ids are dr_moe_route's (moe/moe8.py:1139-1253). */
+#define DR_BALANCE_LOSS 1
+#define DR_BALANCE_GRAD 2 /* dlogits too (the loss and the counts come with either) */
+
+typedef struct dr_balance {
+    const float* logits;   /* [batch * rows][ld_logits] */
+    int64_t ld_logits;
+    int32_t batch, rows;
+    int32_t experts;       /* 1 .. 1024: the logits' columns 0 .. experts - 1 */
+    int32_t width;         /* dlogits' columns: zeros from experts on */
+    const void* ids;       /* [batch * rows][ld_ids] uint16, or uint32 (ids32) */
+    int64_t ld_ids;
+    int32_t ids32;
+    int32_t k;             /* slots a row, 1 .. 16 */
+    int32_t kind;          /* 0 softmax, 1 sigmoid */
+    const uint8_t* mask;   /* [batch * rows], 0: the row does not count; or NULL: all do */
+    float* loss;           /* [batch] */
+    int32_t* counts;       /* [batch][experts] */
+    const float* g;        /* [batch], or NULL: ones */
+    float* dlogits;        /* [batch * rows][ld_dlogits]; rows that do not count get zeros */
+    int64_t ld_dlogits;
+    void* workspace;       /* dr_moe_balance_workspace_bytes, 256-byte aligned; its contents mean nothing between calls */
+    int64_t workspace_bytes;
+    void* stream;
+} dr_balance;
+
+int64_t dr_moe_balance_workspace_bytes(const dr_balance* a, int what);
+int dr_moe_balance(const dr_balance* a, int what);
+
 #ifdef __cplusplus
 }
 #endif

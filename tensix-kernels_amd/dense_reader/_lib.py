@@ -37,11 +37,19 @@ SYMBOLS = (
     "dr_version",
     "dr_head_pick",
     "dr_head_pick_records",
+    "dr_head_loss_workspace_bytes",
+    "dr_head_loss_run",
     "dr_moe_workspace_bytes",
     "dr_moe_matmul",
     "dr_moe_route",
     "dr_moe_route_gate_up",
+    "dr_moe_balance_workspace_bytes",
+    "dr_moe_balance",
 )
+
+DR_LOSS_FORWARD, DR_LOSS_BACKWARD = 1, 2
+DR_LOSS_MAX_K = 64
+DR_BALANCE_LOSS, DR_BALANCE_GRAD = 1, 2
 
 DR_MOE_GATE_UP, DR_MOE_DOWN, DR_MOE_GATE_UP_ROWS, DR_MOE_DOWN_ROWS = 1, 2, 3, 4
 
@@ -166,6 +174,62 @@ class Route(ctypes.Structure):
     ]
 
 
+class HeadLoss(ctypes.Structure):
+    _fields_ = [
+        ("x", c_void_p),
+        ("ldx", c_int64),
+        ("head", c_void_p),
+        ("ld_head", c_int64),
+        ("rows", c_int32),
+        ("dim", c_int32),
+        ("vocab", c_int32),
+        ("valid", c_int32),
+        ("ids", c_void_p),
+        ("ld_ids", c_int64),
+        ("ids64", c_int32),
+        ("k", c_int32),
+        ("vals", c_void_p),
+        ("ld_vals", c_int64),
+        ("temperature", ctypes.c_float),
+        ("loss", c_void_p),
+        ("lse", c_void_p),
+        ("logits", c_void_p),
+        ("g", c_void_p),
+        ("dx", c_void_p),
+        ("ld_dx", c_int64),
+        ("dhead", c_void_p),
+        ("ld_dhead", c_int64),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
+        ("stream", c_void_p),
+    ]
+
+
+class Balance(ctypes.Structure):
+    _fields_ = [
+        ("logits", c_void_p),
+        ("ld_logits", c_int64),
+        ("batch", c_int32),
+        ("rows", c_int32),
+        ("experts", c_int32),
+        ("width", c_int32),
+        ("ids", c_void_p),
+        ("ld_ids", c_int64),
+        ("ids32", c_int32),
+        ("k", c_int32),
+        ("kind", c_int32),
+        ("mask", c_void_p),
+        ("loss", c_void_p),
+        ("counts", c_void_p),
+        ("g", c_void_p),
+        ("dlogits", c_void_p),
+        ("ld_dlogits", c_int64),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
+        ("stream", c_void_p),
+    ]
+
+
 _lib = None
 
 
@@ -225,12 +289,20 @@ def lib():
         L.dr_head_pick_records.restype = c_int
         L.dr_head_pick_records.argtypes = [c_void_p, c_int, c_int, c_int, c_int64, c_void_p, c_void_p, c_void_p,
                                            c_void_p, c_int64, c_void_p]
+        L.dr_head_loss_workspace_bytes.restype = c_int64
+        L.dr_head_loss_workspace_bytes.argtypes = [ctypes.POINTER(HeadLoss), c_int]
+        L.dr_head_loss_run.restype = c_int
+        L.dr_head_loss_run.argtypes = [ctypes.POINTER(HeadLoss), c_int]
         L.dr_moe_workspace_bytes.restype = c_int64
         L.dr_moe_workspace_bytes.argtypes = [ctypes.POINTER(Launch), ctypes.POINTER(Moe)]
         L.dr_moe_matmul.restype = c_int
         L.dr_moe_matmul.argtypes = [ctypes.POINTER(Launch), ctypes.POINTER(Moe)]
         L.dr_moe_route.restype = c_int
         L.dr_moe_route.argtypes = [ctypes.POINTER(Route)]
+        L.dr_moe_balance_workspace_bytes.restype = c_int64
+        L.dr_moe_balance_workspace_bytes.argtypes = [ctypes.POINTER(Balance), c_int]
+        L.dr_moe_balance.restype = c_int
+        L.dr_moe_balance.argtypes = [ctypes.POINTER(Balance), c_int]
         L.dr_moe_route_gate_up.restype = c_int
         L.dr_moe_route_gate_up.argtypes = [ctypes.POINTER(Launch), ctypes.POINTER(Moe), ctypes.POINTER(Route)]
         _lib = L

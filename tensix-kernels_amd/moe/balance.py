@@ -1,0 +1,113 @@
+"""balance.py: the MoE router's balance loss and each expert's count on MI355X, with the gradient of the router's logits.
+The reference (XylolabsInc/tensix-kernels) has no counterpart; logits and ids are moe8.route's (its moe/moe8.py:1139-1253).
+
+  moe8.route(logits, ids, w, k)                              # the picks
+  loss, counts = balance_loss(logits, ids, k)                # differentiable in the logits
+  loss, counts, dlogits = balance_loss_grads(logits, ids, k, g)
+
+Over the rows t of a batch (the second last dim; the dims before it are batches, each with a loss of its own: a sequence's,
+or with one batch the whole step's): p[t] = softmax(logits[t]), or with kind "sigmoid" sigmoid(logits[t]) over its sum;
+counts[e] = the slots that chose expert e; loss = sum over e of E counts[e] / sum(counts) * mean over t of p[t][e], which is
+1 where every expert is chosen alike. The counts have no gradient (a choice has none). mask: the rows that count (a padded
+batch); the others enter nothing, whatever their logits and ids hold, and get zeros. An id at or past E chooses no expert.
+
+The kernels are dr_moe_balance's of libdense_reader.so (include/moe.h); nothing goes to the host, and the memory of a call
+is torch's, on the current stream, so a HIP graph can hold balance_loss and balance_loss_grads (autograd's backward refuses
+to be captured, as lm_head_topk.head_loss's does).
+"""
+
+import ctypes
+import sys
+from pathlib import Path
+
+import torch
+
+sys.path.insert(0, str(Path(__file__).resolve().parents[1]))
+from common import device as dev  # noqa: E402
+from dense_reader import _lib  # noqa: E402
+
+MAX_E = 1024  # experts at most, as moe8.route's
+KINDS = {"softmax": 0, "sigmoid": 1}
+
+
+def _run(logits, ids, k, g, kind, ids32, experts, mask, grad):
+    assert kind in KINDS, f"balance: kind {kind!r}"
+    assert logits.is_cuda and logits.dtype == torch.float32 and logits.dim() >= 2, (logits.device, logits.dtype)
+    *lead, R, W = logits.shape
+    E = W if experts is None else int(experts)
+    assert 1 <= E <= min(W, MAX_E) and 1 <= k <= 16, (E, W, k)
+    batch = 1
+    for n in lead:
+        batch *= n
+    want = (torch.int32, torch.uint32) if ids32 else (torch.int16, torch.uint16)
+    assert ids.dtype in want, f"balance: ids are {ids.dtype}, ids32={ids32} wants {want[0]} or {want[1]}"
+    assert ids.device == logits.device and ids.is_contiguous(), (ids.device, ids.is_contiguous())
+    ld = ids.shape[-1]
+    assert ld >= k and ids.numel() == batch * R * ld, (tuple(ids.shape), tuple(logits.shape), k)
+    lg = logits.detach().contiguous()
+    m = None
+    if mask is not None:
+        assert mask.device == logits.device and mask.dtype in (torch.bool, torch.uint8), (mask.device, mask.dtype)
+        assert mask.numel() == batch * R, (tuple(mask.shape), tuple(logits.shape))
+        m = mask.contiguous()
+    gs = None
+    if g is not None and grad:
+        gs = torch.as_tensor(g, device=logits.device)
+        assert gs.numel() in (1, batch), f"balance: {gs.numel()} weights for {batch} batches"
+        gs = gs.detach().reshape(-1).to(torch.float32).expand(batch).contiguous()
+
+    def new(*shape, dtype=torch.float32):
+        return torch.empty(shape, dtype=dtype, device=logits.device)
+
+    loss, counts = new(*lead), new(*lead, E, dtype=torch.int32)
+    dlogits = new(*logits.shape) if grad else None
+    if batch * R == 0:
+        loss.zero_(), counts.zero_()
+        return loss, counts, dlogits
+    A = _lib.Balance()
+    A.logits, A.ld_logits, A.batch, A.rows, A.experts, A.width = lg.data_ptr(), W, batch, R, E, W
+    A.ids, A.ld_ids, A.ids32, A.k, A.kind = ids.data_ptr(), ld, int(bool(ids32)), k, KINDS[kind]
+    A.mask, A.g, A.dlogits = (None if t is None else t.data_ptr() for t in (m, gs, dlogits))
+    A.loss, A.counts, A.ld_dlogits = loss.data_ptr(), counts.data_ptr(), W
+    what = _lib.DR_BALANCE_GRAD if grad else _lib.DR_BALANCE_LOSS
+    lib = _lib.lib()
+    need = lib.dr_moe_balance_workspace_bytes(ctypes.byref(A), what)
+    _lib.check(_lib.DR_EINVAL if need < 0 else _lib.DR_OK, "dr_moe_balance_workspace_bytes")
+    with torch.cuda.device(logits.device):
+        ws = new(need, dtype=torch.uint8)
+        A.workspace, A.workspace_bytes, A.stream = ws.data_ptr(), need, dev.raw_stream(logits.device)
+        _lib.check(lib.dr_moe_balance(ctypes.byref(A), what), "dr_moe_balance")
+    return loss, counts, dlogits
+
+
+class _Balance(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, k, kind, ids32, experts, mask):
+        loss, counts, _ = _run(logits, ids, k, None, kind, ids32, experts, mask, False)
+        ctx.save_for_backward(logits, ids, mask)
+        ctx.settings = k, kind, ids32, experts
+        ctx.mark_non_differentiable(counts)
+        return loss, counts
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, _):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("balance: a HIP graph captures balance_loss_grads, not backward()")
+        logits, ids, mask = ctx.saved_tensors
+        k, kind, ids32, experts = ctx.settings
+        return (_run(logits, ids, k, g, kind, ids32, experts, mask, True)[2], None, None, None, None, None, None)
+
+
+def balance_loss(logits, ids, k, *, kind="softmax", ids32=False, experts=None, mask=None):
+    """(loss, counts): logits [..., R, W] float32 on the GPU, ids [..., R, >= k] (uint16, or uint32 with ids32: moe8.route's,
+    contiguous; the first k of a row), loss float32 and counts int32 [..., E] for each batch of R rows. experts (default W):
+    the logits' columns 0 .. E - 1. mask [..., R] bool: the rows that count (default all). The loss is differentiable in the
+    logits."""
+    return _Balance.apply(logits, ids, k, kind, ids32, experts, mask)
+
+
+def balance_loss_grads(logits, ids, k, g=None, *, kind="softmax", ids32=False, experts=None, mask=None):
+    """balance_loss and, in the same call, the gradient of the sum over batches of g * loss: (loss, counts, dlogits), dlogits
+    of the logits' shape (zeros past E). g: each batch's weight, one number for all, or None for ones."""
+    return _run(logits, ids, k, g, kind, ids32, experts, mask, True)

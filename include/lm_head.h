@@ -87,9 +87,9 @@ typedef struct dr_head_loss {
     float* lse;           /* [rows] */
     float* logits;        /* [rows][k]: z at the entries (0 where none is held) */
     const float* g;       /* [rows], or NULL: ones */
-    void* dx;             /* [rows][ld_dx] bf16, 8-byte aligned, ld_dx a multiple of 4, or NULL */
+    void* dx;             /* [rows][ld_dx] bf16, 16-byte aligned, ld_dx a multiple of 8, or NULL */
     int64_t ld_dx;
-    void* dhead;          /* [vocab][ld_dhead] bf16, 8-byte aligned, ld_dhead a multiple of 4, or NULL */
+    void* dhead;          /* [vocab][ld_dhead] bf16, 16-byte aligned, ld_dhead a multiple of 8, or NULL */
     int64_t ld_dhead;
     void* workspace;      /* dr_head_loss_workspace_bytes, 256-byte aligned; its contents mean nothing between calls */
     int64_t workspace_bytes;

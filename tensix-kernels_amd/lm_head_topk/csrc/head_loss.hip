@@ -52,32 +52,39 @@ __device__ __forceinline__ void step_barrier() {
 
 // --- the tiled product ------------------------------------------------------------------------------------------------
 
-enum Epi { EPI_STATS, EPI_DZ, EPI_DHEAD, EPI_DX };
+enum Epi { EPI_STATS, EPI_DZ, EPI_DZ1, EPI_DHEAD, EPI_DX };  // (DZ1: tokens, their own logit's 1 taken off there)
 
 struct Gemm {
     const uint16_t *A, *B;  // D[m][n] = sum over k of A[m][k] B[n][k]; an operand lies [rows][k] or (across) [k][rows]
     long long lda, ldb;
     int m, n, k;            // (k: of a [rows][k] operand a multiple of 8)
     int ka;                 // the k rows that an A across has (past them zeros)
+    int nb;                 // dhead: the columns that B has (past them zeros)
+    long long panel;        // dz lies in panels of 256 v: v at (v / 256) panel + row 256 + v % 256
     const int* live;        // the rows that count: n of z and dx, k of dhead
-    int tm, tn, splits, steps;  // tiles; K splits of `steps` steps each
+    int tm, tn, steps;      // tiles; steps of K
     // z's epilogues
     float sc;               // z to the exponent of 2: log2(e) / T
     int v0;                 // z's row 0 is the vocabulary's v0
     const int* idx;         // row that counts -> row, or NULL: itself
     const float* lse;       // [rows]
-    const float* gs;        // [rows that count] g over the largest
+    const float* g;         // [rows], or NULL: ones
+    const float* top;       // the largest |g|
     f32x2* part;            // [m / TM][n] maximum and sum
     long long ld_part;
-    const int* ids;         // [rows][1 << kp] entries, -1 none
+    const int* ids;         // [rows that count][1 << kp] entries, -1 none
+    const void* raw;        // or tokens as they came ([rows] int32, or int64: raw64), those past m none
+    int raw64;
     int kp, kn;
     float* zt;              // [rows][kn]
     // outputs
-    uint16_t* out;          // dz [n][ld_out], dhead [n = v][ld_out]
-    float* acc;             // dx sums [splits][n][ld_out]
-    long long ld_out, acc_stride;
+    uint16_t* out;          // dz (panels), dhead [n = v][ld_out], dx [row][ld_out] or NULL: the sums are not complete
+    long long ld_out;
+    float* acc;             // dx sums [splits][rows that count][ld_acc]
+    long long ld_acc;
+    int plan_steps;         // dx: the steps of a whole piece, which its splits go by
     int add;                // dx: onto the sums so far
-    const float* scale;     // dhead: the factor taken out of dz
+    const float* scale;     // dhead, dx: the factor taken out of dz
 };
 
 // One operand's tile of ROWS x BK values in LDS: 16-byte chunks, laid out so that neither the loads straight from memory
@@ -107,7 +114,9 @@ struct Tile {
     // base: the tile's first value of this step; rows: its rows (across: the step's k) in memory; left: its k (across:
     // its rows) in memory
     __device__ __forceinline__ void load(const uint16_t* base, long long ld, int rows, int left, uint4* lds, int tid) const {
-        const long long bytes = rows > 0 && left > 0 ? ((long long)(rows - 1) * ld + ((left + 7) & ~7)) * 2 : 0;
+        // (no further than the tile's own run of its last row: what comes after may be rows that are not to be read)
+        const int run = min((left + 7) & ~7, T ? ROWS : BK);
+        const long long bytes = rows > 0 && left > 0 ? ((long long)(rows - 1) * ld + run) * 2 : 0;
         const __amdgpu_buffer_rsrc_t r =
             __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, (int)(bytes < 0x7FFFFFFF ? bytes : 0x7FFFFFFF), 0x00020000);
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -123,67 +132,111 @@ struct Tile {
             __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(lds + i * NT + 64 * wave), 16, o, 0, 0, 0);
         }
     }
-    // lane's 8 values of row r0 + lane % 32, k = 16 u + 8 (lane / 32) ..
-    static __device__ __forceinline__ uint4 frag(const uint4* lds, int r0, int u, int lane) {
+    // lane's 8 values of row r0 + lane % 32, k = 16 u + 8 (lane / 32) .., the tile from chunk `from` of the stage on. (One
+    // index from the stage's array: through longer chains the compiler no longer sees which stage a read is of, and has it
+    // wait for the loads to the other.)
+    static __device__ __forceinline__ uint4 frag(const uint4* lds, int from, int r0, int u, int lane) {
         if constexpr (T) {
             constexpr int C = ROWS / 8;
             const int h = lane >> 5, half = (lane >> 4) & 1, i = lane & 15;
-            uint2 q[2];
-#pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                const int k = 16 * u + 8 * h + 4 * p + (i >> 2);
-                const int pair = ((r0 >> 4) + half) ^ turn(k);
-                const uint16_t* at = reinterpret_cast<const uint16_t*>(lds + k * C + 2 * pair) + 4 * (i & 3);
-                q[p] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at));
-            }
-            return make_uint4(q[0].x, q[0].y, q[1].x, q[1].y);
+            const int k = 8 * h + (i >> 2), pair = ((r0 >> 4) + half) ^ turn(k);  // (turn: the same 4 and 16 k further)
+            const int at = (from + k * C + 2 * pair) * 8 + 4 * (i & 3) + 16 * u * ROWS;
+            const uint16_t* v = reinterpret_cast<const uint16_t*>(lds);
+            const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(v + at)));
+            const uint2 hi = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(v + (at + 4 * ROWS))));
+            return make_uint4(lo.x, lo.y, hi.x, hi.y);
         } else {
             const int r = lane & 31, h = lane >> 5;
-            return lds[(r0 + r) * 8 + ((2 * u + h) ^ ((r >> 1) & 7))];
+            return lds[from + (r0 + r) * 8 + ((2 * u + h) ^ ((r >> 1) & 7))];
         }
     }
 };
 
-// workgroups go to the XCDs in turn; each XCD takes a run of tiles, in groups of GM row tiles by all column tiles, so that
-// what runs at once on an XCD shares rows and columns in its L2
-__device__ __forceinline__ void tile_of(const Gemm& a, int& mt, int& nt, int& split) {
-    const int total = a.tm * a.tn * a.splits, xcd = blockIdx.x & 7;
-    int w = xcd * (total >> 3) + min(xcd, total & 7) + (blockIdx.x >> 3);
-    split = w / (a.tm * a.tn);
-    w -= split * a.tm * a.tn;
-    constexpr int GM = 4;
-    const int g = w / (GM * a.tn), first = g * GM, gm = min(GM, a.tm - first);
-    w -= g * GM * a.tn;
-    nt = w / gm;
-    mt = first + w - nt * gm;
+// Tiles and the time (us) that a workgroup takes for a step and for its beginning and end, as many workgroups running at once
+// as fit the CUs: a step of 256 x 256 took 1.88 us, one of 128 x 128, two a CU, 1.0 to 1.1 (8192 x 4096 x 16384: 1240
+// against 1030 TFLOP/s of dx).
+struct Pace {
+    int at_once;
+    float step, ends;
+};
+constexpr int CUS = 256;
+__host__ __device__ constexpr Pace pace(int bm, int bn) {
+    return bn == 64 ? Pace{2 * CUS, 0.6f, 8.f} : bm == 256 ? Pace{CUS, 1.88f, 14.f} : Pace{2 * CUS, 1.1f, 11.f};
 }
 
-template <int BM, int BN, int WM, int WN, bool AT, bool BT, int EPI>
+__host__ __device__ inline float tiled_us(const Pace& p, int tiles, int steps) {
+    return (float)((tiles + p.at_once - 1) / p.at_once) * (p.step * (float)steps + p.ends);
+}
+
+// dx's splits of its long sum, for one or two rounds of workgroups: a split more costs its sums' way through memory. The
+// rows that count are known on the device alone, so every workgroup finds them for itself.
+constexpr int ROUNDS = 2;
+__host__ __device__ inline int dx_splits(const Pace& p, int tiles, int steps, int tile_bytes, float* us = nullptr) {
+    int best = 1;
+    float least = tiled_us(p, tiles, steps);
+    for (int r = 1; r <= ROUNDS; ++r) {
+        int s = r * p.at_once / (tiles > 0 ? tiles : 1);
+        if (s > steps / 4) s = steps / 4;
+        if (s < 2) continue;
+        const float t = tiled_us(p, tiles * s, ((steps + s - 1) / s + 1) & ~1) + 4.f + (float)tiles * (float)s * (float)tile_bytes * 0.5e-6f;
+        if (t < least) least = t, best = s;
+    }
+    if (us) *us = least;
+    return best;
+}
+
+// workgroups go to the XCDs in turn; each XCD takes a run of tiles, in groups of GM row tiles by all column tiles, so that
+// what runs at once on an XCD shares rows and columns in its L2. False past the last.
+__device__ __forceinline__ bool tile_of(int tm, int tn, int splits, int& mt, int& nt, int& split) {
+    const int total = tm * tn * splits, xcd = blockIdx.x & 7, own = (total >> 3) + (xcd < (total & 7));
+    if ((int)(blockIdx.x >> 3) >= own) return false;
+    int w = xcd * (total >> 3) + min(xcd, total & 7) + (blockIdx.x >> 3);
+    split = w / (tm * tn);
+    w -= split * tm * tn;
+    constexpr int GM = 4;
+    const int g = w / (GM * tn), first = g * GM, gm = min(GM, tm - first);
+    w -= g * GM * tn;
+    nt = w / gm;
+    mt = first + w - nt * gm;
+    return true;
+}
+
+template <int BM, int BN, int WM, int WN, int NS, bool AT, bool BT, int EPI>
 __global__ __launch_bounds__(64 * WM * WN) void hl_gemm(const Gemm a) {
-    constexpr int NT = 64 * WM * WN, TM = BM / WM, TN = BN / WN, MI = TM / 32, NI = TN / 32;
+    constexpr int NW = WM * WN, NT = 64 * NW, TM = BM / WM, TN = BN / WN, MI = TM / 32, NI = TN / 32;
     constexpr int CH = (BM + BN) * 8;  // chunks a stage
-    __shared__ uint4 s0[CH], s1[CH];
+    constexpr int NL = CH / NT;        // loads a lane and stage
+    static_assert(NS == 2 || NS == 4, "two or four stages");
+    __shared__ uint4 s0[CH], s1[CH], s2[NS > 2 ? CH : 1], s3[NS > 2 ? CH : 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WN, wn = wave % WN;
-    int mt, nt, split;
-    tile_of(a, mt, nt, split);
-    const int m0 = mt * BM, n0 = nt * BN;
     const int live = a.live ? *a.live : (EPI == EPI_DHEAD ? a.k : a.n);
+    // (dx: the tiles of the rows that count, split as many ways as fill the CUs)
+    const int tn = EPI == EPI_DX ? (live + BN - 1) / BN : a.tn;
+    const int splits = EPI == EPI_DX ? dx_splits(pace(BM, BN), a.tm * tn, a.plan_steps, BM * BN * 8) : 1;
+    int mt, nt, split;
+    if (!tile_of(a.tm, tn, splits, mt, nt, split)) return;
+    const int m0 = mt * BM, n0 = nt * BN;
     const int n_end = EPI == EPI_DHEAD ? a.n : live, k_end = EPI == EPI_DHEAD ? live : a.k;
-    const int ka = EPI == EPI_DHEAD ? live : a.ka;
+    const int nb = EPI == EPI_DHEAD ? a.nb : n_end, ka = EPI == EPI_DHEAD ? live : a.ka;
     if (n0 >= n_end) return;
-    const int step0 = split * a.steps, steps = min(a.steps, (k_end + BK - 1) / BK - step0);
+    // (a split's steps are whole rounds of the stages: the next split's are not its own)
+    const int all = (k_end + BK - 1) / BK, per = ((all + splits - 1) / splits + NS - 1) / NS * NS, step0 = split * per;
+    const int steps = EPI == EPI_DHEAD && n0 >= nb ? 0 : min(per, all - step0);
 
     Tile<BM, AT, NT> ta;
     Tile<BN, BT, NT> tb;
     ta.init(tid, a.lda, a.m - m0);
-    tb.init(tid, a.ldb, n_end - n0);
+    tb.init(tid, a.ldb, nb - n0);
     auto load = [&](int s, uint4* b) {
-        const long long k0 = (long long)(step0 + s) * BK;
-        if constexpr (AT) ta.load(a.A + k0 * a.lda + m0, a.lda, min(BK, ka - (int)k0), a.m - m0, b, tid);
-        else ta.load(a.A + m0 * a.lda + k0, a.lda, min(BM, a.m - m0), k_end - (int)k0, b, tid);
-        if constexpr (BT) tb.load(a.B + k0 * a.ldb + n0, a.ldb, min(BK, k_end - (int)k0), n_end - n0, b + BM * 8, tid);
-        else tb.load(a.B + n0 * a.ldb + k0, a.ldb, min(BN, n_end - n0), k_end - (int)k0, b + BM * 8, tid);
+        const int k0 = (step0 + s) * BK;
+        if constexpr (AT) ta.load(a.A + k0 * a.lda + m0, a.lda, min(BK, ka - k0), a.m - m0, b, tid);
+        else ta.load(a.A + m0 * a.lda + k0, a.lda, min(BM, a.m - m0), k_end - k0, b, tid);
+        if constexpr (EPI == EPI_DHEAD)
+            tb.load(a.B + (n0 >> 8) * a.panel + (n0 & 255) + k0 * a.ldb, a.ldb, min(BK, k_end - k0), nb - n0, b + BM * 8, tid);
+        else if constexpr (EPI == EPI_DX)
+            tb.load(a.B + (k0 >> 8) * a.panel + (k0 & 255) + n0 * a.ldb, a.ldb, min(BN, n_end - n0), k_end - k0, b + BM * 8, tid);
+        else tb.load(a.B + n0 * a.ldb + k0, a.ldb, min(BN, n_end - n0), k_end - k0, b + BM * 8, tid);
     };
     f32x16 acc[MI][NI];
 #pragma unroll
@@ -197,9 +250,9 @@ __global__ __launch_bounds__(64 * WM * WN) void hl_gemm(const Gemm a) {
         for (int u = 0; u < BK / 16; ++u) {
             uint4 fa[MI], fb[NI];
 #pragma unroll
-            for (int j = 0; j < NI; ++j) fb[j] = Tile<BN, BT, NT>::frag(b + BM * 8, wn * TN + 32 * j, u, lane);
+            for (int j = 0; j < NI; ++j) fb[j] = Tile<BN, BT, NT>::frag(b, BM * 8, wn * TN + 32 * j, u, lane);
 #pragma unroll
-            for (int i = 0; i < MI; ++i) fa[i] = Tile<BM, AT, NT>::frag(b, wm * TM + 32 * i, u, lane);
+            for (int i = 0; i < MI; ++i) fa[i] = Tile<BM, AT, NT>::frag(b, 0, wm * TM + 32 * i, u, lane);
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -207,25 +260,62 @@ __global__ __launch_bounds__(64 * WM * WN) void hl_gemm(const Gemm a) {
             __builtin_amdgcn_sched_barrier(0);  // (one u's fragments at a time: the registers hold no more)
         }
     };
-    // (in pairs of steps: one past the last is zeros, as are the loads past the end into a stage that nothing reads. A
-    // last step of its own behind a branch would have the compiler copy every accumulator.)
-    if (steps > 0) load(0, s0);
-    for (int s = 0; s < steps; s += 2) {
-        step_barrier<0>();
-        load(s + 1, s1);
-        sum(s0);
-        step_barrier<0>();
-        load(s + 2, s0);
-        sum(s1);
+    // (whole rounds of the stages: steps past the last are zeros, as are the loads past the end into stages that nothing
+    // reads. A last step of its own behind a branch would have the compiler copy every accumulator.)
+    if (steps > 0) {
+        load(0, s0);
+        if constexpr (NS > 2) load(1, s1), load(2, s2);
+    }
+    for (int s = 0; s < steps; s += NS) {
+        if constexpr (NS == 2) {
+            step_barrier<0>();
+            load(s + 1, s1);
+            sum(s0);
+            step_barrier<0>();
+            load(s + 2, s0);
+            sum(s1);
+        } else {
+            step_barrier<2 * NL>();
+            load(s + 3, s3);
+            sum(s0);
+            step_barrier<2 * NL>();
+            load(s + 4, s0);
+            sum(s1);
+            step_barrier<2 * NL>();
+            load(s + 5, s1);
+            sum(s2);
+            step_barrier<2 * NL>();
+            load(s + 6, s2);
+            sum(s3);
+        }
     }
     step_barrier<0>();  // (the last loads landed: they write this workgroup's LDS)
 
     // lane: columns n = n0 + wn TN + 32 j + lane % 32, rows m0 + wm TM + 32 i + 8 g + 4 (lane / 32) + 0 .. 3 in words 4 g ..
     const int r = lane & 31, h = lane >> 5;
     const int mw = m0 + wm * TM;
+    // the wavefront's own part of the stages: 32 columns of its TM rows in float32
+    constexpr int PER = (NW + NS - 1) / NS;
+    static_assert(PER * 8 * TM <= CH, "a wavefront's sums of 32 columns fit its part of a stage");
+    const int st = wave / PER;
+    uint4* const region = (NS == 2 ? (st ? s1 : s0) : st == 0 ? s0 : st == 1 ? s1 : st == 2 ? s2 : s3) + (wave % PER) * 8 * TM;
+    // 32 columns in bf16, 4 rows of column r at 8-byte unit q: to whole runs of a column's rows in memory
+    uint2* const half = reinterpret_cast<uint2*>(region);
+    constexpr int C16 = TM / 8, SWZ = C16 < 16 ? C16 - 1 : 15;  // 16-byte chunks a column; their turn by column
+    auto put = [&](int q, uint2 v) { half[(r * C16 + ((q >> 1) ^ (r & SWZ))) * 2 + (q & 1)] = v; };
+    auto store = [&](auto&& at, int cols, int rows) {  // at(c, row): column c's place for 8 of its rows from `row` on
+        __builtin_amdgcn_wave_barrier();
+        constexpr int PC = 64 / C16;  // columns a turn
+#pragma unroll
+        for (int t = 0; t < 32 / PC; ++t) {
+            const int c = t * PC + lane / C16, q = lane % C16;
+            if (c < cols && 8 * q < rows) *reinterpret_cast<uint4*>(at(c, 8 * q)) = region[c * C16 + (q ^ (c & SWZ))];
+        }
+        __builtin_amdgcn_wave_barrier();
+    };
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
-        const int n = n0 + wn * TN + 32 * j + r;
+        const int nj = n0 + wn * TN + 32 * j, n = nj + r;
         if constexpr (EPI == EPI_STATS) {
             const int left = a.m - mw;  // vocabulary rows of this wavefront
             if (left < TM) {
@@ -250,20 +340,9 @@ __global__ __launch_bounds__(64 * WM * WN) void hl_gemm(const Gemm a) {
             total += __shfl_xor(total, 32);
             if (h == 0 && n < n_end) a.part[(long long)(mt * WM + wm) * a.ld_part + n] = f32x2{top == -INFINITY ? top : base, total};
             // the entries that lie here: the wavefront's sums of these 32 rows through its own LDS
-            f32x4* mine = reinterpret_cast<f32x4*>(wave < (WM * WN + 1) / 2 ? s0 : s1) + (wave % ((WM * WN + 1) / 2)) * 8 * TM;
-            static_assert((WM * WN + 1) / 2 * 8 * TM <= CH, "a wavefront's sums of 32 rows fit its part of a stage");
-            const int count = 32 << a.kp, nb = n0 + wn * TN + 32 * j;
-            auto entry = [&](int e, long long& row) {  // its row of mw .., or -1
-                const int nn = nb + (e >> a.kp);
-                if (e >= count || nn >= n_end) return -1;
-                row = a.idx ? a.idx[nn] : nn;
-                const int d = a.ids[(row << a.kp) + (e & ((1 << a.kp) - 1))] - mw;
-                return (unsigned)d < (unsigned)min(TM, left) ? d : -1;
-            };
-            long long row = 0;
-            bool any = a.kp >= 4;
-            for (int e = lane; !any && e - lane < count; e += 64) any = __ballot(entry(e, row) >= 0) != 0;
-            if (any) {
+            f32x4* mine = reinterpret_cast<f32x4*>(region);
+            const int here = min(TM, left), w = 1 << a.kp;
+            auto lay = [&] {
 #pragma unroll
                 for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -271,45 +350,109 @@ __global__ __launch_bounds__(64 * WM * WN) void hl_gemm(const Gemm a) {
                         mine[r * (TM / 4) + ((8 * i + 2 * g + h) ^ (r & 7))] =
                             f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
                 __builtin_amdgcn_wave_barrier();
-                for (int e = lane; e - lane < count; e += 64) {
-                    const int d = entry(e, row), t = e >> a.kp;
-                    if (d >= 0) a.zt[row * a.kn + (e & ((1 << a.kp) - 1))] = mine[t * (TM / 4) + ((d >> 2) ^ (t & 7))][d & 3];
+            };
+            auto take = [&](int t, int kk, int d) {  // column t's entry kk at this wavefront's row d
+                const long long row = a.idx ? a.idx[nj + t] : nj + t;
+                a.zt[row * a.kn + kk] = mine[t * (TM / 4) + ((d >> 2) ^ (t & 7))][d & 3];
+            };
+            if (a.kp < 2) {
+                const int t = lane >> a.kp;
+                int d = -1;
+                if (t < 32 && nj + t < n_end) {
+                    if (a.raw) {
+                        const long long id = a.raw64 ? reinterpret_cast<const long long*>(a.raw)[nj + t]
+                                                     : reinterpret_cast<const int*>(a.raw)[nj + t];
+                        d = id >= mw && id < mw + here ? (int)(id - mw) : -1;
+                    } else {
+                        d = a.ids[((long long)nj << a.kp) + lane] - mw;
+                    }
                 }
-                __builtin_amdgcn_wave_barrier();
+                const bool hit = (unsigned)d < (unsigned)here && here > 0;
+                if (__ballot(hit)) {
+                    lay();
+                    if (hit) take(t, lane & (w - 1), d);
+                }
+            } else {  // four a load, eight loads at once
+                const int count = 8 << a.kp;
+                const int4* at = reinterpret_cast<const int4*>(a.ids + ((long long)nj << a.kp));
+                int4 v[8];
+                bool hit = false;
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const int e = lane + 64 * q;
+                    v[q] = e < count && nj + (4 * e >> a.kp) < n_end ? at[e] : make_int4(-1, -1, -1, -1);
+                }
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    v[q].x -= mw, v[q].y -= mw, v[q].z -= mw, v[q].w -= mw;
+                    hit |= (unsigned)v[q].x < (unsigned)here || (unsigned)v[q].y < (unsigned)here ||
+                           (unsigned)v[q].z < (unsigned)here || (unsigned)v[q].w < (unsigned)here;
+                }
+                if (here > 0 && __ballot(hit)) {
+                    lay();
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {
+                        const int e = 4 * (lane + 64 * q), t = e >> a.kp, kk = e & (w - 1);
+                        if ((unsigned)v[q].x < (unsigned)here) take(t, kk, v[q].x);
+                        if ((unsigned)v[q].y < (unsigned)here) take(t, kk + 1, v[q].y);
+                        if ((unsigned)v[q].z < (unsigned)here) take(t, kk + 2, v[q].z);
+                        if ((unsigned)v[q].w < (unsigned)here) take(t, kk + 3, v[q].w);
+                    }
+                }
             }
-        } else if constexpr (EPI == EPI_DZ) {
-            if (n >= n_end) continue;
-            const float l2 = a.lse[a.idx ? a.idx[n] : n] * LOG2E, gs = a.gs[n];
+            __builtin_amdgcn_wave_barrier();
+        } else if constexpr (EPI == EPI_DZ || EPI == EPI_DZ1) {
+            const long long row = n < n_end ? a.idx[n] : 0;
+            const float top = *a.top, l2 = n < n_end ? a.lse[row] * LOG2E : 0.f, gr = a.g && n < n_end ? a.g[row] : 1.f;
+            const float gs = top > 0.f ? gr / top : gr;
             const int left = a.m - mw;
-            uint16_t* o = a.out + n * a.ld_out + mw;
+            const int own = EPI == EPI_DZ1 && n < n_end ? a.ids[n] - a.v0 - mw - 4 * h : -1;  // (the token's own logit)
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const int v = 32 * i + 8 * g + 4 * h;
                     float p[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        p[e] = v + e < left ? gs * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][4 * g + e], a.sc, -l2)) : 0.f;
-                    *reinterpret_cast<uint2*>(o + v) = make_uint2(cvt2(p[0], p[1]), cvt2(p[2], p[3]));
+                    for (int e = 0; e < 4; ++e) {
+                        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][4 * g + e], a.sc, -l2));
+                        if (EPI == EPI_DZ1 && own == 32 * i + 8 * g + e) p[e] -= 1.f;
+                        p[e] *= gs;
+                    }
+                    if (left < TM) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (32 * i + 8 * g + 4 * h + e >= left) p[e] = 0.f;
+                    }
+                    put(8 * i + 2 * g + h, make_uint2(cvt2(p[0], p[1]), cvt2(p[2], p[3])));
                 }
+            uint16_t* o = a.out + (mw >> 8) * a.panel + (long long)nj * 256 + (mw & 255);
+            store([&](int c, int row) { return o + c * 256 + row; }, n_end - nj, TM);
         } else if constexpr (EPI == EPI_DHEAD) {
-            if (n >= n_end) continue;
             const float s = *a.scale;
-            uint16_t* o = a.out + n * a.ld_out + mw;
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    put(8 * i + 2 * g + h, make_uint2(cvt2(acc[i][j][4 * g] * s, acc[i][j][4 * g + 1] * s),
+                                                      cvt2(acc[i][j][4 * g + 2] * s, acc[i][j][4 * g + 3] * s)));
+            uint16_t* o = a.out + nj * a.ld_out + mw;
+            store([&](int c, int row) { return o + c * a.ld_out + row; }, n_end - nj, a.m - mw);
+        } else if (a.out != nullptr && splits == 1) {  // the last sums: dx itself
+            const float s = *a.scale;
+            const long long at = n * a.ld_acc + mw;
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     const int d = 32 * i + 8 * g + 4 * h;
-                    if (mw + d < a.m)
-                        *reinterpret_cast<uint2*>(o + d) =
-                            make_uint2(cvt2(acc[i][j][4 * g] * s, acc[i][j][4 * g + 1] * s),
-                                       cvt2(acc[i][j][4 * g + 2] * s, acc[i][j][4 * g + 3] * s));
+                    f32x4 v = f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+                    if (a.add && n < n_end && mw + d < a.m) v += *reinterpret_cast<const f32x4*>(a.acc + at + d);
+                    put(8 * i + 2 * g + h, make_uint2(cvt2(v[0] * s, v[1] * s), cvt2(v[2] * s, v[3] * s)));
                 }
+            store([&](int c, int row) { return a.out + a.idx[nj + c] * a.ld_out + mw + row; }, n_end - nj, a.m - mw);
         } else {
             if (n >= n_end) continue;
-            float* o = a.acc + split * a.acc_stride + n * a.ld_out + mw;
+            float* o = a.acc + ((long long)split * live + n) * a.ld_acc + mw;
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -330,17 +473,18 @@ __global__ __launch_bounds__(64 * WM * WN) void hl_gemm(const Gemm a) {
 
 struct Prep {
     dr_head_loss a;
-    int kp;        // log2 of the entries' stride
-    int* ids;      // [rows][1 << kp], -1: not held
-    float* q;      // [rows][1 << kp] (a teacher's)
-    float* ent;    // [rows] sum q log q (a teacher's)
-    int* idx;      // [rows] row that counts -> row
-    int* pos;      // [rows] row -> row that counts, -1: left out
-    int* live;     // rows that count
-    float* scale;  // the largest |g| of them, over T
-    float* gs;     // [rows that count]
-    uint16_t* xc;  // [rows that count][dim], or NULL: x where it lies
-    int fwd, back;
+    int kp;         // log2 of the entries' stride
+    int* ids;       // [rows][1 << kp], -1: not held
+    int* idc;       // [rows that count][1 << kp]
+    float* q;       // [rows][1 << kp] (a teacher's)
+    float* ent;     // [rows] sum q log q (a teacher's)
+    uint8_t* held;  // [rows] whether the row counts
+    int* idx;       // [rows] row that counts -> row
+    int* pos;       // [rows] row -> row that counts, -1: left out
+    int* live;      // rows that count
+    float* top;     // the largest |g| of them, and that over T
+    uint16_t* xc;   // [rows that count][dim]
+    uint16_t* dx;   // whose rows left out get zeros, or NULL
 };
 
 __device__ __forceinline__ int entry_id(const dr_head_loss& a, int row, int j) {
@@ -349,10 +493,10 @@ __device__ __forceinline__ int entry_id(const dr_head_loss& a, int row, int j) {
     return id >= 0 && id < a.valid ? (int)id : -1;
 }
 
-// the entries of a row: 1 << kp lanes a row
-__global__ __launch_bounds__(256) void hl_entries(const Prep p) {
-    const int e = blockIdx.x * 256 + threadIdx.x, row = e >> p.kp, w = 1 << p.kp, j = e & (w - 1);
-    const bool in = row < p.a.rows && j < p.a.k;
+// entry e of all rows' (row e >> kp; the lanes of a row are neighbours): id, q, the row's sum; whether the row counts
+__device__ __forceinline__ bool entries_of(const Prep& p, int e, int rows) {
+    const int row = e >> p.kp, w = 1 << p.kp, j = e & (w - 1);
+    const bool in = row < rows && j < p.a.k;
     int id = in ? entry_id(p.a, row, j) : -1;
     if (p.a.vals) {
         float v = in ? p.a.vals[(long long)row * p.a.ld_vals + j] / p.a.temperature : -INFINITY;
@@ -367,137 +511,219 @@ __global__ __launch_bounds__(256) void hl_entries(const Prep p) {
         const float q = id < 0 ? 0.f : x / total;
         float ent = q == 0.f ? 0.f : q * (d - __logf(total));
         for (int o = w >> 1; o; o >>= 1) ent += __shfl_xor(ent, o);
-        if (row < p.a.rows) {
+        if (row < rows) {
             p.q[e] = q;
             if (j == 0) p.ent[row] = ent;
         }
     }
-    if (row < p.a.rows) {
+    const unsigned long long held = __ballot(id >= 0);
+    const int lane = threadIdx.x & 63;
+    const unsigned long long mine = w == 64 ? held : (held >> (lane & ~(w - 1))) & ((1ull << w) - 1);
+    if (row < rows) {
         p.ids[e] = id;
-        if (in && id < 0 && p.fwd) p.a.logits[(long long)row * p.a.k + j] = 0.f;
-        const unsigned long long held = __ballot(id >= 0);
-        const int lane = threadIdx.x & 63;
-        const unsigned long long mine = w == 64 ? held : (held >> (lane & ~(w - 1))) & ((1ull << w) - 1);
-        if (j == 0) p.pos[row] = mine ? 0 : -1;
+        if (j == 0) p.held[row] = mine != 0;
     }
+    return mine != 0;
 }
 
-// the rows that count, in order: each workgroup counts those before its own
-__global__ __launch_bounds__(256) void hl_count(const Prep p) {
-    __shared__ int part[256];
-    __shared__ float gpart[256];
-    const int tid = threadIdx.x, per = (p.a.rows + 255) / 256;
-    const int r0 = min(tid * per, p.a.rows), r1 = min(r0 + per, p.a.rows);
-    int c = 0;
-    float gm = 0.f;
-    for (int r = r0; r < r1; ++r)
-        if (p.pos[r] >= 0) {
-            ++c;
-            const float g = p.a.g ? fabsf(p.a.g[r]) : 1.f;
-            gm = fmaxf(gm, g);
-        }
-    part[tid] = c;
-    gpart[tid] = gm;
-    __syncthreads();
-    int before = 0;
-    for (int i = 0; i < tid; ++i) before += part[i];
-    float top = 0.f;
-    for (int i = 0; i < 256; ++i) top = fmaxf(top, gpart[i]);
-    if (tid == 255) {
-        *p.live = before + c;
-        *p.scale = top / p.a.temperature;
-    }
-    const float inv = top > 0.f ? 1.f / top : 0.f;
-    for (int r = r0; r < r1; ++r)
-        if (p.pos[r] >= 0) {
-            p.pos[r] = before;
-            p.idx[before] = r;
-            if (p.back) p.gs[before] = (p.a.g ? p.a.g[r] : 1.f) == top ? 1.f : (p.a.g ? p.a.g[r] : 1.f) * inv;
-            ++before;
-        }
+__global__ __launch_bounds__(256) void hl_entries(const Prep p) { entries_of(p, blockIdx.x * 256 + threadIdx.x, p.a.rows); }
+
+__device__ __forceinline__ int wave_sum(int v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    return v;
 }
 
+constexpr int GROWS = 16;    // rows a workgroup of hl_gather
+constexpr int FEW = 2048;    // entries that every workgroup looks through itself
+
+// The rows that count, one after another: each workgroup finds the place of its own from the flags of all rows before
+// (16 a load), so that nothing waits for anything; one more finds how many there are and the largest |g|. OWN: the entries
+// too, of few rows, every workgroup looking through all of the ids for the flags (a launch less).
+template <bool OWN>
 __global__ __launch_bounds__(256) void hl_gather(const Prep p) {
-    const int n = blockIdx.x;
-    if (n >= *p.live) return;
-    const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.a.x) + p.idx[n] * p.a.ldx);
-    uint4* dst = reinterpret_cast<uint4*>(p.xc + (long long)n * p.a.dim);
-    for (int c = threadIdx.x; c < p.a.dim / 8; c += 256) dst[c] = src[c];
+    __shared__ int sums[4];
+    __shared__ float tops[4];
+    __shared__ int rows[GROWS];
+    __shared__ uint4 flag4[OWN ? FEW / 16 : 1];
+    uint8_t* const flags = reinterpret_cast<uint8_t*>(flag4);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = p.a.rows;
+    const bool last = blockIdx.x == gridDim.x - 1;
+    const int r0 = last ? n : blockIdx.x * GROWS;
+    const uint8_t* held = p.held;
+    if constexpr (OWN) {
+        for (int i = tid; i < FEW / 16; i += 256) flag4[i] = make_uint4(0u, 0u, 0u, 0u);
+        __syncthreads();
+        const int upto = min(n, r0 + GROWS) << p.kp, w = 1 << p.kp;
+        for (int e = tid; e < upto; e += 256) {
+            const int row = e >> p.kp, j = e & (w - 1);
+            if (j < p.a.k && entry_id(p.a, row, j) >= 0 && (!p.a.vals || p.a.vals[(long long)row * p.a.ld_vals + j] != -INFINITY))
+                flags[row] = 1;
+        }
+        __syncthreads();
+        held = flags;
+        if (!last)
+            for (int e = tid; e < GROWS << p.kp; e += 256) entries_of(p, (r0 << p.kp) + e, min(n, r0 + GROWS));
+    }
+    int c = 0;
+    for (int i = tid; i < r0 / 16; i += 256) {
+        const uint4 f = reinterpret_cast<const uint4*>(held)[i];
+        c += __popc(f.x) + __popc(f.y) + __popc(f.z) + __popc(f.w);
+    }
+    if (last && tid < n % 16) c += held[n / 16 * 16 + tid];
+    c = wave_sum(c);
+    float top = 0.f;
+    if (last && p.a.g) {
+#pragma unroll 8
+        for (int r = tid; r < n; r += 256) {
+            const float g = fabsf(p.a.g[r]);
+            top = fmaxf(top, held[r] ? g : 0.f);
+        }
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    if (lane == 0) sums[wave] = c, tops[wave] = top;
+    __syncthreads();
+    const int before = sums[0] + sums[1] + sums[2] + sums[3];
+    if (last) {
+        if (tid == 0) {
+            top = p.a.g ? fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) : 1.f;
+            *p.live = before;
+            p.top[0] = top;
+            p.top[1] = top / p.a.temperature;
+        }
+        return;
+    }
+    if (wave == 0) {
+        const int r = r0 + lane;
+        const bool on = lane < GROWS && r < n && held[r] != 0;
+        const unsigned long long b = __ballot(on);
+        const int at = before + __popcll(b & ((1ull << lane) - 1));
+        if (lane < GROWS) rows[lane] = on ? at : -1;
+        if (lane < GROWS && r < n) p.pos[r] = on ? at : -1;
+        if (on) p.idx[at] = r;
+    }
+    __syncthreads();  // (OWN: this workgroup's entries are written too)
+    for (int i = wave; i < GROWS; i += 4) {
+        const int at = rows[i];
+        if (at < 0) {
+            if (p.dx && r0 + i < n)  // (a row left out)
+                for (int q = lane; q < p.a.dim / 4; q += 64)
+                    *reinterpret_cast<uint2*>(p.dx + (r0 + i) * p.a.ld_dx + 4 * q) = make_uint2(0u, 0u);
+            continue;
+        }
+        if (lane < 1 << p.kp) p.idc[((long long)at << p.kp) + lane] = p.ids[((long long)(r0 + i) << p.kp) + lane];
+        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.a.x) + (r0 + i) * p.a.ldx);
+        uint4* dst = reinterpret_cast<uint4*>(p.xc + (long long)at * p.a.dim);
+#pragma unroll 8
+        for (int q = lane; q < p.a.dim / 8; q += 64) dst[q] = src[q];
+    }
 }
 
 struct Merge {
     const f32x2* part;
     long long ld;
-    int parts, rows, k, kp, gather;
-    const int *pos;
+    int parts, rows, k, kp;
+    const int* pos;       // NULL: a row's own place
+    const uint8_t* held;  // NULL: tokens as they came
+    const void* raw;
+    int raw64, valid;
+    const int* ids;
     const float *q, *ent;
     float inv_t;
-    float *loss, *lse;
-    const float* zt;
+    float *loss, *lse, *zt;
 };
 
-// TB rows a workgroup, 256 / TB slices of the parts each
-template <int TB>
-__global__ __launch_bounds__(256) void hl_merge(const Merge p) {
-    __shared__ float ms[256], ss[256];
+__device__ __forceinline__ void join(float& m, float& s, float v, float w) {
+    if (v == -INFINITY) return;  // (nothing there)
+    const float top = fmaxf(m, v);
+    s = s * __builtin_amdgcn_exp2f(m - top) + w * __builtin_amdgcn_exp2f(v - top);
+    m = top;
+}
+
+// a row's wavefronts' maxima and sums joined, then lse and loss: TB rows a workgroup of 32 slices (8 of one row)
+template <int TB, int SL>
+__global__ __launch_bounds__(TB* SL) void hl_merge(const Merge p) {
+    __shared__ float ms[TB * SL], ss[TB * SL];
     const int tid = threadIdx.x, t = tid % TB, sl = tid / TB, row = blockIdx.x * TB + t;
-    int n = row < p.rows ? p.pos[row] : -1;
-    if (n >= 0 && !p.gather) n = row;
-    float m = -INFINITY, s = 0.f;
-    if (n >= 0)
-        for (int i = sl; i < p.parts; i += 256 / TB) {
-            const f32x2 v = p.part[i * p.ld + n];
-            if (v[0] == -INFINITY) continue;
-            const float top = fmaxf(m, v[0]);
-            if (top == m) s += v[1] * __builtin_amdgcn_exp2f(v[0] - top);
-            else s = s * __builtin_amdgcn_exp2f(m - top) + v[1], m = top;
+    bool in = false;
+    if (row < p.rows) {
+        if (p.held) {
+            in = p.held[row];
+        } else {
+            const long long id = p.raw64 ? reinterpret_cast<const long long*>(p.raw)[row] : reinterpret_cast<const int*>(p.raw)[row];
+            in = id >= 0 && id < p.valid;
         }
+    }
+    const int n = !in ? -1 : p.pos ? p.pos[row] : row;
+    float m = -INFINITY, s = 0.f;
+    if (n >= 0) {
+        const f32x2* at = p.part + n;
+        int i = sl;
+        for (; i + 3 * SL < p.parts; i += 4 * SL) {
+            f32x2 v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = at[(i + u * SL) * p.ld];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) join(m, s, v[u][0], v[u][1]);
+        }
+        for (; i < p.parts; i += SL) {
+            const f32x2 v = at[i * p.ld];
+            join(m, s, v[0], v[1]);
+        }
+    }
     ms[tid] = m;
     ss[tid] = s;
     __syncthreads();
-    if (sl) return;
-    for (int i = 1; i < 256 / TB; ++i) {
-        const float v = ms[i * TB + t], w = ss[i * TB + t];
-        const float top = fmaxf(m, v);
-        if (top == -INFINITY) continue;
-        s = s * __builtin_amdgcn_exp2f(m - top) + w * __builtin_amdgcn_exp2f(v - top);
-        m = top;
-    }
-    if (row >= p.rows) return;
-    float lse = 0.f, loss = 0.f;
-    if (n >= 0) {
-        lse = (m + __builtin_amdgcn_logf(s)) * LN2;
-        if (p.q) {
-            float c = 0.f;
-            for (int j = 0; j < p.k; ++j) {
-                const float q = p.q[((long long)row << p.kp) + j];
-                if (q != 0.f) c += q * (lse - p.zt[(long long)row * p.k + j] * p.inv_t);
-            }
-            loss = p.ent[row] + c;
-        } else {
-            loss = lse - p.zt[row];
+#pragma unroll
+    for (int o = SL / 2; o; o >>= 1) {
+        if (sl < o) {
+            join(m, s, ms[tid + o * TB], ss[tid + o * TB]);
+            ms[tid] = m;
+            ss[tid] = s;
         }
+        __syncthreads();
     }
+    const float lse = in ? (ms[t] + __builtin_amdgcn_logf(ss[t])) * LN2 : 0.f;
+    __syncthreads();
+    float c = 0.f;
+    float* z = p.zt + (long long)row * p.k;
+    if (p.q) {
+        for (int j = sl; j < p.k && row < p.rows; j += SL) {
+            const long long e = ((long long)row << p.kp) + j;
+            if (p.ids[e] < 0) z[j] = 0.f;
+            else if (const float q = p.q[e]; q != 0.f) c += q * (lse - z[j] * p.inv_t);
+        }
+    } else if (sl == 0 && row < p.rows) {
+        if (in) c = lse - z[0];
+        else z[0] = 0.f;
+    }
+    if (p.q) {
+        ms[tid] = c;
+        __syncthreads();
+        for (int i = 1; sl == 0 && i < SL && i < p.k; ++i) c += ms[i * TB + t];
+    }
+    if (sl || row >= p.rows) return;
     p.lse[row] = lse;
-    p.loss[row] = loss;
+    p.loss[row] = in ? (p.q ? p.ent[row] + c : c) : 0.f;
 }
 
 struct Fix {
     const int *live, *idx, *ids;
-    const float *q, *lse, *zt, *gs;
+    const float *q, *lse, *zt, *g, *top;
     int k, kp, v0, v1;
     float sc;
     uint16_t* dz;
-    long long ld;
+    long long panel;
 };
 
-// the entries' own dz: p less the entries' q of that id
+// a teacher's entries' own dz: p less the entries' q of that id
 __global__ __launch_bounds__(256) void hl_fix(const Fix p) {
     const int e = blockIdx.x * 256 + threadIdx.x, n = e >> p.kp, w = 1 << p.kp, j = e & (w - 1);
     const bool in = n < *p.live;
     const long long row = in ? p.idx[n] : 0;
     const int id = in ? p.ids[(row << p.kp) + j] : -1;
-    const float q = id < 0 ? 0.f : p.q ? p.q[(row << p.kp) + j] : 1.f;
+    const float q = id < 0 ? 0.f : p.q[(row << p.kp) + j];
     float all = 0.f;
     for (int i = 0; i < w; ++i) {
         const int oid = __shfl(id, i, w);
@@ -505,34 +731,45 @@ __global__ __launch_bounds__(256) void hl_fix(const Fix p) {
         if (oid == id) all += oq;
     }
     if (id < p.v0 || id >= p.v1) return;
+    const float top = *p.top, gr = p.g ? p.g[row] : 1.f, gs = top > 0.f ? gr / top : gr;
     const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(p.zt[row * p.k + j], p.sc, -p.lse[row] * LOG2E));
-    p.dz[n * p.ld + (id - p.v0)] = (uint16_t)cvt2(p.gs[n] * (pr - all), 0.f);
+    const int v = id - p.v0;
+    p.dz[(v >> 8) * p.panel + (long long)n * 256 + (v & 255)] = (uint16_t)cvt2(gs * (pr - all), 0.f);
 }
 
 struct Finish {
     const float* acc;
-    long long stride, ld;
-    int splits, rows, dim;
-    const int* pos;
+    int tm, bm, bn, steps, dim;
+    const int *live, *idx;
     const float* scale;
     uint16_t* dx;
     long long ld_dx;
 };
 
+// dx from the splits' sums (none: it is there): 256 columns of a row at a time, a quarter of the splits a wavefront
 __global__ __launch_bounds__(256) void hl_dx(const Finish p) {
-    const int row = blockIdx.x, n = p.pos[row];
+    __shared__ f32x4 part[4][64];
+    const int live = *p.live, splits = dx_splits(pace(p.bm, p.bn), p.tm * ((live + p.bn - 1) / p.bn), p.steps, p.bm * p.bn * 8);
+    if (splits == 1) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, cols = (p.dim + 255) / 256;
     const float s = *p.scale;
-    for (int d = 4 * threadIdx.x; d < p.dim; d += 1024) {
+    const long long stride = (long long)live * p.dim;
+    for (int w = blockIdx.x; w < live * cols; w += gridDim.x) {
+        const int n = w / cols, d = 256 * (w - n * cols) + 4 * lane;
         f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (n >= 0)
-            for (int i = 0; i < p.splits; ++i) v += *reinterpret_cast<const f32x4*>(p.acc + i * p.stride + n * p.ld + d);
-        *reinterpret_cast<uint2*>(p.dx + row * p.ld_dx + d) = make_uint2(cvt2(v[0] * s, v[1] * s), cvt2(v[2] * s, v[3] * s));
+        if (d < p.dim) {
+            const float* at = p.acc + (long long)n * p.dim + d;
+#pragma unroll 8
+            for (int i = wave; i < splits; i += 4) v += *reinterpret_cast<const f32x4*>(at + i * stride);
+        }
+        part[wave][lane] = v;
+        __syncthreads();
+        if (wave == 0 && d < p.dim) {
+            v = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+            *reinterpret_cast<uint2*>(p.dx + p.idx[n] * p.ld_dx + d) = make_uint2(cvt2(v[0] * s, v[1] * s), cvt2(v[2] * s, v[3] * s));
+        }
+        __syncthreads();
     }
-}
-
-__global__ __launch_bounds__(256) void hl_zero_rows(uint16_t* p, long long ld, int dim) {
-    for (int d = 4 * threadIdx.x; d < dim; d += 1024)
-        *reinterpret_cast<uint2*>(p + blockIdx.x * ld + d) = make_uint2(0u, 0u);
 }
 
 // --- the plan ----------------------------------------------------------------------------------------------------------
@@ -542,15 +779,47 @@ constexpr long long DZ_BYTES = 1ll << 30;  // dz a piece at most
 long long up(long long v, long long to) { return (v + to - 1) / to * to; }
 
 struct Plan {
-    int kp, bn, parts, piece, splits;
-    bool gather;
-    long long ids, q, ent, idx, pos, live, gs, xc, part, dz, acc, bytes;
+    int kp, piece;
+    int z, w, d;  // the tiles of z, dhead and dx
+    int parts;
+    bool gather, raw, own;
+    long long ids, idc, q, ent, held, idx, pos, live, xc, part, dz, acc, bytes;
 };
 
 int log2_up(int k) {
     int p = 0;
     while ((1 << p) < k) ++p;
     return p;
+}
+
+enum Tiles { T256, T128, T256x64, T64 };
+struct Size {
+    int bm, bn, tm;  // (a wavefront's rows)
+};
+constexpr Size SIZE[] = {{256, 256, 128}, {128, 128, 64}, {256, 64, 128}, {64, 64, 32}};
+
+int tiles_of(int t, long long m, long long n) {
+    return (int)(up(m, SIZE[t].bm) / SIZE[t].bm * (up(n, SIZE[t].bn) / SIZE[t].bn));
+}
+
+int choose(long long m, long long n, long long k) {
+    const int steps = (int)(up(k, BK) / BK);
+    return tiled_us(pace(128, 128), tiles_of(T128, m, n), steps) < tiled_us(pace(256, 256), tiles_of(T256, m, n), steps) ? T128 : T256;
+}
+
+// z's: up to 64 columns take tiles as narrow, of 256 rows where there are enough of them for every CU (32 rows x 128256 x
+// 4096: 176 us, 6 TB/s), else of 64, four stages deep (48 x 8192 x 1024: 11 us against 16)
+int choose_z(long long m, long long n, long long k) {
+    if (n <= 64) return tiles_of(T256x64, m, n) >= CUS ? T256x64 : T64;
+    return choose(m, n, k);
+}
+
+int choose_dx(long long n, long long d, int steps) {
+    if (n <= 64) return T256x64;
+    float a, b;
+    dx_splits(pace(256, 256), tiles_of(T256, d, n), steps, 256 * 256 * 8, &a);
+    dx_splits(pace(128, 128), tiles_of(T128, d, n), steps, 128 * 128 * 8, &b);
+    return b < a ? T128 : T256;
 }
 
 bool plan_of(const dr_head_loss* a, int what, Plan& p) {
@@ -563,9 +832,11 @@ bool plan_of(const dr_head_loss* a, int what, Plan& p) {
     const bool back = what & DR_LOSS_BACKWARD;
     const long long n = a->rows, np = up(n, 64);
     p.kp = log2_up(a->k);
-    p.bn = n <= 64 ? 64 : n <= 128 ? 128 : 256;
-    p.parts = (int)(up(a->valid, 256) / 128);
+    p.z = choose_z(a->valid, n, a->dim);
+    p.parts = (int)(up(a->valid, SIZE[p.z].bm) / SIZE[p.z].tm);
     p.gather = back || n > 64;
+    p.raw = !p.gather && a->vals == nullptr;  // (tokens read where they are: no launch before z's)
+    p.own = p.gather && n << p.kp <= FEW;
     long long at = 0;
     auto take = [&](long long bytes) {
         const long long here = at;
@@ -573,45 +844,54 @@ bool plan_of(const dr_head_loss* a, int what, Plan& p) {
         return here;
     };
     p.ids = take(n * 4 << p.kp);
+    p.idc = take(p.gather ? n * 4 << p.kp : 0);
     p.q = take(a->vals ? n * 4 << p.kp : 0);
     p.ent = take(a->vals ? n * 4 : 0);
+    p.held = take(n);
     p.idx = take(n * 4);
     p.pos = take(n * 4);
-    p.live = take(8);
-    p.gs = take(back ? n * 4 : 0);
+    p.live = take(12);
     p.xc = take(p.gather ? n * a->dim * 2 : 0);
     p.part = take(what & DR_LOSS_FORWARD ? p.parts * np * 8 : 0);
-    p.piece = 0, p.splits = 1, p.dz = p.acc = 0;
+    p.piece = 0, p.dz = p.acc = 0;
     if (back) {
         // the vocabulary in equal pieces of a multiple of 256
         const long long tiles = up(a->valid, 256) / 256, fit = DZ_BYTES / (n * 512);
         const long long pieces = (tiles + (fit > 1 ? fit : 1) - 1) / (fit > 1 ? fit : 1);
         p.piece = (int)((tiles + pieces - 1) / pieces) * 256;
         p.dz = take(n * p.piece * 2);
+        p.w = choose(a->dim, p.piece, n);
         if (a->dx) {
-            const long long t = up(n, p.bn) / p.bn * (up(a->dim, 256) / 256), most = p.piece / BK;
-            long long s = (512 + t - 1) / t;
-            if (s > most / 4) s = most / 4 > 0 ? most / 4 : 1;
-            p.splits = (int)s;
-            p.acc = take(s * n * a->dim * 4);
+            p.d = choose_dx(n, a->dim, p.piece / BK);
+            // the sums of all rows where there are several pieces; of splits no more than ROUNDS rounds of tiles
+            const long long whole = p.piece < a->valid ? n * a->dim : 0;
+            const Pace pc = pace(SIZE[p.d].bm, SIZE[p.d].bn);
+            const long long split = (long long)ROUNDS * pc.at_once * SIZE[p.d].bm * SIZE[p.d].bn;
+            p.acc = take((whole > split ? whole : split) * 4);
         }
     }
     p.bytes = at;
     return true;
 }
 
-template <int BM, int BN, int WM, int WN, bool AT, bool BT, int EPI>
+template <int BM, int BN, int WM, int WN, int NS, bool AT, bool BT, int EPI>
 void launch(Gemm g, hipStream_t st) {
     g.tm = (g.m + BM - 1) / BM;
     g.tn = (g.n + BN - 1) / BN;
-    hipLaunchKernelGGL((hl_gemm<BM, BN, WM, WN, AT, BT, EPI>), dim3(g.tm * g.tn * g.splits), dim3(64 * WM * WN), 0, st, g);
+    int grid = g.tm * g.tn;
+    if (EPI == EPI_DX) grid = grid > ROUNDS * pace(BM, BN).at_once ? grid : ROUNDS * pace(BM, BN).at_once;
+    grid = (grid + 7) & ~7;  // (as many for each XCD)
+    hipLaunchKernelGGL((hl_gemm<BM, BN, WM, WN, NS, AT, BT, EPI>), dim3(grid), dim3(64 * WM * WN), 0, st, g);
 }
 
-template <bool AT, int EPI>
-void launch_rows(const Gemm& g, int bn, hipStream_t st) {  // (the columns are rows of x)
-    if (bn == 64) launch<256, 64, 2, 2, AT, false, EPI>(g, st);
-    else if (bn == 128) launch<256, 128, 2, 2, AT, false, EPI>(g, st);
-    else launch<256, 256, 2, 4, AT, false, EPI>(g, st);
+template <int EPI>
+void launch_z(const Gemm& g, int t, hipStream_t st) {
+    switch (t) {
+        case T256: return launch<256, 256, 2, 4, 2, false, false, EPI>(g, st);
+        case T128: return launch<128, 128, 2, 2, 2, false, false, EPI>(g, st);
+        case T256x64: return launch<256, 64, 2, 2, 2, false, false, EPI>(g, st);
+        default: return launch<64, 64, 2, 2, 4, false, false, EPI>(g, st);
+    }
 }
 
 }  // namespace
@@ -628,8 +908,8 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
     const bool fwd = what & DR_LOSS_FORWARD, back = what & DR_LOSS_BACKWARD;
     if (!aligned(a->x, 16) || !aligned(a->head, 16) || !aligned(a->ids, a->ids64 ? 8 : 4) || !aligned(a->lse, 4) ||
         !aligned(a->logits, 4) || (fwd && !aligned(a->loss, 4)) || !aligned(a->workspace, 256) || a->workspace_bytes < P.bytes ||
-        (back && a->dx && (!aligned(a->dx, 8) || a->ld_dx < a->dim || a->ld_dx % 4)) ||
-        (back && a->dhead && (!aligned(a->dhead, 8) || a->ld_dhead < a->dim || a->ld_dhead % 4)))
+        (back && a->dx && (!aligned(a->dx, 16) || a->ld_dx < a->dim || a->ld_dx % 8)) ||
+        (back && a->dhead && (!aligned(a->dhead, 16) || a->ld_dhead < a->dim || a->ld_dhead % 8)))
         return DR_EINVAL;
     if (back && !fwd && !a->dx && !a->dhead) return DR_OK;
     const hipStream_t st = reinterpret_cast<hipStream_t>(a->stream);
@@ -641,19 +921,19 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
     p.ids = reinterpret_cast<int*>(ws + P.ids);
     p.q = a->vals ? reinterpret_cast<float*>(ws + P.q) : nullptr;
     p.ent = reinterpret_cast<float*>(ws + P.ent);
+    p.held = reinterpret_cast<uint8_t*>(ws + P.held);
     p.idx = reinterpret_cast<int*>(ws + P.idx);
     p.pos = reinterpret_cast<int*>(ws + P.pos);
     p.live = reinterpret_cast<int*>(ws + P.live);
-    p.scale = reinterpret_cast<float*>(ws + P.live + 4);
-    p.gs = reinterpret_cast<float*>(ws + P.gs);
+    p.top = reinterpret_cast<float*>(ws + P.live + 4);
     p.xc = reinterpret_cast<uint16_t*>(ws + P.xc);
-    p.fwd = fwd, p.back = back;
+    p.dx = back ? reinterpret_cast<uint16_t*>(a->dx) : nullptr;
+    p.idc = reinterpret_cast<int*>(ws + P.idc);
     const int eblocks = (int)((((long long)n << P.kp) + 255) / 256);
-    hipLaunchKernelGGL(hl_entries, dim3(eblocks), dim3(256), 0, st, p);
-    if (P.gather) {
-        hipLaunchKernelGGL(hl_count, dim3(1), dim3(256), 0, st, p);
-        hipLaunchKernelGGL(hl_gather, dim3(n), dim3(256), 0, st, p);
-    }
+    const dim3 gblocks((n + GROWS - 1) / GROWS + 1);
+    if (!P.raw && !P.own) hipLaunchKernelGGL(hl_entries, dim3(eblocks), dim3(256), 0, st, p);
+    if (P.own) hipLaunchKernelGGL(hl_gather<true>, gblocks, dim3(256), 0, st, p);
+    else if (P.gather) hipLaunchKernelGGL(hl_gather<false>, gblocks, dim3(256), 0, st, p);
 
     Gemm z{};  // z of a range of the vocabulary
     z.A = reinterpret_cast<const uint16_t*>(a->head);
@@ -663,66 +943,78 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
     z.n = n, z.k = z.ka = a->dim;
     z.live = P.gather ? p.live : nullptr;
     z.idx = P.gather ? p.idx : nullptr;
-    z.splits = 1, z.steps = (a->dim + BK - 1) / BK;
+    z.steps = (a->dim + BK - 1) / BK;
     z.sc = LOG2E / a->temperature;
-    z.ids = p.ids, z.kp = P.kp, z.kn = kn;
-    z.lse = a->lse, z.gs = p.gs;
+    z.ids = P.gather ? p.idc : p.ids, z.kp = P.kp, z.kn = kn;
+    z.raw = P.raw ? a->ids : nullptr, z.raw64 = a->ids64;
+    z.lse = a->lse, z.g = a->g, z.top = p.top;
     if (fwd) {
         Gemm s = z;
         s.m = a->valid;
         s.part = reinterpret_cast<f32x2*>(ws + P.part);
         s.ld_part = up(n, 64);
         s.zt = a->logits;
-        launch_rows<false, EPI_STATS>(s, P.bn, st);
-        Merge m{s.part, s.ld_part, P.parts, n, kn, P.kp, P.gather, p.pos, p.q, p.ent, 1.f / a->temperature, a->loss, a->lse, a->logits};
-        if (n <= 256) hipLaunchKernelGGL(hl_merge<1>, dim3(n), dim3(256), 0, st, m);
-        else hipLaunchKernelGGL(hl_merge<32>, dim3((n + 31) / 32), dim3(256), 0, st, m);
+        launch_z<EPI_STATS>(s, P.z, st);
+        Merge m{s.part, s.ld_part, P.parts, n, kn, P.kp, P.gather ? p.pos : nullptr, P.raw ? nullptr : p.held, a->ids,
+                a->ids64, a->valid, p.ids, p.q, p.ent, 1.f / a->temperature, a->loss, a->lse, a->logits};
+        if (n <= 64) hipLaunchKernelGGL((hl_merge<1, 256>), dim3(n), dim3(256), 0, st, m);
+        else hipLaunchKernelGGL((hl_merge<32, 32>), dim3((n + 31) / 32), dim3(1024), 0, st, m);
     }
     if (back && (a->dx || a->dhead)) {
         uint16_t* dz = reinterpret_cast<uint16_t*>(ws + P.dz);
+        const long long panel = (long long)n * 256;
         for (int v0 = 0; v0 < a->valid; v0 += P.piece) {
             const int vn = a->valid - v0 < P.piece ? a->valid - v0 : P.piece, vp = (int)up(vn, 256);
             Gemm s = z;
             s.A += (long long)v0 * a->ld_head;
             s.m = vn;
+            s.v0 = v0;
             s.out = dz;
-            s.ld_out = P.piece;
-            launch_rows<false, EPI_DZ>(s, P.bn, st);
-            Fix f{p.live, p.idx, p.ids, p.q, a->lse, a->logits, p.gs, kn, P.kp, v0, v0 + vn, z.sc, dz, P.piece};
-            hipLaunchKernelGGL(hl_fix, dim3(eblocks), dim3(256), 0, st, f);
+            s.panel = panel;
+            if (a->vals) {
+                launch_z<EPI_DZ>(s, P.z, st);
+                Fix f{p.live, p.idx, p.ids, p.q, a->lse, a->logits, a->g, p.top, kn, P.kp, v0, v0 + vn, z.sc, dz, panel};
+                hipLaunchKernelGGL(hl_fix, dim3(eblocks), dim3(256), 0, st, f);
+            } else {
+                launch_z<EPI_DZ1>(s, P.z, st);
+            }
             if (a->dhead) {
                 Gemm w{};
                 w.A = p.xc, w.lda = a->dim;
-                w.B = dz, w.ldb = P.piece;
-                w.m = a->dim, w.n = vn, w.k = n, w.live = p.live;
-                w.splits = 1, w.steps = (n + BK - 1) / BK;
+                w.B = dz, w.ldb = 256, w.panel = panel;
+                // (the rows past valid: zeros, with the last piece)
+                w.m = a->dim, w.nb = vn, w.n = v0 + vn == a->valid ? a->vocab - v0 : vn, w.k = n, w.live = p.live;
+                w.steps = (n + BK - 1) / BK;
                 w.out = reinterpret_cast<uint16_t*>(a->dhead) + (long long)v0 * a->ld_dhead;
                 w.ld_out = a->ld_dhead;
-                w.scale = p.scale;
-                launch<256, 256, 2, 4, true, true, EPI_DHEAD>(w, st);
+                w.scale = p.top + 1;
+                if (P.w == T256) launch<256, 256, 2, 4, 2, true, true, EPI_DHEAD>(w, st);
+                else launch<128, 128, 2, 2, 2, true, true, EPI_DHEAD>(w, st);
             }
             if (a->dx) {
                 Gemm d{};
                 d.A = z.A + (long long)v0 * a->ld_head, d.lda = a->ld_head;
-                d.B = dz, d.ldb = P.piece;
+                d.B = dz, d.ldb = 256, d.panel = panel;
                 d.m = a->dim, d.n = n, d.k = (int)up(vn, 8), d.ka = vn, d.live = p.live;
-                d.splits = P.splits;
-                d.steps = (int)up((vp / BK + P.splits - 1) / P.splits, 2);  // (steps run in pairs)
+                d.steps = vp / BK, d.plan_steps = P.piece / BK;
                 d.acc = reinterpret_cast<float*>(ws + P.acc);
-                d.acc_stride = (long long)n * a->dim;
-                d.ld_out = a->dim;
+                d.ld_acc = a->dim;
                 d.add = v0 > 0;
-                launch_rows<true, EPI_DX>(d, P.bn, st);
+                d.idx = p.idx;
+                d.scale = p.top + 1;
+                if (v0 + vn == a->valid) d.out = reinterpret_cast<uint16_t*>(a->dx), d.ld_out = a->ld_dx;
+                if (P.d == T256x64) launch<256, 64, 2, 2, 2, true, false, EPI_DX>(d, st);
+                else if (P.d == T128) launch<128, 128, 2, 2, 2, true, false, EPI_DX>(d, st);
+                else launch<256, 256, 2, 4, 2, true, false, EPI_DX>(d, st);
             }
         }
         if (a->dx) {
-            Finish f{reinterpret_cast<const float*>(ws + P.acc), (long long)n * a->dim, a->dim, P.splits, n, a->dim, p.pos, p.scale,
-                     reinterpret_cast<uint16_t*>(a->dx), a->ld_dx};
-            hipLaunchKernelGGL(hl_dx, dim3(n), dim3(256), 0, st, f);
+            const Size t = SIZE[P.d];
+            Finish f{reinterpret_cast<const float*>(ws + P.acc), (int)(up(a->dim, t.bm) / t.bm), t.bm, t.bn, P.piece / BK, a->dim, p.live,
+                     p.idx, p.top + 1, reinterpret_cast<uint16_t*>(a->dx), a->ld_dx};
+            const long long items = (long long)n * ((a->dim + 255) / 256);
+            hipLaunchKernelGGL(hl_dx, dim3((unsigned)(items < 4096 ? items : 4096)), dim3(256), 0, st, f);
         }
-        if (a->dhead && a->vocab > a->valid)
-            hipLaunchKernelGGL(hl_zero_rows, dim3(a->vocab - a->valid), dim3(256), 0, st,
-                               reinterpret_cast<uint16_t*>(a->dhead) + (long long)a->valid * a->ld_dhead, a->ld_dhead, a->dim);
     }
     return hipGetLastError() == hipSuccess ? DR_OK : DR_EHIP;
 }

@@ -37,50 +37,47 @@ from lm_head_topk import head_pick  # noqa: E402
 MAX_K = _lib.DR_LOSS_MAX_K  # teacher entries a row at most
 
 
-def _on(device):
-    """device made the current one (a launch goes to the current device's stream)."""
-    return torch.cuda.device(device)
-
-
 class _Call:
     """One call's inputs, checked, and the launch of it."""
 
     def __init__(self, x, rows_t, ids, vals, temperature, valid):
         dim = x.shape[-1]
-        assert isinstance(x, torch.Tensor) and x.is_cuda and x.dtype == torch.bfloat16, (x.device, x.dtype)
+        device = self.device = x.device
+        assert x.is_cuda and x.dtype == torch.bfloat16, (x.device, x.dtype)
         assert dim % 8 == 0, f"head_loss: dim {dim} is not a multiple of 8"
         head_pick.check_rows(rows_t, dim)
-        assert rows_t.device == x.device, (rows_t.device, x.device)
-        self.vocab = rows_t.shape[-2]
-        self.valid = self.vocab if valid is None else int(valid)
-        assert 1 <= self.valid <= self.vocab, (valid, rows_t.shape)
-        x2 = x.detach().reshape(-1, dim)
-        if x2.stride(-1) != 1 or x2.stride(0) % 8 or x2.stride(0) < dim or x2.data_ptr() % 16:
-            x2 = x2.clone(memory_format=torch.contiguous_format)
-        self.x, self.rows_t, self.dim, self.n = x2, rows_t.detach(), dim, x2.shape[0]
+        self.vocab = vocab = rows_t.shape[-2]
+        self.valid = vocab if valid is None else int(valid)
+        assert 1 <= self.valid <= vocab, (valid, rows_t.shape)
+        if x.dim() != 2:
+            x = x.reshape(-1, dim)
+        if x.stride(-1) != 1 or x.stride(0) % 8 or x.stride(0) < dim or x.data_ptr() % 16:
+            x = x.clone(memory_format=torch.contiguous_format)
+        self.x, self.rows_t, self.dim = x, rows_t, dim
+        n = self.n = x.shape[0]
+        self.vals = None
         if vals is None:
-            assert ids.is_cuda and ids.dtype in (torch.int32, torch.int64), (ids.device, ids.dtype)
-            assert ids.numel() == self.n, f"head_loss: {ids.numel()} targets for {self.n} rows"
-            self.shape, self.k, self.vals = ids.shape, 1, None
+            assert ids.dtype in (torch.int32, torch.int64), ids.dtype
+            assert ids.numel() == n, f"head_loss: {ids.numel()} targets for {n} rows"
+            self.shape, self.k = ids.shape, 1
         else:
-            assert ids.is_cuda and ids.dtype == torch.int32, (ids.device, ids.dtype)
-            assert vals.is_cuda and vals.dtype == torch.float32 and vals.shape == ids.shape and vals.dim() >= 1, (
-                vals.dtype, vals.shape, ids.shape)
-            assert vals.device == x.device, (vals.device, x.device)
+            assert ids.dtype == torch.int32, ids.dtype
+            assert vals.device == device and vals.dtype == torch.float32 and vals.shape == ids.shape and vals.dim() >= 1, (
+                vals.device, vals.dtype, vals.shape, ids.shape)
             self.shape, self.k = ids.shape[:-1], ids.shape[-1]
             assert 1 <= self.k <= MAX_K, f"head_loss: 1 to {MAX_K} teacher entries a row, not {self.k}"
-            assert ids.numel() == self.n * self.k, f"head_loss: teacher entries {tuple(ids.shape)} for {self.n} rows"
-            self.vals = vals.detach().reshape(self.n, self.k).contiguous()
-        assert ids.device == x.device, (ids.device, x.device)
-        self.ids = ids.reshape(self.n, self.k).contiguous()
+            assert ids.numel() == n * self.k, f"head_loss: teacher entries {tuple(ids.shape)} for {n} rows"
+            self.vals = vals.contiguous()
+        assert ids.device == device and rows_t.device == device, (ids.device, rows_t.device, device)
+        self.ids = ids.contiguous()
         self.temperature = float(temperature)
         assert 0 < self.temperature < math.inf, f"head_loss: temperature {temperature}"
 
     def empty(self, *shape, dtype=torch.float32):
-        return torch.empty(*shape, dtype=dtype, device=self.x.device)
+        return torch.empty(shape, dtype=dtype, device=self.device)
 
     def outputs(self):
-        """(loss, lse, logits) to be filled."""
+        """(loss, lse, logits) to be filled, and kept for a backward pass."""
         return self.empty(self.n), self.empty(self.n), self.empty(self.n, self.k)
 
     def grads(self, x_grad, head_grad):
@@ -91,33 +88,44 @@ class _Call:
         """The rows' weights as the launch takes them (None: ones)."""
         if g is None:
             return None
-        g = torch.as_tensor(g, device=self.x.device)
+        if not isinstance(g, torch.Tensor):
+            g = torch.tensor(float(g), device=self.device)
+        assert g.device == self.device, (g.device, self.device)
+        if g.dtype == torch.float32 and g.numel() == self.n and g.is_contiguous():
+            return g
         assert g.numel() in (1, self.n), f"head_loss: {g.numel()} weights for {self.n} rows"
         return g.detach().reshape(-1).to(torch.float32).expand(self.n).contiguous()
 
-    def run(self, what, loss, lse, logits, g=None, dx=None, dhead=None):
-        if self.n == 0:
+    def run(self, what, loss, lse=None, logits=None, g=None, dx=None, dhead=None):
+        """The launch; lse and logits lie in its own memory unless given."""
+        n, k, dim = self.n, self.k, self.dim
+        if n == 0:
             if dhead is not None:
                 dhead.zero_()
             return
-        A = _lib.HeadLoss()
-        A.x, A.ldx, A.rows, A.dim = self.x.data_ptr(), self.x.stride(0) if self.n > 1 else self.dim, self.n, self.dim
-        A.head, A.ld_head, A.vocab, A.valid = self.rows_t.data_ptr(), self.dim, self.vocab, self.valid
-        A.ids, A.ld_ids, A.ids64, A.k = self.ids.data_ptr(), self.k, int(self.ids.dtype == torch.int64), self.k
-        if self.vals is not None:
-            A.vals, A.ld_vals = self.vals.data_ptr(), self.k
-        A.temperature = self.temperature
-        A.loss, A.lse, A.logits = (None if t is None else t.data_ptr() for t in (loss, lse, logits))
-        A.g, A.dx, A.dhead = (None if t is None else t.data_ptr() for t in (g, dx, dhead))
-        A.ld_dx = A.ld_dhead = self.dim
+        ptr = torch.Tensor.data_ptr
+        A = _lib.HeadLoss(
+            self.x.data_ptr(), self.x.stride(0) if n > 1 else dim, self.rows_t.data_ptr(), dim, n, dim, self.vocab,
+            self.valid, self.ids.data_ptr(), k, self.ids.dtype == torch.int64, k, None if self.vals is None else ptr(self.vals), k,
+            self.temperature, *(None if t is None else ptr(t) for t in (loss, lse, logits, g, dx)), dim,
+            None if dhead is None else ptr(dhead), dim)
+        ref = ctypes.byref(A)
         lib = _lib.lib()
-        need = lib.dr_head_loss_workspace_bytes(ctypes.byref(A), what)
+        need = lib.dr_head_loss_workspace_bytes(ref, what)
         _lib.check(_lib.DR_EINVAL if need < 0 else _lib.DR_OK, "dr_head_loss_workspace_bytes")
-        with _on(self.x.device):
-            ws = self.empty(need, dtype=torch.uint8)
-            A.workspace, A.workspace_bytes = ws.data_ptr(), need
-            A.stream = dev.raw_stream(self.x.device)
-            _lib.check(lib.dr_head_loss_run(ctypes.byref(A), what), "dr_head_loss_run")
+        own = 0 if lse is not None else 4 * n * (1 + k)
+        ws = self.empty(need + own, dtype=torch.uint8)
+        A.workspace, A.workspace_bytes = ws.data_ptr(), need
+        if own:
+            A.lse, A.logits = A.workspace + need, A.workspace + need + 4 * n
+        A.stream = dev.raw_stream(self.device)
+        if self.device.index == torch.cuda.current_device():
+            st = lib.dr_head_loss_run(ref, what)
+        else:  # (a launch goes to the current device)
+            with torch.cuda.device(self.device):
+                st = lib.dr_head_loss_run(ref, what)
+        if st != _lib.DR_OK:
+            _lib.check(st, "dr_head_loss_run")
 
 
 class _Loss(torch.autograd.Function):
@@ -145,13 +153,21 @@ class _Loss(torch.autograd.Function):
                 None, None, None, None)
 
 
+def _loss(x, rows_t, ids, vals, temperature, valid):
+    if torch.is_grad_enabled() and (x.requires_grad or rows_t.requires_grad):
+        return _Loss.apply(x, rows_t, ids, vals, temperature, valid)
+    c = _Call(x, rows_t, ids, vals, temperature, valid)
+    loss = c.empty(*c.shape)
+    c.run(_lib.DR_LOSS_FORWARD, loss)
+    return loss
+
+
 def _grads(x, rows_t, ids, vals, temperature, valid, g, x_grad, head_grad):
     c = _Call(x, rows_t, ids, vals, temperature, valid)
-    loss, lse, logits = c.outputs()
+    loss = c.empty(*c.shape)
     dx, dhead = c.grads(x_grad, head_grad)
-    c.run(_lib.DR_LOSS_FORWARD | _lib.DR_LOSS_BACKWARD, loss, lse, logits, c.weights(g), dx, dhead)
-    return (loss.reshape(c.shape), None if dx is None else dx.reshape(x.shape),
-            None if dhead is None else dhead.reshape(rows_t.shape))
+    c.run(_lib.DR_LOSS_FORWARD | _lib.DR_LOSS_BACKWARD, loss, g=c.weights(g), dx=dx, dhead=dhead)
+    return (loss, None if dx is None else dx.reshape(x.shape), None if dhead is None else dhead.reshape(rows_t.shape))
 
 
 def token_loss(x, rows_t, targets, valid=None):
@@ -159,7 +175,7 @@ def token_loss(x, rows_t, targets, valid=None):
     shape, differentiable in x and rows_t (head_rows' table, [vocab, dim] or [1, 1, vocab, dim] bf16). targets: int64 or
     int32, one a row; one outside 0 .. valid - 1 leaves its row out. valid: a padded head's real vocabulary (the rows past
     it enter nothing and get zeros; default all)."""
-    return _Loss.apply(x, rows_t, targets, None, 1.0, valid)
+    return _loss(x, rows_t, targets, None, 1.0, valid)
 
 
 def token_loss_grads(x, rows_t, targets, g=None, valid=None, x_grad=True, head_grad=True):
@@ -175,7 +191,7 @@ def distill_loss(x, rows_t, vals, ids, temperature=1.0, valid=None):
     float32 and ids [..., k] int32, k to 64: as linear.topk_merge leaves them (-inf and -1 in empty slots), of a teacher
     of this vocabulary; an id outside 0 .. valid - 1 is an empty slot too, one that comes twice counts twice, and a row of
     empty slots is left out."""
-    return _Loss.apply(x, rows_t, ids, vals, temperature, valid)
+    return _loss(x, rows_t, ids, vals, temperature, valid)
 
 
 def distill_loss_grads(x, rows_t, vals, ids, g=None, temperature=1.0, valid=None, x_grad=True, head_grad=True):

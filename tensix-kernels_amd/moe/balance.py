@@ -44,7 +44,7 @@ def _run(logits, ids, k, g, kind, ids32, experts, mask, grad):
     assert ids.device == logits.device and ids.is_contiguous(), (ids.device, ids.is_contiguous())
     ld = ids.shape[-1]
     assert ld >= k and ids.numel() == batch * R * ld, (tuple(ids.shape), tuple(logits.shape), k)
-    lg = logits.detach().contiguous()
+    lg = logits.contiguous()
     m = None
     if mask is not None:
         assert mask.device == logits.device and mask.dtype in (torch.bool, torch.uint8), (mask.device, mask.dtype)
@@ -52,9 +52,11 @@ def _run(logits, ids, k, g, kind, ids32, experts, mask, grad):
         m = mask.contiguous()
     gs = None
     if g is not None and grad:
-        gs = torch.as_tensor(g, device=logits.device)
+        gs = g if isinstance(g, torch.Tensor) else torch.tensor(float(g), device=logits.device)
+        assert gs.device == logits.device, (gs.device, logits.device)
         assert gs.numel() in (1, batch), f"balance: {gs.numel()} weights for {batch} batches"
-        gs = gs.detach().reshape(-1).to(torch.float32).expand(batch).contiguous()
+        if gs.dtype != torch.float32 or gs.numel() != batch or not gs.is_contiguous():
+            gs = gs.detach().reshape(-1).to(torch.float32).expand(batch).contiguous()
 
     def new(*shape, dtype=torch.float32):
         return torch.empty(shape, dtype=dtype, device=logits.device)
@@ -64,19 +66,24 @@ def _run(logits, ids, k, g, kind, ids32, experts, mask, grad):
     if batch * R == 0:
         loss.zero_(), counts.zero_()
         return loss, counts, dlogits
-    A = _lib.Balance()
-    A.logits, A.ld_logits, A.batch, A.rows, A.experts, A.width = lg.data_ptr(), W, batch, R, E, W
-    A.ids, A.ld_ids, A.ids32, A.k, A.kind = ids.data_ptr(), ld, int(bool(ids32)), k, KINDS[kind]
-    A.mask, A.g, A.dlogits = (None if t is None else t.data_ptr() for t in (m, gs, dlogits))
-    A.loss, A.counts, A.ld_dlogits = loss.data_ptr(), counts.data_ptr(), W
+    ptr = torch.Tensor.data_ptr
+    A = _lib.Balance(
+        ptr(lg), W, batch, R, E, W, ptr(ids), ld, bool(ids32), k, KINDS[kind], None if m is None else ptr(m), ptr(loss),
+        ptr(counts), None if gs is None else ptr(gs), None if dlogits is None else ptr(dlogits), W)
+    ref = ctypes.byref(A)
     what = _lib.DR_BALANCE_GRAD if grad else _lib.DR_BALANCE_LOSS
     lib = _lib.lib()
-    need = lib.dr_moe_balance_workspace_bytes(ctypes.byref(A), what)
+    need = lib.dr_moe_balance_workspace_bytes(ref, what)
     _lib.check(_lib.DR_EINVAL if need < 0 else _lib.DR_OK, "dr_moe_balance_workspace_bytes")
-    with torch.cuda.device(logits.device):
-        ws = new(need, dtype=torch.uint8)
-        A.workspace, A.workspace_bytes, A.stream = ws.data_ptr(), need, dev.raw_stream(logits.device)
-        _lib.check(lib.dr_moe_balance(ctypes.byref(A), what), "dr_moe_balance")
+    ws = new(need, dtype=torch.uint8)
+    A.workspace, A.workspace_bytes, A.stream = ptr(ws), need, dev.raw_stream(logits.device)
+    if logits.device.index == torch.cuda.current_device():
+        st = lib.dr_moe_balance(ref, what)
+    else:  # (a launch goes to the current device)
+        with torch.cuda.device(logits.device):
+            st = lib.dr_moe_balance(ref, what)
+    if st != _lib.DR_OK:
+        _lib.check(st, "dr_moe_balance")
     return loss, counts, dlogits
 
 
@@ -104,7 +111,9 @@ def balance_loss(logits, ids, k, *, kind="softmax", ids32=False, experts=None, m
     contiguous; the first k of a row), loss float32 and counts int32 [..., E] for each batch of R rows. experts (default W):
     the logits' columns 0 .. E - 1. mask [..., R] bool: the rows that count (default all). The loss is differentiable in the
     logits."""
-    return _Balance.apply(logits, ids, k, kind, ids32, experts, mask)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _Balance.apply(logits, ids, k, kind, ids32, experts, mask)
+    return _run(logits, ids, k, None, kind, ids32, experts, mask, False)[:2]
 
 
 def balance_loss_grads(logits, ids, k, g=None, *, kind="softmax", ids32=False, experts=None, mask=None):

@@ -1,10 +1,12 @@
 // moe_balance.hip: the router's balance loss, each expert's count and the gradient of the logits on MI355X (gfx950), behind
-// dr_moe_balance (include/moe.h). A wavefront holds a row's experts (lane l: l, l + 64, ..), so a row's softmax or sigmoids
-// and their sum are a few register operations and one butterfly, and the sums over rows stay in registers until the
-// wavefront's rows are done.
+// dr_moe_balance (include/moe.h).
+//
+// A row lies over L lanes (16 up to 256 experts, a wavefront beyond), each with runs of four experts, so that a load takes 16
+// bytes a lane, a wavefront works on four rows at once, and a row's softmax or sigmoids and their sum are a few register
+// operations and a butterfly of log2(L) steps. The sums over rows stay in registers until the wavefront's rows are done.
 //   balance_sum_k   a workgroup's rows: the sum of p and the counts (LDS), written for the workgroup
-//   balance_join_k  a batch's workgroups' sums in order: counts, f, loss
-//   balance_grad_k  the logits' gradient, p computed again
+//   balance_grad_k  every workgroup joins the workgroups' sums for itself, in order (cheaper than a launch of its own in
+//                   between), then the logits' gradient of its rows, p computed again; balance_join_k: the join alone
 // What bounds it: the logits read twice and the gradient written once; at a few rows the launches.
 
 #include <hip/hip_runtime.h>
@@ -16,207 +18,295 @@
 
 namespace {
 
-constexpr int W = 4;         // wavefronts a workgroup
-constexpr int MAXE = 1024;   // experts
+constexpr int T = 512;      // lanes a workgroup
+constexpr int W = T / 64;
+constexpr int MAXE = 1024;  // experts
 
 struct Bal {
     dr_balance a;
-    float* psum;   // [batch][groups][E]
-    int* csum;     // [batch][groups][E]
-    int* rsum;     // [batch][groups] rows that count
-    float* f;      // [batch][E]: E count / counts
-    float* per;    // [batch]: 1 / rows that count
+    float2* sums;  // [batch][groups][E] sum of p, count (its bits)
+    int* live;     // [batch][groups] rows that count
     int groups;    // workgroups a batch
+    int vec;       // the logits' rows can be read 16 bytes at a time
+    int gvec;      // and dlogits' written so
 };
 
-__device__ __forceinline__ float wave_sum(float v) {
+template <int L>
+__device__ __forceinline__ float sum_over(float v) {
 #pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    for (int o = L / 2; o; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
-__device__ __forceinline__ float wave_max(float v) {
+template <int L>
+__device__ __forceinline__ float max_over(float v) {
 #pragma unroll
-    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    for (int o = L / 2; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
     return v;
 }
 
-// p of a row, lane's experts l + 64 i (0 past the experts); s (sigmoid): the sigmoids. A row of no expert above -inf has
-// p 0 (softmax).
-template <int N>
-__device__ __forceinline__ void row_p(const dr_balance& a, const float* z, int lane, float (&p)[N], float (&s)[N]) {
-    if (a.kind == 0) {
-        float top = -INFINITY;
+// a row's logits: value 4 i + c is expert 4 (l + L i) + c; past the experts -inf
+template <int L, int N>
+__device__ __forceinline__ void row_load(const Bal& b, long long row, int l, float (&z)[4 * N]) {
+    const float* at = b.a.logits + row * b.a.ld_logits;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int e = lane + 64 * i;
-            p[i] = e < a.experts ? z[e] : -INFINITY;
-            top = fmaxf(top, p[i]);
+    for (int i = 0; i < N; ++i) {
+        const int e = 4 * (l + L * i);
+        if (b.vec && e + 4 <= b.a.experts) {
+            const float4 v = *reinterpret_cast<const float4*>(at + e);
+            z[4 * i] = v.x, z[4 * i + 1] = v.y, z[4 * i + 2] = v.z, z[4 * i + 3] = v.w;
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) z[4 * i + c] = e + c < b.a.experts ? at[e + c] : -INFINITY;
         }
-        top = wave_max(top);
-        const float base = top == -INFINITY ? 0.f : top;
-        float total = 0.f;
+    }
+}
+
+// the row's p from its logits, in place (0 past the experts); a row of no expert above -inf has p 0
+template <int L, int N, bool SIG>
+__device__ __forceinline__ void row_p(float (&p)[4 * N], float (&s)[SIG ? 4 * N : 1]) {
+    float total = 0.f;
+    if constexpr (SIG) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
+        for (int i = 0; i < 4 * N; ++i) {
+            s[i] = 1.f / (1.f + expf(-p[i]));
+            total += s[i];
+        }
+    } else {
+        float top = p[0];
+#pragma unroll
+        for (int i = 1; i < 4 * N; ++i) top = fmaxf(top, p[i]);
+        top = max_over<L>(top);
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int i = 0; i < 4 * N; ++i) {
             p[i] = expf(p[i] - base);
             total += p[i];
         }
-        total = wave_sum(total);
-        const float inv = total == 0.f ? 0.f : 1.f / total;
-#pragma unroll
-        for (int i = 0; i < N; ++i) p[i] *= inv, s[i] = 0.f;
-    } else {
-        float total = 0.f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int e = lane + 64 * i;
-            s[i] = e < a.experts ? 1.f / (1.f + expf(-z[e])) : 0.f;
-            total += s[i];
-        }
-        total = wave_sum(total);
-        const float inv = total == 0.f ? 0.f : 1.f / total;
-#pragma unroll
-        for (int i = 0; i < N; ++i) p[i] = s[i] * inv;
     }
+    total = sum_over<L>(total);
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+    for (int i = 0; i < 4 * N; ++i) p[i] = (SIG ? s[i] : p[i]) * inv;
 }
 
-__device__ __forceinline__ bool counts(const dr_balance& a, long long row) { return a.mask == nullptr || a.mask[row] != 0; }
+__device__ __forceinline__ bool row_counts(const dr_balance& a, long long row) { return a.mask == nullptr || a.mask[row] != 0; }
 
-template <int N>
-__global__ __launch_bounds__(64 * W) void balance_sum_k(const Bal b) {
-    __shared__ int cnt[MAXE];
-    __shared__ float ps[W][64 * N];
+template <int L, int N, bool SIG>
+__global__ __launch_bounds__(T) void balance_sum_k(const Bal b) {
+    constexpr int R = T / L;  // rows at once
+    __shared__ int cnt[L * 4 * N];
+    __shared__ float ps[W][L * 4 * N];
     __shared__ int rows[W];
     const dr_balance& a = b.a;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l = tid % L;
     const int g = blockIdx.x % b.groups, batch = blockIdx.x / b.groups;
-    for (int e = tid; e < a.experts; e += 64 * W) cnt[e] = 0;
+    for (int e = tid; e < a.experts; e += T) cnt[e] = 0;
     __syncthreads();
-    float sum[N];
+    float sum[4 * N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) sum[i] = 0.f;
+    for (int i = 0; i < 4 * N; ++i) sum[i] = 0.f;
     int n = 0;
-    for (int r = g * W + wave; r < a.rows; r += b.groups * W) {
+    for (int r0 = g * R; r0 < a.rows; r0 += b.groups * R) {
+        const int r = min(r0 + tid / L, a.rows - 1);  // (the last row again: every lane takes part in the butterflies)
         const long long row = (long long)batch * a.rows + r;
-        if (!counts(a, row)) continue;
-        ++n;
-        float p[N], s[N];
-        row_p<N>(a, a.logits + row * a.ld_logits, lane, p, s);
-#pragma unroll
-        for (int i = 0; i < N; ++i) sum[i] += p[i];
-        if (lane < a.k) {
-            const long long at = row * a.ld_ids + lane;
-            const uint32_t id = a.ids32 ? reinterpret_cast<const uint32_t*>(a.ids)[at] : reinterpret_cast<const uint16_t*>(a.ids)[at];
-            if (id < (uint32_t)a.experts) atomicAdd(&cnt[id], 1);
+        float p[4 * N], s[SIG ? 4 * N : 1];
+        row_load<L, N>(b, row, l, p);
+        uint32_t id = 0xFFFFFFFFu;
+        if (l < a.k) {
+            const long long at = row * a.ld_ids + l;
+            id = a.ids32 ? reinterpret_cast<const uint32_t*>(a.ids)[at] : reinterpret_cast<const uint16_t*>(a.ids)[at];
         }
+        const bool on = r0 + tid / L < a.rows && row_counts(a, row);
+        row_p<L, N, SIG>(p, s);
+#pragma unroll
+        for (int i = 0; i < 4 * N; ++i) sum[i] += on ? p[i] : 0.f;
+        n += on;
+        if (on && id < (uint32_t)a.experts) atomicAdd(&cnt[id], 1);
+    }
+    // the wavefront's rows, then the workgroup's, in order
+#pragma unroll
+    for (int i = 0; i < 4 * N; ++i) {
+#pragma unroll
+        for (int o = L; o < 64; o <<= 1) sum[i] += __shfl_xor(sum[i], o);
     }
 #pragma unroll
-    for (int i = 0; i < N; ++i) ps[wave][lane + 64 * i] = sum[i];
+    for (int o = L; o < 64; o <<= 1) n += __shfl_xor(n, o);
+    if (lane < L) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            *reinterpret_cast<float4*>(&ps[wave][4 * (l + L * i)]) =
+                make_float4(sum[4 * i], sum[4 * i + 1], sum[4 * i + 2], sum[4 * i + 3]);
+    }
     if (lane == 0) rows[wave] = n;
     __syncthreads();
-    const long long at = (long long)blockIdx.x * a.experts;
-    for (int e = tid; e < a.experts; e += 64 * W) {
+    for (int e = tid; e < a.experts; e += T) {
         float v = 0.f;
 #pragma unroll
         for (int w = 0; w < W; ++w) v += ps[w][e];
-        b.psum[at + e] = v;
-        b.csum[at + e] = cnt[e];
+        b.sums[(long long)blockIdx.x * a.experts + e] = make_float2(v, __int_as_float(cnt[e]));
     }
     if (tid == 0) {
         int v = 0;
         for (int w = 0; w < W; ++w) v += rows[w];
-        b.rsum[blockIdx.x] = v;
+        b.live[blockIdx.x] = v;
     }
 }
 
-__global__ __launch_bounds__(1024) void balance_join_k(const Bal b) {
-    __shared__ float red[16];
-    __shared__ int tot[16], live[16];
+struct Joined {
+    float p[MAXE], f[MAXE];  // the sums of p; counts, then E count / counts
+    float2 part[T];          // experts by slices of the workgroups
+    float red[W];
+    int tot[W], live[W];
+};
+
+// A batch's sums over its workgroups: f in LDS; 1 / rows that count is returned. write: the counts and the loss too.
+__device__ __forceinline__ float join(const Bal& b, int batch, bool write, Joined& J) {
     const dr_balance& a = b.a;
-    const int e = threadIdx.x, lane = e & 63, wave = e >> 6, waves = blockDim.x >> 6;
-    const long long at = (long long)blockIdx.x * b.groups;
-    float p = 0.f;
-    int c = 0, r = 0;
-    if (e < a.experts)
-        for (int g = 0; g < b.groups; ++g) {
-            p += b.psum[(at + g) * a.experts + e];
-            c += b.csum[(at + g) * a.experts + e];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const long long at = (long long)batch * b.groups;
+    int pw = 32;  // experts at a time, by T / pw slices of the workgroups
+    while (pw < a.experts && pw < T) pw *= 2;
+    const int e0 = tid & (pw - 1), sl = tid / pw, slices = T / pw;
+    for (int e = e0; e - e0 < a.experts; e += pw) {
+        float p = 0.f;
+        int c = 0;
+        if (e < a.experts) {
+#pragma unroll 8
+            for (int g = sl; g < b.groups; g += slices) {
+                const float2 v = b.sums[(at + g) * a.experts + e];
+                p += v.x;
+                c += __float_as_int(v.y);
+            }
         }
-    for (int g = e; g < b.groups; g += blockDim.x) r += b.rsum[at + g];
-    int cs = c, rs = r;
+        J.part[tid] = make_float2(p, __int_as_float(c));
+        __syncthreads();
+        if (sl == 0 && e < a.experts) {
+            for (int i = 1; i < slices; ++i) {
+                const float2 v = J.part[i * pw + e0];
+                p += v.x;
+                c += __float_as_int(v.y);
+            }
+            J.p[e] = p;
+            J.f[e] = __int_as_float(c);
+        }
+        __syncthreads();
+    }
+    int rows = 0, total = 0;
+    for (int g = tid; g < b.groups; g += T) rows += b.live[at + g];
+    for (int e = tid; e < a.experts; e += T) {
+        const int c = __float_as_int(J.f[e]);
+        total += c;
+        if (write) a.counts[(long long)batch * a.experts + e] = c;
+    }
 #pragma unroll
-    for (int o = 32; o; o >>= 1) cs += __shfl_xor(cs, o), rs += __shfl_xor(rs, o);
-    if (lane == 0) tot[wave] = cs, live[wave] = rs;
+    for (int o = 32; o; o >>= 1) rows += __shfl_xor(rows, o), total += __shfl_xor(total, o);
+    if (lane == 0) J.live[wave] = rows, J.tot[wave] = total;
     __syncthreads();
-    int total = 0, rows = 0;
-    for (int w = 0; w < waves; ++w) total += tot[w], rows += live[w];
-    const float f = total ? (float)a.experts * ((float)c / (float)total) : 0.f, per = rows ? 1.f / (float)rows : 0.f;
-    const float l = wave_sum(f * (p * per));
-    if (lane == 0) red[wave] = l;
+    rows = total = 0;
+    for (int w = 0; w < W; ++w) rows += J.live[w], total += J.tot[w];
+    const float per = rows ? 1.f / (float)rows : 0.f;
+    float loss = 0.f;
+    for (int e = tid; e < a.experts; e += T) {
+        const float f = total ? (float)a.experts * ((float)__float_as_int(J.f[e]) / (float)total) : 0.f;
+        J.f[e] = f;
+        loss += f * (J.p[e] * per);
+    }
+    if (write) {
+        loss = sum_over<64>(loss);
+        if (lane == 0) J.red[wave] = loss;
+    }
     __syncthreads();
-    if (e < a.experts) {
-        a.counts[(long long)blockIdx.x * a.experts + e] = c;
-        b.f[(long long)blockIdx.x * a.experts + e] = f;
+    if (write && tid == 0) {
+        for (int w = 1; w < W; ++w) loss += J.red[w];
+        a.loss[batch] = loss;
     }
-    if (e == 0) {
-        float loss = 0.f;
-        for (int w = 0; w < waves; ++w) loss += red[w];
-        a.loss[blockIdx.x] = loss;
-        b.per[blockIdx.x] = per;
-    }
+    return per;
 }
 
-template <int N>
-__global__ __launch_bounds__(64 * W) void balance_grad_k(const Bal b) {
+__global__ __launch_bounds__(T) void balance_join_k(const Bal b) {
+    __shared__ Joined J;
+    join(b, blockIdx.x, true, J);
+}
+
+template <int L, int N, bool SIG>
+__global__ __launch_bounds__(T) void balance_grad_k(const Bal b) {
+    constexpr int R = T / L;
+    __shared__ Joined J;
     const dr_balance& a = b.a;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int tid = threadIdx.x, l = tid % L;
     const int g = blockIdx.x % b.groups, batch = blockIdx.x / b.groups;
-    float f[N];
+    const float per = join(b, batch, g == 0, J);
+    const float scale = (a.g ? a.g[batch] : 1.f) * per;
+    float f[4 * N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = lane + 64 * i < a.experts ? b.f[(long long)batch * a.experts + lane + 64 * i] : 0.f;
-    const float scale = (a.g ? a.g[batch] : 1.f) * b.per[batch];
-    for (int r = g * W + wave; r < a.rows; r += b.groups * W) {
+    for (int i = 0; i < 4 * N; ++i) {
+        const int e = 4 * (l + L * (i / 4)) + i % 4;
+        f[i] = e < a.experts ? J.f[e] : 0.f;
+    }
+    for (int r0 = g * R; r0 < a.rows; r0 += b.groups * R) {
+        const int r = min(r0 + tid / L, a.rows - 1);
         const long long row = (long long)batch * a.rows + r;
+        const bool on = row_counts(a, row);
+        float p[4 * N], s[SIG ? 4 * N : 1];
+        row_load<L, N>(b, row, l, p);
+        row_p<L, N, SIG>(p, s);
+        float mean = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4 * N; ++i) mean += p[i] * f[i];
+        mean = sum_over<L>(mean);
+        if (r0 + tid / L >= a.rows) continue;
         float* d = a.dlogits + row * a.ld_dlogits;
-        float p[N], s[N], o[N];
-        if (counts(a, row)) {
-            row_p<N>(a, a.logits + row * a.ld_logits, lane, p, s);
-            float mean = 0.f;
 #pragma unroll
-            for (int i = 0; i < N; ++i) mean += p[i] * f[i];
-            mean = wave_sum(mean);
+        for (int i = 0; i < N; ++i) {
+            const int e = 4 * (l + L * i);
+            float o[4];
 #pragma unroll
-            for (int i = 0; i < N; ++i) o[i] = scale * (a.kind ? p[i] * (1.f - s[i]) : p[i]) * (f[i] - mean);
-        } else {
+            for (int c = 0; c < 4; ++c) {
+                const int q = 4 * i + c;
+                o[c] = on ? scale * (SIG ? p[q] * (1.f - s[SIG ? q : 0]) : p[q]) * (f[q] - mean) : 0.f;
+            }
+            if (b.gvec && e + 4 <= a.experts) {
+                *reinterpret_cast<float4*>(d + e) = make_float4(o[0], o[1], o[2], o[3]);
+            } else {
 #pragma unroll
-            for (int i = 0; i < N; ++i) o[i] = 0.f;
+                for (int c = 0; c < 4; ++c)
+                    if (e + c < a.experts) d[e + c] = o[c];
+            }
         }
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (lane + 64 * i < a.experts) d[lane + 64 * i] = o[i];
-        for (int e = a.experts + lane; e < a.width; e += 64) d[e] = 0.f;
+        for (int e = a.experts + l; e < a.width; e += L) d[e] = 0.f;
     }
 }
 
-// workgroups a batch: every CU a few, no more than its rows fill
+// Workgroups a batch: as many as its rows fill, but no more than all the CUs take in one round, and at most 128, since every
+// workgroup of the gradient reads all of their sums (20011 rows x 128 experts: 128 workgroups 5 rows a quarter wavefront).
 int groups_of(const dr_balance* a) {
-    const int fit = (a->rows + W - 1) / W, most = (1024 + a->batch - 1) / a->batch;
+    const int at_once = a->experts <= 256 ? T / 16 : T / 64;
+    int most = 256 / a->batch;
+    most = most < 1 ? 1 : most > 128 ? 128 : most;
+    const int fit = (a->rows + at_once - 1) / at_once;
     return fit < most ? fit : most;
 }
 
 bool valid(const dr_balance* a, int what) {
     return a != nullptr && what >= 1 && what <= 3 && a->batch >= 1 && a->batch <= (1 << 16) && a->rows >= 1 &&
-           (long long)a->batch * a->rows < (1ll << 31) && a->experts >= 1 && a->experts <= MAXE && a->k >= 1 && a->k <= 16 &&
+           (long long)a->batch * a->rows < (1ll << 30) && a->experts >= 1 && a->experts <= MAXE && a->k >= 1 && a->k <= 16 &&
            a->width >= a->experts && a->ld_logits >= a->width && a->ld_ids >= a->k && (a->kind == 0 || a->kind == 1);
 }
 
 long long up256(long long v) { return (v + 255) & ~255ll; }
 
-template <int N>
+template <int L, int N, bool SIG>
 void run(const Bal& b, int what, hipStream_t st) {
     const dim3 grid(b.groups * b.a.batch);
-    hipLaunchKernelGGL(balance_sum_k<N>, grid, dim3(64 * W), 0, st, b);
-    hipLaunchKernelGGL(balance_join_k, dim3(b.a.batch), dim3((b.a.experts + 63) & ~63), 0, st, b);
-    if (what & DR_BALANCE_GRAD) hipLaunchKernelGGL(balance_grad_k<N>, grid, dim3(64 * W), 0, st, b);
+    hipLaunchKernelGGL((balance_sum_k<L, N, SIG>), grid, dim3(T), 0, st, b);
+    if (what & DR_BALANCE_GRAD) hipLaunchKernelGGL((balance_grad_k<L, N, SIG>), grid, dim3(T), 0, st, b);
+    else hipLaunchKernelGGL(balance_join_k, dim3(b.a.batch), dim3(T), 0, st, b);
+}
+
+template <int L, int N>
+void run_kind(const Bal& b, int what, hipStream_t st) {
+    if (b.a.kind) run<L, N, true>(b, what, st);
+    else run<L, N, false>(b, what, st);
 }
 
 }  // namespace
@@ -224,7 +314,7 @@ void run(const Bal& b, int what, hipStream_t st) {
 extern "C" int64_t dr_moe_balance_workspace_bytes(const dr_balance* a, int what) {
     if (!valid(a, what)) return -1;
     const long long w = (long long)a->batch * groups_of(a);
-    return 2 * up256(w * a->experts * 4) + up256(w * 4) + up256((long long)a->batch * a->experts * 4) + up256((long long)a->batch * 4);
+    return up256(w * a->experts * 8) + up256(w * 4);
 }
 
 extern "C" int dr_moe_balance(const dr_balance* a, int what) {
@@ -237,23 +327,17 @@ extern "C" int dr_moe_balance(const dr_balance* a, int what) {
     Bal b{};
     b.a = *a;
     b.groups = groups_of(a);
+    b.vec = aligned(a->logits, 16) && a->ld_logits % 4 == 0;
+    b.gvec = (what & DR_BALANCE_GRAD) && aligned(a->dlogits, 16) && a->ld_dlogits % 4 == 0;
     char* ws = reinterpret_cast<char*>(a->workspace);
     const long long w = (long long)a->batch * b.groups;
-    b.psum = reinterpret_cast<float*>(ws);
-    ws += up256(w * a->experts * 4);
-    b.csum = reinterpret_cast<int*>(ws);
-    ws += up256(w * a->experts * 4);
-    b.rsum = reinterpret_cast<int*>(ws);
-    ws += up256(w * 4);
-    b.f = reinterpret_cast<float*>(ws);
-    ws += up256((long long)a->batch * a->experts * 4);
-    b.per = reinterpret_cast<float*>(ws);
+    b.sums = reinterpret_cast<float2*>(ws);
+    b.live = reinterpret_cast<int*>(ws + up256(w * a->experts * 8));
     const hipStream_t st = reinterpret_cast<hipStream_t>(a->stream);
-    const int n = (a->experts + 63) / 64;
-    if (n <= 1) run<1>(b, what, st);
-    else if (n <= 2) run<2>(b, what, st);
-    else if (n <= 4) run<4>(b, what, st);
-    else if (n <= 8) run<8>(b, what, st);
-    else run<16>(b, what, st);
+    if (a->experts <= 64) run_kind<16, 1>(b, what, st);
+    else if (a->experts <= 128) run_kind<16, 2>(b, what, st);
+    else if (a->experts <= 256) run_kind<16, 4>(b, what, st);
+    else if (a->experts <= 512) run_kind<64, 2>(b, what, st);
+    else run_kind<64, 4>(b, what, st);
     return hipGetLastError() == hipSuccess ? DR_OK : DR_EHIP;
 }

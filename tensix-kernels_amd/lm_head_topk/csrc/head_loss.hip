@@ -29,7 +29,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void* lds_ptr;
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 
-constexpr int BK = 64;                     // k a step
+constexpr int KSTEP = 64;                  // k that plans count in
 constexpr uint32_t PAST = 0x80000000u;     // a buffer offset past every record: the load gives zeros
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
@@ -51,8 +51,6 @@ __device__ __forceinline__ void step_barrier() {
 }
 
 // --- the tiled product ------------------------------------------------------------------------------------------------
-
-enum Epi { EPI_STATS, EPI_DZ, EPI_DZ1, EPI_DHEAD, EPI_DX };  // (DZ1: tokens, their own logit's 1 taken off there)
 
 struct Gemm {
     const uint16_t *A, *B;  // D[m][n] = sum over k of A[m][k] B[n][k]; an operand lies [rows][k] or (across) [k][rows]
@@ -89,48 +87,49 @@ struct Gemm {
 
 // One operand's tile of ROWS x BK values in LDS: 16-byte chunks, laid out so that neither the loads straight from memory
 // (64 chunks in a row a wavefront) nor the fragments' reads meet in a bank.
-template <int ROWS, bool T, int NT>
+template <int ROWS, bool T, int NT, int BK>
 struct Tile {
-    static constexpr int N = ROWS * 8 / NT;  // chunks a lane loads
+    static constexpr int N = ROWS * BK / 8 / NT;  // chunks a lane loads
+    static constexpr int CK = BK / 8;             // chunks of a row's k
     uint32_t off[N];
 
-    // row r's chunk c (8 k) at 8 r + (c ^ (r / 2 % 8)); across: k's chunk c (8 rows), in pairs (32 bytes) shifted by k
+    // row r's chunk c (8 k) turned by row, so that 16 rows' fill all banks; across: k's chunk c (8 rows), in pairs (32 bytes)
+    // turned by k
+    static __device__ __forceinline__ int swz(int r) { return BK == 64 ? (r >> 1) & 7 : (r >> 2) & 3; }
     static __device__ __forceinline__ int turn(int k) { return ROWS >= 128 ? 2 * (k & 3) : ROWS == 64 ? 2 * ((k >> 1) & 1) : 0; }
 
-    __device__ __forceinline__ void init(int tid, long long ld, int left) {
+    __device__ __forceinline__ void init(int tid, int ld, int rows) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int s = i * NT + tid;
             if constexpr (T) {
                 constexpr int C = ROWS / 8;
                 const int k = s / C, c = s % C, src = ((((c >> 1) ^ turn(k))) << 1) | (c & 1);
-                off[i] = 8 * src < left ? (uint32_t)(k * (uint32_t)ld * 2u) + 16u * src : PAST;
+                off[i] = 8 * src < rows ? (uint32_t)(k * ld * 2) + 16u * src : PAST;
             } else {
-                const int r = s >> 3, c = (s & 7) ^ ((r >> 1) & 7);
-                off[i] = (uint32_t)(r * (uint32_t)ld * 2u) + 16u * c;
+                const int r = s / CK, c = (s % CK) ^ swz(r);
+                off[i] = (uint32_t)(r * ld * 2) + 16u * c;
             }
         }
     }
-    // base: the tile's first value of this step; rows: its rows (across: the step's k) in memory; left: its k (across:
-    // its rows) in memory
-    __device__ __forceinline__ void load(const uint16_t* base, long long ld, int rows, int left, uint4* lds, int tid) const {
-        // (no further than the tile's own run of its last row: what comes after may be rows that are not to be read)
-        const int run = min((left + 7) & ~7, T ? ROWS : BK);
-        const long long bytes = rows > 0 && left > 0 ? ((long long)(rows - 1) * ld + run) * 2 : 0;
-        const __amdgpu_buffer_rsrc_t r =
-            __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, (int)(bytes < 0x7FFFFFFF ? bytes : 0x7FFFFFFF), 0x00020000);
-        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            uint32_t o = off[i];
-            if constexpr (!T) {
-                if (left < BK) {  // (the last step of a ragged k)
-                    const int s = i * NT + tid, rr = s >> 3, c = (s & 7) ^ ((rr >> 1) & 7);
-                    if (8 * c >= left) o = PAST;
-                }
+    // The step's loads: at: its first value; ld; rows: the operand's rows in the tile (at least 1); left: its k from this step
+    // on (none left: zeros). Never further than the tile's own run of its last row: what comes after may be rows that are not
+    // to be read.
+    static __device__ __forceinline__ __amdgpu_buffer_rsrc_t source(const uint16_t* at, int ld, int rows, int left) {
+        const int r = T ? min(left, BK) : rows, run = min(T ? (rows + 7) & ~7 : (left + 7) & ~7, T ? ROWS : BK);
+        return __builtin_amdgcn_make_buffer_rsrc((void*)at, (short)0, left > 0 ? ((r - 1) * ld + run) * 2 : 0, 0x00020000);
+    }
+    // the lane's chunk i of it to LDS
+    __device__ __forceinline__ void load(int i, __amdgpu_buffer_rsrc_t from, int left, uint4* lds, int tid) const {
+        uint32_t o = off[i];
+        if constexpr (!T) {
+            if (left < BK) {  // (the last step of a ragged k)
+                const int s = i * NT + tid, c = (s % CK) ^ swz(s / CK);
+                if (8 * c >= left) o = PAST;
             }
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(lds + i * NT + 64 * wave), 16, o, 0, 0, 0);
         }
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_ptr)(lds + i * NT + 64 * __builtin_amdgcn_readfirstlane(tid >> 6)), 16, o,
+                                                 0, 0, 0);
     }
     // lane's 8 values of row r0 + lane % 32, k = 16 u + 8 (lane / 32) .., the tile from chunk `from` of the stage on. (One
     // index from the stage's array: through longer chains the compiler no longer sees which stage a read is of, and has it
@@ -147,14 +146,15 @@ struct Tile {
             return make_uint4(lo.x, lo.y, hi.x, hi.y);
         } else {
             const int r = lane & 31, h = lane >> 5;
-            return lds[from + (r0 + r) * 8 + ((2 * u + h) ^ ((r >> 1) & 7))];
+            return lds[from + (r0 + r) * CK + ((2 * u + h) ^ swz(r))];
         }
     }
 };
 
-// Tiles and the time (us) that a workgroup takes for a step and for its beginning and end, as many workgroups running at once
-// as fit the CUs: a step of 256 x 256 took 1.88 us, one of 128 x 128, two a CU, 1.0 to 1.1 (8192 x 4096 x 16384: 1240
-// against 1030 TFLOP/s of dx).
+// What a workgroup of each tile takes (us): a step, and its beginning and end, as many workgroups at once as fit the CUs (one
+// of 256 x 256, two of the others). From dx at 8192 x 4096 x 16384 (rows x dim x vocabulary): 1240 TFLOP/s in the larger
+// tiles, 1030 in the smaller, which are for what would leave CUs idle.
+enum Epi { EPI_STATS, EPI_DZ, EPI_DZ1, EPI_DHEAD, EPI_DX };  // (DZ1: tokens, their own logit's 1 taken off there)
 struct Pace {
     int at_once;
     float step, ends;
@@ -201,14 +201,18 @@ __device__ __forceinline__ bool tile_of(int tm, int tn, int splits, int& mt, int
     return true;
 }
 
-template <int BM, int BN, int WM, int WN, int NS, bool AT, bool BT, int EPI>
-__global__ __launch_bounds__(64 * WM * WN) void hl_gemm(const Gemm a) {
+template <int BM, int BN, int WM, int WN, int WK, int NS, int BK, bool AT, bool BT, int EPI>
+__global__ __launch_bounds__(64 * WM * WN * WK) void hl_gemm(const Gemm a) {
     constexpr int NW = WM * WN, NT = 64 * NW, TM = BM / WM, TN = BN / WN, MI = TM / 32, NI = TN / 32;
-    constexpr int CH = (BM + BN) * 8;  // chunks a stage
+    constexpr int CA = BM * BK / 8, CH = CA + BN * BK / 8;  // chunks of A, a stage
     constexpr int NL = CH / NT;        // loads a lane and stage
-    static_assert(NS == 2 || NS == 4, "two or four stages");
-    __shared__ uint4 s0[CH], s1[CH], s2[NS > 2 ? CH : 1], s3[NS > 2 ? CH : 1];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    static_assert(NS == 1 || NS == 2 || NS == 4 || NS == 8, "one stage, two, four or eight");
+    constexpr int CM = NS > 1 ? CH : 1, CL = NS > 2 ? CH : 1, CX = NS > 4 ? CH : 1;
+    // (an array each, named where it is used: a read waits for the loads to every array that the compiler cannot rule out)
+    __shared__ uint4 s0[CH * WK], s1[CM * WK], s2[CL * WK], s3[CL * WK], s4[CX], s5[CX], s6[CX], s7[CX];
+    // WK groups of wavefronts, each a share of K in stages of its own, all with the same barriers; tid within the group
+    const int group = WK == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / NT), tid = threadIdx.x - group * NT;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), mine = group * CH;
     const int wm = wave / WN, wn = wave % WN;
     const int live = a.live ? *a.live : (EPI == EPI_DHEAD ? a.k : a.n);
     // (dx: the tiles of the rows that count, split as many ways as fill the CUs)
@@ -223,82 +227,148 @@ __global__ __launch_bounds__(64 * WM * WN) void hl_gemm(const Gemm a) {
     // (a split's steps are whole rounds of the stages: the next split's are not its own)
     const int all = (k_end + BK - 1) / BK, per = ((all + splits - 1) / splits + NS - 1) / NS * NS, step0 = split * per;
     const int steps = EPI == EPI_DHEAD && n0 >= nb ? 0 : min(per, all - step0);
+    const int rounds = ((steps + WK - 1) / WK + NS - 1) / NS;  // (of the stages)
 
-    Tile<BM, AT, NT> ta;
-    Tile<BN, BT, NT> tb;
-    ta.init(tid, a.lda, a.m - m0);
-    tb.init(tid, a.ldb, nb - n0);
-    auto load = [&](int s, uint4* b) {
-        const int k0 = (step0 + s) * BK;
-        if constexpr (AT) ta.load(a.A + k0 * a.lda + m0, a.lda, min(BK, ka - k0), a.m - m0, b, tid);
-        else ta.load(a.A + m0 * a.lda + k0, a.lda, min(BM, a.m - m0), k_end - k0, b, tid);
-        if constexpr (EPI == EPI_DHEAD)
-            tb.load(a.B + (n0 >> 8) * a.panel + (n0 & 255) + k0 * a.ldb, a.ldb, min(BK, k_end - k0), nb - n0, b + BM * 8, tid);
-        else if constexpr (EPI == EPI_DX)
-            tb.load(a.B + (k0 >> 8) * a.panel + (k0 & 255) + n0 * a.ldb, a.ldb, min(BN, n_end - n0), k_end - k0, b + BM * 8, tid);
-        else tb.load(a.B + n0 * a.ldb + k0, a.ldb, min(BN, n_end - n0), k_end - k0, b + BM * 8, tid);
+    Tile<BM, AT, NT, BK> ta;
+    Tile<BN, BT, NT, BK> tb;
+    const int lda = (int)a.lda, ldb = (int)a.ldb, ra = a.m - m0, rb = nb - n0;  // (rows past the tile's)
+    ta.init(tid, lda, ra);
+    tb.init(tid, ldb, rb);
+    // where the next step to be loaded lies, and the k left from it on
+    int k = (step0 + group * rounds * NS) * BK;
+    const uint16_t* pa = a.A + (AT ? k * a.lda + m0 : m0 * a.lda + k);
+    const uint16_t* pb = EPI == EPI_DHEAD ? a.B + (n0 >> 8) * a.panel + (n0 & 255) + k * a.ldb
+                         : EPI == EPI_DX  ? a.B + (k >> 8) * a.panel + (k & 255) + n0 * a.ldb
+                                          : a.B + n0 * a.ldb + k;
+    const long long next_panel = a.panel - 256 + BK;
+    __amdgpu_buffer_rsrc_t from_a, from_b;
+    int left_a, left_b;
+    auto next = [&] {  // the next step to be loaded
+        left_a = (AT ? ka : k_end) - k, left_b = k_end - k;
+        from_a = Tile<BM, AT, NT, BK>::source(pa, lda, AT ? ra : min(BM, ra), left_a);
+        from_b = Tile<BN, BT, NT, BK>::source(pb, ldb, BT ? rb : min(BN, rb), left_b);
+        pa += AT ? (long long)BK * a.lda : BK;
+        pb += BT ? (long long)BK * a.ldb : EPI == EPI_DX && (k & 255) == 256 - BK ? next_panel : BK;
+        k += BK;
     };
-    f32x16 acc[MI][NI];
+    constexpr int NA = CA / NT;
+    auto load = [&](int i0, int i1, uint4* b) {  // its loads i0 .. i1 - 1 of NL
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+        for (int i = i0; i < i1; ++i) {
+            if (i < NA) ta.load(i, from_a, left_a, b + mine, tid);
+            else tb.load(i - NA, from_b, left_b, b + (mine + CA), tid);
+        }
+    };
+    constexpr int CN = MI * NI > 1 ? 1 : 2;  // sums of one tile: two in turn, which need not wait for each other
+    f32x16 acc[MI][NI], odd;
 #pragma unroll
-        for (int j = 0; j < NI; ++j)
+    for (int e = 0; e < 16; ++e) {
+        odd[e] = 0.f;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    auto sum = [&](const uint4* b) {
+        for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int u = 0; u < BK / 16; ++u) {
+            for (int j = 0; j < NI; ++j) acc[i][j][e] = 0.f;
+    }
+    // A step's sums from one stage, the loads of a later step to another, with four stages between the sums: a wavefront that
+    // issues all of its loads at once stands still until the memory pipeline has taken them, and all do after the barrier.
+    // (With two they would land too late for the next step.)
+    auto sum = [&](const uint4* b, uint4* to) {
+        constexpr int U = BK / 16;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
             uint4 fa[MI], fb[NI];
 #pragma unroll
-            for (int j = 0; j < NI; ++j) fb[j] = Tile<BN, BT, NT>::frag(b, BM * 8, wn * TN + 32 * j, u, lane);
+            for (int j = 0; j < NI; ++j) fb[j] = Tile<BN, BT, NT, BK>::frag(b, mine + CA, wn * TN + 32 * j, u, lane);
 #pragma unroll
-            for (int i = 0; i < MI; ++i) fa[i] = Tile<BM, AT, NT>::frag(b, 0, wm * TM + 32 * i, u, lane);
+            for (int i = 0; i < MI; ++i) fa[i] = Tile<BM, AT, NT, BK>::frag(b, mine, wm * TM + 32 * i, u, lane);
+            if constexpr (NS >= 4) load(u * NL / U, (u + 1) * NL / U, to);
+            else if (NS == 2 && u == 0) load(0, NL, to);
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
-                for (int j = 0; j < NI; ++j) acc[i][j] = mfma32(fa[i], fb[j], acc[i][j]);
-            __builtin_amdgcn_sched_barrier(0);  // (one u's fragments at a time: the registers hold no more)
+                for (int j = 0; j < NI; ++j) {
+                    f32x16& to = CN == 2 && (u & 1) ? odd : acc[i][j];
+                    to = mfma32(fa[i], fb[j], to);
+                }
+            // (one u's fragments at a time: the registers hold no more; a small tile reads them all at once)
+            if constexpr (MI * NI > 1) __builtin_amdgcn_sched_barrier(0);
         }
     };
     // (whole rounds of the stages: steps past the last are zeros, as are the loads past the end into stages that nothing
     // reads. A last step of its own behind a branch would have the compiler copy every accumulator.)
+    auto step = [&](uint4* to, const uint4* from) {
+        step_barrier<NS >= 4 ? (NS - 2) * NL : 0>();
+        next();
+        sum(from, to);
+    };
+    auto first = [&](uint4* to) {
+        next();
+        load(0, NL, to);
+    };
     if (steps > 0) {
-        load(0, s0);
-        if constexpr (NS > 2) load(1, s1), load(2, s2);
+        first(s0);
+        if constexpr (NS >= 4) first(s1), first(s2);
+        if constexpr (NS == 8) first(s3), first(s4), first(s5), first(s6);
     }
-    for (int s = 0; s < steps; s += NS) {
-        if constexpr (NS == 2) {
+    for (int s = 0; s < rounds; ++s) {
+        if constexpr (NS == 1) {  // (more workgroups instead)
             step_barrier<0>();
-            load(s + 1, s1);
-            sum(s0);
-            step_barrier<0>();
-            load(s + 2, s0);
-            sum(s1);
+            sum(s0, s0);
+            if (s + 1 < rounds) {
+                step_barrier<0>();
+                first(s0);
+            }
+        } else if constexpr (NS == 2) {
+            step(s1, s0);
+            step(s0, s1);
+        } else if constexpr (NS == 4) {
+            step(s3, s0);
+            step(s0, s1);
+            step(s1, s2);
+            step(s2, s3);
         } else {
-            step_barrier<2 * NL>();
-            load(s + 3, s3);
-            sum(s0);
-            step_barrier<2 * NL>();
-            load(s + 4, s0);
-            sum(s1);
-            step_barrier<2 * NL>();
-            load(s + 5, s1);
-            sum(s2);
-            step_barrier<2 * NL>();
-            load(s + 6, s2);
-            sum(s3);
+            step(s7, s0);
+            step(s0, s1);
+            step(s1, s2);
+            step(s2, s3);
+            step(s3, s4);
+            step(s4, s5);
+            step(s5, s6);
+            step(s6, s7);
         }
     }
     step_barrier<0>();  // (the last loads landed: they write this workgroup's LDS)
+    if constexpr (CN == 2) acc[0][0] += odd;
+    if constexpr (WK == 2) {  // the second group's sums to the first
+        static_assert(WK == 1 || (MI * NI == 1 && NW * 256 <= CM * WK), "their sums fit a stage");
+        f32x4* at = reinterpret_cast<f32x4*>(s1) + wave * 256 + lane;
+        if (group) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                at[64 * g] = f32x4{acc[0][0][4 * g], acc[0][0][4 * g + 1], acc[0][0][4 * g + 2], acc[0][0][4 * g + 3]};
+        }
+        step_barrier<0>();
+        if (group) return;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const f32x4 v = at[64 * g];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[0][0][4 * g + e] += v[e];
+        }
+    }
 
     // lane: columns n = n0 + wn TN + 32 j + lane % 32, rows m0 + wm TM + 32 i + 8 g + 4 (lane / 32) + 0 .. 3 in words 4 g ..
     const int r = lane & 31, h = lane >> 5;
     const int mw = m0 + wm * TM;
     // the wavefront's own part of the stages: 32 columns of its TM rows in float32
-    constexpr int PER = (NW + NS - 1) / NS;
-    static_assert(PER * 8 * TM <= CH, "a wavefront's sums of 32 columns fit its part of a stage");
-    const int st = wave / PER;
-    uint4* const region = (NS == 2 ? (st ? s1 : s0) : st == 0 ? s0 : st == 1 ? s1 : st == 2 ? s2 : s3) + (wave % PER) * 8 * TM;
+    constexpr int PER = NS == 1 || WK > 1 ? NW : NS == 4 ? (NW + 3) / 4 : (NW + 1) / 2;
+    static_assert(PER * 8 * TM <= CH * WK, "a wavefront's sums of 32 columns fit its part of a stage");
+    uint4* region = s0 + (wave % PER) * 8 * TM;
+    if constexpr (PER < NW) {
+        const int at = wave / PER;
+        if constexpr (NS == 4) region = (at == 0 ? s0 : at == 1 ? s1 : at == 2 ? s2 : s3) + (wave % PER) * 8 * TM;
+        else region = (at ? s1 : s0) + (wave % PER) * 8 * TM;
+    }
     // 32 columns in bf16, 4 rows of column r at 8-byte unit q: to whole runs of a column's rows in memory
     uint2* const half = reinterpret_cast<uint2*>(region);
     constexpr int C16 = TM / 8, SWZ = C16 < 16 ? C16 - 1 : 15;  // 16-byte chunks a column; their turn by column
@@ -534,7 +604,7 @@ __device__ __forceinline__ int wave_sum(int v) {
     return v;
 }
 
-constexpr int GROWS = 16;    // rows a workgroup of hl_gather
+constexpr int GROWS = 4;     // rows a workgroup of hl_gather, one a wavefront
 constexpr int FEW = 2048;    // entries that every workgroup looks through itself
 
 // The rows that count, one after another: each workgroup finds the place of its own from the flags of all rows before
@@ -570,7 +640,7 @@ __global__ __launch_bounds__(256) void hl_gather(const Prep p) {
         const uint4 f = reinterpret_cast<const uint4*>(held)[i];
         c += __popc(f.x) + __popc(f.y) + __popc(f.z) + __popc(f.w);
     }
-    if (last && tid < n % 16) c += held[n / 16 * 16 + tid];
+    if (tid < r0 % 16) c += held[r0 / 16 * 16 + tid];
     c = wave_sum(c);
     float top = 0.f;
     if (last && p.a.g) {
@@ -604,13 +674,13 @@ __global__ __launch_bounds__(256) void hl_gather(const Prep p) {
         if (on) p.idx[at] = r;
     }
     __syncthreads();  // (OWN: this workgroup's entries are written too)
-    for (int i = wave; i < GROWS; i += 4) {
-        const int at = rows[i];
+    {
+        const int i = wave, at = rows[i];
         if (at < 0) {
             if (p.dx && r0 + i < n)  // (a row left out)
                 for (int q = lane; q < p.a.dim / 4; q += 64)
                     *reinterpret_cast<uint2*>(p.dx + (r0 + i) * p.a.ld_dx + 4 * q) = make_uint2(0u, 0u);
-            continue;
+            return;
         }
         if (lane < 1 << p.kp) p.idc[((long long)at << p.kp) + lane] = p.ids[((long long)(r0 + i) << p.kp) + lane];
         const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.a.x) + (r0 + i) * p.a.ldx);
@@ -672,11 +742,16 @@ __global__ __launch_bounds__(TB* SL) void hl_merge(const Merge p) {
             join(m, s, v[0], v[1]);
         }
     }
-    ms[tid] = m;
-    ss[tid] = s;
-    __syncthreads();
+    if constexpr (TB == 1) {  // (a row's slices are whole wavefronts)
 #pragma unroll
-    for (int o = SL / 2; o; o >>= 1) {
+        for (int o = 32; o; o >>= 1) join(m, s, __shfl_xor(m, o), __shfl_xor(s, o));
+    }
+    constexpr int LEFT = TB == 1 ? SL / 64 : SL;  // slices that are left
+    if (TB > 1 || (tid & 63) == 0) ms[TB == 1 ? tid >> 6 : tid] = m, ss[TB == 1 ? tid >> 6 : tid] = s;
+    __syncthreads();
+    if constexpr (TB == 1) m = ms[tid % LEFT], s = ss[tid % LEFT];
+#pragma unroll
+    for (int o = LEFT / 2; o; o >>= 1) {
         if (sl < o) {
             join(m, s, ms[tid + o * TB], ss[tid + o * TB]);
             ms[tid] = m;
@@ -780,7 +855,7 @@ long long up(long long v, long long to) { return (v + to - 1) / to * to; }
 
 struct Plan {
     int kp, piece;
-    int z, w, d;  // the tiles of z, dhead and dx
+    int z, y, w, d;  // the tiles of z for the statistics and for dz, of dhead and of dx
     int parts;
     bool gather, raw, own;
     long long ids, idc, q, ent, held, idx, pos, live, xc, part, dz, acc, bytes;
@@ -803,7 +878,7 @@ int tiles_of(int t, long long m, long long n) {
 }
 
 int choose(long long m, long long n, long long k) {
-    const int steps = (int)(up(k, BK) / BK);
+    const int steps = (int)(up(k, KSTEP) / KSTEP);
     return tiled_us(pace(128, 128), tiles_of(T128, m, n), steps) < tiled_us(pace(256, 256), tiles_of(T256, m, n), steps) ? T128 : T256;
 }
 
@@ -860,9 +935,10 @@ bool plan_of(const dr_head_loss* a, int what, Plan& p) {
         const long long pieces = (tiles + (fit > 1 ? fit : 1) - 1) / (fit > 1 ? fit : 1);
         p.piece = (int)((tiles + pieces - 1) / pieces) * 256;
         p.dz = take(n * p.piece * 2);
+        p.y = choose_z(p.piece, n, a->dim);
         p.w = choose(a->dim, p.piece, n);
         if (a->dx) {
-            p.d = choose_dx(n, a->dim, p.piece / BK);
+            p.d = choose_dx(n, a->dim, p.piece / KSTEP);
             // the sums of all rows where there are several pieces; of splits no more than ROUNDS rounds of tiles
             const long long whole = p.piece < a->valid ? n * a->dim : 0;
             const Pace pc = pace(SIZE[p.d].bm, SIZE[p.d].bn);
@@ -874,23 +950,23 @@ bool plan_of(const dr_head_loss* a, int what, Plan& p) {
     return true;
 }
 
-template <int BM, int BN, int WM, int WN, int NS, bool AT, bool BT, int EPI>
+template <int BM, int BN, int WM, int WN, int WK, int NS, int BK, bool AT, bool BT, int EPI>
 void launch(Gemm g, hipStream_t st) {
     g.tm = (g.m + BM - 1) / BM;
     g.tn = (g.n + BN - 1) / BN;
     int grid = g.tm * g.tn;
     if (EPI == EPI_DX) grid = grid > ROUNDS * pace(BM, BN).at_once ? grid : ROUNDS * pace(BM, BN).at_once;
     grid = (grid + 7) & ~7;  // (as many for each XCD)
-    hipLaunchKernelGGL((hl_gemm<BM, BN, WM, WN, NS, AT, BT, EPI>), dim3(grid), dim3(64 * WM * WN), 0, st, g);
+    hipLaunchKernelGGL((hl_gemm<BM, BN, WM, WN, WK, NS, BK, AT, BT, EPI>), dim3(grid), dim3(64 * WM * WN * WK), 0, st, g);
 }
 
 template <int EPI>
 void launch_z(const Gemm& g, int t, hipStream_t st) {
     switch (t) {
-        case T256: return launch<256, 256, 2, 4, 2, false, false, EPI>(g, st);
-        case T128: return launch<128, 128, 2, 2, 2, false, false, EPI>(g, st);
-        case T256x64: return launch<256, 64, 2, 2, 2, false, false, EPI>(g, st);
-        default: return launch<64, 64, 2, 2, 4, false, false, EPI>(g, st);
+        case T256: return launch<256, 256, 2, 4, 1, 2, 64, false, false, EPI>(g, st);
+        case T128: return launch<128, 128, 2, 2, 1, 2, 64, false, false, EPI>(g, st);
+        case T256x64: return launch<256, 64, 2, 2, 1, 2, 64, false, false, EPI>(g, st);
+        default: return launch<64, 64, 2, 2, 2, 4, 64, false, false, EPI>(g, st);
     }
 }
 
@@ -943,7 +1019,7 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
     z.n = n, z.k = z.ka = a->dim;
     z.live = P.gather ? p.live : nullptr;
     z.idx = P.gather ? p.idx : nullptr;
-    z.steps = (a->dim + BK - 1) / BK;
+    z.steps = (a->dim + KSTEP - 1) / KSTEP;
     z.sc = LOG2E / a->temperature;
     z.ids = P.gather ? p.idc : p.ids, z.kp = P.kp, z.kn = kn;
     z.raw = P.raw ? a->ids : nullptr, z.raw64 = a->ids64;
@@ -972,11 +1048,11 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
             s.out = dz;
             s.panel = panel;
             if (a->vals) {
-                launch_z<EPI_DZ>(s, P.z, st);
+                launch_z<EPI_DZ>(s, P.y, st);
                 Fix f{p.live, p.idx, p.ids, p.q, a->lse, a->logits, a->g, p.top, kn, P.kp, v0, v0 + vn, z.sc, dz, panel};
                 hipLaunchKernelGGL(hl_fix, dim3(eblocks), dim3(256), 0, st, f);
             } else {
-                launch_z<EPI_DZ1>(s, P.z, st);
+                launch_z<EPI_DZ1>(s, P.y, st);
             }
             if (a->dhead) {
                 Gemm w{};
@@ -984,33 +1060,34 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
                 w.B = dz, w.ldb = 256, w.panel = panel;
                 // (the rows past valid: zeros, with the last piece)
                 w.m = a->dim, w.nb = vn, w.n = v0 + vn == a->valid ? a->vocab - v0 : vn, w.k = n, w.live = p.live;
-                w.steps = (n + BK - 1) / BK;
+                w.steps = (n + KSTEP - 1) / KSTEP;
                 w.out = reinterpret_cast<uint16_t*>(a->dhead) + (long long)v0 * a->ld_dhead;
                 w.ld_out = a->ld_dhead;
                 w.scale = p.top + 1;
-                if (P.w == T256) launch<256, 256, 2, 4, 2, true, true, EPI_DHEAD>(w, st);
-                else launch<128, 128, 2, 2, 2, true, true, EPI_DHEAD>(w, st);
+                if (n <= KSTEP) launch<128, 128, 2, 2, 1, 1, 64, true, true, EPI_DHEAD>(w, st);
+                else if (P.w == T256) launch<256, 256, 2, 4, 1, 4, 32, true, true, EPI_DHEAD>(w, st);
+                else launch<128, 128, 2, 2, 1, 4, 32, true, true, EPI_DHEAD>(w, st);
             }
             if (a->dx) {
                 Gemm d{};
                 d.A = z.A + (long long)v0 * a->ld_head, d.lda = a->ld_head;
                 d.B = dz, d.ldb = 256, d.panel = panel;
                 d.m = a->dim, d.n = n, d.k = (int)up(vn, 8), d.ka = vn, d.live = p.live;
-                d.steps = vp / BK, d.plan_steps = P.piece / BK;
+                d.steps = vp / KSTEP, d.plan_steps = P.piece / KSTEP;
                 d.acc = reinterpret_cast<float*>(ws + P.acc);
                 d.ld_acc = a->dim;
                 d.add = v0 > 0;
                 d.idx = p.idx;
                 d.scale = p.top + 1;
                 if (v0 + vn == a->valid) d.out = reinterpret_cast<uint16_t*>(a->dx), d.ld_out = a->ld_dx;
-                if (P.d == T256x64) launch<256, 64, 2, 2, 2, true, false, EPI_DX>(d, st);
-                else if (P.d == T128) launch<128, 128, 2, 2, 2, true, false, EPI_DX>(d, st);
-                else launch<256, 256, 2, 4, 2, true, false, EPI_DX>(d, st);
+                if (P.d == T256x64) launch<256, 64, 2, 2, 1, 4, 32, true, false, EPI_DX>(d, st);
+                else if (P.d == T128) launch<128, 128, 2, 2, 1, 4, 32, true, false, EPI_DX>(d, st);
+                else launch<256, 256, 2, 4, 1, 4, 32, true, false, EPI_DX>(d, st);
             }
         }
         if (a->dx) {
             const Size t = SIZE[P.d];
-            Finish f{reinterpret_cast<const float*>(ws + P.acc), (int)(up(a->dim, t.bm) / t.bm), t.bm, t.bn, P.piece / BK, a->dim, p.live,
+            Finish f{reinterpret_cast<const float*>(ws + P.acc), (int)(up(a->dim, t.bm) / t.bm), t.bm, t.bn, P.piece / KSTEP, a->dim, p.live,
                      p.idx, p.top + 1, reinterpret_cast<uint16_t*>(a->dx), a->ld_dx};
             const long long items = (long long)n * ((a->dim + 255) / 256);
             hipLaunchKernelGGL(hl_dx, dim3((unsigned)(items < 4096 ? items : 4096)), dim3(256), 0, st, f);

@@ -89,7 +89,7 @@ class _Call:
         if g is None:
             return None
         if not isinstance(g, torch.Tensor):
-            g = torch.tensor(float(g), device=self.device)
+            return self.empty(self.n).fill_(float(g))  # (a copy from the host could not be captured)
         assert g.device == self.device, (g.device, self.device)
         if g.dtype == torch.float32 and g.numel() == self.n and g.is_contiguous():
             return g

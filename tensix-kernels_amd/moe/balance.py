@@ -52,7 +52,8 @@ def _run(logits, ids, k, g, kind, ids32, experts, mask, grad):
         m = mask.contiguous()
     gs = None
     if g is not None and grad:
-        gs = g if isinstance(g, torch.Tensor) else torch.tensor(float(g), device=logits.device)
+        # (a number filled in: a copy from the host could not be captured)
+        gs = g if isinstance(g, torch.Tensor) else torch.full((batch,), float(g), device=logits.device)
         assert gs.device == logits.device, (gs.device, logits.device)
         assert gs.numel() in (1, batch), f"balance: {gs.numel()} weights for {batch} batches"
         if gs.dtype != torch.float32 or gs.numel() != batch or not gs.is_contiguous():

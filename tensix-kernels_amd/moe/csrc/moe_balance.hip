@@ -68,7 +68,7 @@ __device__ __forceinline__ void row_p(float (&p)[4 * N], float (&s)[SIG ? 4 * N 
     if constexpr (SIG) {
 #pragma unroll
         for (int i = 0; i < 4 * N; ++i) {
-            s[i] = 1.f / (1.f + expf(-p[i]));
+            s[i] = __builtin_amdgcn_rcpf(1.f + __expf(-p[i]));
             total += s[i];
         }
     } else {
@@ -79,7 +79,7 @@ __device__ __forceinline__ void row_p(float (&p)[4 * N], float (&s)[SIG ? 4 * N 
         const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
         for (int i = 0; i < 4 * N; ++i) {
-            p[i] = expf(p[i] - base);
+            p[i] = __expf(p[i] - base);
             total += p[i];
         }
     }
@@ -106,11 +106,15 @@ __global__ __launch_bounds__(T) void balance_sum_k(const Bal b) {
 #pragma unroll
     for (int i = 0; i < 4 * N; ++i) sum[i] = 0.f;
     int n = 0;
+    float z[4 * N];  // (the next row's logits are asked for before this one's are worked on)
+    row_load<L, N>(b, (long long)batch * a.rows + min(g * R + tid / L, a.rows - 1), l, z);
     for (int r0 = g * R; r0 < a.rows; r0 += b.groups * R) {
         const int r = min(r0 + tid / L, a.rows - 1);  // (the last row again: every lane takes part in the butterflies)
         const long long row = (long long)batch * a.rows + r;
         float p[4 * N], s[SIG ? 4 * N : 1];
-        row_load<L, N>(b, row, l, p);
+#pragma unroll
+        for (int i = 0; i < 4 * N; ++i) p[i] = z[i];
+        row_load<L, N>(b, (long long)batch * a.rows + min(r + b.groups * R, a.rows - 1), l, z);
         uint32_t id = 0xFFFFFFFFu;
         if (l < a.k) {
             const long long at = row * a.ld_ids + l;
@@ -235,6 +239,8 @@ __global__ __launch_bounds__(T) void balance_grad_k(const Bal b) {
     const dr_balance& a = b.a;
     const int tid = threadIdx.x, l = tid % L;
     const int g = blockIdx.x % b.groups, batch = blockIdx.x / b.groups;
+    float z[4 * N];
+    row_load<L, N>(b, (long long)batch * a.rows + min(g * R + tid / L, a.rows - 1), l, z);
     const float per = join(b, batch, g == 0, J);
     const float scale = (a.g ? a.g[batch] : 1.f) * per;
     float f[4 * N];
@@ -248,7 +254,9 @@ __global__ __launch_bounds__(T) void balance_grad_k(const Bal b) {
         const long long row = (long long)batch * a.rows + r;
         const bool on = row_counts(a, row);
         float p[4 * N], s[SIG ? 4 * N : 1];
-        row_load<L, N>(b, row, l, p);
+#pragma unroll
+        for (int i = 0; i < 4 * N; ++i) p[i] = z[i];
+        row_load<L, N>(b, (long long)batch * a.rows + min(r + b.groups * R, a.rows - 1), l, z);
         row_p<L, N, SIG>(p, s);
         float mean = 0.f;
 #pragma unroll

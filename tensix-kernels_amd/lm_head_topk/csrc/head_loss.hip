@@ -161,6 +161,7 @@ struct Pace {
 };
 constexpr int CUS = 256;
 __host__ __device__ constexpr Pace pace(int bm, int bn) {
+    if (bm == 64) return Pace{CUS, 0.25f, 5.f};
     return bn == 64 ? Pace{2 * CUS, 0.6f, 8.f} : bm == 256 ? Pace{CUS, 1.88f, 14.f} : Pace{2 * CUS, 1.1f, 11.f};
 }
 
@@ -225,7 +226,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void hl_gemm(const Gemm a) {
     const int nb = EPI == EPI_DHEAD ? a.nb : n_end, ka = EPI == EPI_DHEAD ? live : a.ka;
     if (n0 >= n_end) return;
     // (a split's steps are whole rounds of the stages: the next split's are not its own)
-    const int all = (k_end + BK - 1) / BK, per = ((all + splits - 1) / splits + NS - 1) / NS * NS, step0 = split * per;
+    constexpr int ROUND = NS * WK;
+    const int all = (k_end + BK - 1) / BK, per = ((all + splits - 1) / splits + ROUND - 1) / ROUND * ROUND, step0 = split * per;
     const int steps = EPI == EPI_DHEAD && n0 >= nb ? 0 : min(per, all - step0);
     const int rounds = ((steps + WK - 1) / WK + NS - 1) / NS;  // (of the stages)
 
@@ -890,7 +892,12 @@ int choose_z(long long m, long long n, long long k) {
 }
 
 int choose_dx(long long n, long long d, int steps) {
-    if (n <= 64) return T256x64;
+    if (n <= 64) {
+        float a, b;
+        dx_splits(pace(256, 64), tiles_of(T256x64, d, n), steps, 256 * 64 * 8, &a);
+        dx_splits(pace(64, 64), tiles_of(T64, d, n), steps, 64 * 64 * 8, &b);
+        return b < a ? T64 : T256x64;
+    }
     float a, b;
     dx_splits(pace(256, 256), tiles_of(T256, d, n), steps, 256 * 256 * 8, &a);
     dx_splits(pace(128, 128), tiles_of(T128, d, n), steps, 128 * 128 * 8, &b);
@@ -906,6 +913,7 @@ bool plan_of(const dr_head_loss* a, int what, Plan& p) {
         return false;
     const bool back = what & DR_LOSS_BACKWARD;
     const long long n = a->rows, np = up(n, 64);
+    if (up(a->valid, 64) / 64 * (np / 64) > 1 << 30) return false;  // (tiles a launch counts)
     p.kp = log2_up(a->k);
     p.z = choose_z(a->valid, n, a->dim);
     p.parts = (int)(up(a->valid, SIZE[p.z].bm) / SIZE[p.z].tm);
@@ -1080,7 +1088,8 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
                 d.idx = p.idx;
                 d.scale = p.top + 1;
                 if (v0 + vn == a->valid) d.out = reinterpret_cast<uint16_t*>(a->dx), d.ld_out = a->ld_dx;
-                if (P.d == T256x64) launch<256, 64, 2, 2, 1, 4, 32, true, false, EPI_DX>(d, st);
+                if (P.d == T64) launch<64, 64, 2, 2, 2, 4, 64, true, false, EPI_DX>(d, st);
+                else if (P.d == T256x64) launch<256, 64, 2, 2, 1, 4, 32, true, false, EPI_DX>(d, st);
                 else if (P.d == T128) launch<128, 128, 2, 2, 1, 4, 32, true, false, EPI_DX>(d, st);
                 else launch<256, 256, 2, 4, 1, 4, 32, true, false, EPI_DX>(d, st);
             }

@@ -15,7 +15,7 @@ import pytest
 
 
 def k_loops(asm):
-    """[(function, instructions)] of the innermost loops of hl_gemm that hold a matrix instruction."""
+    """[(function, instructions)] of the innermost loops of hl_gemm that hold matrix instructions and loads to LDS."""
     out = []
     for name, body in re.findall(r"^(_Z\S*hl_gemm\S+):(.*?)^\.Lfunc_end", asm, re.M | re.S):
         lines = [s.split(";")[0].strip() for s in body.split("\n")]
@@ -26,7 +26,7 @@ def k_loops(asm):
             if any((b, e) != (b2, e2) and b <= b2 and e2 <= e for b2, e2 in loops):
                 continue
             part = [s for s in lines[b:e] if s and not s.endswith(":")]
-            if any(s.startswith("v_mfma") for s in part):
+            if any(s.startswith("v_mfma") for s in part) and any(re.match(r"buffer_load.*\blds$", s) for s in part):
                 out.append((name, part))
     return out
 
@@ -37,7 +37,7 @@ def extra_waits(asm):
             if sum(s.startswith("s_waitcnt") and "vmcnt" in s for s in part) > sum(s == "s_barrier" for s in part)]
 
 
-_LOOP = """_Z7hl_gemm:
+_LOOP = """_Z7hl_gemmILi1EEvv:
 .LBB0_1:
 \ts_waitcnt vmcnt(0) lgkmcnt(0)
 \ts_barrier

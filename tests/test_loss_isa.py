@@ -15,7 +15,8 @@ import pytest
 
 
 def k_loops(asm):
-    """[(function, instructions)] of the innermost loops of hl_gemm that hold matrix instructions and loads to LDS."""
+    """[(function, instructions)] of the innermost loops of hl_gemm that hold matrix instructions and no other memory access
+    than loads to LDS and reads of it (a branch back over code laid in between, an epilogue's, makes none)."""
     out = []
     for name, body in re.findall(r"^(_Z\S*hl_gemm\S+):(.*?)^\.Lfunc_end", asm, re.M | re.S):
         lines = [s.split(";")[0].strip() for s in body.split("\n")]
@@ -26,7 +27,7 @@ def k_loops(asm):
             if any((b, e) != (b2, e2) and b <= b2 and e2 <= e for b2, e2 in loops):
                 continue
             part = [s for s in lines[b:e] if s and not s.endswith(":")]
-            if any(s.startswith("v_mfma") for s in part) and any(re.match(r"buffer_load.*\blds$", s) for s in part):
+            if any(s.startswith("v_mfma") for s in part) and not any(s.startswith("global_") for s in part):
                 out.append((name, part))
     return out
 

@@ -13,6 +13,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 #include "dense_reader.h"
 #include "lm_head.h"
 
@@ -151,26 +153,33 @@ struct Tile {
     }
 };
 
-// What a workgroup of each tile takes (us): a step, and its beginning and end, as many workgroups at once as fit the CUs (one
-// of 256 x 256, two of the others). From dx at 8192 x 4096 x 16384 (rows x dim x vocabulary): 1240 TFLOP/s in the larger
-// tiles, 1030 in the smaller, which are for what would leave CUs idle.
+// About the time (us) that a workgroup of each product and tile takes for a step of 64 k (more with more of the CUs at work:
+// the memory and the power are shared) and for its beginning and end, as many workgroups at once as fit the CUs. Fitted to the
+// kernels' times at eight shapes of 73 to 8192 rows, 584 to 4096 values and 2898 to 94639 tokens, most within 15 %; what
+// decides between two tiles is mostly how many rounds they take.
 enum Epi { EPI_STATS, EPI_DZ, EPI_DZ1, EPI_DHEAD, EPI_DX };  // (DZ1: tokens, their own logit's 1 taken off there)
 struct Pace {
     int at_once;
-    float step, ends;
+    float step, shared, ends;
 };
 constexpr int CUS = 256;
-__host__ __device__ constexpr Pace pace(int bm, int bn) {
-    if (bm == 64) return Pace{CUS, 0.25f, 5.f};
-    return bn == 64 ? Pace{2 * CUS, 0.6f, 8.f} : bm == 256 ? Pace{CUS, 1.88f, 14.f} : Pace{2 * CUS, 1.1f, 11.f};
+__host__ __device__ constexpr Pace pace(int epi, int bm, int bn, int wk) {
+    const bool dx = epi == EPI_DX, dhead = epi == EPI_DHEAD;
+    if (wk == 2) return Pace{CUS, dx ? 0.23f : 0.28f, 0.f, dx ? 4.5f : 2.8f};  // 64 x 64, two groups of wavefronts
+    if (bm == 64) return Pace{2 * CUS, 0.32f, 0.16f, 3.5f};
+    if (bn == 64) return Pace{2 * CUS, 0.6f, 0.9f, 8.f};
+    if (bm == 256) return Pace{CUS, dx ? 1.05f : dhead ? 1.15f : 1.2f, 0.45f, dx ? 13.f : dhead ? 8.f : 12.f};
+    return Pace{2 * CUS, dx ? 0.75f : dhead ? 0.6f : 0.62f, dhead ? 0.3f : 0.35f, dx ? 7.f : dhead ? 4.f : 8.f};
 }
 
 __host__ __device__ inline float tiled_us(const Pace& p, int tiles, int steps) {
-    return (float)((tiles + p.at_once - 1) / p.at_once) * (p.step * (float)steps + p.ends);
+    const int rounds = (tiles + p.at_once - 1) / p.at_once;
+    const float full = rounds ? (float)tiles / (float)(rounds * p.at_once) : 0.f;
+    return (float)rounds * ((p.step + p.shared * full) * (float)steps + p.ends);
 }
 
-// dx's splits of its long sum, for one or two rounds of workgroups: a split more costs its sums' way through memory. The
-// rows that count are known on the device alone, so every workgroup finds them for itself.
+// dx's splits of its long sum, for one or two rounds of workgroups: their sums' way back through memory costs a launch and
+// about 3.5 TB/s. The rows that count are known on the device alone, so every workgroup finds the splits for itself.
 constexpr int ROUNDS = 2;
 __host__ __device__ inline int dx_splits(const Pace& p, int tiles, int steps, int tile_bytes, float* us = nullptr) {
     int best = 1;
@@ -179,7 +188,7 @@ __host__ __device__ inline int dx_splits(const Pace& p, int tiles, int steps, in
         int s = r * p.at_once / (tiles > 0 ? tiles : 1);
         if (s > steps / 4) s = steps / 4;
         if (s < 2) continue;
-        const float t = tiled_us(p, tiles * s, ((steps + s - 1) / s + 1) & ~1) + 4.f + (float)tiles * (float)s * (float)tile_bytes * 0.5e-6f;
+        const float t = tiled_us(p, tiles * s, ((steps + s - 1) / s + 1) & ~1) + 4.f + (float)tiles * (float)s * (float)tile_bytes * 0.28e-6f;
         if (t < least) least = t, best = s;
     }
     if (us) *us = least;
@@ -218,7 +227,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void hl_gemm(const Gemm a) {
     const int live = a.live ? *a.live : (EPI == EPI_DHEAD ? a.k : a.n);
     // (dx: the tiles of the rows that count, split as many ways as fill the CUs)
     const int tn = EPI == EPI_DX ? (live + BN - 1) / BN : a.tn;
-    const int splits = EPI == EPI_DX ? dx_splits(pace(BM, BN), a.tm * tn, a.plan_steps, BM * BN * 8) : 1;
+    const int splits = EPI == EPI_DX ? dx_splits(pace(EPI, BM, BN, WK), a.tm * tn, a.plan_steps, BM * BN * 4) : 1;
     int mt, nt, split;
     if (!tile_of(a.tm, tn, splits, mt, nt, split)) return;
     const int m0 = mt * BM, n0 = nt * BN;
@@ -816,7 +825,7 @@ __global__ __launch_bounds__(256) void hl_fix(const Fix p) {
 
 struct Finish {
     const float* acc;
-    int tm, bm, bn, steps, dim;
+    int tm, bm, bn, wk, steps, dim;
     const int *live, *idx;
     const float* scale;
     uint16_t* dx;
@@ -826,7 +835,7 @@ struct Finish {
 // dx from the splits' sums (none: it is there): 256 columns of a row at a time, a quarter of the splits a wavefront
 __global__ __launch_bounds__(256) void hl_dx(const Finish p) {
     __shared__ f32x4 part[4][64];
-    const int live = *p.live, splits = dx_splits(pace(p.bm, p.bn), p.tm * ((live + p.bn - 1) / p.bn), p.steps, p.bm * p.bn * 8);
+    const int live = *p.live, splits = dx_splits(pace(EPI_DX, p.bm, p.bn, p.wk), p.tm * ((live + p.bn - 1) / p.bn), p.steps, p.bm * p.bn * 4);
     if (splits == 1) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, cols = (p.dim + 255) / 256;
     const float s = *p.scale;
@@ -869,39 +878,37 @@ int log2_up(int k) {
     return p;
 }
 
-enum Tiles { T256, T128, T256x64, T64 };
+enum Tiles { T256, T128, T64, T64K, T256x64 };  // (T64K: two groups of wavefronts split K)
 struct Size {
-    int bm, bn, tm;  // (a wavefront's rows)
+    int bm, bn, tm, wk;  // (tm: a wavefront's rows)
 };
-constexpr Size SIZE[] = {{256, 256, 128}, {128, 128, 64}, {256, 64, 128}, {64, 64, 32}};
+constexpr Size SIZE[] = {{256, 256, 128, 1}, {128, 128, 64, 1}, {64, 64, 32, 1}, {64, 64, 32, 2}, {256, 64, 128, 1}};
+
+constexpr Pace pace_of(int epi, int t) { return pace(epi, SIZE[t].bm, SIZE[t].bn, SIZE[t].wk); }
 
 int tiles_of(int t, long long m, long long n) {
     return (int)(up(m, SIZE[t].bm) / SIZE[t].bm * (up(n, SIZE[t].bn) / SIZE[t].bn));
 }
 
-int choose(long long m, long long n, long long k) {
+// the tile of `tiles` that takes the least time for a product of m rows by n columns, summed over k
+int choose(int epi, long long m, long long n, long long k, std::initializer_list<int> tiles) {
+    int best = 0;
+    float least = 1e30f;
     const int steps = (int)(up(k, KSTEP) / KSTEP);
-    return tiled_us(pace(128, 128), tiles_of(T128, m, n), steps) < tiled_us(pace(256, 256), tiles_of(T256, m, n), steps) ? T128 : T256;
+    for (int t : tiles) {
+        float us;
+        if (epi == EPI_DX) dx_splits(pace_of(epi, t), tiles_of(t, m, n), steps, SIZE[t].bm * SIZE[t].bn * 4, &us);
+        else us = tiled_us(pace_of(epi, t), tiles_of(t, m, n), steps);
+        if (us < least) least = us, best = t;
+    }
+    return best;
 }
 
 // z's: up to 64 columns take tiles as narrow, of 256 rows where there are enough of them for every CU (32 rows x 128256 x
-// 4096: 176 us, 6 TB/s), else of 64, four stages deep (48 x 8192 x 1024: 11 us against 16)
+// 4096: 176 us, 6 TB/s)
 int choose_z(long long m, long long n, long long k) {
-    if (n <= 64) return tiles_of(T256x64, m, n) >= CUS ? T256x64 : T64;
-    return choose(m, n, k);
-}
-
-int choose_dx(long long n, long long d, int steps) {
-    if (n <= 64) {
-        float a, b;
-        dx_splits(pace(256, 64), tiles_of(T256x64, d, n), steps, 256 * 64 * 8, &a);
-        dx_splits(pace(64, 64), tiles_of(T64, d, n), steps, 64 * 64 * 8, &b);
-        return b < a ? T64 : T256x64;
-    }
-    float a, b;
-    dx_splits(pace(256, 256), tiles_of(T256, d, n), steps, 256 * 256 * 8, &a);
-    dx_splits(pace(128, 128), tiles_of(T128, d, n), steps, 128 * 128 * 8, &b);
-    return b < a ? T128 : T256;
+    if (n <= 64 && tiles_of(T256x64, m, n) >= CUS) return T256x64;
+    return n <= 64 ? choose(EPI_DZ, m, n, k, {T64, T64K}) : choose(EPI_DZ, m, n, k, {T256, T128, T64, T64K});
 }
 
 bool plan_of(const dr_head_loss* a, int what, Plan& p) {
@@ -917,7 +924,8 @@ bool plan_of(const dr_head_loss* a, int what, Plan& p) {
     p.kp = log2_up(a->k);
     p.z = choose_z(a->valid, n, a->dim);
     p.parts = (int)(up(a->valid, SIZE[p.z].bm) / SIZE[p.z].tm);
-    p.gather = back || n > 64;
+    // (forward alone, the rows that count are gathered where leaving out the others may save more than that takes, about 10 us)
+    p.gather = back || (double)n * a->valid * a->dim > 3e10;
     p.raw = !p.gather && a->vals == nullptr;  // (tokens read where they are: no launch before z's)
     p.own = p.gather && n << p.kp <= FEW;
     long long at = 0;
@@ -944,13 +952,12 @@ bool plan_of(const dr_head_loss* a, int what, Plan& p) {
         p.piece = (int)((tiles + pieces - 1) / pieces) * 256;
         p.dz = take(n * p.piece * 2);
         p.y = choose_z(p.piece, n, a->dim);
-        p.w = choose(a->dim, p.piece, n);
+        p.w = choose(EPI_DHEAD, a->dim, p.piece, n, {T256, T128});
         if (a->dx) {
-            p.d = choose_dx(n, a->dim, p.piece / KSTEP);
+            p.d = n <= 64 ? choose(EPI_DX, a->dim, n, p.piece, {T256x64, T64K}) : choose(EPI_DX, a->dim, n, p.piece, {T256, T128, T64K});
             // the sums of all rows where there are several pieces; of splits no more than ROUNDS rounds of tiles
             const long long whole = p.piece < a->valid ? n * a->dim : 0;
-            const Pace pc = pace(SIZE[p.d].bm, SIZE[p.d].bn);
-            const long long split = (long long)ROUNDS * pc.at_once * SIZE[p.d].bm * SIZE[p.d].bn;
+            const long long split = (long long)ROUNDS * pace_of(EPI_DX, p.d).at_once * SIZE[p.d].bm * SIZE[p.d].bn;
             p.acc = take((whole > split ? whole : split) * 4);
         }
     }
@@ -963,7 +970,8 @@ void launch(Gemm g, hipStream_t st) {
     g.tm = (g.m + BM - 1) / BM;
     g.tn = (g.n + BN - 1) / BN;
     int grid = g.tm * g.tn;
-    if (EPI == EPI_DX) grid = grid > ROUNDS * pace(BM, BN).at_once ? grid : ROUNDS * pace(BM, BN).at_once;
+    constexpr int most = ROUNDS * pace(EPI, BM, BN, WK).at_once;
+    if (EPI == EPI_DX && grid < most) grid = most;
     grid = (grid + 7) & ~7;  // (as many for each XCD)
     hipLaunchKernelGGL((hl_gemm<BM, BN, WM, WN, WK, NS, BK, AT, BT, EPI>), dim3(grid), dim3(64 * WM * WN * WK), 0, st, g);
 }
@@ -974,6 +982,7 @@ void launch_z(const Gemm& g, int t, hipStream_t st) {
         case T256: return launch<256, 256, 2, 4, 1, 2, 64, false, false, EPI>(g, st);
         case T128: return launch<128, 128, 2, 2, 1, 2, 64, false, false, EPI>(g, st);
         case T256x64: return launch<256, 64, 2, 2, 1, 2, 64, false, false, EPI>(g, st);
+        case T64: return launch<64, 64, 2, 2, 1, 4, 64, false, false, EPI>(g, st);
         default: return launch<64, 64, 2, 2, 2, 4, 64, false, false, EPI>(g, st);
     }
 }
@@ -1088,7 +1097,7 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
                 d.idx = p.idx;
                 d.scale = p.top + 1;
                 if (v0 + vn == a->valid) d.out = reinterpret_cast<uint16_t*>(a->dx), d.ld_out = a->ld_dx;
-                if (P.d == T64) launch<64, 64, 2, 2, 2, 4, 64, true, false, EPI_DX>(d, st);
+                if (P.d == T64K) launch<64, 64, 2, 2, 2, 4, 64, true, false, EPI_DX>(d, st);
                 else if (P.d == T256x64) launch<256, 64, 2, 2, 1, 4, 32, true, false, EPI_DX>(d, st);
                 else if (P.d == T128) launch<128, 128, 2, 2, 1, 4, 32, true, false, EPI_DX>(d, st);
                 else launch<256, 256, 2, 4, 1, 4, 32, true, false, EPI_DX>(d, st);
@@ -1096,7 +1105,7 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
         }
         if (a->dx) {
             const Size t = SIZE[P.d];
-            Finish f{reinterpret_cast<const float*>(ws + P.acc), (int)(up(a->dim, t.bm) / t.bm), t.bm, t.bn, P.piece / KSTEP, a->dim, p.live,
+            Finish f{reinterpret_cast<const float*>(ws + P.acc), (int)(up(a->dim, t.bm) / t.bm), t.bm, t.bn, t.wk, P.piece / KSTEP, a->dim, p.live,
                      p.idx, p.top + 1, reinterpret_cast<uint16_t*>(a->dx), a->ld_dx};
             const long long items = (long long)n * ((a->dim + 255) / 256);
             hipLaunchKernelGGL(hl_dx, dim3((unsigned)(items < 4096 ? items : 4096)), dim3(256), 0, st, f);

@@ -111,7 +111,8 @@ int dr_moe_route_gate_up(const dr_launch* launch, const dr_moe* moe, const dr_ro
 
 /* The router's balance loss of batches of rows (a batch: a sequence, or all of a step's tokens), each expert's count and
  * the gradient of the logits. Per batch, over its rows t that count:
- *   p[t] = softmax of the logits (kind 0; a row with none above -inf: 0), or their sigmoids over the sigmoids' sum (kind 1);
+ *   p[t] = softmax of the logits (kind 0; a row with none above -inf: 0), or their sigmoids over the sigmoids' sum (kind 1;
+ *     a row whose sigmoids are all 0 in float32, logits below -87: 0);
  *   counts[e] = the rows' slots that chose e (an id >= experts chooses none), f[e] = experts * counts[e] / sum of counts;
  *   loss = sum over e of f[e] * mean over t of p[t][e]  (1 where all are chosen alike; 0 where no row counts);
  *   dlogits = g times its gradient, the counts taken as constants (as the choice has none).

@@ -69,7 +69,7 @@ struct Gemm {
     const int* idx;         // row that counts -> row, or NULL: itself
     const float* lse;       // [rows]
     const float* g;         // [rows], or NULL: ones
-    const float* top;       // the largest |g|
+    const float* top;       // the factor taken out of dz
     f32x2* part;            // [m / TM][n] maximum and sum
     long long ld_part;
     const int* ids;         // [rows that count][1 << kp] entries, -1 none
@@ -563,7 +563,7 @@ struct Prep {
     int* idx;       // [rows] row that counts -> row
     int* pos;       // [rows] row -> row that counts, -1: left out
     int* live;      // rows that count
-    float* top;     // the largest |g| of them, and that over T
+    float* top;     // the factor taken out of dz, the largest |g| of them, and that over T
     uint16_t* xc;   // [rows that count][dim]
     uint16_t* dx;   // whose rows left out get zeros, or NULL
 };
@@ -624,7 +624,7 @@ constexpr int FEW = 2048;    // entries that every workgroup looks through itsel
 template <bool OWN>
 __global__ __launch_bounds__(256) void hl_gather(const Prep p) {
     __shared__ int sums[4];
-    __shared__ float tops[4];
+    __shared__ float tops[4], lows[4];
     __shared__ int rows[GROWS];
     __shared__ uint4 flag4[OWN ? FEW / 16 : 1];
     uint8_t* const flags = reinterpret_cast<uint8_t*>(flag4);
@@ -653,22 +653,27 @@ __global__ __launch_bounds__(256) void hl_gather(const Prep p) {
     }
     if (tid < r0 % 16) c += held[r0 / 16 * 16 + tid];
     c = wave_sum(c);
-    float top = 0.f;
+    float top = 0.f, low = INFINITY;
     if (last && p.a.g) {
 #pragma unroll 8
         for (int r = tid; r < n; r += 256) {
             const float g = fabsf(p.a.g[r]);
-            top = fmaxf(top, held[r] ? g : 0.f);
+            const bool in = held[r] && g > 0.f && g < INFINITY;  // (an infinite weight stays in its row)
+            top = fmaxf(top, in ? g : 0.f);
+            low = fminf(low, in ? g : INFINITY);
         }
     }
 #pragma unroll
-    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    if (lane == 0) sums[wave] = c, tops[wave] = top;
+    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o)), low = fminf(low, __shfl_xor(low, o));
+    if (lane == 0) sums[wave] = c, tops[wave] = top, lows[wave] = low;
     __syncthreads();
     const int before = sums[0] + sums[1] + sums[2] + sums[3];
     if (last) {
         if (tid == 0) {
             top = p.a.g ? fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) : 1.f;
+            low = fminf(fminf(lows[0], lows[1]), fminf(lows[2], lows[3]));
+            // (weights so far apart that the smallest over the largest would near the smallest float32: as they are)
+            if (p.a.g && !(low > top * 0x1p-40f)) top = 1.f;
             *p.live = before;
             p.top[0] = top;
             p.top[1] = top / p.a.temperature;

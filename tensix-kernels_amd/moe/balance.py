@@ -8,8 +8,9 @@ The reference (XylolabsInc/tensix-kernels) has no counterpart; logits and ids ar
 Over the rows t of a batch (the second last dim; the dims before it are batches, each with a loss of its own: a sequence's,
 or with one batch the whole step's): p[t] = softmax(logits[t]), or with kind "sigmoid" sigmoid(logits[t]) over its sum;
 counts[e] = the slots that chose expert e; loss = sum over e of E counts[e] / sum(counts) * mean over t of p[t][e], which is
-1 where every expert is chosen alike. The counts have no gradient (a choice has none). mask: the rows that count (a padded
-batch); the others enter nothing, whatever their logits and ids hold, and get zeros. An id at or past E chooses no expert.
+1 where every expert is chosen alike. (A row with no logit above -inf, or whose sigmoids are all 0 in float32, has p 0.) The
+counts have no gradient (a choice has none). mask: the rows that count (a padded batch); the others enter nothing, whatever
+their logits and ids hold, and get zeros. An id at or past E chooses no expert.
 
 The kernels are dr_moe_balance's of libdense_reader.so (include/moe.h); nothing goes to the host, and the memory of a call
 is torch's, on the current stream, so a HIP graph can hold balance_loss and balance_loss_grads (autograd's backward refuses

@@ -77,6 +77,15 @@ def test_balance(device, kind, batch, rows, width, experts, k, ids32):
         same("the counts alone", counts, got[1])
 
 
+def test_first_slots_of_wider_ids(device):
+    """Of ids with more slots a row than k (a shared expert's slot behind the picks, say), the first k count."""
+    logits, ids, mask, g = inputs(device, 2, 60, 64, 64, 5, 7, ids32=True)
+    got = balance.balance_loss_grads(logits, ids, 4, g, ids32=True, mask=mask)
+    check("the first four of five", got, expected(logits, ids, 4, "softmax", 64, mask, g))
+    for a, b in zip(got, balance.balance_loss_grads(logits, ids[..., :4].contiguous(), 4, g, ids32=True, mask=mask)):
+        same("the four alone", a, b)
+
+
 def test_rows_that_do_not_count(device):
     """Whatever rows that do not count hold changes nothing; a batch of none gives zeros; so do ids that choose none."""
     logits, ids, mask, g = inputs(device, 3, 50, 64, 64, 4, 1)

@@ -102,7 +102,8 @@ def teacher(n, k, valid, g, device, empty=True):
 
 TOKEN = [(1, 1, 1, 8), (1, 1000, 1000, 64), (2, 257, 257, 72), (33, 999, 998, 520), (64, 8192, 8192, 1024),
          (65, 513, 500, 96), (127, 3000, 3000, 200), (128, 255, 255, 264), (129, 1025, 1024, 64), (300, 2048, 2047, 384),
-         (513, 769, 769, 1000), (1000, 5003, 5000, 128)]
+         (513, 769, 769, 1000), (1000, 5003, 5000, 128),
+         (40, 70001, 70000, 64), (700, 2900, 2899, 520), (2100, 20000, 19999, 72), (70000, 300, 300, 8)]
 
 
 @pytest.mark.parametrize("n, v, valid, d", TOKEN)
@@ -141,6 +142,55 @@ def test_distill(device, n, v, valid, d, k, t):
     if n > 2:
         assert out[0][0] == 0 and out[0][2] == 0 and not out[1][[0, 2]].any()
     same("the loss alone", head_loss.distill_loss(x, head, vals, ids, temperature=t, valid=valid), out[0])
+
+
+@pytest.mark.parametrize("k", [0, 4])
+def test_pieces_of_the_vocabulary(device, k):
+    """So many rows and tokens that the logits' gradient comes in two pieces: dx sums over both, dhead's rows come from each,
+    entries lie in both."""
+    n, v, valid, d = 8200, 66000, 65990, 64
+    x, head, w, g = inputs(device, n, v, d, 20 + k)
+    if k:
+        ids, vals = teacher(n, k, valid, g, device)
+        out = head_loss.distill_loss_grads(x, head, vals, ids, w, valid=valid)
+    else:
+        ids, vals = torch.randint(-valid // 4, valid, (n,), generator=g).to(device.torch), None
+        out = head_loss.token_loss_grads(x, head, ids, w, valid=valid)
+    check(f"pieces, k {k}", out, expected(x, head, ids, vals, 1.0, valid, w))
+
+
+def test_offsets_past_32_bits(device):
+    """A head of more than 2^32 bytes and 2^31 values: the loss against a chunked sum in 64 bits, dhead's last rows against
+    the formula's."""
+    n, v, d = 5, 530_003, 4096
+    x, _, w, g = inputs(device, n, 8, d, 22)
+    gen = torch.Generator(device=device.torch).manual_seed(23)
+    head = torch.empty(v, d, dtype=torch.bfloat16, device=device.torch)
+    step = 32768
+    for i in range(0, v, step):
+        head[i : i + step] = torch.randn(min(step, v - i), d, generator=gen, device=device.torch) * 0.05
+    ids = torch.tensor([v - 1, 0, v - 3, -100, v // 2], device=device.torch)
+    loss, dx, dhead = head_loss.token_loss_grads(x, head, ids, w)
+    z = torch.cat([x.double() @ head[i : i + step].double().T for i in range(0, v, step)], 1)
+    lse = torch.logsumexp(z, 1)
+    on = ids >= 0
+    want = torch.where(on, lse - z.gather(1, ids.clamp(min=0)[:, None])[:, 0], 0.0)
+    ez = (d + 2) * U * (x.double().abs().sum(1) * 0.4)  # (|head| < 0.4)
+    assert float(head.abs().max()) < 0.4
+    within("loss", loss, want, 2 * ez + (4096 + 64) * U + 16 * U * (lse.abs() + z.abs().amax(1)) + 1e-30)
+    dz = (z - lse[:, None]).exp()
+    dz[torch.arange(n, device=device.torch)[on], ids[on]] -= 1
+    dz = dz * torch.where(on, w.double(), 0.0)[:, None]
+    ep = (3 * ez + (4096 + 64) * U + 16 * U * (lse.abs() + z.abs().amax(1)))[:, None] * (dz.abs() + 1e-12)
+    for rows in (slice(0, 300), slice(v - 300, v)):
+        e = ((ep + (B + 4 * U) * (dz.abs() + ep))[:, rows]).T @ x.double().abs() * 1.01
+        val = dz[:, rows].T @ x.double()
+        within(f"dhead rows {rows.start} ..", dhead[rows], val, e + (B + 4 * U) * (val.abs() + e) + 2.0**-133)
+    val = sum(dz[:, i : i + step] @ head[i : i + step].double() for i in range(0, v, step))
+    mag = sum(dz.abs()[:, i : i + step] @ head[i : i + step].double().abs() for i in range(0, v, step))
+    err = sum((ep + (B + 4 * U) * (dz.abs() + ep))[:, i : i + step] @ head[i : i + step].double().abs() for i in range(0, v, step))
+    e = err + (v + 64) * U * 1.01 * mag
+    within("dx", dx, val, e + (B + 4 * U) * (val.abs() + e) + 2.0**-133)
 
 
 def test_every_row_left_out(device):
@@ -206,6 +256,28 @@ def test_masked_vocabulary_and_extremes(device):
     assert loss.isnan().nonzero().tolist() == [[5]]
 
 
+def test_weights(device):
+    """Weights of zero, and of both signs and far apart; an infinite one or a NaN stays in its row's dx."""
+    n, v, d = 40, 300, 64
+    x, head, w, g = inputs(device, n, v, d, 30)
+    ids = torch.randint(0, v, (n,), generator=g).to(device.torch)
+    zero = head_loss.token_loss_grads(x, head, ids, torch.zeros_like(w))
+    assert not zero[1].any() and not zero[2].any() and bool((zero[0] > 0).all())
+    signs = (w - 0.5) * 10.0 ** torch.arange(-20, 20, device=device.torch)
+    out = head_loss.token_loss_grads(x, head, ids, signs)
+    check("weights far apart", (None, out[1], out[2]), expected(x, head, ids, None, 1.0, v, signs))
+    w = w / w.max()
+    want = head_loss.token_loss_grads(x, head, ids, w)[1]
+    top = int(w.argmax())
+    for bad in (float("inf"), float("nan")):
+        odd = w.clone()
+        odd[(top + 1) % n] = bad
+        got = head_loss.token_loss_grads(x, head, ids, odd)[1]
+        rest = torch.arange(n, device=device.torch) != (top + 1) % n
+        same(f"rows beside a weight of {bad}", got[rest], want[rest])
+        assert not torch.isfinite(got[(top + 1) % n]).all()
+
+
 @pytest.mark.parametrize("n", [7, 90])
 def test_layouts(device, n):
     """x as a view with a longer row, off its alignment, transposed, of rank 4; targets of any shape; the head of rank 4."""
@@ -225,7 +297,7 @@ def test_layouts(device, n):
     assert got[0].shape == (1, n) and got[1].shape == (1, 1, n, d) and got[2].shape == (1, 1, v, d)
     for a, b in zip(got, want):
         same("rank 4", a.reshape(b.shape), b)
-    for g1 in (2.0, torch.tensor(2.0, device=device.torch), None):
+    for g1 in (2.0, torch.tensor(2.0, device=device.torch), torch.full((n,), 2.0, dtype=torch.float64, device=device.torch), None):
         a = head_loss.token_loss_grads(x, head, ids, g1)
         b = head_loss.token_loss_grads(x, head, ids, torch.full((n,), 1.0 if g1 is None else 2.0, device=device.torch))
         same("one weight for all", a[2], b[2])
@@ -373,6 +445,8 @@ def test_refusals(device):
         ("temperature NaN", lambda: D(x, head, vals, ti, temperature=float("nan"))),
     ):
         raises(name, AssertionError, fn)
+    odd = torch.empty(300 * 64 + 1, dtype=torch.bfloat16, device=device.torch)[1:].view(300, 64)
+    raises("a head off its alignment", ValueError, lambda: T(x, odd, ids))
 
 
 def test_a_training_step(device):

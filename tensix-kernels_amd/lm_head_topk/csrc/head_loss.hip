@@ -62,6 +62,9 @@ struct Gemm {
     int nb;                 // dhead: the columns that B has (past them zeros)
     long long panel;        // dz lies in panels of 256 v: v at (v / 256) panel + row 256 + v % 256
     const int* live;        // the rows that count: n of z and dx, k of dhead
+    const uint16_t* whole;  // x where it lies ([rows][ldx]), for B of z and A of dhead where every row counts; or NULL
+    long long ldx;
+    int rows;
     int tm, tn, steps;      // tiles; steps of K
     // z's epilogues
     float sc;               // z to the exponent of 2: log2(e) / T
@@ -242,15 +245,19 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void hl_gemm(const Gemm a) {
 
     Tile<BM, AT, NT, BK> ta;
     Tile<BN, BT, NT, BK> tb;
-    const int lda = (int)a.lda, ldb = (int)a.ldb, ra = a.m - m0, rb = nb - n0;  // (rows past the tile's)
+    constexpr bool X_A = EPI == EPI_DHEAD, X_B = EPI == EPI_STATS || EPI == EPI_DZ || EPI == EPI_DZ1;
+    const bool whole = (X_A || X_B) && a.whole && live == a.rows;
+    const uint16_t *A = X_A && whole ? a.whole : a.A, *B = X_B && whole ? a.whole : a.B;
+    const long long la = X_A && whole ? a.ldx : a.lda, lb = X_B && whole ? a.ldx : a.ldb;
+    const int lda = (int)la, ldb = (int)lb, ra = a.m - m0, rb = nb - n0;  // (rows past the tile's)
     ta.init(tid, lda, ra);
     tb.init(tid, ldb, rb);
     // where the next step to be loaded lies, and the k left from it on
     int k = (step0 + group * rounds * NS) * BK;
-    const uint16_t* pa = a.A + (AT ? k * a.lda + m0 : m0 * a.lda + k);
-    const uint16_t* pb = EPI == EPI_DHEAD ? a.B + (n0 >> 8) * a.panel + (n0 & 255) + k * a.ldb
-                         : EPI == EPI_DX  ? a.B + (k >> 8) * a.panel + (k & 255) + n0 * a.ldb
-                                          : a.B + n0 * a.ldb + k;
+    const uint16_t* pa = A + (AT ? k * la + m0 : m0 * la + k);
+    const uint16_t* pb = EPI == EPI_DHEAD ? B + (n0 >> 8) * a.panel + (n0 & 255) + k * lb
+                         : EPI == EPI_DX  ? B + (k >> 8) * a.panel + (k & 255) + n0 * lb
+                                          : B + n0 * lb + k;
     const long long next_panel = a.panel - 256 + BK;
     __amdgpu_buffer_rsrc_t from_a, from_b;
     int left_a, left_b;
@@ -258,8 +265,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void hl_gemm(const Gemm a) {
         left_a = (AT ? ka : k_end) - k, left_b = k_end - k;
         from_a = Tile<BM, AT, NT, BK>::source(pa, lda, AT ? ra : min(BM, ra), left_a);
         from_b = Tile<BN, BT, NT, BK>::source(pb, ldb, BT ? rb : min(BN, rb), left_b);
-        pa += AT ? (long long)BK * a.lda : BK;
-        pb += BT ? (long long)BK * a.ldb : EPI == EPI_DX && (k & 255) == 256 - BK ? next_panel : BK;
+        pa += AT ? BK * la : BK;
+        pb += BT ? BK * lb : EPI == EPI_DX && (k & 255) == 256 - BK ? next_panel : BK;
         k += BK;
     };
     constexpr int NA = CA / NT;
@@ -619,7 +626,8 @@ constexpr int GROWS = 4;     // rows a workgroup of hl_gather, one a wavefront
 constexpr int FEW = 2048;    // entries that every workgroup looks through itself
 
 // The rows that count, one after another: each workgroup finds the place of its own from the flags of all rows before
-// (16 a load), so that nothing waits for anything; one more finds how many there are and the largest |g|. OWN: the entries
+// (16 a load), so that nothing waits for anything; one more finds how many there are and the largest |g|. Where every row
+// counts none is copied. OWN: the entries
 // too, of few rows, every workgroup looking through all of the ids for the flags (a launch less).
 template <bool OWN>
 __global__ __launch_bounds__(256) void hl_gather(const Prep p) {
@@ -635,7 +643,7 @@ __global__ __launch_bounds__(256) void hl_gather(const Prep p) {
     if constexpr (OWN) {
         for (int i = tid; i < FEW / 16; i += 256) flag4[i] = make_uint4(0u, 0u, 0u, 0u);
         __syncthreads();
-        const int upto = min(n, r0 + GROWS) << p.kp, w = 1 << p.kp;
+        const int upto = n << p.kp, w = 1 << p.kp;
         for (int e = tid; e < upto; e += 256) {
             const int row = e >> p.kp, j = e & (w - 1);
             if (j < p.a.k && entry_id(p.a, row, j) >= 0 && (!p.a.vals || p.a.vals[(long long)row * p.a.ld_vals + j] != -INFINITY))
@@ -646,13 +654,17 @@ __global__ __launch_bounds__(256) void hl_gather(const Prep p) {
         if (!last)
             for (int e = tid; e < GROWS << p.kp; e += 256) entries_of(p, (r0 << p.kp) + e, min(n, r0 + GROWS));
     }
-    int c = 0;
-    for (int i = tid; i < r0 / 16; i += 256) {
+    int c = 0, out = 0;  // rows that count before this workgroup's; rows left out, all of them
+    for (int i = tid; i < n / 16; i += 256) {
         const uint4 f = reinterpret_cast<const uint4*>(held)[i];
-        c += __popc(f.x) + __popc(f.y) + __popc(f.z) + __popc(f.w);
+        const int here = __popc(f.x) + __popc(f.y) + __popc(f.z) + __popc(f.w);
+        c += i < r0 / 16 ? here : 0;
+        out += 16 - here;
     }
     if (tid < r0 % 16) c += held[r0 / 16 * 16 + tid];
+    if (tid < n % 16) out += 1 - held[n / 16 * 16 + tid];
     c = wave_sum(c);
+    const bool some = __syncthreads_or(out != 0);
     float top = 0.f, low = INFINITY;
     if (last && p.a.g) {
 #pragma unroll 8
@@ -699,6 +711,7 @@ __global__ __launch_bounds__(256) void hl_gather(const Prep p) {
             return;
         }
         if (lane < 1 << p.kp) p.idc[((long long)at << p.kp) + lane] = p.ids[((long long)(r0 + i) << p.kp) + lane];
+        if (!some) return;  // (every row counts: x is read where it lies)
         const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.a.x) + (r0 + i) * p.a.ldx);
         uint4* dst = reinterpret_cast<uint4*>(p.xc + (long long)at * p.a.dim);
 #pragma unroll 8
@@ -1039,6 +1052,7 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
     z.B = P.gather ? p.xc : reinterpret_cast<const uint16_t*>(a->x);
     z.ldb = P.gather ? a->dim : a->ldx;
     z.n = n, z.k = z.ka = a->dim;
+    z.whole = P.gather ? reinterpret_cast<const uint16_t*>(a->x) : nullptr, z.ldx = a->ldx, z.rows = n;
     z.live = P.gather ? p.live : nullptr;
     z.idx = P.gather ? p.idx : nullptr;
     z.steps = (a->dim + KSTEP - 1) / KSTEP;
@@ -1079,6 +1093,7 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
             if (a->dhead) {
                 Gemm w{};
                 w.A = p.xc, w.lda = a->dim;
+                w.whole = z.whole, w.ldx = z.ldx, w.rows = n;
                 w.B = dz, w.ldb = 256, w.panel = panel;
                 // (the rows past valid: zeros, with the last piece)
                 w.m = a->dim, w.nb = vn, w.n = v0 + vn == a->valid ? a->vocab - v0 : vn, w.k = n, w.live = p.live;

@@ -52,6 +52,14 @@ __device__ __forceinline__ void step_barrier() {
     asm volatile("" ::: "memory");
 }
 
+// two maxima, in the exponent of 2, and sums of what exceeds them
+__device__ __forceinline__ void join(float& m, float& s, float v, float w) {
+    if (v == -INFINITY) return;  // (nothing there)
+    const float top = fmaxf(m, v);
+    s = s * __builtin_amdgcn_exp2f(m - top) + w * __builtin_amdgcn_exp2f(v - top);
+    m = top;
+}
+
 // --- the tiled product ------------------------------------------------------------------------------------------------
 
 struct Gemm {
@@ -73,7 +81,7 @@ struct Gemm {
     const float* lse;       // [rows]
     const float* g;         // [rows], or NULL: ones
     const float* top;       // the factor taken out of dz
-    f32x2* part;            // [m / TM][n] maximum and sum
+    f32x2* part;            // [m / BM][n] maximum and sum
     long long ld_part;
     const int* ids;         // [rows that count][1 << kp] entries, -1 none
     const void* raw;        // or tokens as they came ([rows] int32, or int64: raw64), those past m none
@@ -219,10 +227,11 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void hl_gemm(const Gemm a) {
     constexpr int NW = WM * WN, NT = 64 * NW, TM = BM / WM, TN = BN / WN, MI = TM / 32, NI = TN / 32;
     constexpr int CA = BM * BK / 8, CH = CA + BN * BK / 8;  // chunks of A, a stage
     constexpr int NL = CH / NT;        // loads a lane and stage
-    static_assert(NS == 1 || NS == 2 || NS == 4 || NS == 8, "one stage, two, four or eight");
-    constexpr int CM = NS > 1 ? CH : 1, CL = NS > 2 ? CH : 1, CX = NS > 4 ? CH : 1;
+    static_assert(NS >= 1 && NS <= 4, "one to four stages");
+    constexpr int C1 = NS > 1 ? CH * WK : 1, C2 = NS > 2 ? CH * WK : 1, C3 = NS > 3 ? CH * WK : 1;
     // (an array each, named where it is used: a read waits for the loads to every array that the compiler cannot rule out)
-    __shared__ uint4 s0[CH * WK], s1[CM * WK], s2[CL * WK], s3[CL * WK], s4[CX], s5[CX], s6[CX], s7[CX];
+    __shared__ uint4 s0[CH * WK], s1[C1], s2[C2], s3[C3];
+    __shared__ f32x2 stat[EPI == EPI_STATS ? WM : 1][EPI == EPI_STATS ? BN : 1];
     // WK groups of wavefronts, each a share of K in stages of its own, all with the same barriers; tid within the group
     const int group = WK == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / NT), tid = threadIdx.x - group * NT;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), mine = group * CH;
@@ -287,7 +296,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void hl_gemm(const Gemm a) {
 #pragma unroll
             for (int j = 0; j < NI; ++j) acc[i][j][e] = 0.f;
     }
-    // A step's sums from one stage, the loads of a later step to another, with four stages between the sums: a wavefront that
+    // A step's sums from one stage, the loads of a later step to another, with three stages and more between the sums: a wavefront that
     // issues all of its loads at once stands still until the memory pipeline has taken them, and all do after the barrier.
     // (With two they would land too late for the next step.)
     auto sum = [&](const uint4* b, uint4* to) {
@@ -299,7 +308,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void hl_gemm(const Gemm a) {
             for (int j = 0; j < NI; ++j) fb[j] = Tile<BN, BT, NT, BK>::frag(b, mine + CA, wn * TN + 32 * j, u, lane);
 #pragma unroll
             for (int i = 0; i < MI; ++i) fa[i] = Tile<BM, AT, NT, BK>::frag(b, mine, wm * TM + 32 * i, u, lane);
-            if constexpr (NS >= 4) load(u * NL / U, (u + 1) * NL / U, to);
+            if constexpr (NS >= 3) load(u * NL / U, (u + 1) * NL / U, to);
             else if (NS == 2 && u == 0) load(0, NL, to);
 #pragma unroll
             for (int i = 0; i < MI; ++i)
@@ -315,7 +324,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void hl_gemm(const Gemm a) {
     // (whole rounds of the stages: steps past the last are zeros, as are the loads past the end into stages that nothing
     // reads. A last step of its own behind a branch would have the compiler copy every accumulator.)
     auto step = [&](uint4* to, const uint4* from) {
-        step_barrier<NS >= 4 ? (NS - 2) * NL : 0>();
+        step_barrier<NS >= 3 ? (NS - 2) * NL : 0>();
         next();
         sum(from, to);
     };
@@ -325,8 +334,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void hl_gemm(const Gemm a) {
     };
     if (steps > 0) {
         first(s0);
-        if constexpr (NS >= 4) first(s1), first(s2);
-        if constexpr (NS == 8) first(s3), first(s4), first(s5), first(s6);
+        if constexpr (NS >= 3) first(s1);
+        if constexpr (NS >= 4) first(s2);
     }
     for (int s = 0; s < rounds; ++s) {
         if constexpr (NS == 1) {  // (more workgroups instead)
@@ -339,26 +348,21 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void hl_gemm(const Gemm a) {
         } else if constexpr (NS == 2) {
             step(s1, s0);
             step(s0, s1);
-        } else if constexpr (NS == 4) {
+        } else if constexpr (NS == 3) {
+            step(s2, s0);
+            step(s0, s1);
+            step(s1, s2);
+        } else {
             step(s3, s0);
             step(s0, s1);
             step(s1, s2);
             step(s2, s3);
-        } else {
-            step(s7, s0);
-            step(s0, s1);
-            step(s1, s2);
-            step(s2, s3);
-            step(s3, s4);
-            step(s4, s5);
-            step(s5, s6);
-            step(s6, s7);
         }
     }
     step_barrier<0>();  // (the last loads landed: they write this workgroup's LDS)
     if constexpr (CN == 2) acc[0][0] += odd;
     if constexpr (WK == 2) {  // the second group's sums to the first
-        static_assert(WK == 1 || (MI * NI == 1 && NW * 256 <= CM * WK), "their sums fit a stage");
+        static_assert(WK == 1 || (MI * NI == 1 && NW * 256 <= C1), "their sums fit a stage");
         f32x4* at = reinterpret_cast<f32x4*>(s1) + wave * 256 + lane;
         if (group) {
 #pragma unroll
@@ -426,7 +430,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void hl_gemm(const Gemm a) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) total += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], a.sc, -base));
             total += __shfl_xor(total, 32);
-            if (h == 0 && n < n_end) a.part[(long long)(mt * WM + wm) * a.ld_part + n] = f32x2{top == -INFINITY ? top : base, total};
+            if (h == 0) stat[wm][wn * TN + 32 * j + r] = f32x2{top == -INFINITY ? top : base, total};
             // the entries that lie here: the wavefront's sums of these 32 rows through its own LDS
             f32x4* mine = reinterpret_cast<f32x4*>(region);
             const int here = min(TM, left), w = 1 << a.kp;
@@ -553,6 +557,19 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void hl_gemm(const Gemm a) {
                         *p = v;
                     }
                 }
+        }
+    }
+    if constexpr (EPI == EPI_STATS) {  // the wavefronts' rows of a column together
+        __syncthreads();
+        if (wm == 0 && h == 0) {
+#pragma unroll
+            for (int j = 0; j < NI; ++j) {
+                const int c = wn * TN + 32 * j + r;
+                float m = stat[0][c][0], s = stat[0][c][1];
+#pragma unroll
+                for (int i = 1; i < WM; ++i) join(m, s, stat[i][c][0], stat[i][c][1]);
+                if (n0 + c < n_end) a.part[mt * a.ld_part + n0 + c] = f32x2{m, s};
+            }
         }
     }
 }
@@ -733,14 +750,7 @@ struct Merge {
     float *loss, *lse, *zt;
 };
 
-__device__ __forceinline__ void join(float& m, float& s, float v, float w) {
-    if (v == -INFINITY) return;  // (nothing there)
-    const float top = fmaxf(m, v);
-    s = s * __builtin_amdgcn_exp2f(m - top) + w * __builtin_amdgcn_exp2f(v - top);
-    m = top;
-}
-
-// a row's wavefronts' maxima and sums joined, then lse and loss: TB rows a workgroup of 32 slices (8 of one row)
+// a row's tiles' maxima and sums joined, then lse and loss: TB rows a workgroup of 32 slices (8 of one row)
 template <int TB, int SL>
 __global__ __launch_bounds__(TB* SL) void hl_merge(const Merge p) {
     __shared__ float ms[TB * SL], ss[TB * SL];
@@ -896,11 +906,11 @@ int log2_up(int k) {
     return p;
 }
 
-enum Tiles { T256, T128, T64, T64K, T256x64 };  // (T64K: two groups of wavefronts split K)
+enum Tiles { T256, T128, T64, T64K, T256x64, T128x64 };  // (T64K: two groups of wavefronts split K)
 struct Size {
-    int bm, bn, tm, wk;  // (tm: a wavefront's rows)
+    int bm, bn, wk;
 };
-constexpr Size SIZE[] = {{256, 256, 128, 1}, {128, 128, 64, 1}, {64, 64, 32, 1}, {64, 64, 32, 2}, {256, 64, 128, 1}};
+constexpr Size SIZE[] = {{256, 256, 1}, {128, 128, 1}, {64, 64, 1}, {64, 64, 2}, {256, 64, 1}, {128, 64, 1}};
 
 constexpr Pace pace_of(int epi, int t) { return pace(epi, SIZE[t].bm, SIZE[t].bn, SIZE[t].wk); }
 
@@ -922,10 +932,10 @@ int choose(int epi, long long m, long long n, long long k, std::initializer_list
     return best;
 }
 
-// z's: up to 64 columns take tiles as narrow, of 256 rows where there are enough of them for every CU (32 rows x 128256 x
-// 4096: 176 us, 6 TB/s)
+// z's: up to 64 columns take tiles as narrow, of 128 rows where there are two a CU and more, which then only wait for the head
+// (32 rows x 4096: 131072 tokens 171 us, 6.2 TB/s, 65536 tokens 110; in tiles of 256 rows 174 and 136)
 int choose_z(long long m, long long n, long long k) {
-    if (n <= 64 && tiles_of(T256x64, m, n) >= CUS) return T256x64;
+    if (n <= 64 && tiles_of(T128x64, m, n) >= 2 * CUS) return T128x64;
     return n <= 64 ? choose(EPI_DZ, m, n, k, {T64, T64K}) : choose(EPI_DZ, m, n, k, {T256, T128, T64, T64K});
 }
 
@@ -941,7 +951,7 @@ bool plan_of(const dr_head_loss* a, int what, Plan& p) {
     if (up(a->valid, 64) / 64 * (np / 64) > 1 << 30) return false;  // (tiles a launch counts)
     p.kp = log2_up(a->k);
     p.z = choose_z(a->valid, n, a->dim);
-    p.parts = (int)(up(a->valid, SIZE[p.z].bm) / SIZE[p.z].tm);
+    p.parts = (int)(up(a->valid, SIZE[p.z].bm) / SIZE[p.z].bm);
     // (forward alone, the rows that count are gathered where leaving out the others may save more than that takes, about 10 us)
     p.gather = back || (double)n * a->valid * a->dim > 3e10;
     p.raw = !p.gather && a->vals == nullptr;  // (tokens read where they are: no launch before z's)
@@ -999,7 +1009,7 @@ void launch_z(const Gemm& g, int t, hipStream_t st) {
     switch (t) {
         case T256: return launch<256, 256, 2, 4, 1, 2, 64, false, false, EPI>(g, st);
         case T128: return launch<128, 128, 2, 2, 1, 2, 64, false, false, EPI>(g, st);
-        case T256x64: return launch<256, 64, 2, 2, 1, 2, 64, false, false, EPI>(g, st);
+        case T128x64: return launch<128, 64, 2, 2, 1, 3, 64, false, false, EPI>(g, st);
         case T64: return launch<64, 64, 2, 2, 1, 4, 64, false, false, EPI>(g, st);
         default: return launch<64, 64, 2, 2, 2, 4, 64, false, false, EPI>(g, st);
     }

@@ -5,10 +5,16 @@
 //   z  [v][n]  = head . x^T      summed over dim;    the softmax's statistics, or dz, are its epilogue
 //   dhead [v][d] = dz^T . x      summed over rows;   x and dz across
 //   dx [n][d]  = dz . head       summed over v;      head across
-// A call is a few launches: the entries (ids checked, the teacher's softmax), the rows that count gathered into a
-// contiguous x (rows left out cost nothing and whatever they hold enters no sum), z with each wavefront's maximum and sum
-// of a row, their merge into lse and loss; backward, piece by piece of the vocabulary, dz from z computed again, the
-// entries' own dz, dhead's rows, dx's sum so far.
+// A call is a few launches: the entries (ids checked, the teacher's softmax), the rows that count found (and gathered, where
+// some do not: rows left out cost nothing and whatever they hold enters no sum), z with each tile's maximum and sum of a row,
+// their merge into lse and loss; backward, piece by piece of the vocabulary, dz from z computed again, a teacher's entries' own
+// dz, dhead's rows, dx's sum so far. The logits are never kept: that is one product more than a program that keeps them.
+//
+// What bounds them (8192 rows x 4096 against 128256 tokens, 27.3 ms; a large library product of the same layouts runs at 1200,
+// 985 and 1110 TFLOP/s): z 7.05 ms (1220 TFLOP/s), dz 7.16 (1200), dhead 6.69 (1286), dx 6.85 (1256). With zeros for inputs
+// the same kernels run at 1530 to 1790 TFLOP/s and 2.4 GHz: the power that random values draw, at 1.8 GHz, holds them there.
+// 32 rows: 176 us for the 1.05 GB of the head, 6.0 TB/s. A few rows against a small vocabulary: each launch's start, its first
+// loads and a chain of LDS reads and matrix instructions (48 x 1024 against 8192: 7 launches of 4 to 9 us).
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -73,7 +79,7 @@ struct Gemm {
     const uint16_t* whole;  // x where it lies ([rows][ldx]), for B of z and A of dhead where every row counts; or NULL
     long long ldx;
     int rows;
-    int tm, tn, steps;      // tiles; steps of K
+    int tm, tn;             // tiles
     // z's epilogues
     float sc;               // z to the exponent of 2: log2(e) / T
     int v0;                 // z's row 0 is the vocabulary's v0
@@ -222,6 +228,19 @@ __device__ __forceinline__ bool tile_of(int tm, int tn, int splits, int& mt, int
     return true;
 }
 
+// D[m][n] in tiles of BM x BN, a wavefront BM / WM x BN / WN of 32x32x16 matrix instructions; NS stages of BK k in LDS, filled
+// straight from memory.
+// - 256 x 256 by 8 wavefronts: the largest that the registers hold, so the fewest bytes into a CU for each operation. Its
+//   operands along k (z) come in steps of 64, a whole 128-byte line of a row, two stages; those across (dhead, dx) in four
+//   stages of 32 k, which leaves the loads three steps: dhead 1270 -> 1305 TFLOP/s, z the other way round (1210 to 1284 in two
+//   stages of 64, 1194 to 1241 in four of 32). 4 wavefronts of 128 x 128 read a third less LDS, but nothing runs beside them
+//   (1190 to 1270); 256 x 128 twice a CU 950 to 1060; fragments read a step ahead or wave priorities change nothing.
+//   (8192 x 4096 x 16384.)
+// - 128 x 128 and 64 x 64, twice a CU, where larger tiles would leave CUs idle (choose); 64 x 64 also by two groups of
+//   wavefronts that split K, where there is at most one tile a CU.
+// - 128 x 64 for up to 64 rows of x: the head is read once, at the memory's rate.
+// The epilogues' bf16 leave through LDS in whole runs of a row (with that and dz in panels dhead of 64128 tokens went from 4840
+// to 4593 us).
 template <int BM, int BN, int WM, int WN, int WK, int NS, int BK, bool AT, bool BT, int EPI>
 __global__ __launch_bounds__(64 * WM * WN * WK) void hl_gemm(const Gemm a) {
     constexpr int NW = WM * WN, NT = 64 * NW, TM = BM / WM, TN = BN / WN, MI = TM / 32, NI = TN / 32;
@@ -1065,7 +1084,6 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
     z.whole = P.gather ? reinterpret_cast<const uint16_t*>(a->x) : nullptr, z.ldx = a->ldx, z.rows = n;
     z.live = P.gather ? p.live : nullptr;
     z.idx = P.gather ? p.idx : nullptr;
-    z.steps = (a->dim + KSTEP - 1) / KSTEP;
     z.sc = LOG2E / a->temperature;
     z.ids = P.gather ? p.idc : p.ids, z.kp = P.kp, z.kn = kn;
     z.raw = P.raw ? a->ids : nullptr, z.raw64 = a->ids64;
@@ -1086,7 +1104,7 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
         uint16_t* dz = reinterpret_cast<uint16_t*>(ws + P.dz);
         const long long panel = (long long)n * 256;
         for (int v0 = 0; v0 < a->valid; v0 += P.piece) {
-            const int vn = a->valid - v0 < P.piece ? a->valid - v0 : P.piece, vp = (int)up(vn, 256);
+            const int vn = a->valid - v0 < P.piece ? a->valid - v0 : P.piece;
             Gemm s = z;
             s.A += (long long)v0 * a->ld_head;
             s.m = vn;
@@ -1107,7 +1125,6 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
                 w.B = dz, w.ldb = 256, w.panel = panel;
                 // (the rows past valid: zeros, with the last piece)
                 w.m = a->dim, w.nb = vn, w.n = v0 + vn == a->valid ? a->vocab - v0 : vn, w.k = n, w.live = p.live;
-                w.steps = (n + KSTEP - 1) / KSTEP;
                 w.out = reinterpret_cast<uint16_t*>(a->dhead) + (long long)v0 * a->ld_dhead;
                 w.ld_out = a->ld_dhead;
                 w.scale = p.top + 1;
@@ -1120,7 +1137,7 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
                 d.A = z.A + (long long)v0 * a->ld_head, d.lda = a->ld_head;
                 d.B = dz, d.ldb = 256, d.panel = panel;
                 d.m = a->dim, d.n = n, d.k = (int)up(vn, 8), d.ka = vn, d.live = p.live;
-                d.steps = vp / KSTEP, d.plan_steps = P.piece / KSTEP;
+                d.plan_steps = P.piece / KSTEP;
                 d.acc = reinterpret_cast<float*>(ws + P.acc);
                 d.ld_acc = a->dim;
                 d.add = v0 > 0;

@@ -623,12 +623,13 @@ __device__ __forceinline__ bool entries_of(const Prep& p, int e, int rows) {
     const bool in = row < rows && j < p.a.k;
     int id = in ? entry_id(p.a, row, j) : -1;
     if (p.a.vals) {
-        float v = in ? p.a.vals[(long long)row * p.a.ld_vals + j] / p.a.temperature : -INFINITY;
+        // (the temperature after the difference: the type's lowest value, at a temperature below 1, is still no empty slot)
+        float v = in ? p.a.vals[(long long)row * p.a.ld_vals + j] : -INFINITY;
         if (v == -INFINITY) id = -1;
         if (id < 0) v = -INFINITY;
         float top = v;
         for (int o = w >> 1; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-        const float d = id < 0 ? 0.f : v - top;
+        const float d = id < 0 ? 0.f : (v - top) / p.a.temperature;
         const float x = id < 0 ? 0.f : __expf(d);
         float total = x;
         for (int o = w >> 1; o; o >>= 1) total += __shfl_xor(total, o);

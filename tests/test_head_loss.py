@@ -256,6 +256,23 @@ def test_masked_vocabulary_and_extremes(device):
     assert loss.isnan().nonzero().tolist() == [[5]]
 
 
+@pytest.mark.parametrize("n", [20, 700])
+def test_teacher_of_lowest_values(device, n):
+    """The type's lowest value, at a temperature that takes it past float32, is an entry of probability 0, and a row of
+    nothing else one of equal probabilities: bit by bit what the same entries give with a value of little and of 0."""
+    x, head, w, g = inputs(device, n, 500, 64, n)
+    ids, vals = teacher(n, 8, 500, g, device, empty=False)
+    plain = vals.clone()
+    low = torch.rand(n, 8, generator=g).to(device.torch) < 0.5
+    low[:, 0], low[3], low[n - 1] = False, True, True
+    vals[low], plain[low] = torch.finfo(torch.float32).min, -200.0  # (exp(-200 / 0.5) is 0 in float32 and below any bound)
+    plain[3] = plain[n - 1] = 0.0
+    want = head_loss.distill_loss_grads(x, head, plain, ids, w, temperature=0.5)
+    check(f"lowest values, {n} rows", want, expected(x, head, ids, plain, 0.5, 500, w))
+    for part, a, b in zip(("loss", "dx", "dhead"), head_loss.distill_loss_grads(x, head, vals, ids, w, temperature=0.5), want):
+        same(part, a, b)
+
+
 def test_weights(device):
     """Weights of zero, and of both signs and far apart; an infinite one or a NaN stays in its row's dx."""
     n, v, d = 40, 300, 64

@@ -449,7 +449,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void hl_gemm(const Gemm a) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) total += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], a.sc, -base));
             total += __shfl_xor(total, 32);
-            if (h == 0) stat[wm][wn * TN + 32 * j + r] = f32x2{top == -INFINITY ? top : base, total};
+            // (no sum: nothing there; a NaN with nothing else beside it is something)
+            if (h == 0) stat[wm][wn * TN + 32 * j + r] = f32x2{total == 0.f ? -INFINITY : base, total};
             // the entries that lie here: the wavefront's sums of these 32 rows through its own LDS
             f32x4* mine = reinterpret_cast<f32x4*>(region);
             const int here = min(TM, left), w = 1 << a.kp;

@@ -256,6 +256,21 @@ def test_masked_vocabulary_and_extremes(device):
     assert loss.isnan().nonzero().tolist() == [[5]]
 
 
+@pytest.mark.parametrize("n", [1, 40, 100, 1000])
+def test_a_row_of_nan_in_the_head(device, n):
+    """A NaN in one row of the head is in every row's loss, also where that row is alone in its tile."""
+    x, head, w, g = inputs(device, n, 2049, 64, n)
+    ids = torch.randint(0, 64, (n,), generator=g).to(device.torch)
+    head[64], head[256], head[2048] = 0.0, 0.0, 0.0
+    for valid in (65, 257, 2049):
+        assert not head_loss.token_loss(x, head, ids, valid=valid).isnan().any()
+        head[valid - 1] = float("nan")
+        assert bool(head_loss.token_loss(x, head, ids, valid=valid).isnan().all()), valid
+        loss, dx, _ = head_loss.token_loss_grads(x, head, ids, valid=valid)
+        assert bool(loss.isnan().all()) and bool(dx.isnan().all()), valid
+        head[valid - 1] = 0.0
+
+
 @pytest.mark.parametrize("n", [20, 700])
 def test_teacher_of_lowest_values(device, n):
     """The type's lowest value, at a temperature that takes it past float32, is an entry of probability 0, and a row of

@@ -61,15 +61,18 @@ __device__ __forceinline__ void row_load(const Bal& b, long long row, int l, flo
     }
 }
 
-// the row's p from its logits, in place (0 past the experts); a row of no expert above -inf has p 0
+// the row's p from its logits, in place (0 past the experts); a row of no expert above -inf has p 0. down: 1 less the sigmoid,
+// as a product, which keeps its accuracy where the sigmoid nears 1.
 template <int L, int N, bool SIG>
-__device__ __forceinline__ void row_p(float (&p)[4 * N], float (&s)[SIG ? 4 * N : 1]) {
+__device__ __forceinline__ void row_p(float (&p)[4 * N], float (&down)[SIG ? 4 * N : 1]) {
     float total = 0.f;
     if constexpr (SIG) {
 #pragma unroll
         for (int i = 0; i < 4 * N; ++i) {
-            s[i] = __builtin_amdgcn_rcpf(1.f + __expf(-p[i]));
-            total += s[i];
+            const float x = __expf(-p[i]);
+            p[i] = __builtin_amdgcn_rcpf(1.f + x);
+            down[i] = x == INFINITY ? 1.f : x * p[i];
+            total += p[i];
         }
     } else {
         float top = p[0];
@@ -86,7 +89,7 @@ __device__ __forceinline__ void row_p(float (&p)[4 * N], float (&s)[SIG ? 4 * N 
     total = sum_over<L>(total);
     const float inv = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
-    for (int i = 0; i < 4 * N; ++i) p[i] = (SIG ? s[i] : p[i]) * inv;
+    for (int i = 0; i < 4 * N; ++i) p[i] *= inv;
 }
 
 __device__ __forceinline__ bool row_counts(const dr_balance& a, long long row) { return a.mask == nullptr || a.mask[row] != 0; }
@@ -111,7 +114,7 @@ __global__ __launch_bounds__(T) void balance_sum_k(const Bal b) {
     for (int r0 = g * R; r0 < a.rows; r0 += b.groups * R) {
         const int r = min(r0 + tid / L, a.rows - 1);  // (the last row again: every lane takes part in the butterflies)
         const long long row = (long long)batch * a.rows + r;
-        float p[4 * N], s[SIG ? 4 * N : 1];
+        float p[4 * N], down[SIG ? 4 * N : 1];
 #pragma unroll
         for (int i = 0; i < 4 * N; ++i) p[i] = z[i];
         row_load<L, N>(b, (long long)batch * a.rows + min(r + b.groups * R, a.rows - 1), l, z);
@@ -121,7 +124,7 @@ __global__ __launch_bounds__(T) void balance_sum_k(const Bal b) {
             id = a.ids32 ? reinterpret_cast<const uint32_t*>(a.ids)[at] : reinterpret_cast<const uint16_t*>(a.ids)[at];
         }
         const bool on = r0 + tid / L < a.rows && row_counts(a, row);
-        row_p<L, N, SIG>(p, s);
+        row_p<L, N, SIG>(p, down);
 #pragma unroll
         for (int i = 0; i < 4 * N; ++i) sum[i] += on ? p[i] : 0.f;
         n += on;
@@ -253,11 +256,11 @@ __global__ __launch_bounds__(T) void balance_grad_k(const Bal b) {
         const int r = min(r0 + tid / L, a.rows - 1);
         const long long row = (long long)batch * a.rows + r;
         const bool on = row_counts(a, row);
-        float p[4 * N], s[SIG ? 4 * N : 1];
+        float p[4 * N], down[SIG ? 4 * N : 1];
 #pragma unroll
         for (int i = 0; i < 4 * N; ++i) p[i] = z[i];
         row_load<L, N>(b, (long long)batch * a.rows + min(r + b.groups * R, a.rows - 1), l, z);
-        row_p<L, N, SIG>(p, s);
+        row_p<L, N, SIG>(p, down);
         float mean = 0.f;
 #pragma unroll
         for (int i = 0; i < 4 * N; ++i) mean += p[i] * f[i];
@@ -271,7 +274,7 @@ __global__ __launch_bounds__(T) void balance_grad_k(const Bal b) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int q = 4 * i + c;
-                o[c] = on ? scale * (SIG ? p[q] * (1.f - s[SIG ? q : 0]) : p[q]) * (f[q] - mean) : 0.f;
+                o[c] = on ? scale * (SIG ? p[q] * down[SIG ? q : 0] : p[q]) * (f[q] - mean) : 0.f;
             }
             if (b.gvec && e + 4 <= a.experts) {
                 *reinterpret_cast<float4*>(d + e) = make_float4(o[0], o[1], o[2], o[3]);

@@ -116,6 +116,25 @@ def test_extreme_logits(device, kind):
     assert bad[1].isnan() and torch.equal(bad[0], got[0][0])
 
 
+def test_gradients_of_large_sigmoids(device):
+    """Where the sigmoid nears 1, its slope keeps float32's accuracy: off by its own roundings alone."""
+    logits, ids, mask, g = inputs(device, 2, 40, 32, 32, 4, 8)
+    logits = logits.abs() + 10
+    logits[0, 3, 5], logits[1, 4, 6] = 100.0, -torch.inf
+    loss, eloss, counts, d, _ = expected(logits, ids, 4, "sigmoid", 32, mask, g)
+    got = balance.balance_loss_grads(logits, ids, 4, g, kind="sigmoid", mask=mask)
+    s = torch.sigmoid(logits.double())
+    down = torch.sigmoid(-logits.double())
+    f = (32 * counts.double() / counts.sum(1, keepdim=True))[:, None]
+    p = s / s.sum(-1, keepdim=True)
+    rows = mask.sum(1).double()[:, None, None]
+    scale = g.double()[:, None, None] / rows * mask[..., None]
+    mean = (p * f).sum(-1, keepdim=True)
+    # (the exponent's argument |z| u, and what rel and expected's bounds count)
+    rel = 3 * (32 + 64 + 4 * logits[logits.isfinite()].double().abs().amax()) * U
+    within("dlogits", got[2], scale * p * down * (f - mean), scale * p * down * (f + mean) * rel + 1e-37)
+
+
 def test_shapes_autograd_and_differences(device):
     logits, ids, mask, g = inputs(device, 1, 30, 96, 96, 4, 3)
     flat = logits[0].clone().requires_grad_()

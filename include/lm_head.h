@@ -74,7 +74,7 @@ typedef struct dr_head_loss {
     int64_t ldx;
     const void* head;     /* [vocab][ld_head] bf16, 16-byte aligned, ld_head a multiple of 8 */
     int64_t ld_head;
-    int32_t rows, dim;    /* dim a multiple of 8 */
+    int32_t rows, dim;    /* rows to 2^20, dim a multiple of 8; rows * valid to about 2^39 */
     int32_t vocab, valid; /* 1 <= valid <= vocab: the head's rows that take part */
     const void* ids;      /* [rows][ld_ids] int32, or int64 (ids64) */
     int64_t ld_ids;

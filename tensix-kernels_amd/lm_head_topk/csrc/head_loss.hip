@@ -910,6 +910,7 @@ __global__ __launch_bounds__(256) void hl_dx(const Finish p) {
 // --- the plan ----------------------------------------------------------------------------------------------------------
 
 constexpr long long DZ_BYTES = 1ll << 30;  // dz a piece at most
+constexpr int MOST_TILES = (1 << 23) - 8;  // of 512 lanes: a launch holds fewer than 2^32
 
 long long up(long long v, long long to) { return (v + to - 1) / to * to; }
 
@@ -969,9 +970,10 @@ bool plan_of(const dr_head_loss* a, int what, Plan& p) {
         return false;
     const bool back = what & DR_LOSS_BACKWARD;
     const long long n = a->rows, np = up(n, 64);
-    if (up(a->valid, 64) / 64 * (np / 64) > 1 << 30) return false;  // (tiles a launch counts)
+    if (up(a->valid, 64) / 64 * (np / 64) > 1 << 30) return false;  // (tiles counted in 32 bits)
     p.kp = log2_up(a->k);
     p.z = choose_z(a->valid, n, a->dim);
+    if (tiles_of(p.z, a->valid, n) >= MOST_TILES) return false;
     p.parts = (int)(up(a->valid, SIZE[p.z].bm) / SIZE[p.z].bm);
     // (forward alone, the rows that count are gathered where leaving out the others may save more than that takes, about 10 us)
     p.gather = back || (double)n * a->valid * a->dim > 3e10;

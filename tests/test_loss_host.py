@@ -80,6 +80,16 @@ def test_head_loss_refuses_what_it_does_not_know():
     assert _lib.lib().dr_head_loss_workspace_bytes(ctypes.byref(_head()), 1) > 0
 
 
+def test_head_loss_refuses_more_tiles_than_a_launch_holds():
+    """A launch holds fewer than 2^32 lanes: more rows and tokens than that are refused before any of its kernels runs."""
+    ask = _lib.lib().dr_head_loss_workspace_bytes
+    for rows, valid, ok in ((1 << 20, 1 << 18, True), (1 << 19, 1 << 23, False), (1 << 20, 1 << 20, False), (64, 1 << 28, True)):
+        A = _head(rows=rows, dim=8, ldx=8, ld_head=8, ld_dx=8, ld_dhead=8, vocab=valid, valid=valid, workspace_bytes=1 << 62)
+        assert (ask(ctypes.byref(A), 1) > 0) == ok, (rows, valid)
+        if not ok:
+            assert _lib.lib().dr_head_loss_run(ctypes.byref(A), 1) == _lib.DR_EINVAL, (rows, valid)
+
+
 def test_head_loss_workspace_keeps_no_logits():
     """The backward's workspace holds a piece of the logits' gradient, never all of it: with eight times the vocabulary it
     stays the same; nor does the forward's hold the logits."""

@@ -82,7 +82,7 @@ typedef struct dr_head_loss {
     int32_t k;            /* entries a row, 1 .. DR_LOSS_MAX_K */
     const float* vals;    /* [rows][ld_vals] the teacher's logits, or NULL: tokens (k 1) */
     int64_t ld_vals;
-    float temperature;    /* T > 0, finite (tokens: 1) */
+    float temperature;    /* T from 2^-20 on, finite (tokens: 1) */
     float* loss;          /* [rows] */
     float* lse;           /* [rows] */
     float* logits;        /* [rows][k]: z at the entries (0 where none is held) */

@@ -71,7 +71,7 @@ class _Call:
         assert ids.device == device and rows_t.device == device, (ids.device, rows_t.device, device)
         self.ids = ids.contiguous()
         self.temperature = float(temperature)
-        assert 0 < self.temperature < math.inf, f"head_loss: temperature {temperature}"
+        assert 2.0**-20 <= self.temperature < math.inf, f"head_loss: temperature {temperature}"
 
     def empty(self, *shape, dtype=torch.float32):
         return torch.empty(shape, dtype=dtype, device=self.device)
@@ -190,7 +190,7 @@ def distill_loss(x, rows_t, vals, ids, temperature=1.0, valid=None):
     teacher's q = softmax(vals / temperature) over the row's entries: float32, differentiable in x and rows_t. vals [..., k]
     float32 and ids [..., k] int32, k to 64: as linear.topk_merge leaves them (-inf and -1 in empty slots), of a teacher
     of this vocabulary; an id outside 0 .. valid - 1 is an empty slot too, one that comes twice counts twice, and a row of
-    empty slots is left out."""
+    empty slots is left out. temperature: from 2^-20 on (a probability is off by |logit| / temperature * 2^-23 of itself)."""
     return _loss(x, rows_t, ids, vals, temperature, valid)
 
 

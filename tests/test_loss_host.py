@@ -80,6 +80,15 @@ def test_head_loss_refuses_what_it_does_not_know():
     assert _lib.lib().dr_head_loss_workspace_bytes(ctypes.byref(_head()), 1) > 0
 
 
+@pytest.mark.parametrize("t", [2.0**-21, 1e-39, 1e-50])
+def test_head_loss_refuses_temperatures_without_an_inverse(t):
+    A = _head(vals=4096, k=4, ld_ids=4, ld_vals=4, temperature=t)
+    for what in (1, 2, 3):
+        assert _lib.lib().dr_head_loss_run(ctypes.byref(A), what) == _lib.DR_EINVAL, t
+    A.temperature = 2.0**-20
+    assert _lib.lib().dr_head_loss_workspace_bytes(ctypes.byref(A), 3) > 0
+
+
 def test_head_loss_refuses_more_tiles_than_a_launch_holds():
     """A launch holds fewer than 2^32 lanes: more rows and tokens than that are refused before any of its kernels runs."""
     ask = _lib.lib().dr_head_loss_workspace_bytes

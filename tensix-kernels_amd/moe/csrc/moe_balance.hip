@@ -301,6 +301,7 @@ int groups_of(const dr_balance* a) {
 bool valid(const dr_balance* a, int what) {
     return a != nullptr && what >= 1 && what <= 3 && a->batch >= 1 && a->batch <= (1 << 16) && a->rows >= 1 &&
            (long long)a->batch * a->rows < (1ll << 30) && a->experts >= 1 && a->experts <= MAXE && a->k >= 1 && a->k <= 16 &&
+           (long long)a->rows * a->k < (1ll << 31) &&  // (the counts are int32)
            a->width >= a->experts && a->ld_logits >= a->width && a->ld_ids >= a->k && (a->kind == 0 || a->kind == 1);
 }
 

@@ -124,7 +124,7 @@ def _balance(**kw):
 @pytest.mark.parametrize("bad", [
     dict(batch=0), dict(batch=65537), dict(rows=0), dict(rows=1 << 30), dict(experts=0), dict(experts=1025, width=1025,
     ld_logits=1025, ld_dlogits=1025), dict(experts=33), dict(width=33), dict(k=0), dict(k=5), dict(k=17, ld_ids=17),
-    dict(kind=2), dict(kind=-1),
+    dict(kind=2), dict(kind=-1), dict(batch=1, rows=1 << 27, k=16, ld_ids=16),
 ])
 def test_balance_refuses_sizes(bad):
     A = _balance(**bad)

@@ -137,7 +137,7 @@ typedef struct dr_balance {
     const float* g;        /* [batch], or NULL: ones */
     float* dlogits;        /* [batch * rows][ld_dlogits]; rows that do not count get zeros */
     int64_t ld_dlogits;
-    void* workspace;       /* dr_moe_balance_workspace_bytes, 256-byte aligned; its contents mean nothing between calls */
+    void* workspace;       /* dr_moe_balance_workspace_bytes (0: not read), 256-byte aligned; it keeps nothing between calls */
     int64_t workspace_bytes;
     void* stream;
 } dr_balance;

@@ -74,7 +74,7 @@ class _Call:
         assert 2.0**-20 <= self.temperature < math.inf, f"head_loss: temperature {temperature}"
 
     def empty(self, *shape, dtype=torch.float32):
-        return torch.empty(shape, dtype=dtype, device=self.device)
+        return torch.empty(*shape or ((),), dtype=dtype, device=self.device)
 
     def outputs(self):
         """(loss, lse, logits) to be filled, and kept for a backward pass."""
@@ -103,12 +103,14 @@ class _Call:
             if dhead is not None:
                 dhead.zero_()
             return
-        ptr = torch.Tensor.data_ptr
+
+        def ptr(t):
+            return None if t is None else t.data_ptr()
+
         A = _lib.HeadLoss(
             self.x.data_ptr(), self.x.stride(0) if n > 1 else dim, self.rows_t.data_ptr(), dim, n, dim, self.vocab,
-            self.valid, self.ids.data_ptr(), k, self.ids.dtype == torch.int64, k, None if self.vals is None else ptr(self.vals), k,
-            self.temperature, *(None if t is None else ptr(t) for t in (loss, lse, logits, g, dx)), dim,
-            None if dhead is None else ptr(dhead), dim)
+            self.valid, self.ids.data_ptr(), k, self.ids.dtype == torch.int64, k, ptr(self.vals), k, self.temperature,
+            ptr(loss), ptr(lse), ptr(logits), ptr(g), ptr(dx), dim, ptr(dhead), dim)
         ref = ctypes.byref(A)
         lib = _lib.lib()
         need = lib.dr_head_loss_workspace_bytes(ref, what)

@@ -60,11 +60,10 @@ def _run(logits, ids, k, g, kind, ids32, experts, mask, grad):
         if gs.dtype != torch.float32 or gs.numel() != batch or not gs.is_contiguous():
             gs = gs.detach().reshape(-1).to(torch.float32).expand(batch).contiguous()
 
-    def new(*shape, dtype=torch.float32):
-        return torch.empty(shape, dtype=dtype, device=logits.device)
-
-    loss, counts = new(*lead), new(*lead, E, dtype=torch.int32)
-    dlogits = new(*logits.shape) if grad else None
+    device = logits.device
+    loss = torch.empty(lead, dtype=torch.float32, device=device)
+    counts = torch.empty((*lead, E), dtype=torch.int32, device=device)
+    dlogits = torch.empty_like(lg) if grad else None
     if batch * R == 0:
         loss.zero_(), counts.zero_()
         return loss, counts, dlogits
@@ -77,12 +76,14 @@ def _run(logits, ids, k, g, kind, ids32, experts, mask, grad):
     lib = _lib.lib()
     need = lib.dr_moe_balance_workspace_bytes(ref, what)
     _lib.check(_lib.DR_EINVAL if need < 0 else _lib.DR_OK, "dr_moe_balance_workspace_bytes")
-    ws = new(need, dtype=torch.uint8)
-    A.workspace, A.workspace_bytes, A.stream = ptr(ws), need, dev.raw_stream(logits.device)
-    if logits.device.index == torch.cuda.current_device():
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        A.workspace, A.workspace_bytes = ptr(ws), need
+    A.stream = dev.raw_stream(device)
+    if device.index == torch.cuda.current_device():
         st = lib.dr_moe_balance(ref, what)
     else:  # (a launch goes to the current device)
-        with torch.cuda.device(logits.device):
+        with torch.cuda.device(device):
             st = lib.dr_moe_balance(ref, what)
     if st != _lib.DR_OK:
         _lib.check(st, "dr_moe_balance")

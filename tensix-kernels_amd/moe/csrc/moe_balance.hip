@@ -7,6 +7,8 @@
 //   balance_sum_k   a workgroup's rows: the sum of p and the counts (LDS), written for the workgroup
 //   balance_grad_k  every workgroup joins the workgroups' sums for itself, in order (cheaper than a launch of its own in
 //                   between), then the logits' gradient of its rows, p computed again; balance_join_k: the join alone
+//   balance_one_k   all of it by one workgroup, a batch of few rows or one of many batches: one launch and no memory between
+//                   (32 rows x 32 experts: 5.2 us in a graph, two launches 8.2; called eagerly 11.8 and 16.0, all of it the host's)
 // What bounds it: the logits read twice and the gradient written once; at a few rows the launches.
 
 #include <hip/hip_runtime.h>
@@ -94,16 +96,20 @@ __device__ __forceinline__ void row_p(float (&p)[4 * N], float (&down)[SIG ? 4 *
 
 __device__ __forceinline__ bool row_counts(const dr_balance& a, long long row) { return a.mask == nullptr || a.mask[row] != 0; }
 
+// a workgroup's rows in LDS: cnt, and by wavefront the sum of p and the rows that count
+template <int L, int N>
+struct Sums {
+    int cnt[L * 4 * N];
+    float p[W][L * 4 * N];
+    int rows[W];
+};
+
 template <int L, int N, bool SIG>
-__global__ __launch_bounds__(T) void balance_sum_k(const Bal b) {
+__device__ __forceinline__ void sum_rows(const Bal& b, int g, int batch, Sums<L, N>& S) {
     constexpr int R = T / L;  // rows at once
-    __shared__ int cnt[L * 4 * N];
-    __shared__ float ps[W][L * 4 * N];
-    __shared__ int rows[W];
     const dr_balance& a = b.a;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l = tid % L;
-    const int g = blockIdx.x % b.groups, batch = blockIdx.x / b.groups;
-    for (int e = tid; e < a.experts; e += T) cnt[e] = 0;
+    for (int e = tid; e < a.experts; e += T) S.cnt[e] = 0;
     __syncthreads();
     float sum[4 * N];
 #pragma unroll
@@ -128,7 +134,7 @@ __global__ __launch_bounds__(T) void balance_sum_k(const Bal b) {
 #pragma unroll
         for (int i = 0; i < 4 * N; ++i) sum[i] += on ? p[i] : 0.f;
         n += on;
-        if (on && id < (uint32_t)a.experts) atomicAdd(&cnt[id], 1);
+        if (on && id < (uint32_t)a.experts) atomicAdd(&S.cnt[id], 1);
     }
     // the wavefront's rows, then the workgroup's, in order
 #pragma unroll
@@ -141,20 +147,28 @@ __global__ __launch_bounds__(T) void balance_sum_k(const Bal b) {
     if (lane < L) {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            *reinterpret_cast<float4*>(&ps[wave][4 * (l + L * i)]) =
+            *reinterpret_cast<float4*>(&S.p[wave][4 * (l + L * i)]) =
                 make_float4(sum[4 * i], sum[4 * i + 1], sum[4 * i + 2], sum[4 * i + 3]);
     }
-    if (lane == 0) rows[wave] = n;
+    if (lane == 0) S.rows[wave] = n;
     __syncthreads();
+}
+
+template <int L, int N, bool SIG>
+__global__ __launch_bounds__(T) void balance_sum_k(const Bal b) {
+    __shared__ __attribute__((aligned(16))) Sums<L, N> S;
+    const dr_balance& a = b.a;
+    const int tid = threadIdx.x, g = blockIdx.x % b.groups, batch = blockIdx.x / b.groups;
+    sum_rows<L, N, SIG>(b, g, batch, S);
     for (int e = tid; e < a.experts; e += T) {
         float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < W; ++w) v += ps[w][e];
-        b.sums[(long long)blockIdx.x * a.experts + e] = make_float2(v, __int_as_float(cnt[e]));
+        for (int w = 0; w < W; ++w) v += S.p[w][e];
+        b.sums[(long long)blockIdx.x * a.experts + e] = make_float2(v, __int_as_float(S.cnt[e]));
     }
     if (tid == 0) {
         int v = 0;
-        for (int w = 0; w < W; ++w) v += rows[w];
+        for (int w = 0; w < W; ++w) v += S.rows[w];
         b.live[blockIdx.x] = v;
     }
 }
@@ -166,40 +180,12 @@ struct Joined {
     int tot[W], live[W];
 };
 
-// A batch's sums over its workgroups: f in LDS; 1 / rows that count is returned. write: the counts and the loss too.
-__device__ __forceinline__ float join(const Bal& b, int batch, bool write, Joined& J) {
+// A batch's sums (J.p, J.f) and the lane's share of its rows that count to f; 1 / those rows is returned. write: the counts and
+// the loss too.
+__device__ __forceinline__ float finish(const Bal& b, int batch, bool write, int rows, Joined& J) {
     const dr_balance& a = b.a;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const long long at = (long long)batch * b.groups;
-    int pw = 32;  // experts at a time, by T / pw slices of the workgroups
-    while (pw < a.experts && pw < T) pw *= 2;
-    const int e0 = tid & (pw - 1), sl = tid / pw, slices = T / pw;
-    for (int e = e0; e - e0 < a.experts; e += pw) {
-        float p = 0.f;
-        int c = 0;
-        if (e < a.experts) {
-#pragma unroll 8
-            for (int g = sl; g < b.groups; g += slices) {
-                const float2 v = b.sums[(at + g) * a.experts + e];
-                p += v.x;
-                c += __float_as_int(v.y);
-            }
-        }
-        J.part[tid] = make_float2(p, __int_as_float(c));
-        __syncthreads();
-        if (sl == 0 && e < a.experts) {
-            for (int i = 1; i < slices; ++i) {
-                const float2 v = J.part[i * pw + e0];
-                p += v.x;
-                c += __float_as_int(v.y);
-            }
-            J.p[e] = p;
-            J.f[e] = __int_as_float(c);
-        }
-        __syncthreads();
-    }
-    int rows = 0, total = 0;
-    for (int g = tid; g < b.groups; g += T) rows += b.live[at + g];
+    int total = 0;
     for (int e = tid; e < a.experts; e += T) {
         const int c = __float_as_int(J.f[e]);
         total += c;
@@ -230,21 +216,54 @@ __device__ __forceinline__ float join(const Bal& b, int batch, bool write, Joine
     return per;
 }
 
+// the batch's sums over its workgroups, finished
+__device__ __forceinline__ float join(const Bal& b, int batch, bool write, Joined& J) {
+    const dr_balance& a = b.a;
+    const int tid = threadIdx.x;
+    const long long at = (long long)batch * b.groups;
+    int pw = 32;  // experts at a time, by T / pw slices of the workgroups
+    while (pw < a.experts && pw < T) pw *= 2;
+    const int e0 = tid & (pw - 1), sl = tid / pw, slices = T / pw;
+    for (int e = e0; e - e0 < a.experts; e += pw) {
+        float p = 0.f;
+        int c = 0;
+        if (e < a.experts) {
+#pragma unroll 8
+            for (int g = sl; g < b.groups; g += slices) {
+                const float2 v = b.sums[(at + g) * a.experts + e];
+                p += v.x;
+                c += __float_as_int(v.y);
+            }
+        }
+        J.part[tid] = make_float2(p, __int_as_float(c));
+        __syncthreads();
+        if (sl == 0 && e < a.experts) {
+            for (int i = 1; i < slices; ++i) {
+                const float2 v = J.part[i * pw + e0];
+                p += v.x;
+                c += __float_as_int(v.y);
+            }
+            J.p[e] = p;
+            J.f[e] = __int_as_float(c);
+        }
+        __syncthreads();
+    }
+    int rows = 0;
+    for (int g = tid; g < b.groups; g += T) rows += b.live[at + g];
+    return finish(b, batch, write, rows, J);
+}
+
 __global__ __launch_bounds__(T) void balance_join_k(const Bal b) {
     __shared__ Joined J;
     join(b, blockIdx.x, true, J);
 }
 
+// the gradient of a workgroup's rows; z: the first one's logits
 template <int L, int N, bool SIG>
-__global__ __launch_bounds__(T) void balance_grad_k(const Bal b) {
+__device__ __forceinline__ void grad_rows(const Bal& b, int g, int batch, float per, float (&z)[4 * N], const Joined& J) {
     constexpr int R = T / L;
-    __shared__ Joined J;
     const dr_balance& a = b.a;
     const int tid = threadIdx.x, l = tid % L;
-    const int g = blockIdx.x % b.groups, batch = blockIdx.x / b.groups;
-    float z[4 * N];
-    row_load<L, N>(b, (long long)batch * a.rows + min(g * R + tid / L, a.rows - 1), l, z);
-    const float per = join(b, batch, g == 0, J);
     const float scale = (a.g ? a.g[batch] : 1.f) * per;
     float f[4 * N];
 #pragma unroll
@@ -288,13 +307,44 @@ __global__ __launch_bounds__(T) void balance_grad_k(const Bal b) {
     }
 }
 
+template <int L, int N, bool SIG>
+__global__ __launch_bounds__(T) void balance_grad_k(const Bal b) {
+    __shared__ Joined J;
+    const int g = blockIdx.x % b.groups, batch = blockIdx.x / b.groups;
+    float z[4 * N];
+    row_load<L, N>(b, (long long)batch * b.a.rows + min(g * (T / L) + (int)threadIdx.x / L, b.a.rows - 1), threadIdx.x % L, z);
+    const float per = join(b, batch, g == 0, J);
+    grad_rows<L, N, SIG>(b, g, batch, per, z, J);
+}
+
+template <int L, int N, bool SIG>
+__global__ __launch_bounds__(T) void balance_one_k(const Bal b, int grad) {
+    __shared__ __attribute__((aligned(16))) Sums<L, N> S;
+    __shared__ Joined J;
+    const int tid = threadIdx.x, batch = blockIdx.x;
+    sum_rows<L, N, SIG>(b, 0, batch, S);
+    float z[4 * N];
+    if (grad) row_load<L, N>(b, (long long)batch * b.a.rows + min(tid / L, b.a.rows - 1), tid % L, z);
+    for (int e = tid; e < b.a.experts; e += T) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) v += S.p[w][e];
+        J.p[e] = v;
+        J.f[e] = __int_as_float(S.cnt[e]);
+    }
+    const float per = finish(b, batch, true, tid < W ? S.rows[tid] : 0, J);
+    if (grad) grad_rows<L, N, SIG>(b, 0, batch, per, z, J);
+}
+
 // Workgroups a batch: as many as its rows fill, but no more than all the CUs take in one round, and at most 128, since every
-// workgroup of the gradient reads all of their sums (20011 rows x 128 experts: 128 workgroups 5 rows a quarter wavefront).
+// workgroup of the gradient reads all of their sums (20011 rows x 128 experts: 128 workgroups 5 rows a quarter wavefront). Up to
+// twice a workgroup's rows one takes all (64 rows x 32 experts in a graph: 6.8 us, 8.0 in two launches; 128 rows 10.0 and 8.3).
 int groups_of(const dr_balance* a) {
     const int at_once = a->experts <= 256 ? T / 16 : T / 64;
     int most = 256 / a->batch;
     most = most < 1 ? 1 : most > 128 ? 128 : most;
     const int fit = (a->rows + at_once - 1) / at_once;
+    if (fit <= 2) return 1;
     return fit < most ? fit : most;
 }
 
@@ -309,6 +359,10 @@ long long up256(long long v) { return (v + 255) & ~255ll; }
 
 template <int L, int N, bool SIG>
 void run(const Bal& b, int what, hipStream_t st) {
+    if (b.groups == 1) {
+        hipLaunchKernelGGL((balance_one_k<L, N, SIG>), dim3(b.a.batch), dim3(T), 0, st, b, what & DR_BALANCE_GRAD);
+        return;
+    }
     const dim3 grid(b.groups * b.a.batch);
     hipLaunchKernelGGL((balance_sum_k<L, N, SIG>), grid, dim3(T), 0, st, b);
     if (what & DR_BALANCE_GRAD) hipLaunchKernelGGL((balance_grad_k<L, N, SIG>), grid, dim3(T), 0, st, b);
@@ -325,15 +379,16 @@ void run_kind(const Bal& b, int what, hipStream_t st) {
 
 extern "C" int64_t dr_moe_balance_workspace_bytes(const dr_balance* a, int what) {
     if (!valid(a, what)) return -1;
-    const long long w = (long long)a->batch * groups_of(a);
+    const long long w = groups_of(a) > 1 ? (long long)a->batch * groups_of(a) : 0;
     return up256(w * a->experts * 8) + up256(w * 4);
 }
 
 extern "C" int dr_moe_balance(const dr_balance* a, int what) {
     if (!valid(a, what)) return DR_EINVAL;
+    const long long need = dr_moe_balance_workspace_bytes(a, what);
     auto aligned = [](const void* p, uintptr_t to) { return p != nullptr && reinterpret_cast<uintptr_t>(p) % to == 0; };
     if (!aligned(a->logits, 4) || !aligned(a->ids, a->ids32 ? 4 : 2) || !aligned(a->loss, 4) || !aligned(a->counts, 4) ||
-        !aligned(a->workspace, 256) || a->workspace_bytes < dr_moe_balance_workspace_bytes(a, what) ||
+        (need > 0 && !aligned(a->workspace, 256)) || a->workspace_bytes < need ||
         ((what & DR_BALANCE_GRAD) && (!aligned(a->dlogits, 4) || a->ld_dlogits < a->width)))
         return DR_EINVAL;
     Bal b{};

@@ -77,6 +77,22 @@ def test_balance(device, kind, batch, rows, width, experts, k, ids32):
         same("the counts alone", counts, got[1])
 
 
+@pytest.mark.parametrize("kind", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("batch, rows, width, experts, k", [
+    (300, 100, 41, 40, 4), (257, 33, 260, 257, 2), (1, 64, 32, 32, 4), (1, 65, 32, 32, 4), (2, 16, 512, 512, 8),
+    (2, 17, 512, 512, 8),
+])
+def test_a_workgroup_a_batch(device, kind, batch, rows, width, experts, k):
+    """Many batches, and as many rows as one workgroup takes and one more."""
+    logits, ids, mask, g = inputs(device, batch, rows, width, experts, k, batch + rows + width)
+    mask[0] = False
+    got = balance.balance_loss_grads(logits, ids, k, g, kind=kind, experts=experts, mask=mask)
+    check(f"{kind} {batch} x {rows} x {experts}", got, expected(logits, ids, k, kind, experts, mask, g))
+    loss, counts = balance.balance_loss(logits, ids, k, kind=kind, experts=experts, mask=mask)
+    same("the loss alone", loss, got[0])
+    same("the counts alone", counts, got[1])
+
+
 def test_first_slots_of_wider_ids(device):
     """Of ids with more slots a row than k (a shared expert's slot behind the picks, say), the first k count."""
     logits, ids, mask, g = inputs(device, 2, 60, 64, 64, 5, 7, ids32=True)

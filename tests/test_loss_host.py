@@ -114,7 +114,7 @@ def _balance(**kw):
     A = _lib.Balance()
     for f in ("logits", "ids", "loss", "counts", "dlogits", "workspace"):
         setattr(A, f, 4096)
-    A.batch, A.rows, A.experts, A.width, A.ld_logits, A.ld_dlogits, A.ld_ids, A.k = 2, 10, 32, 32, 32, 32, 4, 4
+    A.batch, A.rows, A.experts, A.width, A.ld_logits, A.ld_dlogits, A.ld_ids, A.k = 2, 100, 32, 32, 32, 32, 4, 4
     A.workspace_bytes = 1 << 40
     for name, v in kw.items():
         setattr(A, name, v)

@@ -6,9 +6,10 @@
 // operations and a butterfly of log2(L) steps. The sums over rows stay in registers until the wavefront's rows are done.
 //   balance_sum_k   a workgroup's rows: the sum of p and the counts (LDS), written for the workgroup
 //   balance_grad_k  every workgroup joins the workgroups' sums for itself, in order (cheaper than a launch of its own in
-//                   between), then the logits' gradient of its rows, p computed again; balance_join_k: the join alone
+//                   between while they are few; balance_slice_k otherwise), then the logits' gradient of its rows, p computed
+//                   again; balance_join_k: the join alone
 //   balance_one_k   all of it by one workgroup, a batch of few rows or one of many batches: one launch and no memory between
-//                   (32 rows x 32 experts: 5.2 us in a graph, two launches 8.2; called eagerly 11.8 and 16.0, all of it the host's)
+//                   (32 rows x 32 experts: 4.8 us in a graph, two launches 8; called eagerly 12 and 16, the host's)
 // What bounds it: the logits read twice and the gradient written once; at a few rows the launches.
 
 #include <hip/hip_runtime.h>
@@ -29,21 +30,36 @@ struct Bal {
     float2* sums;  // [batch][groups][E] sum of p, count (its bits)
     int* live;     // [batch][groups] rows that count
     int groups;    // workgroups a batch
+    const float2* in;    // [batch][parts][E], [batch][parts]: the sums to be joined, the workgroups' or (parts 1) balance_slice_k's
+    const int* in_live;
+    int parts;
     int vec;       // the logits' rows can be read 16 bytes at a time
     int gvec;      // and dlogits' written so
 };
 
-template <int L>
-__device__ __forceinline__ float sum_over(float v) {
+// v of the lane that a row's DPP control names: neighbours, pairs, the quads and the halves of 16 lanes changed over. (A turn is
+// a few cycles; the general shuffle, through LDS, about a hundred, and a row takes twelve to twenty of them one after another.)
+template <int CONTROL>
+__device__ __forceinline__ float turned(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CONTROL, 0xF, 0xF, true));
+}
+template <int L, typename F>
+__device__ __forceinline__ float over(float v, F&& f) {
+    v = f(v, turned<0xB1>(v));   // quad_perm 1 0 3 2
+    v = f(v, turned<0x4E>(v));   // quad_perm 2 3 0 1
+    v = f(v, turned<0x141>(v));  // row_half_mirror
+    v = f(v, turned<0x140>(v));  // row_mirror
 #pragma unroll
-    for (int o = L / 2; o; o >>= 1) v += __shfl_xor(v, o);
+    for (int o = 16; o < L; o <<= 1) v = f(v, __shfl_xor(v, o));
     return v;
 }
 template <int L>
+__device__ __forceinline__ float sum_over(float v) {
+    return over<L>(v, [](float a, float b) { return a + b; });
+}
+template <int L>
 __device__ __forceinline__ float max_over(float v) {
-#pragma unroll
-    for (int o = L / 2; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
+    return over<L>(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
 // a row's logits: value 4 i + c is expert 4 (l + L i) + c; past the experts -inf
@@ -61,6 +77,29 @@ __device__ __forceinline__ void row_load(const Bal& b, long long row, int l, flo
             for (int c = 0; c < 4; ++c) z[4 * i + c] = e + c < b.a.experts ? at[e + c] : -INFINITY;
         }
     }
+}
+
+// What a row takes from memory, asked for before the row ahead of it is worked on (two rows ahead: the same, within 3 %). Past
+// the batch's last row that one again: every lane takes part in the butterflies.
+template <int N>
+struct Row {
+    float z[4 * N];
+    uint32_t id;  // lane l's slot
+    uint8_t on;
+};
+template <int L, int N, bool IDS>
+__device__ __forceinline__ void row_get(const Bal& b, int batch, int r, int l, Row<N>& to) {
+    const dr_balance& a = b.a;
+    const long long row = (long long)batch * a.rows + min(r, a.rows - 1);
+    row_load<L, N>(b, row, l, to.z);
+    if constexpr (IDS) {
+        to.id = 0xFFFFFFFFu;
+        if (l < a.k) {
+            const long long at = row * a.ld_ids + l;
+            to.id = a.ids32 ? reinterpret_cast<const uint32_t*>(a.ids)[at] : reinterpret_cast<const uint16_t*>(a.ids)[at];
+        }
+    }
+    to.on = a.mask ? a.mask[row] : 1;
 }
 
 // the row's p from its logits, in place (0 past the experts); a row of no expert above -inf has p 0. down: 1 less the sigmoid,
@@ -94,8 +133,6 @@ __device__ __forceinline__ void row_p(float (&p)[4 * N], float (&down)[SIG ? 4 *
     for (int i = 0; i < 4 * N; ++i) p[i] *= inv;
 }
 
-__device__ __forceinline__ bool row_counts(const dr_balance& a, long long row) { return a.mask == nullptr || a.mask[row] != 0; }
-
 // a workgroup's rows in LDS: cnt, and by wavefront the sum of p and the rows that count
 template <int L, int N>
 struct Sums {
@@ -115,26 +152,19 @@ __device__ __forceinline__ void sum_rows(const Bal& b, int g, int batch, Sums<L,
 #pragma unroll
     for (int i = 0; i < 4 * N; ++i) sum[i] = 0.f;
     int n = 0;
-    float z[4 * N];  // (the next row's logits are asked for before this one's are worked on)
-    row_load<L, N>(b, (long long)batch * a.rows + min(g * R + tid / L, a.rows - 1), l, z);
-    for (int r0 = g * R; r0 < a.rows; r0 += b.groups * R) {
-        const int r = min(r0 + tid / L, a.rows - 1);  // (the last row again: every lane takes part in the butterflies)
-        const long long row = (long long)batch * a.rows + r;
-        float p[4 * N], down[SIG ? 4 * N : 1];
+    const int step = b.groups * R;
+    Row<N> next;
+    row_get<L, N, true>(b, batch, g * R + tid / L, l, next);
+    for (int r = g * R + tid / L; r - tid / L < a.rows; r += step) {
+        Row<N> now = next;
+        row_get<L, N, true>(b, batch, r + step, l, next);
+        const bool on = r < a.rows && now.on;
+        float down[SIG ? 4 * N : 1];
+        row_p<L, N, SIG>(now.z, down);
 #pragma unroll
-        for (int i = 0; i < 4 * N; ++i) p[i] = z[i];
-        row_load<L, N>(b, (long long)batch * a.rows + min(r + b.groups * R, a.rows - 1), l, z);
-        uint32_t id = 0xFFFFFFFFu;
-        if (l < a.k) {
-            const long long at = row * a.ld_ids + l;
-            id = a.ids32 ? reinterpret_cast<const uint32_t*>(a.ids)[at] : reinterpret_cast<const uint16_t*>(a.ids)[at];
-        }
-        const bool on = r0 + tid / L < a.rows && row_counts(a, row);
-        row_p<L, N, SIG>(p, down);
-#pragma unroll
-        for (int i = 0; i < 4 * N; ++i) sum[i] += on ? p[i] : 0.f;
+        for (int i = 0; i < 4 * N; ++i) sum[i] += on ? now.z[i] : 0.f;
         n += on;
-        if (on && id < (uint32_t)a.experts) atomicAdd(&S.cnt[id], 1);
+        if (on && now.id < (uint32_t)a.experts) atomicAdd(&S.cnt[now.id], 1);
     }
     // the wavefront's rows, then the workgroup's, in order
 #pragma unroll
@@ -216,11 +246,11 @@ __device__ __forceinline__ float finish(const Bal& b, int batch, bool write, int
     return per;
 }
 
-// the batch's sums over its workgroups, finished
+// the batch's sums over its parts, finished
 __device__ __forceinline__ float join(const Bal& b, int batch, bool write, Joined& J) {
     const dr_balance& a = b.a;
     const int tid = threadIdx.x;
-    const long long at = (long long)batch * b.groups;
+    const long long at = (long long)batch * b.parts;
     int pw = 32;  // experts at a time, by T / pw slices of the workgroups
     while (pw < a.experts && pw < T) pw *= 2;
     const int e0 = tid & (pw - 1), sl = tid / pw, slices = T / pw;
@@ -228,9 +258,9 @@ __device__ __forceinline__ float join(const Bal& b, int batch, bool write, Joine
         float p = 0.f;
         int c = 0;
         if (e < a.experts) {
-#pragma unroll 8
-            for (int g = sl; g < b.groups; g += slices) {
-                const float2 v = b.sums[(at + g) * a.experts + e];
+#pragma unroll 16
+            for (int g = sl; g < b.parts; g += slices) {
+                const float2 v = b.in[(at + g) * a.experts + e];
                 p += v.x;
                 c += __float_as_int(v.y);
             }
@@ -249,8 +279,44 @@ __device__ __forceinline__ float join(const Bal& b, int batch, bool write, Joine
         __syncthreads();
     }
     int rows = 0;
-    for (int g = tid; g < b.groups; g += T) rows += b.live[at + g];
+    for (int g = tid; g < b.parts; g += T) rows += b.in_live[at + g];
     return finish(b, batch, write, rows, J);
+}
+
+// the workgroups' sums of 64 experts of a batch, an eighth of the workgroups a wavefront
+__global__ __launch_bounds__(T) void balance_slice_k(const Bal b, float2* sums, int* live) {
+    __shared__ float2 part[W][64];
+    __shared__ int rows[W];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, E = b.a.experts;
+    const int slices = (E + 63) / 64, batch = blockIdx.x / slices, slice = blockIdx.x % slices, e = 64 * slice + lane;
+    const long long at = (long long)batch * b.groups;
+    float p = 0.f;
+    int c = 0;
+    if (e < E) {
+#pragma unroll 16
+        for (int g = wave; g < b.groups; g += W) {
+            const float2 v = b.sums[(at + g) * E + e];
+            p += v.x;
+            c += __float_as_int(v.y);
+        }
+    }
+    part[wave][lane] = make_float2(p, __int_as_float(c));
+    int n = 0;
+    if (slice == 0)
+        for (int g = tid; g < b.groups; g += T) n += b.live[at + g];
+#pragma unroll
+    for (int o = 32; o; o >>= 1) n += __shfl_xor(n, o);
+    if (lane == 0) rows[wave] = n;
+    __syncthreads();
+    if (wave == 0 && e < E) {
+#pragma unroll
+        for (int w = 1; w < W; ++w) p += part[w][lane].x, c += __float_as_int(part[w][lane].y);
+        sums[(long long)batch * E + e] = make_float2(p, __int_as_float(c));
+    }
+    if (slice == 0 && tid == 0) {
+        for (int w = 1; w < W; ++w) n += rows[w];
+        live[batch] = n;
+    }
 }
 
 __global__ __launch_bounds__(T) void balance_join_k(const Bal b) {
@@ -258,12 +324,12 @@ __global__ __launch_bounds__(T) void balance_join_k(const Bal b) {
     join(b, blockIdx.x, true, J);
 }
 
-// the gradient of a workgroup's rows; z: the first one's logits
+// the gradient of a workgroup's rows; next: the first of them, asked for before the sums are joined
 template <int L, int N, bool SIG>
-__device__ __forceinline__ void grad_rows(const Bal& b, int g, int batch, float per, float (&z)[4 * N], const Joined& J) {
+__device__ __forceinline__ void grad_rows(const Bal& b, int g, int batch, float per, Row<N>& next, const Joined& J) {
     constexpr int R = T / L;
     const dr_balance& a = b.a;
-    const int tid = threadIdx.x, l = tid % L;
+    const int tid = threadIdx.x, l = tid % L, step = b.groups * R;
     const float scale = (a.g ? a.g[batch] : 1.f) * per;
     float f[4 * N];
 #pragma unroll
@@ -271,21 +337,17 @@ __device__ __forceinline__ void grad_rows(const Bal& b, int g, int batch, float 
         const int e = 4 * (l + L * (i / 4)) + i % 4;
         f[i] = e < a.experts ? J.f[e] : 0.f;
     }
-    for (int r0 = g * R; r0 < a.rows; r0 += b.groups * R) {
-        const int r = min(r0 + tid / L, a.rows - 1);
-        const long long row = (long long)batch * a.rows + r;
-        const bool on = row_counts(a, row);
-        float p[4 * N], down[SIG ? 4 * N : 1];
-#pragma unroll
-        for (int i = 0; i < 4 * N; ++i) p[i] = z[i];
-        row_load<L, N>(b, (long long)batch * a.rows + min(r + b.groups * R, a.rows - 1), l, z);
+    for (int r = g * R + tid / L; r - tid / L < a.rows; r += step) {
+        Row<N> now = next;
+        row_get<L, N, false>(b, batch, r + step, l, next);
+        float (&p)[4 * N] = now.z, down[SIG ? 4 * N : 1];
         row_p<L, N, SIG>(p, down);
         float mean = 0.f;
 #pragma unroll
         for (int i = 0; i < 4 * N; ++i) mean += p[i] * f[i];
         mean = sum_over<L>(mean);
-        if (r0 + tid / L >= a.rows) continue;
-        float* d = a.dlogits + row * a.ld_dlogits;
+        if (r >= a.rows) continue;
+        float* d = a.dlogits + ((long long)batch * a.rows + r) * a.ld_dlogits;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int e = 4 * (l + L * i);
@@ -293,7 +355,7 @@ __device__ __forceinline__ void grad_rows(const Bal& b, int g, int batch, float 
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int q = 4 * i + c;
-                o[c] = on ? scale * (SIG ? p[q] * down[SIG ? q : 0] : p[q]) * (f[q] - mean) : 0.f;
+                o[c] = now.on ? scale * (SIG ? p[q] * down[SIG ? q : 0] : p[q]) * (f[q] - mean) : 0.f;
             }
             if (b.gvec && e + 4 <= a.experts) {
                 *reinterpret_cast<float4*>(d + e) = make_float4(o[0], o[1], o[2], o[3]);
@@ -311,20 +373,20 @@ template <int L, int N, bool SIG>
 __global__ __launch_bounds__(T) void balance_grad_k(const Bal b) {
     __shared__ Joined J;
     const int g = blockIdx.x % b.groups, batch = blockIdx.x / b.groups;
-    float z[4 * N];
-    row_load<L, N>(b, (long long)batch * b.a.rows + min(g * (T / L) + (int)threadIdx.x / L, b.a.rows - 1), threadIdx.x % L, z);
+    Row<N> next;
+    row_get<L, N, false>(b, batch, g * (T / L) + threadIdx.x / L, threadIdx.x % L, next);
     const float per = join(b, batch, g == 0, J);
-    grad_rows<L, N, SIG>(b, g, batch, per, z, J);
+    grad_rows<L, N, SIG>(b, g, batch, per, next, J);
 }
 
 template <int L, int N, bool SIG>
-__global__ __launch_bounds__(T) void balance_one_k(const Bal b, int grad) {
+__global__ __launch_bounds__(T) void balance_one_k(const Bal b, int gradient) {
     __shared__ __attribute__((aligned(16))) Sums<L, N> S;
     __shared__ Joined J;
     const int tid = threadIdx.x, batch = blockIdx.x;
     sum_rows<L, N, SIG>(b, 0, batch, S);
-    float z[4 * N];
-    if (grad) row_load<L, N>(b, (long long)batch * b.a.rows + min(tid / L, b.a.rows - 1), tid % L, z);
+    Row<N> next;
+    if (gradient) row_get<L, N, false>(b, batch, tid / L, tid % L, next);
     for (int e = tid; e < b.a.experts; e += T) {
         float v = 0.f;
 #pragma unroll
@@ -333,19 +395,26 @@ __global__ __launch_bounds__(T) void balance_one_k(const Bal b, int grad) {
         J.f[e] = __int_as_float(S.cnt[e]);
     }
     const float per = finish(b, batch, true, tid < W ? S.rows[tid] : 0, J);
-    if (grad) grad_rows<L, N, SIG>(b, 0, batch, per, z, J);
+    if (gradient) grad_rows<L, N, SIG>(b, 0, batch, per, next, J);
 }
 
-// Workgroups a batch: as many as its rows fill, but no more than all the CUs take in one round, and at most 128, since every
-// workgroup of the gradient reads all of their sums (20011 rows x 128 experts: 128 workgroups 5 rows a quarter wavefront). Up to
-// twice a workgroup's rows one takes all (64 rows x 32 experts in a graph: 6.8 us, 8.0 in two launches; 128 rows 10.0 and 8.3).
-int groups_of(const dr_balance* a) {
+// Workgroups a batch, and whether their sums are joined by a launch of its own: as many workgroups as the rows fill, but no more
+// than all the CUs take in one round (65536 rows x 128 experts: 26.1 us, 33.3 by 128 workgroups; two rounds and four are slower
+// too, 16384 x 1024 48 and 63 to 43). Every workgroup of the gradient reads all of a batch's sums, which a launch of its own saves
+// where they are more than 256 KB: 16384 rows x 1024 experts 43 us (67 without), 8192 x 256 15.9 (19.5); at 8 batches of 4096 x
+// 256, 64 KB each, 25.8 (23.4 without). Up to twice a workgroup's rows one takes all (64 rows x 32 experts 6.2 us, 8.1 in two
+// launches; 128 rows 9.6 and 8.1). Times in a graph.
+struct Split {
+    int groups;
+    bool slices;
+};
+constexpr int JOINED = 32768;  // sums of 8 bytes that every workgroup may read
+Split split_of(const dr_balance* a) {
     const int at_once = a->experts <= 256 ? T / 16 : T / 64;
-    int most = 256 / a->batch;
-    most = most < 1 ? 1 : most > 128 ? 128 : most;
     const int fit = (a->rows + at_once - 1) / at_once;
-    if (fit <= 2) return 1;
-    return fit < most ? fit : most;
+    if (fit <= 2) return {1, false};
+    const int most = a->batch < 256 ? 256 / a->batch : 1, groups = fit < most ? fit : most;
+    return {groups, groups * a->experts > JOINED};
 }
 
 bool valid(const dr_balance* a, int what) {
@@ -365,6 +434,9 @@ void run(const Bal& b, int what, hipStream_t st) {
     }
     const dim3 grid(b.groups * b.a.batch);
     hipLaunchKernelGGL((balance_sum_k<L, N, SIG>), grid, dim3(T), 0, st, b);
+    if (b.parts == 1)
+        hipLaunchKernelGGL(balance_slice_k, dim3(b.a.batch * ((b.a.experts + 63) / 64)), dim3(T), 0, st, b,
+                           const_cast<float2*>(b.in), const_cast<int*>(b.in_live));
     if (what & DR_BALANCE_GRAD) hipLaunchKernelGGL((balance_grad_k<L, N, SIG>), grid, dim3(T), 0, st, b);
     else hipLaunchKernelGGL(balance_join_k, dim3(b.a.batch), dim3(T), 0, st, b);
 }
@@ -379,7 +451,8 @@ void run_kind(const Bal& b, int what, hipStream_t st) {
 
 extern "C" int64_t dr_moe_balance_workspace_bytes(const dr_balance* a, int what) {
     if (!valid(a, what)) return -1;
-    const long long w = groups_of(a) > 1 ? (long long)a->batch * groups_of(a) : 0;
+    const Split s = split_of(a);
+    const long long w = s.groups > 1 ? (long long)a->batch * (s.groups + s.slices) : 0;
     return up256(w * a->experts * 8) + up256(w * 4);
 }
 
@@ -393,13 +466,16 @@ extern "C" int dr_moe_balance(const dr_balance* a, int what) {
         return DR_EINVAL;
     Bal b{};
     b.a = *a;
-    b.groups = groups_of(a);
+    const Split s = split_of(a);
+    b.groups = s.groups;
     b.vec = aligned(a->logits, 16) && a->ld_logits % 4 == 0;
     b.gvec = (what & DR_BALANCE_GRAD) && aligned(a->dlogits, 16) && a->ld_dlogits % 4 == 0;
-    char* ws = reinterpret_cast<char*>(a->workspace);
-    const long long w = (long long)a->batch * b.groups;
-    b.sums = reinterpret_cast<float2*>(ws);
-    b.live = reinterpret_cast<int*>(ws + up256(w * a->experts * 8));
+    const long long w = (long long)a->batch * b.groups;  // (the slices' sums behind the workgroups')
+    b.sums = reinterpret_cast<float2*>(a->workspace);
+    b.live = reinterpret_cast<int*>(reinterpret_cast<char*>(a->workspace) + up256((w + s.slices * a->batch) * a->experts * 8));
+    b.in = s.slices ? b.sums + w * a->experts : b.sums;
+    b.in_live = s.slices ? b.live + w : b.live;
+    b.parts = s.slices ? 1 : b.groups;
     const hipStream_t st = reinterpret_cast<hipStream_t>(a->stream);
     if (a->experts <= 64) run_kind<16, 1>(b, what, st);
     else if (a->experts <= 128) run_kind<16, 2>(b, what, st);

@@ -80,10 +80,10 @@ def test_balance(device, kind, batch, rows, width, experts, k, ids32):
 @pytest.mark.parametrize("kind", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("batch, rows, width, experts, k", [
     (300, 100, 41, 40, 4), (257, 33, 260, 257, 2), (1, 64, 32, 32, 4), (1, 65, 32, 32, 4), (2, 16, 512, 512, 8),
-    (2, 17, 512, 512, 8),
+    (2, 17, 512, 512, 8), (1, 600, 1030, 1000, 8), (3, 700, 512, 500, 4), (1, 8200, 256, 250, 6),
 ])
-def test_a_workgroup_a_batch(device, kind, batch, rows, width, experts, k):
-    """Many batches, and as many rows as one workgroup takes and one more."""
+def test_many_workgroups_and_one(device, kind, batch, rows, width, experts, k):
+    """Many batches, as many rows as one workgroup takes and one more, and sums that a launch of its own joins."""
     logits, ids, mask, g = inputs(device, batch, rows, width, experts, k, batch + rows + width)
     mask[0] = False
     got = balance.balance_loss_grads(logits, ids, k, g, kind=kind, experts=experts, mask=mask)

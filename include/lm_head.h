@@ -47,7 +47,8 @@ int dr_head_pick_records(const void* records, int n_records, int rows, int k, in
                          void* out, void* ids_out, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* The losses. A head [vocab][dim] bf16 (one row a token, as dr_head_pick reads it) against rows x [rows][dim] bf16:
- * z = x . head^T, float32 sums, never in memory as a whole. Per row, with lse = log(sum over v < valid of exp(z[v] / T)):
+ * z = x . head^T, float32 sums, of which no call has more than 2 GiB in memory. Per row, with lse = log(sum over
+ * v < valid of exp(z[v] / T)):
  *   tokens (vals NULL, k 1, T 1): loss = lse - z[id];
  *   a teacher's best k logits (vals): over the entries held, q = softmax(vals / T),
  *     loss = sum q (log q - z[id] / T + lse), the divergence of the row's softmax at temperature T from the teacher's
@@ -56,9 +57,10 @@ int dr_head_pick_records(const void* records, int n_records, int rows, int k, in
  * left out: loss, lse, logits and dx 0, nothing into dhead, whatever x, g or vals hold there.
  *
  * Gradients of sum over rows of g[row] * loss[row]: dz[v] = g / T (p[v] - sum of q over entries of id v), p = exp(z / T -
- * lse); dx = dz . head, dhead = dz^T . x (rows valid .. vocab - 1 zeros). z is computed again, piece by piece of the
- * vocabulary; dz is rounded to bf16 (divided by the largest |g| of the rows that count, which the float32 sums get back,
- * unless their weights lie further apart than 2^40), the sums are float32, dx and dhead rounded once.
+ * lse); dx = dz . head, dhead = dz^T . x (rows valid .. vocab - 1 zeros). Piece by piece of the vocabulary (dz to 1 GiB)
+ * z is computed again; a call of both directions and one piece may keep it in its workspace instead. dz is rounded to
+ * bf16 (divided by the largest |g| of the rows that count, which the float32 sums get back, unless their weights lie
+ * further apart than 2^40), the sums are float32, dx and dhead rounded once.
  *
  * No counterpart in the reference, which has no training: the head and the teacher's records are its
  * lm_head_topk/head_pick.py:43-52 and dense_reader/linear.py:747-768.

@@ -8,13 +8,15 @@
 // A call is a few launches: the entries (ids checked, the teacher's softmax), the rows that count found (and gathered, where
 // some do not: rows left out cost nothing and whatever they hold enters no sum), z with each tile's maximum and sum of a row,
 // their merge into lse and loss; backward, piece by piece of the vocabulary, dz from z computed again, a teacher's entries' own
-// dz, dhead's rows, dx's sum so far. The logits are never kept: that is one product more than a program that keeps them.
+// dz, dhead's rows, dx's sum so far. Large calls do not keep the logits: that is one product more than a program that keeps
+// them. One of both directions whose dz is one piece (1 GB) keeps them from the loss to dz where that is faster (KEEP_DIM), and
+// of few rows takes all between the products in one launch (hl_few).
 //
 // What bounds them (8192 rows x 4096 against 128256 tokens, 27.3 ms; a large library product of the same layouts runs at 1200,
 // 985 and 1110 TFLOP/s): z 7.05 ms (1220 TFLOP/s), dz 7.16 (1200), dhead 6.69 (1286), dx 6.85 (1256). With zeros for inputs
 // the same kernels run at 1530 to 1790 TFLOP/s and 2.4 GHz: the power that random values draw, at 1.8 GHz, holds them there.
 // 32 rows: 176 us for the 1.05 GB of the head, 6.0 TB/s. A few rows against a small vocabulary: each launch's start, its first
-// loads and a chain of LDS reads and matrix instructions (48 x 1024 against 8192: 7 launches of 4 to 9 us).
+// loads and a chain of LDS reads and matrix instructions (48 x 1024 against 8192: 5 launches of 4 to 9 us).
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -94,6 +96,7 @@ struct Gemm {
     int raw64;
     int kp, kn;
     float* zt;              // [rows][kn]
+    float* kept;            // z itself for hl_dz, in panels as dz, or NULL
     // outputs
     uint16_t* out;          // dz (panels), dhead [n = v][ld_out], dx [row][ld_out] or NULL: the sums are not complete
     long long ld_out;
@@ -467,7 +470,16 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void hl_gemm(const Gemm a) {
                 const long long row = a.idx ? a.idx[nj + t] : nj + t;
                 a.zt[row * a.kn + kk] = mine[t * (TM / 4) + ((d >> 2) ^ (t & 7))][d & 3];
             };
-            if (a.kp < 2) {
+            if (a.kept) {  // (the entries are read from it)
+                lay();
+                constexpr int C4 = TM / 4, PC = 64 / C4;  // 16-byte chunks a column, columns a turn
+                float* o = a.kept + (mw >> 8) * a.panel + (long long)nj * 256 + (mw & 255);
+#pragma unroll 2
+                for (int t = 0; t < 32 / PC; ++t) {
+                    const int c = t * PC + lane / C4, q = lane % C4;
+                    if (nj + c < n_end) *reinterpret_cast<f32x4*>(o + c * 256 + 4 * q) = mine[c * C4 + (q ^ (c & 7))];
+                }
+            } else if (a.kp < 2) {
                 const int t = lane >> a.kp;
                 int d = -1;
                 if (t < 32 && nj + t < n_end) {
@@ -618,25 +630,31 @@ __device__ __forceinline__ int entry_id(const dr_head_loss& a, int row, int j) {
     return id >= 0 && id < a.valid ? (int)id : -1;
 }
 
+// A row's softmax over w lanes, of entries v (-inf and id -1: none), and its sum of q log q. (The temperature after the
+// difference: the type's lowest value, at a temperature below 1, is still no empty slot.)
+__device__ __forceinline__ void teacher(float v, int id, int w, float temperature, float& q, float& ent) {
+    float top = v;
+    for (int o = w >> 1; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    const float d = id < 0 ? 0.f : (v - top) / temperature;
+    const float x = id < 0 ? 0.f : __expf(d);
+    float total = x;
+    for (int o = w >> 1; o; o >>= 1) total += __shfl_xor(total, o);
+    q = id < 0 ? 0.f : x / total;
+    ent = q == 0.f ? 0.f : q * (d - __logf(total));
+    for (int o = w >> 1; o; o >>= 1) ent += __shfl_xor(ent, o);
+}
+
 // entry e of all rows' (row e >> kp; the lanes of a row are neighbours): id, q, the row's sum; whether the row counts
 __device__ __forceinline__ bool entries_of(const Prep& p, int e, int rows) {
     const int row = e >> p.kp, w = 1 << p.kp, j = e & (w - 1);
     const bool in = row < rows && j < p.a.k;
     int id = in ? entry_id(p.a, row, j) : -1;
     if (p.a.vals) {
-        // (the temperature after the difference: the type's lowest value, at a temperature below 1, is still no empty slot)
         float v = in ? p.a.vals[(long long)row * p.a.ld_vals + j] : -INFINITY;
         if (v == -INFINITY) id = -1;
         if (id < 0) v = -INFINITY;
-        float top = v;
-        for (int o = w >> 1; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-        const float d = id < 0 ? 0.f : (v - top) / p.a.temperature;
-        const float x = id < 0 ? 0.f : __expf(d);
-        float total = x;
-        for (int o = w >> 1; o; o >>= 1) total += __shfl_xor(total, o);
-        const float q = id < 0 ? 0.f : x / total;
-        float ent = q == 0.f ? 0.f : q * (d - __logf(total));
-        for (int o = w >> 1; o; o >>= 1) ent += __shfl_xor(ent, o);
+        float q, ent;
+        teacher(v, id, w, p.a.temperature, q, ent);
         if (row < rows) {
             p.q[e] = q;
             if (j == 0) p.ent[row] = ent;
@@ -659,6 +677,10 @@ __device__ __forceinline__ int wave_sum(int v) {
     for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
+
+// the factor taken out of dz, of the rows' weights that count (positive, finite) the largest; weights so far apart that the
+// smallest over the largest would near the smallest float32: as they are
+__device__ __forceinline__ float factor(float top, float low) { return low > top * 0x1p-40f ? top : 1.f; }
 
 constexpr int GROWS = 4;     // rows a workgroup of hl_gather, one a wavefront
 constexpr int FEW = 2048;    // entries that every workgroup looks through itself
@@ -722,8 +744,7 @@ __global__ __launch_bounds__(256) void hl_gather(const Prep p) {
         if (tid == 0) {
             top = p.a.g ? fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) : 1.f;
             low = fminf(fminf(lows[0], lows[1]), fminf(lows[2], lows[3]));
-            // (weights so far apart that the smallest over the largest would near the smallest float32: as they are)
-            if (p.a.g && !(low > top * 0x1p-40f)) top = 1.f;
+            if (p.a.g) top = factor(top, low);
             *p.live = before;
             p.top[0] = top;
             p.top[1] = top / p.a.temperature;
@@ -769,7 +790,30 @@ struct Merge {
     const float *q, *ent;
     float inv_t;
     float *loss, *lse, *zt;
+    const float* kept;    // z itself, the entries' not taken yet; or NULL
+    long long panel;
 };
+
+// a row's tiles' maxima and sums, one slice of SL: from `sl` on
+template <int SL>
+__device__ __forceinline__ void slice_of(const f32x2* at, long long ld, int parts, int sl, float& m, float& s) {
+    int i = sl;
+    for (; i + 3 * SL < parts; i += 4 * SL) {
+        f32x2 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = at[(i + u * SL) * ld];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) join(m, s, v[u][0], v[u][1]);
+    }
+    for (; i < parts; i += SL) {
+        const f32x2 v = at[i * ld];
+        join(m, s, v[0], v[1]);
+    }
+}
+__device__ __forceinline__ void wave_join(float& m, float& s) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) join(m, s, __shfl_xor(m, o), __shfl_xor(s, o));
+}
 
 // a row's tiles' maxima and sums joined, then lse and loss: TB rows a workgroup of 32 slices (8 of one row)
 template <int TB, int SL>
@@ -787,25 +831,8 @@ __global__ __launch_bounds__(TB* SL) void hl_merge(const Merge p) {
     }
     const int n = !in ? -1 : p.pos ? p.pos[row] : row;
     float m = -INFINITY, s = 0.f;
-    if (n >= 0) {
-        const f32x2* at = p.part + n;
-        int i = sl;
-        for (; i + 3 * SL < p.parts; i += 4 * SL) {
-            f32x2 v[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) v[u] = at[(i + u * SL) * p.ld];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) join(m, s, v[u][0], v[u][1]);
-        }
-        for (; i < p.parts; i += SL) {
-            const f32x2 v = at[i * p.ld];
-            join(m, s, v[0], v[1]);
-        }
-    }
-    if constexpr (TB == 1) {  // (a row's slices are whole wavefronts)
-#pragma unroll
-        for (int o = 32; o; o >>= 1) join(m, s, __shfl_xor(m, o), __shfl_xor(s, o));
-    }
+    if (n >= 0) slice_of<SL>(p.part + n, p.ld, p.parts, sl, m, s);
+    if constexpr (TB == 1) wave_join(m, s);  // (a row's slices are whole wavefronts)
     constexpr int LEFT = TB == 1 ? SL / 64 : SL;  // slices that are left
     if (TB > 1 || (tid & 63) == 0) ms[TB == 1 ? tid >> 6 : tid] = m, ss[TB == 1 ? tid >> 6 : tid] = s;
     __syncthreads();
@@ -823,6 +850,12 @@ __global__ __launch_bounds__(TB* SL) void hl_merge(const Merge p) {
     __syncthreads();
     float c = 0.f;
     float* z = p.zt + (long long)row * p.k;
+    if (p.kept && in) {  // (each read by the lane that took it)
+        for (int j = sl; j < p.k; j += SL) {
+            const int id = p.ids[((long long)row << p.kp) + j];
+            z[j] = id < 0 ? 0.f : p.kept[(id >> 8) * p.panel + (long long)n * 256 + (id & 255)];
+        }
+    }
     if (p.q) {
         for (int j = sl; j < p.k && row < p.rows; j += SL) {
             const long long e = ((long long)row << p.kp) + j;
@@ -841,6 +874,147 @@ __global__ __launch_bounds__(TB* SL) void hl_merge(const Merge p) {
     if (sl || row >= p.rows) return;
     p.lse[row] = lse;
     p.loss[row] = in ? (p.q ? p.ent[row] + c : c) : 0.f;
+}
+
+struct Dz {
+    const int *live, *idx, *ids;  // (ids: tokens' own, of the rows that count, or NULL)
+    const float *z, *lse, *g, *top;
+    uint16_t* dz;
+    long long panel;
+    int valid;
+    float sc;
+};
+
+// dz from z as the loss left it: a wavefront's rows of one panel, 1 KB read and 512 bytes written each (1842 rows against 128256
+// tokens: 275 us, 5.2 TB/s)
+constexpr int DZ_ROWS = 8;  // a wavefront, asked for at once
+__global__ __launch_bounds__(256) void hl_dz(const Dz p) {
+    const int live = *p.live, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = (blockIdx.y * 4 + wave) * DZ_ROWS, v0 = blockIdx.x * 256 + 4 * lane;
+    if (n0 >= live) return;
+    const float top = *p.top;
+    const long long at = blockIdx.x * p.panel + (long long)n0 * 256 + 4 * lane;
+    f32x4 z[DZ_ROWS];
+#pragma unroll
+    for (int i = 0; i < DZ_ROWS; ++i) z[i] = *reinterpret_cast<const f32x4*>(p.z + at + min(i, live - 1 - n0) * 256);
+#pragma unroll
+    for (int i = 0; i < DZ_ROWS; ++i) {
+        const int n = n0 + i;
+        if (n >= live) break;
+        const int row = p.idx[n], own = p.ids ? p.ids[n] - v0 : -1;
+        const float l2 = p.lse[row] * LOG2E, gr = p.g ? p.g[row] : 1.f, gs = top > 0.f ? gr / top : gr;
+        float d[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            d[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i][e], p.sc, -l2));
+            if (own == e) d[e] -= 1.f;
+            d[e] = v0 + e < p.valid ? d[e] * gs : 0.f;
+        }
+        *reinterpret_cast<uint2*>(p.dz + at + i * 256) = make_uint2(cvt2(d[0], d[1]), cvt2(d[2], d[3]));
+    }
+}
+
+struct Few {
+    dr_head_loss a;
+    int kp, parts;
+    const f32x2* part;
+    long long ld;
+    const float* kept;
+    uint16_t* dz;
+    long long panel;
+    float sc, inv_t;
+    int *idx, *live;
+    float* top;
+    uint16_t *xc, *dx;
+};
+
+// Few rows (one a wavefront and panel), from z as the loss left it: what hl_gather, hl_merge, hl_dz and hl_fix do, in one launch.
+// Every wavefront joins its row's tiles for itself and counts the rows that count from all of the ids; the first panel's write
+// what there is one of.
+constexpr int FEW_ROWS = 64, FEW_PARTS = 512;  // (a ballot's; eight parts a lane)
+__global__ __launch_bounds__(256) void hl_few(const Few p) {
+    __shared__ uint32_t flags[FEW_ROWS];
+    __shared__ f32x4 taken[4][64];  // the entries' q in the wavefront's panel
+    const dr_head_loss& a = p.a;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), w = 1 << p.kp;
+    const int r = blockIdx.y * 4 + wave, row = min(r, a.rows - 1), v0 = blockIdx.x * 256;
+    const bool first = blockIdx.x == 0;
+    const f32x4 z = *reinterpret_cast<const f32x4*>(p.kept + blockIdx.x * p.panel + row * 256 + 4 * lane);
+    float m = -INFINITY, s = 0.f;
+    slice_of<64>(p.part + row, p.ld, p.parts, lane, m, s);
+    if (tid < FEW_ROWS) flags[tid] = 0;
+    taken[wave][lane] = f32x4{0.f, 0.f, 0.f, 0.f};
+    __syncthreads();
+    for (int e = tid; e < a.rows << p.kp; e += 256) {
+        const int er = e >> p.kp, j = e & (w - 1);
+        if (j < a.k && entry_id(a, er, j) >= 0 && (!a.vals || a.vals[(long long)er * a.ld_vals + j] != -INFINITY)) flags[er] = 1;
+    }
+    __syncthreads();
+    const unsigned long long on = __ballot(flags[lane] != 0);
+    const int live = __popcll(on), at = __popcll(on & ((1ull << row) - 1));
+    float top = 0.f, low = INFINITY;
+    if (a.g && lane < a.rows) {
+        const float g = fabsf(a.g[lane]);
+        const bool in = (on >> lane & 1) && g > 0.f && g < INFINITY;
+        top = in ? g : 0.f, low = in ? g : INFINITY;
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o)), low = fminf(low, __shfl_xor(low, o));
+    top = a.g ? factor(top, low) : 1.f;
+    if (first && r == 0 && lane == 0) {
+        *p.live = live;
+        p.top[0] = top;
+        p.top[1] = top / a.temperature;
+    }
+    if (r >= a.rows) return;
+    float* const zt = a.logits + (long long)row * a.k;
+    if (!(on >> row & 1)) {  // (a row left out)
+        if (!first) return;
+        if (lane < a.k) zt[lane] = 0.f;
+        if (lane == 0) a.loss[row] = a.lse[row] = 0.f;
+        if (p.dx)
+            for (int q = lane; q < a.dim / 4; q += 64) *reinterpret_cast<uint2*>(p.dx + row * a.ld_dx + 4 * q) = make_uint2(0u, 0u);
+        return;
+    }
+    wave_join(m, s);
+    const float lse = (m + __builtin_amdgcn_logf(s)) * LN2;
+    int id = lane < a.k ? entry_id(a, row, lane) : -1;
+    float q = id < 0 ? 0.f : 1.f, ent = 0.f;
+    if (a.vals) {
+        float v = lane < a.k ? a.vals[(long long)row * a.ld_vals + lane] : -INFINITY;
+        if (v == -INFINITY) id = -1;
+        if (id < 0) v = -INFINITY;
+        teacher(v, id, w, a.temperature, q, ent);
+    }
+    float all = 0.f;  // (an id that comes twice)
+    for (int i = 0; i < a.k; ++i) {
+        const float other = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(q), i));
+        if (__builtin_amdgcn_readlane(id, i) == id) all += other;
+    }
+    if (id >= v0 && id < v0 + 256) reinterpret_cast<float*>(taken[wave])[id - v0] = all;
+    __builtin_amdgcn_wave_barrier();
+    const f32x4 less = taken[wave][lane];
+    const float l2 = lse * LOG2E, gr = a.g ? a.g[row] : 1.f, gs = top > 0.f ? gr / top : gr;
+    float d[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        d[e] = v0 + 4 * lane + e < a.valid ? (__builtin_amdgcn_exp2f(__builtin_fmaf(z[e], p.sc, -l2)) - less[e]) * gs : 0.f;
+    *reinterpret_cast<uint2*>(p.dz + blockIdx.x * p.panel + at * 256 + 4 * lane) = make_uint2(cvt2(d[0], d[1]), cvt2(d[2], d[3]));
+    if (!first) return;
+    const float zj = id < 0 ? 0.f : p.kept[(id >> 8) * p.panel + row * 256 + (id & 255)];
+    if (lane < a.k) zt[lane] = zj;
+    float c = id < 0 || q == 0.f ? 0.f : q * (lse - zj * p.inv_t), loss = 0.f;
+    for (int i = 0; i < a.k; ++i) loss += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(c), i));
+    if (lane == 0) {
+        a.lse[row] = lse;
+        a.loss[row] = a.vals ? ent + loss : loss;
+        p.idx[at] = row;
+    }
+    if (live == a.rows) return;  // (x is read where it lies)
+    const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.x) + (long long)row * a.ldx);
+    uint4* dst = reinterpret_cast<uint4*>(p.xc + (long long)at * a.dim);
+#pragma unroll 8
+    for (int i = lane; i < a.dim / 8; i += 64) dst[i] = src[i];
 }
 
 struct Fix {
@@ -910,6 +1084,10 @@ __global__ __launch_bounds__(256) void hl_dx(const Finish p) {
 // --- the plan ----------------------------------------------------------------------------------------------------------
 
 constexpr long long DZ_BYTES = 1ll << 30;  // dz a piece at most
+// z of a call that is one piece (float32, 2 GB at most) is kept from the loss to dz where computing it again takes longer than
+// writing and reading it: 2048 rows x 1024 against 128256 tokens 1.88 ms kept, 2.03 again, x 768 1.59 and 1.62, x 512 1.26 and
+// 1.20, x 64 0.83 and 0.59; 4096 x 2048 6.20 and 7.29.
+constexpr int KEEP_DIM = 768;
 constexpr int MOST_TILES = (1 << 23) - 8;  // of 512 lanes: a launch holds fewer than 2^32
 
 long long up(long long v, long long to) { return (v + to - 1) / to * to; }
@@ -918,8 +1096,8 @@ struct Plan {
     int kp, piece;
     int z, y, w, d;  // the tiles of z for the statistics and for dz, of dhead and of dx
     int parts;
-    bool gather, raw, own;
-    long long ids, idc, q, ent, held, idx, pos, live, xc, part, dz, acc, bytes;
+    bool gather, raw, own, keep, few;
+    long long kept, ids, idc, q, ent, held, idx, pos, live, xc, part, dz, acc, bytes;
 };
 
 int log2_up(int k) {
@@ -995,13 +1173,17 @@ bool plan_of(const dr_head_loss* a, int what, Plan& p) {
     p.live = take(12);
     p.xc = take(p.gather ? n * a->dim * 2 : 0);
     p.part = take(what & DR_LOSS_FORWARD ? p.parts * np * 8 : 0);
-    p.piece = 0, p.dz = p.acc = 0;
+    p.piece = 0, p.dz = p.acc = p.kept = 0, p.keep = p.few = false;
     if (back) {
         // the vocabulary in equal pieces of a multiple of 256
         const long long tiles = up(a->valid, 256) / 256, fit = DZ_BYTES / (n * 512);
         const long long pieces = (tiles + (fit > 1 ? fit : 1) - 1) / (fit > 1 ? fit : 1);
         p.piece = (int)((tiles + pieces - 1) / pieces) * 256;
         p.dz = take(n * p.piece * 2);
+        p.keep = what == (DR_LOSS_FORWARD | DR_LOSS_BACKWARD) && pieces == 1 && (a->dx || a->dhead);
+        p.few = p.keep && n <= FEW_ROWS && p.parts <= FEW_PARTS;
+        p.keep = p.few || (p.keep && a->dim >= KEEP_DIM);
+        p.kept = take(p.keep ? n * p.piece * 4 : 0);
         p.y = choose_z(p.piece, n, a->dim);
         p.w = choose(EPI_DHEAD, a->dim, p.piece, n, {T256, T128});
         if (a->dx) {
@@ -1075,19 +1257,20 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
     p.idc = reinterpret_cast<int*>(ws + P.idc);
     const int eblocks = (int)((((long long)n << P.kp) + 255) / 256);
     const dim3 gblocks((n + GROWS - 1) / GROWS + 1);
-    if (!P.raw && !P.own) hipLaunchKernelGGL(hl_entries, dim3(eblocks), dim3(256), 0, st, p);
-    if (P.own) hipLaunchKernelGGL(hl_gather<true>, gblocks, dim3(256), 0, st, p);
-    else if (P.gather) hipLaunchKernelGGL(hl_gather<false>, gblocks, dim3(256), 0, st, p);
+    const bool gather = P.gather && !P.few;  // (before the products)
+    if (!P.raw && !P.own && !P.few) hipLaunchKernelGGL(hl_entries, dim3(eblocks), dim3(256), 0, st, p);
+    if (gather && P.own) hipLaunchKernelGGL(hl_gather<true>, gblocks, dim3(256), 0, st, p);
+    else if (gather) hipLaunchKernelGGL(hl_gather<false>, gblocks, dim3(256), 0, st, p);
 
     Gemm z{};  // z of a range of the vocabulary
     z.A = reinterpret_cast<const uint16_t*>(a->head);
     z.lda = a->ld_head;
-    z.B = P.gather ? p.xc : reinterpret_cast<const uint16_t*>(a->x);
-    z.ldb = P.gather ? a->dim : a->ldx;
+    z.B = gather ? p.xc : reinterpret_cast<const uint16_t*>(a->x);
+    z.ldb = gather ? a->dim : a->ldx;
     z.n = n, z.k = z.ka = a->dim;
     z.whole = P.gather ? reinterpret_cast<const uint16_t*>(a->x) : nullptr, z.ldx = a->ldx, z.rows = n;
-    z.live = P.gather ? p.live : nullptr;
-    z.idx = P.gather ? p.idx : nullptr;
+    z.live = gather ? p.live : nullptr;
+    z.idx = gather ? p.idx : nullptr;
     z.sc = LOG2E / a->temperature;
     z.ids = P.gather ? p.idc : p.ids, z.kp = P.kp, z.kn = kn;
     z.raw = P.raw ? a->ids : nullptr, z.raw64 = a->ids64;
@@ -1098,10 +1281,18 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
         s.part = reinterpret_cast<f32x2*>(ws + P.part);
         s.ld_part = up(n, 64);
         s.zt = a->logits;
+        s.kept = P.keep ? reinterpret_cast<float*>(ws + P.kept) : nullptr;
+        s.panel = (long long)n * 256;
         launch_z<EPI_STATS>(s, P.z, st);
         Merge m{s.part, s.ld_part, P.parts, n, kn, P.kp, P.gather ? p.pos : nullptr, P.raw ? nullptr : p.held, a->ids,
-                a->ids64, a->valid, p.ids, p.q, p.ent, 1.f / a->temperature, a->loss, a->lse, a->logits};
-        if (n <= 64) hipLaunchKernelGGL((hl_merge<1, 256>), dim3(n), dim3(256), 0, st, m);
+                a->ids64, a->valid, p.ids, p.q, p.ent, 1.f / a->temperature, a->loss, a->lse, a->logits, s.kept, s.panel};
+        if (P.few) {
+            Few f{*a, P.kp, P.parts, s.part, s.ld_part, s.kept, reinterpret_cast<uint16_t*>(ws + P.dz), s.panel, z.sc,
+                  1.f / a->temperature, p.idx, p.live, p.top, p.xc, p.dx};
+            hipLaunchKernelGGL(hl_few, dim3((a->valid + 255) / 256, (n + 3) / 4), dim3(256), 0, st, f);
+        } else if (n <= 64 && P.parts <= FEW_PARTS) {
+            hipLaunchKernelGGL((hl_merge<1, 64>), dim3(n), dim3(64), 0, st, m);
+        } else if (n <= 64) hipLaunchKernelGGL((hl_merge<1, 256>), dim3(n), dim3(256), 0, st, m);
         else hipLaunchKernelGGL((hl_merge<32, 32>), dim3((n + 31) / 32), dim3(1024), 0, st, m);
     }
     if (back && (a->dx || a->dhead)) {
@@ -1115,12 +1306,18 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
             s.v0 = v0;
             s.out = dz;
             s.panel = panel;
-            if (a->vals) {
+            if (P.keep && !P.few) {
+                Dz d{p.live, p.idx, a->vals ? nullptr : p.idc, reinterpret_cast<const float*>(ws + P.kept), a->lse, a->g, p.top,
+                     dz, panel, vn, z.sc};
+                hipLaunchKernelGGL(hl_dz, dim3((vn + 255) / 256, (n + 4 * DZ_ROWS - 1) / (4 * DZ_ROWS)), dim3(256), 0, st, d);
+            } else if (!P.few && a->vals) {
                 launch_z<EPI_DZ>(s, P.y, st);
+            } else if (!P.few) {
+                launch_z<EPI_DZ1>(s, P.y, st);
+            }
+            if (a->vals && !P.few) {
                 Fix f{p.live, p.idx, p.ids, p.q, a->lse, a->logits, a->g, p.top, kn, P.kp, v0, v0 + vn, z.sc, dz, panel};
                 hipLaunchKernelGGL(hl_fix, dim3(eblocks), dim3(256), 0, st, f);
-            } else {
-                launch_z<EPI_DZ1>(s, P.y, st);
             }
             if (a->dhead) {
                 Gemm w{};

@@ -27,18 +27,16 @@ constexpr int MAXE = 1024;  // experts
 
 struct Bal {
     dr_balance a;
-    float2* sums;  // [batch][groups][E] sum of p, count (its bits)
-    int* live;     // [batch][groups] rows that count
-    int groups;    // workgroups a batch
-    const float2* in;    // [batch][parts][E], [batch][parts]: the sums to be joined, the workgroups' or (parts 1) balance_slice_k's
-    const int* in_live;
+    float2* sums;         // [batch][groups][E] sum of p, count (its bits)
+    int* live;            // [batch][groups] rows that count
+    int groups;           // workgroups a batch
+    const float2* in;     // [batch][parts][E], [batch][parts]: the sums to be joined, the workgroups' own or (parts 1) what
+    const int* in_live;   //     balance_slice_k made of them
     int parts;
-    int vec;       // the logits' rows can be read 16 bytes at a time
-    int gvec;      // and dlogits' written so
+    int vec;              // the logits' rows can be read 16 bytes at a time
+    int gvec;             // and dlogits' written so
 };
 
-// v of the lane that a row's DPP control names: neighbours, pairs, the quads and the halves of 16 lanes changed over. (A turn is
-// a few cycles; the general shuffle, through LDS, about a hundred, and a row takes twelve to twenty of them one after another.)
 template <int CONTROL>
 __device__ __forceinline__ float turned(float v) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CONTROL, 0xF, 0xF, true));

@@ -144,6 +144,41 @@ def test_distill(device, n, v, valid, d, k, t):
     same("the loss alone", head_loss.distill_loss(x, head, vals, ids, temperature=t, valid=valid), out[0])
 
 
+@pytest.mark.parametrize("n, v, valid, d, k", [
+    (100, 700, 690, 768, 0), (70, 257, 257, 2048, 0), (300, 5003, 5000, 1024, 0), (2100, 2900, 2899, 776, 0),
+    (600, 20000, 19990, 800, 0), (100, 700, 690, 768, 64), (70, 257, 257, 2048, 1), (300, 5003, 5000, 1024, 5),
+    (2100, 2900, 2899, 776, 16), (600, 20000, 19990, 800, 2), (64, 32768, 32768, 64, 0), (64, 32769, 32769, 64, 0),
+    (64, 32768, 32760, 64, 64), (63, 40000, 40000, 72, 7), (5, 300, 299, 8, 64), (64, 513, 512, 1024, 3),
+])
+def test_logits_kept_for_the_gradient(device, n, v, valid, d, k):
+    """Many values a row, and few rows: the gradient is made of the loss's own logits. Some rows are left out, one id comes in
+    every slot, weights and vocabularies of any size."""
+    x, head, w, g = inputs(device, n, v, d, n + v + d + k)
+    w[0] = -2.0
+    if k:
+        ids, vals = teacher(n, k, valid, g, device)
+        ids[1], vals[2], ids[3] = 7, -math.inf, -1
+        x[2:4] = math.nan
+        run = lambda fn, *a, **kw: fn(x, head, vals, ids, *a, temperature=1.5, valid=valid, **kw)
+        loss, grads = head_loss.distill_loss, head_loss.distill_loss_grads
+        want = expected(x, head, ids, vals, 1.5, valid, w)
+    else:
+        ids = torch.randint(0, valid, (n,), generator=g)
+        ids[torch.rand(n, generator=g) < 0.2] = -100
+        ids[0], ids[1], ids[2] = valid, valid - 1, 0
+        ids = ids.to(device.torch)
+        x[0] = math.nan
+        run = lambda fn, *a, **kw: fn(x, head, ids, *a, valid=valid, **kw)
+        loss, grads = head_loss.token_loss, head_loss.token_loss_grads
+        want = expected(x, head, ids, None, 1.0, valid, w)
+    out = run(grads, w)
+    check(f"{n} x {v} ({valid}) x {d}, {k} entries", out, want)
+    same("the loss alone", run(loss), out[0])
+    same("dx alone", run(grads, w, head_grad=False)[1], out[1])
+    same("dhead alone", run(grads, w, x_grad=False)[2], out[2])
+    same("again", run(grads, w)[1], out[1])
+
+
 @pytest.mark.parametrize("k", [0, 4])
 def test_pieces_of_the_vocabulary(device, k):
     """So many rows and tokens that the logits' gradient comes in two pieces: dx sums over both, dhead's rows come from each,

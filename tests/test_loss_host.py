@@ -108,6 +108,9 @@ def test_head_loss_workspace_keeps_no_logits():
     assert sizes[1] < 1.2 * sizes[0] and sizes[0] < 65536 * 128256 * 2 / 4, sizes
     fwd = _lib.lib().dr_head_loss_workspace_bytes(ctypes.byref(_head(**big, vocab=128256, valid=128256)), 1)
     assert fwd < 65536 * 128256 * 4 / 16, fwd
+    both = [_lib.lib().dr_head_loss_workspace_bytes(ctypes.byref(_head(**big, vocab=v, valid=v)), 3) for v in (8192, 128256)]
+    kept = 65536 * 8192 * 4  # (one piece: 2 GiB)
+    assert kept < both[0] < 2 * kept and both[1] < sizes[0] + 1.1 * fwd, both
 
 
 def _balance(**kw):

@@ -931,9 +931,16 @@ struct Few {
 // Few rows (one a wavefront and panel), from z as the loss left it: what hl_gather, hl_merge, hl_dz and hl_fix do, in one launch.
 // Every wavefront joins its row's tiles for itself and counts the rows that count from all of the ids; the first panel's write
 // what there is one of.
-constexpr int FEW_ROWS = 64, FEW_PARTS = 512;  // (a ballot's; eight parts a lane)
+constexpr int FEW_ROWS = 256, FEW_PARTS = 512, FEW_IDS = 4096;
+// (every panel's wavefronts join the parts again: 64 rows x 1024 against 16384 tokens, 256 parts, 42.2 us, 49.0 in launches of
+// their own; against 32768 65.4 and 64.7; 128 rows against 8192 37.7 and 45.7, 16384 57.4 and 56.4)
+constexpr int FEW_JOINS = 16384;
+__host__ __device__ inline bool few_parts(int rows, int parts) {
+    return rows <= FEW_ROWS && parts <= FEW_PARTS && rows * parts <= FEW_JOINS;
+}
 __global__ __launch_bounds__(256) void hl_few(const Few p) {
     __shared__ uint32_t flags[FEW_ROWS];
+    static_assert(FEW_ROWS == 256, "a flag a lane");
     __shared__ f32x4 taken[4][64];  // the entries' q in the wavefront's panel
     const dr_head_loss& a = p.a;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), w = 1 << p.kp;
@@ -942,7 +949,7 @@ __global__ __launch_bounds__(256) void hl_few(const Few p) {
     const f32x4 z = *reinterpret_cast<const f32x4*>(p.kept + blockIdx.x * p.panel + row * 256 + 4 * lane);
     float m = -INFINITY, s = 0.f;
     slice_of<64>(p.part + row, p.ld, p.parts, lane, m, s);
-    if (tid < FEW_ROWS) flags[tid] = 0;
+    flags[tid] = 0;
     taken[wave][lane] = f32x4{0.f, 0.f, 0.f, 0.f};
     __syncthreads();
     for (int e = tid; e < a.rows << p.kp; e += 256) {
@@ -950,13 +957,19 @@ __global__ __launch_bounds__(256) void hl_few(const Few p) {
         if (j < a.k && entry_id(a, er, j) >= 0 && (!a.vals || a.vals[(long long)er * a.ld_vals + j] != -INFINITY)) flags[er] = 1;
     }
     __syncthreads();
-    const unsigned long long on = __ballot(flags[lane] != 0);
-    const int live = __popcll(on), at = __popcll(on & ((1ull << row) - 1));
+    int live = 0, at = 0;  // the rows that count; those before this one
+    bool in = false;
     float top = 0.f, low = INFINITY;
-    if (a.g && lane < a.rows) {
-        const float g = fabsf(a.g[lane]);
-        const bool in = (on >> lane & 1) && g > 0.f && g < INFINITY;
-        top = in ? g : 0.f, low = in ? g : INFINITY;
+#pragma unroll
+    for (int i = 0; i < FEW_ROWS / 64; ++i) {
+        const bool mine = flags[64 * i + lane] != 0;
+        const unsigned long long on = __ballot(mine);
+        const int here = row - 64 * i;
+        live += __popcll(on);
+        at += here >= 64 ? __popcll(on) : here > 0 ? __popcll(on & ((1ull << here) - 1)) : 0;
+        in |= here >= 0 && here < 64 && (on >> (here & 63) & 1);
+        const float g = a.g && mine ? fabsf(a.g[64 * i + lane]) : 0.f;
+        if (g > 0.f && g < INFINITY) top = fmaxf(top, g), low = fminf(low, g);
     }
 #pragma unroll
     for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o)), low = fminf(low, __shfl_xor(low, o));
@@ -968,7 +981,7 @@ __global__ __launch_bounds__(256) void hl_few(const Few p) {
     }
     if (r >= a.rows) return;
     float* const zt = a.logits + (long long)row * a.k;
-    if (!(on >> row & 1)) {  // (a row left out)
+    if (!in) {  // (a row left out)
         if (!first) return;
         if (lane < a.k) zt[lane] = 0.f;
         if (lane == 0) a.loss[row] = a.lse[row] = 0.f;
@@ -1181,7 +1194,7 @@ bool plan_of(const dr_head_loss* a, int what, Plan& p) {
         p.piece = (int)((tiles + pieces - 1) / pieces) * 256;
         p.dz = take(n * p.piece * 2);
         p.keep = what == (DR_LOSS_FORWARD | DR_LOSS_BACKWARD) && pieces == 1 && (a->dx || a->dhead);
-        p.few = p.keep && n <= FEW_ROWS && p.parts <= FEW_PARTS;
+        p.few = p.keep && few_parts((int)n, p.parts) && n << p.kp <= FEW_IDS;
         p.keep = p.few || (p.keep && a->dim >= KEEP_DIM);
         p.kept = take(p.keep ? n * p.piece * 4 : 0);
         p.y = choose_z(p.piece, n, a->dim);
@@ -1290,7 +1303,7 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
             Few f{*a, P.kp, P.parts, s.part, s.ld_part, s.kept, reinterpret_cast<uint16_t*>(ws + P.dz), s.panel, z.sc,
                   1.f / a->temperature, p.idx, p.live, p.top, p.xc, p.dx};
             hipLaunchKernelGGL(hl_few, dim3((a->valid + 255) / 256, (n + 3) / 4), dim3(256), 0, st, f);
-        } else if (n <= 64 && P.parts <= FEW_PARTS) {
+        } else if (few_parts(n, P.parts)) {  // (in hl_few's order: the loss alone is the same)
             hipLaunchKernelGGL((hl_merge<1, 64>), dim3(n), dim3(64), 0, st, m);
         } else if (n <= 64) hipLaunchKernelGGL((hl_merge<1, 256>), dim3(n), dim3(256), 0, st, m);
         else hipLaunchKernelGGL((hl_merge<32, 32>), dim3((n + 31) / 32), dim3(1024), 0, st, m);

@@ -149,6 +149,8 @@ def test_distill(device, n, v, valid, d, k, t):
     (600, 20000, 19990, 800, 0), (100, 700, 690, 768, 64), (70, 257, 257, 2048, 1), (300, 5003, 5000, 1024, 5),
     (2100, 2900, 2899, 776, 16), (600, 20000, 19990, 800, 2), (64, 32768, 32768, 64, 0), (64, 32769, 32769, 64, 0),
     (64, 32768, 32760, 64, 64), (63, 40000, 40000, 72, 7), (5, 300, 299, 8, 64), (64, 513, 512, 1024, 3),
+    (256, 1000, 999, 64, 0), (129, 2900, 2899, 264, 0), (193, 600, 600, 72, 16), (256, 1000, 1000, 64, 17),
+    (257, 600, 600, 64, 0),
 ])
 def test_logits_kept_for_the_gradient(device, n, v, valid, d, k):
     """Many values a row, and few rows: the gradient is made of the loss's own logits. Some rows are left out, one id comes in

@@ -429,9 +429,9 @@ def test_gradients_against_differences(device):
         assert abs(mine - slope) <= slack, (which, mine, slope, slack)
 
 
-def test_repeats_streams_and_graphs(device):
+@pytest.mark.parametrize("n, v, d", [(200, 1500, 136), (600, 3000, 136), (600, 3000, 776)])
+def test_repeats_streams_and_graphs(device, n, v, d):
     """The same call twice, on another stream, and replayed in two graphs with eager work between: bit for bit."""
-    n, v, d = 200, 1500, 136
     x, head, w, g = inputs(device, n, v, d, 13)
     ids = torch.randint(-100, v, (n,), generator=g).to(device.torch)
     ti, tv = teacher(n, 8, v, g, device)

@@ -96,7 +96,7 @@ struct Gemm {
     int raw64;
     int kp, kn;
     float* zt;              // [rows][kn]
-    float* kept;            // z itself for hl_dz, in panels as dz, or NULL
+    float* kept;            // KEEP: z itself, in panels as dz
     // outputs
     uint16_t* out;          // dz (panels), dhead [n = v][ld_out], dx [row][ld_out] or NULL: the sums are not complete
     long long ld_out;
@@ -177,7 +177,8 @@ struct Tile {
 // the memory and the power are shared) and for its beginning and end, as many workgroups at once as fit the CUs. Fitted to the
 // kernels' times at eight shapes of 73 to 8192 rows, 584 to 4096 values and 2898 to 94639 tokens, most within 15 %; what
 // decides between two tiles is mostly how many rounds they take.
-enum Epi { EPI_STATS, EPI_DZ, EPI_DZ1, EPI_DHEAD, EPI_DX };  // (DZ1: tokens, their own logit's 1 taken off there)
+// (KEEP: the statistics, z kept instead of the entries' taken; DZ1: tokens, their own logit's 1 taken off there)
+enum Epi { EPI_STATS, EPI_KEEP, EPI_DZ, EPI_DZ1, EPI_DHEAD, EPI_DX };
 struct Pace {
     int at_once;
     float step, shared, ends;
@@ -253,7 +254,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void hl_gemm(const Gemm a) {
     constexpr int C1 = NS > 1 ? CH * WK : 1, C2 = NS > 2 ? CH * WK : 1, C3 = NS > 3 ? CH * WK : 1;
     // (an array each, named where it is used: a read waits for the loads to every array that the compiler cannot rule out)
     __shared__ uint4 s0[CH * WK], s1[C1], s2[C2], s3[C3];
-    __shared__ f32x2 stat[EPI == EPI_STATS ? WM : 1][EPI == EPI_STATS ? BN : 1];
+    constexpr bool STATS = EPI == EPI_STATS || EPI == EPI_KEEP;
+    __shared__ f32x2 stat[STATS ? WM : 1][STATS ? BN : 1];
     // WK groups of wavefronts, each a share of K in stages of its own, all with the same barriers; tid within the group
     const int group = WK == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / NT), tid = threadIdx.x - group * NT;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), mine = group * CH;
@@ -276,7 +278,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void hl_gemm(const Gemm a) {
 
     Tile<BM, AT, NT, BK> ta;
     Tile<BN, BT, NT, BK> tb;
-    constexpr bool X_A = EPI == EPI_DHEAD, X_B = EPI == EPI_STATS || EPI == EPI_DZ || EPI == EPI_DZ1;
+    constexpr bool X_A = EPI == EPI_DHEAD, X_B = STATS || EPI == EPI_DZ || EPI == EPI_DZ1;
     const bool whole = (X_A || X_B) && a.whole && live == a.rows;
     const uint16_t *A = X_A && whole ? a.whole : a.A, *B = X_B && whole ? a.whole : a.B;
     const long long la = X_A && whole ? a.ldx : a.lda, lb = X_B && whole ? a.ldx : a.ldb;
@@ -430,7 +432,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void hl_gemm(const Gemm a) {
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
         const int nj = n0 + wn * TN + 32 * j, n = nj + r;
-        if constexpr (EPI == EPI_STATS) {
+        if constexpr (STATS) {
             const int left = a.m - mw;  // vocabulary rows of this wavefront
             if (left < TM) {
 #pragma unroll
@@ -470,14 +472,15 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void hl_gemm(const Gemm a) {
                 const long long row = a.idx ? a.idx[nj + t] : nj + t;
                 a.zt[row * a.kn + kk] = mine[t * (TM / 4) + ((d >> 2) ^ (t & 7))][d & 3];
             };
-            if (a.kept) {  // (the entries are read from it)
+            if constexpr (EPI == EPI_KEEP) {  // (the entries are read from it)
                 lay();
                 constexpr int C4 = TM / 4, PC = 64 / C4;  // 16-byte chunks a column, columns a turn
                 float* o = a.kept + (mw >> 8) * a.panel + (long long)nj * 256 + (mw & 255);
 #pragma unroll 2
                 for (int t = 0; t < 32 / PC; ++t) {
                     const int c = t * PC + lane / C4, q = lane % C4;
-                    if (nj + c < n_end) *reinterpret_cast<f32x4*>(o + c * 256 + 4 * q) = mine[c * C4 + (q ^ (c & 7))];
+                    if (nj + c < n_end)  // (read once, much later)
+                        __builtin_nontemporal_store(mine[c * C4 + (q ^ (c & 7))], reinterpret_cast<f32x4*>(o + c * 256 + 4 * q));
                 }
             } else if (a.kp < 2) {
                 const int t = lane >> a.kp;
@@ -591,7 +594,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void hl_gemm(const Gemm a) {
                 }
         }
     }
-    if constexpr (EPI == EPI_STATS) {  // the wavefronts' rows of a column together
+    if constexpr (STATS) {  // the wavefronts' rows of a column together
         __syncthreads();
         if (wm == 0 && h == 0) {
 #pragma unroll
@@ -896,7 +899,7 @@ __global__ __launch_bounds__(256) void hl_dz(const Dz p) {
     const long long at = blockIdx.x * p.panel + (long long)n0 * 256 + 4 * lane;
     f32x4 z[DZ_ROWS];
 #pragma unroll
-    for (int i = 0; i < DZ_ROWS; ++i) z[i] = *reinterpret_cast<const f32x4*>(p.z + at + min(i, live - 1 - n0) * 256);
+    for (int i = 0; i < DZ_ROWS; ++i) z[i] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p.z + at + min(i, live - 1 - n0) * 256));
 #pragma unroll
     for (int i = 0; i < DZ_ROWS; ++i) {
         const int n = n0 + i;
@@ -1296,7 +1299,8 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
         s.zt = a->logits;
         s.kept = P.keep ? reinterpret_cast<float*>(ws + P.kept) : nullptr;
         s.panel = (long long)n * 256;
-        launch_z<EPI_STATS>(s, P.z, st);
+        if (P.keep) launch_z<EPI_KEEP>(s, P.z, st);
+        else launch_z<EPI_STATS>(s, P.z, st);
         Merge m{s.part, s.ld_part, P.parts, n, kn, P.kp, P.gather ? p.pos : nullptr, P.raw ? nullptr : p.held, a->ids,
                 a->ids64, a->valid, p.ids, p.q, p.ent, 1.f / a->temperature, a->loss, a->lse, a->logits, s.kept, s.panel};
         if (P.few) {

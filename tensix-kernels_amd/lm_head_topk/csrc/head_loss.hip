@@ -1346,7 +1346,9 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
                 w.out = reinterpret_cast<uint16_t*>(a->dhead) + (long long)v0 * a->ld_dhead;
                 w.ld_out = a->ld_dhead;
                 w.scale = p.top + 1;
-                if (n <= KSTEP) launch<128, 128, 2, 2, 1, 1, 64, true, true, EPI_DHEAD>(w, st);
+                // (few steps: one stage and five workgroups a CU instead of four and two; 400 rows x 2880 against 50257 tokens, dx
+                // aside, 365 us and 382, 1003 rows 709 and 711, 1500 x 1024 against 8192 98.7 and 94.0)
+                if (n <= KSTEP || (P.w == T128 && n <= 1024)) launch<128, 128, 2, 2, 1, 1, 64, true, true, EPI_DHEAD>(w, st);
                 else if (P.w == T256) launch<256, 256, 2, 4, 1, 4, 32, true, true, EPI_DHEAD>(w, st);
                 else launch<128, 128, 2, 2, 1, 4, 32, true, true, EPI_DHEAD>(w, st);
             }

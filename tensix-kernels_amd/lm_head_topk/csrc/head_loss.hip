@@ -681,27 +681,30 @@ __device__ __forceinline__ int wave_sum(int v) {
     return v;
 }
 
+constexpr int GROWS = 4;     // rows a workgroup of hl_gather, one a wavefront
+constexpr int MANY = 32768;  // rows past which it takes 64, and looks through the flags a sixteenth as often (2^18 rows x 64
+                             // against 300 tokens, the whole call: 1.97 ms, 2.50 by 4; 2^20 8.97 and 17.0; 2^15 the same)
+constexpr int FEW = 2048;    // entries that every workgroup looks through itself
+
 // the factor taken out of dz, of the rows' weights that count (positive, finite) the largest; weights so far apart that the
 // smallest over the largest would near the smallest float32: as they are
 __device__ __forceinline__ float factor(float top, float low) { return low > top * 0x1p-40f ? top : 1.f; }
 
-constexpr int GROWS = 4;     // rows a workgroup of hl_gather, one a wavefront
-constexpr int FEW = 2048;    // entries that every workgroup looks through itself
 
 // The rows that count, one after another: each workgroup finds the place of its own from the flags of all rows before
 // (16 a load), so that nothing waits for anything; one more finds how many there are and the largest |g|. Where every row
-// counts none is copied. OWN: the entries
-// too, of few rows, every workgroup looking through all of the ids for the flags (a launch less).
-template <bool OWN>
+// counts none is copied. OWN: the entries too, of few rows, every workgroup looking through all of the ids for the flags (a
+// launch less).
+template <bool OWN, int GR>
 __global__ __launch_bounds__(256) void hl_gather(const Prep p) {
     __shared__ int sums[4];
     __shared__ float tops[4], lows[4];
-    __shared__ int rows[GROWS];
+    __shared__ int rows[GR];
     __shared__ uint4 flag4[OWN ? FEW / 16 : 1];
     uint8_t* const flags = reinterpret_cast<uint8_t*>(flag4);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = p.a.rows;
     const bool last = blockIdx.x == gridDim.x - 1;
-    const int r0 = last ? n : blockIdx.x * GROWS;
+    const int r0 = last ? n : blockIdx.x * GR;
     const uint8_t* held = p.held;
     if constexpr (OWN) {
         for (int i = tid; i < FEW / 16; i += 256) flag4[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -715,7 +718,7 @@ __global__ __launch_bounds__(256) void hl_gather(const Prep p) {
         __syncthreads();
         held = flags;
         if (!last)
-            for (int e = tid; e < GROWS << p.kp; e += 256) entries_of(p, (r0 << p.kp) + e, min(n, r0 + GROWS));
+            for (int e = tid; e < GR << p.kp; e += 256) entries_of(p, (r0 << p.kp) + e, min(n, r0 + GR));
     }
     int c = 0, out = 0;  // rows that count before this workgroup's; rows left out, all of them
     for (int i = tid; i < n / 16; i += 256) {
@@ -756,24 +759,24 @@ __global__ __launch_bounds__(256) void hl_gather(const Prep p) {
     }
     if (wave == 0) {
         const int r = r0 + lane;
-        const bool on = lane < GROWS && r < n && held[r] != 0;
+        const bool on = lane < GR && r < n && held[r] != 0;
         const unsigned long long b = __ballot(on);
         const int at = before + __popcll(b & ((1ull << lane) - 1));
-        if (lane < GROWS) rows[lane] = on ? at : -1;
-        if (lane < GROWS && r < n) p.pos[r] = on ? at : -1;
+        if (lane < GR) rows[lane] = on ? at : -1;
+        if (lane < GR && r < n) p.pos[r] = on ? at : -1;
         if (on) p.idx[at] = r;
     }
     __syncthreads();  // (OWN: this workgroup's entries are written too)
-    {
-        const int i = wave, at = rows[i];
+    for (int i = wave; i < GR; i += 4) {
+        const int at = rows[i];
         if (at < 0) {
             if (p.dx && r0 + i < n)  // (a row left out)
                 for (int q = lane; q < p.a.dim / 4; q += 64)
                     *reinterpret_cast<uint2*>(p.dx + (r0 + i) * p.a.ld_dx + 4 * q) = make_uint2(0u, 0u);
-            return;
+            continue;
         }
         if (lane < 1 << p.kp) p.idc[((long long)at << p.kp) + lane] = p.ids[((long long)(r0 + i) << p.kp) + lane];
-        if (!some) return;  // (every row counts: x is read where it lies)
+        if (!some) continue;  // (every row counts: x is read where it lies)
         const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.a.x) + (r0 + i) * p.a.ldx);
         uint4* dst = reinterpret_cast<uint4*>(p.xc + (long long)at * p.a.dim);
 #pragma unroll 8
@@ -1283,8 +1286,9 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
     const dim3 gblocks((n + GROWS - 1) / GROWS + 1);
     const bool gather = P.gather && !P.few;  // (before the products)
     if (!P.raw && !P.own && !P.few) hipLaunchKernelGGL(hl_entries, dim3(eblocks), dim3(256), 0, st, p);
-    if (gather && P.own) hipLaunchKernelGGL(hl_gather<true>, gblocks, dim3(256), 0, st, p);
-    else if (gather) hipLaunchKernelGGL(hl_gather<false>, gblocks, dim3(256), 0, st, p);
+    if (gather && P.own) hipLaunchKernelGGL((hl_gather<true, GROWS>), gblocks, dim3(256), 0, st, p);
+    else if (gather && n <= MANY) hipLaunchKernelGGL((hl_gather<false, GROWS>), gblocks, dim3(256), 0, st, p);
+    else if (gather) hipLaunchKernelGGL((hl_gather<false, 64>), dim3((n + 63) / 64 + 1), dim3(256), 0, st, p);
 
     Gemm z{};  // z of a range of the vocabulary
     z.A = reinterpret_cast<const uint16_t*>(a->head);

@@ -58,9 +58,10 @@ int dr_head_pick_records(const void* records, int n_records, int rows, int k, in
  *
  * Gradients of sum over rows of g[row] * loss[row]: dz[v] = g / T (p[v] - sum of q over entries of id v), p = exp(z / T -
  * lse); dx = dz . head, dhead = dz^T . x (rows valid .. vocab - 1 zeros). Piece by piece of the vocabulary (dz to 1 GiB)
- * z is computed again; a call of both directions and one piece may keep it in its workspace instead. dz is rounded to
+ * z is computed again; a call of one piece may keep it in its workspace instead. dz is rounded to
  * bf16 (divided by the largest |g| of the rows that count, which the float32 sums get back, unless their weights lie
- * further apart than 2^40), the sums are float32, dx and dhead rounded once.
+ * further apart than 2^40; up to 32 rows and one piece, what that leaves is rounded and summed too), the sums are
+ * float32, dx and dhead rounded once.
  *
  * No counterpart in the reference, which has no training: the head and the teacher's records are its
  * lm_head_topk/head_pick.py:43-52 and dense_reader/linear.py:747-768.

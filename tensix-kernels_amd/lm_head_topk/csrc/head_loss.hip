@@ -928,12 +928,29 @@ struct Few {
     long long ld;
     const float* kept;
     uint16_t* dz;
-    long long panel;
+    long long panel, dz_panel;
     float sc, inv_t;
     int *idx, *live;
     float* top;
     uint16_t *xc, *dx;
+    int fine;  // what dz's rounding leaves, rounded too, as so many rows more (of x as well)
 };
+
+// a row's tiles' maxima and sums joined, in hl_merge<1, 256>'s order: one part a row for hl_few
+__global__ __launch_bounds__(256) void hl_join(const f32x2* part, long long ld, int parts, f32x2* out) {
+    __shared__ float ms[4], ss[4];
+    const int tid = threadIdx.x;
+    float m = -INFINITY, s = 0.f;
+    slice_of<256>(part + blockIdx.x, ld, parts, tid, m, s);
+    wave_join(m, s);
+    if ((tid & 63) == 0) ms[tid >> 6] = m, ss[tid >> 6] = s;
+    __syncthreads();
+    if (tid) return;
+    join(ms[0], ss[0], ms[2], ss[2]);
+    join(ms[1], ss[1], ms[3], ss[3]);
+    join(ms[0], ss[0], ms[1], ss[1]);
+    out[blockIdx.x] = f32x2{ms[0], ss[0]};
+}
 
 // Few rows (one a wavefront and panel), from z as the loss left it: what hl_gather, hl_merge, hl_dz and hl_fix do, in one launch.
 // Every wavefront joins its row's tiles for itself and counts the rows that count from all of the ids; the first panel's write
@@ -982,7 +999,7 @@ __global__ __launch_bounds__(256) void hl_few(const Few p) {
     for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o)), low = fminf(low, __shfl_xor(low, o));
     top = a.g ? factor(top, low) : 1.f;
     if (first && r == 0 && lane == 0) {
-        *p.live = live;
+        *p.live = p.fine ? 2 * live : live;
         p.top[0] = top;
         p.top[1] = top / a.temperature;
     }
@@ -990,8 +1007,8 @@ __global__ __launch_bounds__(256) void hl_few(const Few p) {
     float* const zt = a.logits + (long long)row * a.k;
     if (!in) {  // (a row left out)
         if (!first) return;
-        if (lane < a.k) zt[lane] = 0.f;
-        if (lane == 0) a.loss[row] = a.lse[row] = 0.f;
+        if (a.loss && lane < a.k) zt[lane] = 0.f;
+        if (a.loss && lane == 0) a.loss[row] = a.lse[row] = 0.f;
         if (p.dx)
             for (int q = lane; q < a.dim / 4; q += 64) *reinterpret_cast<uint2*>(p.dx + row * a.ld_dx + 4 * q) = make_uint2(0u, 0u);
         return;
@@ -1019,22 +1036,36 @@ __global__ __launch_bounds__(256) void hl_few(const Few p) {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         d[e] = v0 + 4 * lane + e < a.valid ? (__builtin_amdgcn_exp2f(__builtin_fmaf(z[e], p.sc, -l2)) - less[e]) * gs : 0.f;
-    *reinterpret_cast<uint2*>(p.dz + blockIdx.x * p.panel + at * 256 + 4 * lane) = make_uint2(cvt2(d[0], d[1]), cvt2(d[2], d[3]));
-    if (!first) return;
-    const float zj = id < 0 ? 0.f : p.kept[(id >> 8) * p.panel + row * 256 + (id & 255)];
-    if (lane < a.k) zt[lane] = zj;
-    float c = id < 0 || q == 0.f ? 0.f : q * (lse - zj * p.inv_t), loss = 0.f;
-    for (int i = 0; i < a.k; ++i) loss += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(c), i));
-    if (lane == 0) {
-        a.lse[row] = lse;
-        a.loss[row] = a.vals ? ent + loss : loss;
-        p.idx[at] = row;
+    const uint2 hi = make_uint2(cvt2(d[0], d[1]), cvt2(d[2], d[3]));
+    uint16_t* const dz = p.dz + blockIdx.x * p.dz_panel + 4 * lane;
+    *reinterpret_cast<uint2*>(dz + at * 256) = hi;
+    if (p.fine) {
+        d[0] -= __uint_as_float(hi.x << 16), d[1] -= __uint_as_float(hi.x & 0xFFFF0000u);
+        d[2] -= __uint_as_float(hi.y << 16), d[3] -= __uint_as_float(hi.y & 0xFFFF0000u);
+        *reinterpret_cast<uint2*>(dz + (live + at) * 256) = make_uint2(cvt2(d[0], d[1]), cvt2(d[2], d[3]));
     }
-    if (live == a.rows) return;  // (x is read where it lies)
+    if (!first) return;
+    if (lane == 0) p.idx[at] = row;
+    if (a.loss) {
+        const float zj = id < 0 ? 0.f : p.kept[(id >> 8) * p.panel + row * 256 + (id & 255)];
+        if (lane < a.k) zt[lane] = zj;
+        const float c = id < 0 || q == 0.f ? 0.f : q * (lse - zj * p.inv_t);
+        float loss = 0.f;
+        for (int i = 0; i < a.k; ++i) loss += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(c), i));
+        if (lane == 0) {
+            a.lse[row] = lse;
+            a.loss[row] = a.vals ? ent + loss : loss;
+        }
+    }
+    if (live == a.rows && !p.fine) return;  // (x is read where it lies)
     const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.x) + (long long)row * a.ldx);
-    uint4* dst = reinterpret_cast<uint4*>(p.xc + (long long)at * a.dim);
-#pragma unroll 8
-    for (int i = lane; i < a.dim / 8; i += 64) dst[i] = src[i];
+    uint4 *dst = reinterpret_cast<uint4*>(p.xc + (long long)at * a.dim), *more = dst + (long long)live * (a.dim / 8);
+#pragma unroll 4
+    for (int i = lane; i < a.dim / 8; i += 64) {
+        const uint4 v = src[i];
+        dst[i] = v;
+        if (p.fine) more[i] = v;
+    }
 }
 
 struct Fix {
@@ -1080,23 +1111,26 @@ struct Finish {
     const float* scale;
     uint16_t* dx;
     long long ld_dx;
+    int fine;  // two rows of sums each
 };
 
 // dx from the splits' sums (none: it is there): 256 columns of a row at a time, a quarter of the splits a wavefront
 __global__ __launch_bounds__(256) void hl_dx(const Finish p) {
     __shared__ f32x4 part[4][64];
     const int live = *p.live, splits = dx_splits(pace(EPI_DX, p.bm, p.bn, p.wk), p.tm * ((live + p.bn - 1) / p.bn), p.steps, p.bm * p.bn * 4);
-    if (splits == 1) return;
+    if (splits == 1 && !p.fine) return;
+    const int sums = splits << p.fine, rows = live >> p.fine;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, cols = (p.dim + 255) / 256;
     const float s = *p.scale;
     const long long stride = (long long)live * p.dim;
-    for (int w = blockIdx.x; w < live * cols; w += gridDim.x) {
+    for (int w = blockIdx.x; w < rows * cols; w += gridDim.x) {
         const int n = w / cols, d = 256 * (w - n * cols) + 4 * lane;
         f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
         if (d < p.dim) {
             const float* at = p.acc + (long long)n * p.dim + d;
 #pragma unroll 8
-            for (int i = wave; i < splits; i += 4) v += *reinterpret_cast<const f32x4*>(at + i * stride);
+            for (int i = wave; i < sums; i += 4)
+                v += *reinterpret_cast<const f32x4*>(at + (i >> p.fine) * stride + (i & p.fine) * (long long)rows * p.dim);
         }
         part[wave][lane] = v;
         __syncthreads();
@@ -1115,6 +1149,11 @@ constexpr long long DZ_BYTES = 1ll << 30;  // dz a piece at most
 // writing and reading it: 2048 rows x 1024 against 128256 tokens 1.88 ms kept, 2.03 again, x 768 1.59 and 1.62, x 512 1.26 and
 // 1.20, x 64 0.83 and 0.59; 4096 x 2048 6.20 and 7.29.
 constexpr int KEEP_DIM = 768;
+
+// Few rows' sums over them (of one piece) do not average what dz's rounding to bf16 leaves (one row x 552, 5 entries: dhead off by 2.8e-3 of its
+// norm, by its own rounding alone 1.7e-3). Up to 32 rows that rest goes through the products as rows of its own, which a tile
+// of 64 has room for (8 rows x 1024 against 8192 tokens 34 us with it and without, 32 x 4096 against 128256 677 and 659).
+constexpr int FINE_ROWS = 32;
 constexpr int MOST_TILES = (1 << 23) - 8;  // of 512 lanes: a launch holds fewer than 2^32
 
 long long up(long long v, long long to) { return (v + to - 1) / to * to; }
@@ -1123,8 +1162,9 @@ struct Plan {
     int kp, piece;
     int z, y, w, d;  // the tiles of z for the statistics and for dz, of dhead and of dx
     int parts;
-    bool gather, raw, own, keep, few;
-    long long kept, ids, idc, q, ent, held, idx, pos, live, xc, part, dz, acc, bytes;
+    bool gather, raw, own, keep, few, fine;
+    int dz_rows;  // the rows of dz and of what is made of it
+    long long joined, kept, ids, idc, q, ent, held, idx, pos, live, xc, part, dz, acc, bytes;
 };
 
 int log2_up(int k) {
@@ -1180,6 +1220,14 @@ bool plan_of(const dr_head_loss* a, int what, Plan& p) {
     p.z = choose_z(a->valid, n, a->dim);
     if (tiles_of(p.z, a->valid, n) >= MOST_TILES) return false;
     p.parts = (int)(up(a->valid, SIZE[p.z].bm) / SIZE[p.z].bm);
+    // the vocabulary in equal pieces of a multiple of 256; what is made of one
+    const long long tiles = up(a->valid, 256) / 256, fit = DZ_BYTES / (n * 512);
+    const long long pieces = (tiles + (fit > 1 ? fit : 1) - 1) / (fit > 1 ? fit : 1);
+    p.piece = back ? (int)((tiles + pieces - 1) / pieces) * 256 : 0;
+    const bool one = back && pieces == 1 && (a->dx || a->dhead);
+    p.few = one && (n <= FINE_ROWS || few_parts((int)n, p.parts)) && n << p.kp <= FEW_IDS;
+    p.fine = p.few && n <= FINE_ROWS;
+    p.keep = p.few || (one && what & DR_LOSS_FORWARD && a->dim >= KEEP_DIM);
     // (forward alone, the rows that count are gathered where leaving out the others may save more than that takes, about 10 us)
     p.gather = back || (double)n * a->valid * a->dim > 3e10;
     p.raw = !p.gather && a->vals == nullptr;  // (tokens read where they are: no launch before z's)
@@ -1198,25 +1246,22 @@ bool plan_of(const dr_head_loss* a, int what, Plan& p) {
     p.idx = take(n * 4);
     p.pos = take(n * 4);
     p.live = take(12);
-    p.xc = take(p.gather ? n * a->dim * 2 : 0);
-    p.part = take(what & DR_LOSS_FORWARD ? p.parts * np * 8 : 0);
-    p.piece = 0, p.dz = p.acc = p.kept = 0, p.keep = p.few = false;
+    p.xc = take(p.gather ? (p.fine ? 2 : 1) * n * a->dim * 2 : 0);
+    p.part = take(what & DR_LOSS_FORWARD || p.few ? p.parts * np * 8 : 0);
+    p.dz = p.acc = p.kept = p.joined = p.dz_rows = 0;
     if (back) {
-        // the vocabulary in equal pieces of a multiple of 256
-        const long long tiles = up(a->valid, 256) / 256, fit = DZ_BYTES / (n * 512);
-        const long long pieces = (tiles + (fit > 1 ? fit : 1) - 1) / (fit > 1 ? fit : 1);
-        p.piece = (int)((tiles + pieces - 1) / pieces) * 256;
-        p.dz = take(n * p.piece * 2);
-        p.keep = what == (DR_LOSS_FORWARD | DR_LOSS_BACKWARD) && pieces == 1 && (a->dx || a->dhead);
-        p.few = p.keep && few_parts((int)n, p.parts) && n << p.kp <= FEW_IDS;
-        p.keep = p.few || (p.keep && a->dim >= KEEP_DIM);
+        const long long nr = p.dz_rows = (int)(p.fine ? 2 * n : n);
+        p.dz = take(nr * p.piece * 2);
+        p.joined = take(p.few ? n * 8 : 0);
         p.kept = take(p.keep ? n * p.piece * 4 : 0);
         p.y = choose_z(p.piece, n, a->dim);
-        p.w = choose(EPI_DHEAD, a->dim, p.piece, n, {T256, T128});
+        p.w = choose(EPI_DHEAD, a->dim, p.piece, nr, {T256, T128});
         if (a->dx) {
-            p.d = n <= 64 ? choose(EPI_DX, a->dim, n, p.piece, {T256x64, T64K}) : choose(EPI_DX, a->dim, n, p.piece, {T256, T128, T64K});
-            // the sums of all rows where there are several pieces; of splits no more than ROUNDS rounds of tiles
-            const long long whole = p.piece < a->valid ? n * a->dim : 0;
+            p.d = nr <= 64 ? choose(EPI_DX, a->dim, nr, p.piece, {T256x64, T64K})
+                           : choose(EPI_DX, a->dim, nr, p.piece, {T256, T128, T64K});
+            // the sums of all rows where there are several pieces, or two rows of sums for one; of splits no more than ROUNDS
+            // rounds of tiles
+            const long long whole = p.piece < a->valid || p.fine ? nr * a->dim : 0;
             const long long split = (long long)ROUNDS * pace_of(EPI_DX, p.d).at_once * SIZE[p.d].bm * SIZE[p.d].bn;
             p.acc = take((whole > split ? whole : split) * 4);
         }
@@ -1303,7 +1348,7 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
     z.ids = P.gather ? p.idc : p.ids, z.kp = P.kp, z.kn = kn;
     z.raw = P.raw ? a->ids : nullptr, z.raw64 = a->ids64;
     z.lse = a->lse, z.g = a->g, z.top = p.top;
-    if (fwd) {
+    if (fwd || P.few) {  // (few rows' gradients are the same with and without their loss)
         Gemm s = z;
         s.m = a->valid;
         s.part = reinterpret_cast<f32x2*>(ws + P.part);
@@ -1316,8 +1361,12 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
         Merge m{s.part, s.ld_part, P.parts, n, kn, P.kp, P.gather ? p.pos : nullptr, P.raw ? nullptr : p.held, a->ids,
                 a->ids64, a->valid, p.ids, p.q, p.ent, 1.f / a->temperature, a->loss, a->lse, a->logits, s.kept, s.panel};
         if (P.few) {
-            Few f{*a, P.kp, P.parts, s.part, s.ld_part, s.kept, reinterpret_cast<uint16_t*>(ws + P.dz), s.panel, z.sc,
-                  1.f / a->temperature, p.idx, p.live, p.top, p.xc, p.dx};
+            const bool few = few_parts(n, P.parts);  // (more are joined once, by a launch of its own)
+            f32x2* joined = reinterpret_cast<f32x2*>(ws + P.joined);
+            if (!few) hipLaunchKernelGGL(hl_join, dim3(n), dim3(256), 0, st, s.part, s.ld_part, P.parts, joined);
+            Few f{*a, P.kp, few ? P.parts : 1, few ? s.part : joined, s.ld_part, s.kept, reinterpret_cast<uint16_t*>(ws + P.dz),
+                  s.panel, 256ll * P.dz_rows, z.sc, 1.f / a->temperature, p.idx, p.live, p.top, p.xc, p.dx, P.fine};
+            if (!fwd) f.a.loss = nullptr;
             hipLaunchKernelGGL(hl_few, dim3((a->valid + 255) / 256, (n + 3) / 4), dim3(256), 0, st, f);
         } else if (few_parts(n, P.parts)) {  // (in hl_few's order: the loss alone is the same)
             hipLaunchKernelGGL((hl_merge<1, 64>), dim3(n), dim3(64), 0, st, m);
@@ -1326,7 +1375,7 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
     }
     if (back && (a->dx || a->dhead)) {
         uint16_t* dz = reinterpret_cast<uint16_t*>(ws + P.dz);
-        const long long panel = (long long)n * 256;
+        const long long panel = 256ll * P.dz_rows;
         for (int v0 = 0; v0 < a->valid; v0 += P.piece) {
             const int vn = a->valid - v0 < P.piece ? a->valid - v0 : P.piece;
             Gemm s = z;
@@ -1351,16 +1400,16 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
             if (a->dhead) {
                 Gemm w{};
                 w.A = p.xc, w.lda = a->dim;
-                w.whole = z.whole, w.ldx = z.ldx, w.rows = n;
+                w.whole = P.fine ? nullptr : z.whole, w.ldx = z.ldx, w.rows = n;
                 w.B = dz, w.ldb = 256, w.panel = panel;
                 // (the rows past valid: zeros, with the last piece)
-                w.m = a->dim, w.nb = vn, w.n = v0 + vn == a->valid ? a->vocab - v0 : vn, w.k = n, w.live = p.live;
+                w.m = a->dim, w.nb = vn, w.n = v0 + vn == a->valid ? a->vocab - v0 : vn, w.k = P.dz_rows, w.live = p.live;
                 w.out = reinterpret_cast<uint16_t*>(a->dhead) + (long long)v0 * a->ld_dhead;
                 w.ld_out = a->ld_dhead;
                 w.scale = p.top + 1;
                 // (few steps: one stage and five workgroups a CU instead of four and two; 400 rows x 2880 against 50257 tokens, dx
                 // aside, 365 us and 382, 1003 rows 709 and 711, 1500 x 1024 against 8192 98.7 and 94.0)
-                if (n <= KSTEP || (P.w == T128 && n <= 1024)) launch<128, 128, 2, 2, 1, 1, 64, true, true, EPI_DHEAD>(w, st);
+                if (P.dz_rows <= KSTEP || (P.w == T128 && n <= 1024)) launch<128, 128, 2, 2, 1, 1, 64, true, true, EPI_DHEAD>(w, st);
                 else if (P.w == T256) launch<256, 256, 2, 4, 1, 4, 32, true, true, EPI_DHEAD>(w, st);
                 else launch<128, 128, 2, 2, 1, 4, 32, true, true, EPI_DHEAD>(w, st);
             }
@@ -1368,14 +1417,14 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
                 Gemm d{};
                 d.A = z.A + (long long)v0 * a->ld_head, d.lda = a->ld_head;
                 d.B = dz, d.ldb = 256, d.panel = panel;
-                d.m = a->dim, d.n = n, d.k = (int)up(vn, 8), d.ka = vn, d.live = p.live;
+                d.m = a->dim, d.n = P.dz_rows, d.k = (int)up(vn, 8), d.ka = vn, d.live = p.live;
                 d.plan_steps = P.piece / KSTEP;
                 d.acc = reinterpret_cast<float*>(ws + P.acc);
                 d.ld_acc = a->dim;
                 d.add = v0 > 0;
                 d.idx = p.idx;
                 d.scale = p.top + 1;
-                if (v0 + vn == a->valid) d.out = reinterpret_cast<uint16_t*>(a->dx), d.ld_out = a->ld_dx;
+                if (v0 + vn == a->valid && !P.fine) d.out = reinterpret_cast<uint16_t*>(a->dx), d.ld_out = a->ld_dx;
                 if (P.d == T64K) launch<64, 64, 2, 2, 2, 4, 64, true, false, EPI_DX>(d, st);
                 else if (P.d == T256x64) launch<256, 64, 2, 2, 1, 4, 32, true, false, EPI_DX>(d, st);
                 else if (P.d == T128) launch<128, 128, 2, 2, 1, 4, 32, true, false, EPI_DX>(d, st);
@@ -1385,7 +1434,7 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
         if (a->dx) {
             const Size t = SIZE[P.d];
             Finish f{reinterpret_cast<const float*>(ws + P.acc), (int)(up(a->dim, t.bm) / t.bm), t.bm, t.bn, t.wk, P.piece / KSTEP, a->dim, p.live,
-                     p.idx, p.top + 1, reinterpret_cast<uint16_t*>(a->dx), a->ld_dx};
+                     p.idx, p.top + 1, reinterpret_cast<uint16_t*>(a->dx), a->ld_dx, P.fine};
             const long long items = (long long)n * ((a->dim + 255) / 256);
             hipLaunchKernelGGL(hl_dx, dim3((unsigned)(items < 4096 ? items : 4096)), dim3(256), 0, st, f);
         }

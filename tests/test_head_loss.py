@@ -49,8 +49,8 @@ def entries(ids, vals, valid, t):
     return torch.where(held, ids, 0).long(), q, on, -torch.special.entr(q).sum(1)
 
 
-def expected(x, head, ids, vals, t, valid, g):
-    """[(value, bound)] of loss, dx and dhead, in 64 bits."""
+def expected(x, head, ids, vals, t, valid, g, b=B):
+    """[(value, bound)] of loss, dx and dhead, in 64 bits; b: how far dz's rounding is off."""
     n, d = x.shape
     ids, q, on, ent = entries(ids, vals, valid, t)
     x = torch.where(on[:, None], x.double(), 0.0)
@@ -72,7 +72,7 @@ def expected(x, head, ids, vals, t, valid, g):
     evals = 0 if vals is None else torch.where(q > 0, vals.double(), 0.0).abs().amax(1)[:, None] / t
     ep += eq * (64 + 8 + 4 * evals) * U * (vals is not None)
     dz, ep = (dz - eq) * gt, ep * gt.abs()
-    ez2 = ep + (B + 4 * U) * (dz.abs() + ep)
+    ez2 = ep + (b + 4 * U) * (dz.abs() + ep)
     out = [(loss, eloss)]
     for val, err, mag, depth in (
         (dz @ w, ez2 @ w.abs(), dz.abs() @ w.abs(), valid),
@@ -179,6 +179,26 @@ def test_logits_kept_for_the_gradient(device, n, v, valid, d, k):
     same("dx alone", run(grads, w, head_grad=False)[1], out[1])
     same("dhead alone", run(grads, w, x_grad=False)[2], out[2])
     same("again", run(grads, w)[1], out[1])
+
+
+@pytest.mark.parametrize("n, v, valid, d, k", [
+    (1, 2900, 2899, 552, 5), (1, 1, 1, 8, 0), (2, 257, 256, 64, 0), (32, 8192, 8192, 1024, 8), (31, 40000, 40000, 72, 64),
+    (17, 5000, 4999, 264, 0), (8, 100, 100, 4096, 3),
+])
+def test_few_rows_keep_what_rounding_leaves(device, n, v, valid, d, k):
+    """Of up to 32 rows the products take dz with what its rounding to bf16 leaves, rounded too: off by b^2 instead of b."""
+    x, head, w, g = inputs(device, n, v, d, n + v + d + k)
+    if k:
+        ids, vals = teacher(n, k, valid, g, device)
+        if n > 2:
+            ids[1] = -1
+        out = head_loss.distill_loss_grads(x, head, vals, ids, w, valid=valid)
+    else:
+        ids, vals = torch.randint(0, valid, (n,), generator=g).to(device.torch), None
+        if n > 2:
+            ids[1] = -100
+        out = head_loss.token_loss_grads(x, head, ids, w, valid=valid)
+    check(f"{n} x {v} x {d}, {k}", out, expected(x, head, ids, vals, 1.0, valid, w, B * B))
 
 
 @pytest.mark.parametrize("k", [0, 4])

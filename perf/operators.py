@@ -18,8 +18,6 @@ from pathlib import Path
 
 import torch
 
-sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "tensix-kernels_amd"))  # (imported from where `own` is true)
-
 own = False
 
 
@@ -130,6 +128,7 @@ def prepare(case, seed):
 
 
 def _own(s):
+    sys.path[:0] = [p for p in [str(Path(__file__).resolve().parents[1] / "tensix-kernels_amd")] if p not in sys.path]
     case = s["case"]
     if case["kind"] == "balance":
         from moe import balance

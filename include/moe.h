@@ -119,6 +119,8 @@ int dr_moe_route_gate_up(const dr_launch* launch, const dr_moe* moe, const dr_ro
  * No counterpart in the reference, which has no training: logits and ids are dr_moe_route's (moe/moe8.py:1139-1253). */
 #define DR_BALANCE_LOSS 1
 #define DR_BALANCE_GRAD 2 /* dlogits too (the loss and the counts come with either) */
+#define DR_BALANCE_BACKWARD 8 /* dlogits alone, from kept as a call of the same rows and mask left it: the bits of that call's
+                               * own gradient; ids, loss, counts and workspace are not read */
 
 typedef struct dr_balance {
     const float* logits;   /* [batch * rows][ld_logits] */
@@ -134,6 +136,7 @@ typedef struct dr_balance {
     const uint8_t* mask;   /* [batch * rows], 0: the row does not count; or NULL: all do */
     float* loss;           /* [batch] */
     int32_t* counts;       /* [batch][experts] */
+    int32_t* kept;         /* [batch][1 + experts] the rows that count, then the counts again, for DR_BALANCE_BACKWARD; or NULL */
     const float* g;        /* [batch], or NULL: ones */
     float* dlogits;        /* [batch * rows][ld_dlogits]; rows that do not count get zeros */
     int64_t ld_dlogits;

@@ -49,7 +49,7 @@ SYMBOLS = (
 
 DR_LOSS_FORWARD, DR_LOSS_BACKWARD = 1, 2
 DR_LOSS_MAX_K = 64
-DR_BALANCE_LOSS, DR_BALANCE_GRAD = 1, 2
+DR_BALANCE_LOSS, DR_BALANCE_GRAD, DR_BALANCE_BACKWARD = 1, 2, 8
 
 DR_MOE_GATE_UP, DR_MOE_DOWN, DR_MOE_GATE_UP_ROWS, DR_MOE_DOWN_ROWS = 1, 2, 3, 4
 
@@ -221,6 +221,7 @@ class Balance(ctypes.Structure):
         ("mask", c_void_p),
         ("loss", c_void_p),
         ("counts", c_void_p),
+        ("kept", c_void_p),
         ("g", c_void_p),
         ("dlogits", c_void_p),
         ("ld_dlogits", c_int64),

@@ -7,7 +7,8 @@
 //   balance_sum_k   a workgroup's rows: the sum of p and the counts (LDS), written for the workgroup
 //   balance_grad_k  every workgroup joins the workgroups' sums for itself, in order (cheaper than a launch of its own in
 //                   between while they are few; balance_slice_k otherwise), then the logits' gradient of its rows, p computed
-//                   again; balance_join_k: the join alone
+//                   again; balance_join_k: the join alone. After a call that kept the counts (DR_BALANCE_BACKWARD) there is nothing to
+//                   join, and balance_grad_k is all that runs
 //   balance_one_k   all of it by one workgroup, a batch of few rows or one of many batches: one launch and no memory between
 //                   (32 rows x 32 experts: 4.8 us in a graph, two launches 8; called eagerly 12 and 16, the host's)
 // What bounds it: the logits read twice and the gradient written once; at a few rows the launches.
@@ -35,6 +36,7 @@ struct Bal {
     int parts;
     int vec;              // the logits' rows can be read 16 bytes at a time
     int gvec;             // and dlogits' written so
+    int given;            // the gradient alone: a.kept holds the rows that count and the counts
 };
 
 template <int CONTROL>
@@ -208,16 +210,17 @@ struct Joined {
     int tot[W], live[W];
 };
 
-// A batch's sums (J.p, J.f) and the lane's share of its rows that count to f; 1 / those rows is returned. write: the counts and
-// the loss too.
+// A batch's sums (J.p, J.f) and the lane's share of its rows that count to f; 1 / those rows is returned. write: the counts, the
+// loss and what a backward takes too.
 __device__ __forceinline__ float finish(const Bal& b, int batch, bool write, int rows, Joined& J) {
     const dr_balance& a = b.a;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int total = 0;
+    int total = 0, *kept = write && a.kept ? a.kept + (long long)batch * (1 + a.experts) : nullptr;
     for (int e = tid; e < a.experts; e += T) {
         const int c = __float_as_int(J.f[e]);
         total += c;
         if (write) a.counts[(long long)batch * a.experts + e] = c;
+        if (kept) kept[1 + e] = c;
     }
 #pragma unroll
     for (int o = 32; o; o >>= 1) rows += __shfl_xor(rows, o), total += __shfl_xor(total, o);
@@ -225,6 +228,7 @@ __device__ __forceinline__ float finish(const Bal& b, int batch, bool write, int
     __syncthreads();
     rows = total = 0;
     for (int w = 0; w < W; ++w) rows += J.live[w], total += J.tot[w];
+    if (kept && tid == 0) *kept = rows;
     const float per = rows ? 1.f / (float)rows : 0.f;
     float loss = 0.f;
     for (int e = tid; e < a.experts; e += T) {
@@ -242,6 +246,16 @@ __device__ __forceinline__ float finish(const Bal& b, int batch, bool write, int
         a.loss[batch] = loss;
     }
     return per;
+}
+
+// f from the rows and counts that an earlier call kept; no sums of p, which the gradient does not need
+__device__ __forceinline__ float given(const Bal& b, int batch, Joined& J) {
+    const int tid = threadIdx.x, *kept = b.a.kept + (long long)batch * (1 + b.a.experts);
+    for (int e = tid; e < b.a.experts; e += T) {
+        J.p[e] = 0.f;
+        J.f[e] = __int_as_float(kept[1 + e]);
+    }
+    return finish(b, batch, false, tid == 0 ? *kept : 0, J);
 }
 
 // the batch's sums over its parts, finished
@@ -373,7 +387,7 @@ __global__ __launch_bounds__(T) void balance_grad_k(const Bal b) {
     const int g = blockIdx.x % b.groups, batch = blockIdx.x / b.groups;
     Row<N> next;
     row_get<L, N, false>(b, batch, g * (T / L) + threadIdx.x / L, threadIdx.x % L, next);
-    const float per = join(b, batch, g == 0, J);
+    const float per = b.given ? given(b, batch, J) : join(b, batch, g == 0, J);
     grad_rows<L, N, SIG>(b, g, batch, per, next, J);
 }
 
@@ -416,7 +430,7 @@ Split split_of(const dr_balance* a) {
 }
 
 bool valid(const dr_balance* a, int what) {
-    return a != nullptr && what >= 1 && what <= 3 && a->batch >= 1 && a->batch <= (1 << 16) && a->rows >= 1 &&
+    return a != nullptr && ((what >= 1 && what <= 3) || what == DR_BALANCE_BACKWARD) && a->batch >= 1 && a->batch <= (1 << 16) && a->rows >= 1 &&
            (long long)a->batch * a->rows < (1ll << 30) && a->experts >= 1 && a->experts <= MAXE && a->k >= 1 && a->k <= 16 &&
            (long long)a->rows * a->k < (1ll << 31) &&  // (the counts are int32)
            a->width >= a->experts && a->ld_logits >= a->width && a->ld_ids >= a->k && (a->kind == 0 || a->kind == 1);
@@ -426,6 +440,10 @@ long long up256(long long v) { return (v + 255) & ~255ll; }
 
 template <int L, int N, bool SIG>
 void run(const Bal& b, int what, hipStream_t st) {
+    if (b.given) {
+        hipLaunchKernelGGL((balance_grad_k<L, N, SIG>), dim3(b.groups * b.a.batch), dim3(T), 0, st, b);
+        return;
+    }
     if (b.groups == 1) {
         hipLaunchKernelGGL((balance_one_k<L, N, SIG>), dim3(b.a.batch), dim3(T), 0, st, b, what & DR_BALANCE_GRAD);
         return;
@@ -449,6 +467,7 @@ void run_kind(const Bal& b, int what, hipStream_t st) {
 
 extern "C" int64_t dr_moe_balance_workspace_bytes(const dr_balance* a, int what) {
     if (!valid(a, what)) return -1;
+    if (what == DR_BALANCE_BACKWARD) return 0;
     const Split s = split_of(a);
     const long long w = s.groups > 1 ? (long long)a->batch * (s.groups + s.slices) : 0;
     return up256(w * a->experts * 8) + up256(w * 4);
@@ -458,16 +477,19 @@ extern "C" int dr_moe_balance(const dr_balance* a, int what) {
     if (!valid(a, what)) return DR_EINVAL;
     const long long need = dr_moe_balance_workspace_bytes(a, what);
     auto aligned = [](const void* p, uintptr_t to) { return p != nullptr && reinterpret_cast<uintptr_t>(p) % to == 0; };
-    if (!aligned(a->logits, 4) || !aligned(a->ids, a->ids32 ? 4 : 2) || !aligned(a->loss, 4) || !aligned(a->counts, 4) ||
-        (need > 0 && !aligned(a->workspace, 256)) || a->workspace_bytes < need ||
-        ((what & DR_BALANCE_GRAD) && (!aligned(a->dlogits, 4) || a->ld_dlogits < a->width)))
+    const bool given = what == DR_BALANCE_BACKWARD, grad = given || what & DR_BALANCE_GRAD;
+    if (!aligned(a->logits, 4) ||
+        (!given && (!aligned(a->ids, a->ids32 ? 4 : 2) || !aligned(a->loss, 4) || !aligned(a->counts, 4))) ||
+        ((given || a->kept) && !aligned(a->kept, 4)) || (need > 0 && !aligned(a->workspace, 256)) ||
+        a->workspace_bytes < need || (grad && (!aligned(a->dlogits, 4) || a->ld_dlogits < a->width)))
         return DR_EINVAL;
     Bal b{};
     b.a = *a;
     const Split s = split_of(a);
     b.groups = s.groups;
+    b.given = given;
     b.vec = aligned(a->logits, 16) && a->ld_logits % 4 == 0;
-    b.gvec = (what & DR_BALANCE_GRAD) && aligned(a->dlogits, 16) && a->ld_dlogits % 4 == 0;
+    b.gvec = grad && aligned(a->dlogits, 16) && a->ld_dlogits % 4 == 0;
     const long long w = (long long)a->batch * b.groups;  // (the slices' sums behind the workgroups')
     b.sums = reinterpret_cast<float2*>(a->workspace);
     b.live = reinterpret_cast<int*>(reinterpret_cast<char*>(a->workspace) + up256((w + s.slices * a->batch) * a->experts * 8));

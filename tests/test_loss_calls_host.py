@@ -1,0 +1,35 @@
+"""The losses' C entries on the host (no GPU): refusals before anything is launched, workspaces, and plans."""
+
+import ctypes
+import re
+from pathlib import Path
+
+import pytest
+
+from dense_reader import _lib
+
+ROOT = Path(__file__).resolve().parents[1]
+
+
+def test_backward_constant_matches_the_header():
+    text = (ROOT / "include" / "moe.h").read_text()
+    assert int(re.search(r"^#define DR_BALANCE_BACKWARD (\d+)", text, re.M).group(1)) == _lib.DR_BALANCE_BACKWARD
+
+
+@pytest.mark.parametrize("bad", [
+    dict(logits=None), dict(logits=4098), dict(kept=None), dict(kept=4098), dict(dlogits=None), dict(dlogits=4098),
+    dict(ld_dlogits=31), dict(rows=0), dict(experts=33), dict(kind=2),
+])
+def test_balance_backward_refuses(bad):
+    A = _lib.Balance(logits=4096, kept=4096, dlogits=4096, batch=2, rows=100, experts=32, width=32, ld_logits=32, ld_dlogits=32,
+                     ld_ids=1, k=1)
+    assert _lib.lib().dr_moe_balance_workspace_bytes(ctypes.byref(A), _lib.DR_BALANCE_BACKWARD) == 0
+    for name, v in bad.items():
+        setattr(A, name, v)
+    assert _lib.lib().dr_moe_balance(ctypes.byref(A), _lib.DR_BALANCE_BACKWARD) == _lib.DR_EINVAL, bad
+
+
+def test_balance_refuses_a_misaligned_kept():
+    A = _lib.Balance(logits=4096, ids=4096, loss=4096, counts=4096, kept=4098, batch=2, rows=10, experts=32, width=32,
+                     ld_logits=32, ld_ids=4, k=4)
+    assert _lib.lib().dr_moe_balance(ctypes.byref(A), _lib.DR_BALANCE_LOSS) == _lib.DR_EINVAL

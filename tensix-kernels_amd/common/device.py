@@ -94,6 +94,12 @@ def raw_stream(device):
     return torch._C._cuda_getCurrentRawStream(device.index if device.index is not None else torch.cuda.current_device())
 
 
+def written(*tensors):
+    """The library has been given these tensors of a caller's (or None) to write into: for autograd a change in place, so
+    that a backward that would find other values than its forward refuses (0.4 us; it sees no write through a pointer)."""
+    torch.autograd.graph.increment_version([t for t in tensors if t is not None])
+
+
 def open_device(device_id=0):
     return Device(device_id)
 

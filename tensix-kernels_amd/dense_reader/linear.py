@@ -517,6 +517,8 @@ def matmul(
     L, y, keep = _launch(x, w, scale, topk=topk, out=out, col0=col0, w_up=w_up, max_banks=max_banks, **opts)
     run(L, x.device, "dr_matmul")
     del keep
+    if out is not None and (topk is None or L.topk.write_y):
+        dev.written(out)
     return y
 
 

@@ -114,6 +114,7 @@ def pick(records, x, rows_t, nrows, k, top=16, logits="bf16", out=None, valid=No
         stream,
     )
     _lib.check(st, "dr_head_pick")
+    dev.written(out, ids_out)
     return out
 
 
@@ -156,6 +157,7 @@ def pick_records(records, nrows, k, vocab, tmap=None, out=None, ids_out=None):
         None if ids_out is None else ids_out.data_ptr(), wp, wn, stream,
     )
     _lib.check(st, "dr_head_pick_records")
+    dev.written(out, ids_out)
     return out
 
 

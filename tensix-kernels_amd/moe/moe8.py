@@ -688,6 +688,7 @@ def route(logits, ids, w, k, *, kind="softmax", bias=None, ids32=False, experts=
     Keys and weights in double, rounded to bf16 at the end. Returns w (reference moe8.py:1139-1253)."""
     A = _route_args(logits, ids, w, k, kind, bias, ids32, experts, shared, scale, norm, groups, slot)
     _lib.check(_lib.lib().dr_moe_route(ctypes.byref(A)), "dr_moe_route")
+    dev.written(ids, w, shared)
     return w
 
 
@@ -717,7 +718,9 @@ def route_gate_up(logits, x, P, ids, w, k, *, act="silu", kind="softmax", bias=N
     assert not P["gu_bias"] or split, "moe8: gate_up's bias needs two loaders (loaders=2)"
     x2 = _x_rows(x, 1, H)[:1]
     h = torch.empty(1, 1, 1, kk * I, dtype=torch.bfloat16, device=x2.device)
-    return _run(P, x2, 1, H, H, h, kk * I, True, _lib.DR_MOE_GATE_UP, ids, ids32, w, kk, 1, act, route=A)
+    _run(P, x2, 1, H, H, h, kk * I, True, _lib.DR_MOE_GATE_UP, ids, ids32, w, kk, 1, act, route=A)
+    dev.written(ids, w, shared)
+    return h
 
 
 def route_reference(logits, k, kind="softmax", bias=None, scale=1.0, norm=True, groups=None, slot=None):

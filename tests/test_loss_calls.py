@@ -4,10 +4,19 @@ Most compare two calls that mean the same, bit for bit."""
 import pytest
 import torch
 
-from common.testing import same
+from common.testing import raises, same
+from dense_reader import linear
+from lm_head_topk import head_loss, lmhead
 from moe import balance, moe8
 
 pytestmark = pytest.mark.gpu
+
+
+def head_inputs(device, n, v, d, seed):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(n, d, generator=g).to(torch.bfloat16).to(device.torch)
+    head = (torch.randn(v, d, generator=g) * 0.1).to(torch.bfloat16).to(device.torch)
+    return x, head, torch.rand(n, generator=g).to(device.torch) + 0.25, g
 
 
 def router_inputs(device, batch, rows, width, experts, k, seed):
@@ -53,3 +62,38 @@ def test_balance_backward_is_the_one_call(device, kind, batch, rows, width, expe
         mine.fill_(0), counts.add_(1)
         (loss * g).sum().backward()
         same(f"{kind} {batch} x {rows} x {experts} of {width}", leaf.grad, want[2])
+
+
+def test_inputs_that_the_library_writes_again(device):
+    """What the library writes into a caller's tensor counts for autograd as a change of it: a backward that would read the
+    new values where the forward read the old ones is refused."""
+    n, d, v = 8, 256, 512
+    x, head, _, g = head_inputs(device, n, v, d, 2)
+    w, _ = linear.native_weight(device, torch.randn(d, d, generator=g) * 0.1, linear.bfloat8_b)
+    buf = torch.empty(1, 1, n, d, dtype=torch.bfloat16, device=device.torch)
+    ids = torch.randint(0, v, (n,), generator=g).to(device.torch)
+    leaf = head.clone().requires_grad_()
+    linear.matmul(x.reshape(1, 1, n, d), w, None, out=buf)
+    loss = head_loss.token_loss(buf, leaf, ids)
+    loss.sum().backward()  # (nothing in between)
+    same("nothing written", leaf.grad, head_loss.token_loss_grads(buf, head, ids)[2])
+    loss = head_loss.token_loss(buf, leaf, ids)
+    linear.matmul(x.reshape(1, 1, n, d) * 2, w, None, out=buf)
+    raises("x written by a matmul", RuntimeError, lambda: loss.sum().backward())
+
+    slots = torch.zeros(1, 1, n, 4, dtype=torch.int16, device=device.torch)
+    weights = torch.ones(1, 1, n, 4, dtype=torch.bfloat16, device=device.torch)
+    y = (weights.clone().requires_grad_() * weights).sum()
+    moe8.route(torch.randn(1, 1, n, 64, generator=g).to(device.torch), slots, weights, 4)
+    raises("weights written by the router", RuntimeError, y.backward)
+
+    token = torch.zeros(1, dtype=torch.int32, device=device.torch)
+    one = x[:1].reshape(1, 1, 1, d)
+    for rescore in (True, False):
+        teacher = lmhead.DeviceHead(device, head.cpu(), fmt="bf16", chunks=1, k=8, rescore=rescore, device_pick=True)
+        teacher.logits_topk(one, 1, ids_out=token)
+        for what, t in (("page", teacher.picks[1][0, 0, :1, 0]), ("token", token)):
+            loss = head_loss.token_loss(x[:1], leaf, t)
+            teacher.logits_topk(one, 1, ids_out=token)
+            raises(f"a {what} written by the pick, rescore {rescore}", RuntimeError, lambda: loss.sum().backward())
+        teacher.deallocate()

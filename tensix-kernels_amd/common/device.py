@@ -17,6 +17,7 @@ import math
 from dataclasses import dataclass
 
 import torch
+from torch.autograd import forward_ad
 
 TILE = 32
 
@@ -98,6 +99,15 @@ def written(*tensors):
     """The library has been given these tensors of a caller's (or None) to write into: for autograd a change in place, so
     that a backward that would find other values than its forward refuses (0.4 us; it sees no write through a pointer)."""
     torch.autograd.graph.increment_version([t for t in tensors if t is not None])
+
+
+def no_tangents(what, *tensors):
+    """Refuse dual tensors (torch.autograd.forward_ad): an op without a rule for them would drop their tangents unseen. (Of
+    tensors outside a dual level, all but always the case, only the level is looked at.)"""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what}: no forward-mode derivative")
 
 
 def open_device(device_id=0):

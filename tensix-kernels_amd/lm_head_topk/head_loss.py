@@ -42,6 +42,7 @@ class _Call:
     """One call's inputs, checked, and the launch of it."""
 
     def __init__(self, x, rows_t, ids, vals, temperature, valid):
+        dev.no_tangents("head_loss", x, rows_t, vals)
         dim = x.shape[-1]
         device = self.device = x.device
         assert x.is_cuda and x.dtype == torch.bfloat16, (x.device, x.dtype)
@@ -89,6 +90,7 @@ class _Call:
         """The rows' weights as the launch takes them (None: ones)."""
         if g is None:
             return None
+        dev.no_tangents("head_loss", g)
         if not isinstance(g, torch.Tensor):
             return self.empty(self.n).fill_(float(g))  # (a copy from the host could not be captured)
         assert g.device == self.device, (g.device, self.device)

@@ -36,6 +36,7 @@ def _weights(g, batch, device):
     """The batches' weights as the launch takes them (None: ones)."""
     if g is None:
         return None
+    dev.no_tangents("balance", g)
     # (a number filled in: a copy from the host could not be captured)
     gs = g if isinstance(g, torch.Tensor) else torch.full((batch,), float(g), device=device)
     assert gs.device == device, (gs.device, device)
@@ -60,6 +61,7 @@ def _launch(A, what, device):
 
 def _run(logits, ids, k, g, kind, ids32, experts, mask, grad, keep=False):
     """(loss, counts, dlogits or None, what a backward takes or None)."""
+    dev.no_tangents("balance", logits)
     assert kind in KINDS, f"balance: kind {kind!r}"
     assert logits.is_cuda and logits.dtype == torch.float32 and logits.dim() >= 2, (logits.device, logits.dtype)
     *lead, R, W = logits.shape

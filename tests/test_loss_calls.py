@@ -1,8 +1,11 @@
 """Calls of the losses (lm_head_topk/head_loss.py, moe/balance.py) that a program makes and their operators' own tests do not.
 Most compare two calls that mean the same, bit for bit."""
 
+import math
+
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from common.testing import raises, same
 from dense_reader import linear
@@ -17,6 +20,13 @@ def head_inputs(device, n, v, d, seed):
     x = torch.randn(n, d, generator=g).to(torch.bfloat16).to(device.torch)
     head = (torch.randn(v, d, generator=g) * 0.1).to(torch.bfloat16).to(device.torch)
     return x, head, torch.rand(n, generator=g).to(device.torch) + 0.25, g
+
+
+def teacher(n, k, v, g, device):
+    ids = torch.randint(0, v, (n, k), generator=g).int()
+    vals = torch.randn(n, k, generator=g) * 3
+    vals[torch.rand(n, k, generator=g) < 0.1] = -math.inf
+    return ids.to(device.torch), vals.to(device.torch)
 
 
 def router_inputs(device, batch, rows, width, experts, k, seed):
@@ -90,10 +100,34 @@ def test_inputs_that_the_library_writes_again(device):
     token = torch.zeros(1, dtype=torch.int32, device=device.torch)
     one = x[:1].reshape(1, 1, 1, d)
     for rescore in (True, False):
-        teacher = lmhead.DeviceHead(device, head.cpu(), fmt="bf16", chunks=1, k=8, rescore=rescore, device_pick=True)
-        teacher.logits_topk(one, 1, ids_out=token)
-        for what, t in (("page", teacher.picks[1][0, 0, :1, 0]), ("token", token)):
+        th = lmhead.DeviceHead(device, head.cpu(), fmt="bf16", chunks=1, k=8, rescore=rescore, device_pick=True)
+        th.logits_topk(one, 1, ids_out=token)
+        for what, t in (("page", th.picks[1][0, 0, :1, 0]), ("token", token)):
             loss = head_loss.token_loss(x[:1], leaf, t)
-            teacher.logits_topk(one, 1, ids_out=token)
+            th.logits_topk(one, 1, ids_out=token)
             raises(f"a {what} written by the pick, rescore {rescore}", RuntimeError, lambda: loss.sum().backward())
-        teacher.deallocate()
+        th.deallocate()
+
+
+def test_forward_mode_is_refused(device):
+    """A dual tensor's tangent has no rule here: an error, never a loss without it."""
+    x, head, w, g = head_inputs(device, 6, 100, 64, 3)
+    ids = torch.randint(0, 100, (6,), generator=g).to(device.torch)
+    ti, tv = teacher(6, 3, 100, g, device)
+    logits, slots, mask, gb = router_inputs(device, 2, 10, 32, 32, 4, 3)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+        for name, fn in (
+            ("x", lambda: head_loss.token_loss(dual(x), head, ids)),
+            ("the head", lambda: head_loss.token_loss(x, dual(head), ids)),
+            ("x that needs a gradient too", lambda: head_loss.token_loss(dual(x.clone().requires_grad_()), head, ids)),
+            ("x of both at once", lambda: head_loss.token_loss_grads(dual(x), head, ids)),
+            ("weights", lambda: head_loss.token_loss_grads(x, head, ids, dual(w))),
+            ("a teacher's values", lambda: head_loss.distill_loss(x, head, dual(tv), ti)),
+            ("a teacher's values, both at once", lambda: head_loss.distill_loss_grads(x, head, dual(tv), ti)),
+            ("logits", lambda: balance.balance_loss(dual(logits), slots, 4)),
+            ("logits of both at once", lambda: balance.balance_loss_grads(dual(logits), slots, 4)),
+            ("weights of batches", lambda: balance.balance_loss_grads(logits, slots, 4, dual(gb))),
+        ):
+            raises(f"forward mode, {name}", RuntimeError, fn)
+        same("nothing dual", head_loss.token_loss(x, head, ids), head_loss.token_loss_grads(x, head, ids)[0])

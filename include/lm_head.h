@@ -67,15 +67,16 @@ int dr_head_pick_records(const void* records, int n_records, int rows, int k, in
  * lm_head_topk/head_pick.py:43-52 and dense_reader/linear.py:747-768.
  */
 #define DR_LOSS_MAX_K 64
+#define DR_LOSS_MAX_LD (1 << 21) /* ldx and ld_head at most */
 
 /* what a call computes */
 #define DR_LOSS_FORWARD 1  /* loss, lse, logits */
 #define DR_LOSS_BACKWARD 2 /* dx, dhead, from lse and logits (a forward call's, of the same inputs) */
 
 typedef struct dr_head_loss {
-    const void* x;        /* [rows][ldx] bf16, 16-byte aligned, ldx a multiple of 8 */
+    const void* x;        /* [rows][ldx] bf16, 16-byte aligned, ldx a multiple of 8, to DR_LOSS_MAX_LD */
     int64_t ldx;
-    const void* head;     /* [vocab][ld_head] bf16, 16-byte aligned, ld_head a multiple of 8 */
+    const void* head;     /* [vocab][ld_head] bf16, the same */
     int64_t ld_head;
     int32_t rows, dim;    /* rows to 2^20, dim a multiple of 8; rows * valid to about 2^39 */
     int32_t vocab, valid; /* 1 <= valid <= vocab: the head's rows that take part */

@@ -49,6 +49,7 @@ SYMBOLS = (
 
 DR_LOSS_FORWARD, DR_LOSS_BACKWARD = 1, 2
 DR_LOSS_MAX_K = 64
+DR_LOSS_MAX_LD = 1 << 21
 DR_BALANCE_LOSS, DR_BALANCE_GRAD, DR_BALANCE_BACKWARD = 1, 2, 8
 
 DR_MOE_GATE_UP, DR_MOE_DOWN, DR_MOE_GATE_UP_ROWS, DR_MOE_DOWN_ROWS = 1, 2, 3, 4

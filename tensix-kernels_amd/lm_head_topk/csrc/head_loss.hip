@@ -1211,7 +1211,7 @@ bool plan_of(const dr_head_loss* a, int what, Plan& p) {
         a->dim > (1 << 17) || a->vocab < 1 || a->vocab > (1 << 28) || a->valid < 1 || a->valid > a->vocab || a->k < 1 ||
         a->k > DR_LOSS_MAX_K || (a->vals == nullptr && (a->k != 1 || a->temperature != 1.f)) ||
         !(a->temperature >= 0x1p-20f && a->temperature < INFINITY) || a->ldx < a->dim || a->ldx % 8 || a->ld_head < a->dim ||
-        a->ld_head % 8 || a->ldx > (1 << 21) || a->ld_head > (1 << 21) || a->ld_ids < a->k || (a->vals && a->ld_vals < a->k))
+        a->ld_head % 8 || a->ldx > DR_LOSS_MAX_LD || a->ld_head > DR_LOSS_MAX_LD || a->ld_ids < a->k || (a->vals && a->ld_vals < a->k))
         return false;
     const bool back = what & DR_LOSS_BACKWARD;
     const long long n = a->rows, np = up(n, 64);

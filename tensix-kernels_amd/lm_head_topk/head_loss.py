@@ -36,6 +36,7 @@ from dense_reader import _lib  # noqa: E402
 from lm_head_topk import head_pick  # noqa: E402
 
 MAX_K = _lib.DR_LOSS_MAX_K  # teacher entries a row at most
+MAX_LD = _lib.DR_LOSS_MAX_LD  # values from a row of x to the next at most, else it is copied
 
 
 class _Call:
@@ -53,7 +54,8 @@ class _Call:
         assert 1 <= self.valid <= vocab, (valid, rows_t.shape)
         if x.dim() != 2:
             x = x.reshape(-1, dim)
-        if x.stride(-1) != 1 or x.stride(0) % 8 or x.stride(0) < dim or x.data_ptr() % 16:
+        # (past MAX_LD the offsets in a tile pass the kernels' 32 bits: a few positions of long sequences, say)
+        if x.stride(-1) != 1 or x.stride(0) % 8 or not dim <= x.stride(0) <= MAX_LD or x.data_ptr() % 16:
             x = x.clone(memory_format=torch.contiguous_format)
         self.x, self.rows_t, self.dim = x, rows_t, dim
         n = self.n = x.shape[0]

@@ -131,3 +131,21 @@ def test_forward_mode_is_refused(device):
         ):
             raises(f"forward mode, {name}", RuntimeError, fn)
         same("nothing dual", head_loss.token_loss(x, head, ids), head_loss.token_loss_grads(x, head, ids)[0])
+
+
+@pytest.mark.parametrize("n, s, d", [(8, 1024, 4096), (3, 70000, 64), (1, 1024, 4096)])
+def test_rows_far_apart(device, n, s, d):
+    """The last position of each of a batch's sequences, read where the whole batch lies, at any distance."""
+    g = torch.Generator().manual_seed(4)
+    hidden = torch.full((n, s, d), float("nan"), dtype=torch.bfloat16, device=device.torch)
+    hidden[:, -1] = torch.randn(n, d, generator=g).to(device.torch)
+    head = (torch.randn(300, d, generator=g) * 0.1).to(torch.bfloat16).to(device.torch)
+    ids = torch.randint(0, 300, (n,), generator=g).to(device.torch)
+    x = hidden[:, -1]
+    want = head_loss.token_loss_grads(x.contiguous(), head, ids)
+    assert n == 1 or x.stride(0) > 1 << 21
+    for part, a, b in zip(("loss", "dx", "dhead"), head_loss.token_loss_grads(x, head, ids), want):
+        same(part, a, b)
+    leaf = x.detach().requires_grad_()
+    head_loss.token_loss(leaf, head, ids).sum().backward()
+    same("backward", leaf.grad, want[1])

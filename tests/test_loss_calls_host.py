@@ -16,6 +16,26 @@ def test_backward_constant_matches_the_header():
     assert int(re.search(r"^#define DR_BALANCE_BACKWARD (\d+)", text, re.M).group(1)) == _lib.DR_BALANCE_BACKWARD
 
 
+def head(**kw):
+    """A dr_head_loss whose pointers are never read."""
+    A = _lib.HeadLoss(rows=100, dim=64, ldx=64, ld_head=64, vocab=1000, valid=1000, ld_ids=1, k=1, temperature=1.0, ld_dx=64,
+                      ld_dhead=64, workspace_bytes=1 << 62)
+    for f in ("x", "head", "ids", "loss", "lse", "logits", "dx", "dhead", "workspace"):
+        setattr(A, f, 4096)
+    for name, v in kw.items():
+        setattr(A, name, v)
+    return A
+
+
+def test_farthest_rows():
+    """The limit on a row's distance is the header's, and holds."""
+    text = (ROOT / "include" / "lm_head.h").read_text()
+    assert 1 << int(re.search(r"^#define DR_LOSS_MAX_LD \(1 << (\d+)\)", text, re.M).group(1)) == _lib.DR_LOSS_MAX_LD
+    for name in ("ldx", "ld_head"):
+        for ld, ok in ((_lib.DR_LOSS_MAX_LD, True), (_lib.DR_LOSS_MAX_LD + 8, False)):
+            assert (_lib.lib().dr_head_loss_workspace_bytes(ctypes.byref(head(**{name: ld})), 3) > 0) == ok
+
+
 @pytest.mark.parametrize("bad", [
     dict(logits=None), dict(logits=4098), dict(kept=None), dict(kept=4098), dict(dlogits=None), dict(dlogits=4098),
     dict(ld_dlogits=31), dict(rows=0), dict(experts=33), dict(kind=2),

@@ -92,7 +92,7 @@ struct Gemm {
     f32x2* part;            // [m / BM][n] maximum and sum
     long long ld_part;
     const int* ids;         // [rows that count][1 << kp] entries, -1 none
-    const void* raw;        // or tokens as they came ([rows] int32, or int64: raw64), those past m none
+    const void* raw;        // or tokens as they came ([rows] int32, or int64: raw64; one after another), those past m none
     int raw64;
     int kp, kn;
     float* zt;              // [rows][kn]
@@ -1230,7 +1230,7 @@ bool plan_of(const dr_head_loss* a, int what, Plan& p) {
     p.keep = p.few || (one && what & DR_LOSS_FORWARD && a->dim >= KEEP_DIM);
     // (forward alone, the rows that count are gathered where leaving out the others may save more than that takes, about 10 us)
     p.gather = back || (double)n * a->valid * a->dim > 3e10;
-    p.raw = !p.gather && a->vals == nullptr;  // (tokens read where they are: no launch before z's)
+    p.raw = !p.gather && a->vals == nullptr && a->ld_ids == 1;  // (tokens read where they are: no launch before z's)
     p.own = p.gather && n << p.kp <= FEW;
     long long at = 0;
     auto take = [&](long long bytes) {

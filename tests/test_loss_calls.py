@@ -1,14 +1,16 @@
 """Calls of the losses (lm_head_topk/head_loss.py, moe/balance.py) that a program makes and their operators' own tests do not.
 Most compare two calls that mean the same, bit for bit."""
 
+import ctypes
 import math
 
 import pytest
 import torch
 from torch.autograd import forward_ad
 
+from common import device as cdev
 from common.testing import raises, same
-from dense_reader import linear
+from dense_reader import _lib, linear
 from lm_head_topk import head_loss, lmhead
 from moe import balance, moe8
 
@@ -149,3 +151,89 @@ def test_rows_far_apart(device, n, s, d):
     leaf = x.detach().requires_grad_()
     head_loss.token_loss(leaf, head, ids).sum().backward()
     same("backward", leaf.grad, want[1])
+
+
+def laid(t, ld, fill):
+    """t's rows ld apart, what lies between them filled: (the memory, a check that it still holds that)."""
+    wide = torch.full((t.shape[0], ld), fill, dtype=t.dtype, device=t.device)
+    wide[:, : t.shape[1]] = t
+    gap = wide[:, t.shape[1] :].clone()
+
+    def untouched(what):
+        got = wide[:, t.shape[1] :]
+        assert torch.equal(torch.nan_to_num(got.double(), 3.0), torch.nan_to_num(gap.double(), 3.0)), f"{what}: between its rows"
+
+    return wide, untouched
+
+
+@pytest.mark.parametrize("n, v, valid, d, k", [
+    (5, 300, 299, 64, 0), (40, 900, 890, 136, 0), (300, 2100, 2100, 264, 0), (1100, 5000, 4999, 800, 0),
+    (5, 300, 299, 64, 3), (40, 900, 890, 136, 16), (300, 2100, 2100, 264, 5), (1100, 5000, 4999, 800, 2),
+])
+def test_head_loss_rows_at_any_distance(device, n, v, valid, d, k):
+    """Every operand of the C entry with rows further apart than they are long: what the packed ones give, alone and with the
+    gradients, and nothing between the rows is read into a sum or written."""
+    x, head, g, gen = head_inputs(device, n, v, d, n + k)
+    if k:
+        ids, vals = teacher(n, k, valid, gen, device)
+    else:
+        ids, vals = torch.randint(-20, valid, (n, 1), generator=gen).to(device.torch), None
+    m = max(1, k)
+    lib, dt = _lib.lib(), device.torch
+    wx, _ = laid(x, d + 24, math.nan)
+    wh, _ = laid(head, d + 8, math.nan)
+    wi, _ = laid(ids, m + 3, 1)  # (a token of the vocabulary: read as a row's target it would change the loss)
+    wv, _ = laid(vals, m + 2, 100.0) if k else (None, None)
+
+    def call(what, far):
+        loss, lse, logits = torch.empty(n, device=dt), torch.empty(n, device=dt), torch.empty(n, m, device=dt)
+        dx, dxu = laid(torch.full((n, d), 7.0, dtype=torch.bfloat16, device=dt), d + 16 if far else d, 7.0)
+        dh, dhu = laid(torch.full((v, d), 7.0, dtype=torch.bfloat16, device=dt), d + 32 if far else d, 7.0)
+        X, H, I, V = (wx, wh, wi, wv) if far else (x, head, ids, vals)
+        A = _lib.HeadLoss()
+        A.x, A.ldx, A.head, A.ld_head = X.data_ptr(), X.stride(0), H.data_ptr(), H.stride(0)
+        A.rows, A.dim, A.vocab, A.valid = n, d, v, valid
+        A.ids, A.ld_ids, A.ids64, A.k = I.data_ptr(), I.stride(0), int(I.dtype == torch.int64), m
+        if k:
+            A.vals, A.ld_vals = V.data_ptr(), V.stride(0)
+        A.temperature = 1.0
+        A.loss, A.lse, A.logits, A.g = loss.data_ptr(), lse.data_ptr(), logits.data_ptr(), g.data_ptr()
+        if what & _lib.DR_LOSS_BACKWARD:
+            A.dx, A.ld_dx, A.dhead, A.ld_dhead = dx.data_ptr(), dx.stride(0), dh.data_ptr(), dh.stride(0)
+        need = lib.dr_head_loss_workspace_bytes(ctypes.byref(A), what)
+        assert need > 0
+        ws = torch.empty(need, dtype=torch.uint8, device=dt)
+        A.workspace, A.workspace_bytes, A.stream = ws.data_ptr(), need, cdev.raw_stream(dt)
+        assert lib.dr_head_loss_run(ctypes.byref(A), what) == _lib.DR_OK
+        torch.cuda.synchronize()
+        dxu("dx"), dhu("dhead")
+        return loss, lse, logits, dx[:, :d], dh[:, :d]
+
+    for what in (_lib.DR_LOSS_FORWARD, _lib.DR_LOSS_FORWARD | _lib.DR_LOSS_BACKWARD):
+        for part, a, b in zip(("loss", "lse", "logits", "dx", "dhead"), call(what, True), call(what, False)):
+            same(f"{what}: {part}", a, b)
+
+
+@pytest.mark.parametrize("batch, rows, width, experts, k", [(2, 33, 70, 64, 4), (1, 3000, 128, 100, 8), (1, 600, 1030, 1000, 3)])
+def test_balance_rows_at_any_distance(device, batch, rows, width, experts, k):
+    logits, ids, mask, g = router_inputs(device, batch, rows, width, experts, k, rows)
+    want = balance.balance_loss_grads(logits, ids, k, g, experts=experts, mask=mask)
+    dt = device.torch
+    for more in (1, 4):
+        wl, _ = laid(logits.reshape(-1, width), width + more, math.nan)
+        wi, _ = laid(ids.reshape(-1, k), k + 3, 1)
+        d, untouched = laid(torch.full((batch * rows, width), 7.0, device=dt), width + more, 7.0)
+        loss, counts = torch.empty(batch, device=dt), torch.empty(batch, experts, dtype=torch.int32, device=dt)
+        A = _lib.Balance()
+        A.logits, A.ld_logits, A.batch, A.rows, A.experts, A.width = wl.data_ptr(), width + more, batch, rows, experts, width
+        A.ids, A.ld_ids, A.k, A.mask = wi.data_ptr(), k + 3, k, mask.data_ptr()
+        A.loss, A.counts, A.g, A.dlogits, A.ld_dlogits = loss.data_ptr(), counts.data_ptr(), g.data_ptr(), d.data_ptr(), width + more
+        need = _lib.lib().dr_moe_balance_workspace_bytes(ctypes.byref(A), _lib.DR_BALANCE_GRAD)
+        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dt)
+        A.workspace, A.workspace_bytes, A.stream = ws.data_ptr(), need, cdev.raw_stream(dt)
+        assert _lib.lib().dr_moe_balance(ctypes.byref(A), _lib.DR_BALANCE_GRAD) == _lib.DR_OK
+        torch.cuda.synchronize()
+        untouched("dlogits")
+        same("loss", loss, want[0])
+        same("counts", counts, want[1])
+        same("dlogits", d[:, :width].reshape(want[2].shape), want[2])

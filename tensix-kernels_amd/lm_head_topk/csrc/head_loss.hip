@@ -531,7 +531,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void hl_gemm(const Gemm a) {
         } else if constexpr (EPI == EPI_DZ || EPI == EPI_DZ1) {
             const long long row = n < n_end ? a.idx[n] : 0;
             const float top = *a.top, l2 = n < n_end ? a.lse[row] * LOG2E : 0.f, gr = a.g && n < n_end ? a.g[row] : 1.f;
-            const float gs = top > 0.f ? gr / top : gr;
+            const float gs = gr / top;
             const int left = a.m - mw;
             const int own = EPI == EPI_DZ1 && n < n_end ? a.ids[n] - a.v0 - mw - 4 * h : -1;  // (the token's own logit)
 #pragma unroll
@@ -687,8 +687,8 @@ constexpr int MANY = 32768;  // rows past which it takes 64, and looks through t
 constexpr int FEW = 2048;    // entries that every workgroup looks through itself
 
 // the factor taken out of dz, of the rows' weights that count (positive, finite) the largest; weights so far apart that the
-// smallest over the largest would near the smallest float32: as they are
-__device__ __forceinline__ float factor(float top, float low) { return low > top * 0x1p-40f ? top : 1.f; }
+// smallest over the largest would near the smallest float32, or none (all 0, or infinite: 0 times those is a NaN): as they are
+__device__ __forceinline__ float factor(float top, float low) { return top > 0.f && low > top * 0x1p-40f ? top : 1.f; }
 
 
 // The rows that count, one after another: each workgroup finds the place of its own from the flags of all rows before
@@ -909,7 +909,7 @@ __global__ __launch_bounds__(256) void hl_dz(const Dz p) {
         const int n = n0 + i;
         if (n >= live) break;
         const int row = p.idx[n], own = p.ids ? p.ids[n] - v0 : -1;
-        const float l2 = p.lse[row] * LOG2E, gr = p.g ? p.g[row] : 1.f, gs = top > 0.f ? gr / top : gr;
+        const float l2 = p.lse[row] * LOG2E, gr = p.g ? p.g[row] : 1.f, gs = gr / top;
         float d[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -1031,7 +1031,7 @@ __global__ __launch_bounds__(256) void hl_few(const Few p) {
     if (id >= v0 && id < v0 + 256) reinterpret_cast<float*>(taken[wave])[id - v0] = all;
     __builtin_amdgcn_wave_barrier();
     const f32x4 less = taken[wave][lane];
-    const float l2 = lse * LOG2E, gr = a.g ? a.g[row] : 1.f, gs = top > 0.f ? gr / top : gr;
+    const float l2 = lse * LOG2E, gr = a.g ? a.g[row] : 1.f, gs = gr / top;
     float d[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -1040,8 +1040,12 @@ __global__ __launch_bounds__(256) void hl_few(const Few p) {
     uint16_t* const dz = p.dz + blockIdx.x * p.dz_panel + 4 * lane;
     *reinterpret_cast<uint2*>(dz + at * 256) = hi;
     if (p.fine) {
-        d[0] -= __uint_as_float(hi.x << 16), d[1] -= __uint_as_float(hi.x & 0xFFFF0000u);
-        d[2] -= __uint_as_float(hi.y << 16), d[3] -= __uint_as_float(hi.y & 0xFFFF0000u);
+        const uint32_t bits[4] = {hi.x << 16, hi.x & 0xFFFF0000u, hi.y << 16, hi.y & 0xFFFF0000u};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // (of an infinite value nothing is left)
+            const float h = __uint_as_float(bits[e]);
+            d[e] = __builtin_fabsf(h) == INFINITY ? 0.f : d[e] - h;
+        }
         *reinterpret_cast<uint2*>(dz + (live + at) * 256) = make_uint2(cvt2(d[0], d[1]), cvt2(d[2], d[3]));
     }
     if (!first) return;
@@ -1098,7 +1102,7 @@ __global__ __launch_bounds__(256) void hl_fix(const Fix p) {
         }
     }
     if (id < p.v0 || id >= p.v1) return;
-    const float top = *p.top, gr = p.g ? p.g[row] : 1.f, gs = top > 0.f ? gr / top : gr;
+    const float top = *p.top, gr = p.g ? p.g[row] : 1.f, gs = gr / top;
     const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(p.zt[row * p.k + j], p.sc, -p.lse[row] * LOG2E));
     const int v = id - p.v0;
     p.dz[(v >> 8) * p.panel + (long long)n * 256 + (v & 255)] = (uint16_t)cvt2(gs * (pr - all), 0.f);

@@ -237,3 +237,19 @@ def test_balance_rows_at_any_distance(device, batch, rows, width, experts, k):
         same("loss", loss, want[0])
         same("counts", counts, want[1])
         same("dlogits", d[:, :width].reshape(want[2].shape), want[2])
+
+
+@pytest.mark.parametrize("n", [1, 5, 32, 33, 300])
+@pytest.mark.parametrize("others", [0.0, 0.5])
+def test_infinite_weights(device, n, others):
+    """A row of infinite weight gives dhead infinities of the sign of its dz x, whatever the number of rows and with weights of
+    0 beside it: no NaN, as the formula has none (every p above 0, no x of 0)."""
+    x, head, w, g = head_inputs(device, n, 300, 64, 5)
+    x = torch.where(x == 0, torch.ones_like(x), x)
+    ids = torch.randint(0, 300, (n,), generator=g).to(device.torch)
+    w.fill_(others)
+    w[n // 2] = math.inf
+    dhead = head_loss.token_loss_grads(x, head, ids, w)[2]
+    sign = torch.ones(300, 1, dtype=torch.float64, device=device.torch)
+    sign[ids[n // 2]] = -1  # (p - 1 at the row's own token)
+    same(f"{n} rows", dhead.double(), math.inf * sign * x[n // 2].double().sign())

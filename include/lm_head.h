@@ -100,7 +100,8 @@ typedef struct dr_head_loss {
     void* stream;
 } dr_head_loss;
 
-/* Bytes of workspace the call needs (what: DR_LOSS_FORWARD, DR_LOSS_BACKWARD or both), -1 if it is invalid. */
+/* Bytes of workspace the call needs (what: DR_LOSS_FORWARD, DR_LOSS_BACKWARD or both; dx and dhead NULL or not as in the call:
+ * asked for neither, a backward needs and does nothing), -1 if it is invalid. */
 int64_t dr_head_loss_workspace_bytes(const dr_head_loss* a, int what);
 
 /* Enqueues the call on the stream: nothing is allocated, kept or waited for, so it can be captured. */

@@ -1217,7 +1217,7 @@ bool plan_of(const dr_head_loss* a, int what, Plan& p) {
         !(a->temperature >= 0x1p-20f && a->temperature < INFINITY) || a->ldx < a->dim || a->ldx % 8 || a->ld_head < a->dim ||
         a->ld_head % 8 || a->ldx > DR_LOSS_MAX_LD || a->ld_head > DR_LOSS_MAX_LD || a->ld_ids < a->k || (a->vals && a->ld_vals < a->k))
         return false;
-    const bool back = what & DR_LOSS_BACKWARD;
+    const bool back = what & DR_LOSS_BACKWARD && (a->dx || a->dhead);  // (asked for neither: the forward alone)
     const long long n = a->rows, np = up(n, 64);
     if (up(a->valid, 64) / 64 * (np / 64) > 1 << 30) return false;  // (tiles counted in 32 bits)
     p.kp = log2_up(a->k);
@@ -1228,7 +1228,7 @@ bool plan_of(const dr_head_loss* a, int what, Plan& p) {
     const long long tiles = up(a->valid, 256) / 256, fit = DZ_BYTES / (n * 512);
     const long long pieces = (tiles + (fit > 1 ? fit : 1) - 1) / (fit > 1 ? fit : 1);
     p.piece = back ? (int)((tiles + pieces - 1) / pieces) * 256 : 0;
-    const bool one = back && pieces == 1 && (a->dx || a->dhead);
+    const bool one = back && pieces == 1;
     p.few = one && (n <= FINE_ROWS || few_parts((int)n, p.parts)) && n << p.kp <= FEW_IDS;
     p.fine = p.few && n <= FINE_ROWS;
     p.keep = p.few || (one && what & DR_LOSS_FORWARD && a->dim >= KEEP_DIM);
@@ -1307,13 +1307,13 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
     Plan P;
     if (!plan_of(a, what, P)) return DR_EINVAL;
     auto aligned = [](const void* p, uintptr_t to) { return p != nullptr && reinterpret_cast<uintptr_t>(p) % to == 0; };
-    const bool fwd = what & DR_LOSS_FORWARD, back = what & DR_LOSS_BACKWARD;
+    const bool fwd = what & DR_LOSS_FORWARD, back = what & DR_LOSS_BACKWARD && (a->dx || a->dhead);
     if (!aligned(a->x, 16) || !aligned(a->head, 16) || !aligned(a->ids, a->ids64 ? 8 : 4) || !aligned(a->lse, 4) ||
         !aligned(a->logits, 4) || (fwd && !aligned(a->loss, 4)) || !aligned(a->workspace, 256) || a->workspace_bytes < P.bytes ||
         (back && a->dx && (!aligned(a->dx, 16) || a->ld_dx < a->dim || a->ld_dx % 8)) ||
         (back && a->dhead && (!aligned(a->dhead, 16) || a->ld_dhead < a->dim || a->ld_dhead % 8)))
         return DR_EINVAL;
-    if (back && !fwd && !a->dx && !a->dhead) return DR_OK;
+    if (!fwd && !back) return DR_OK;
     const hipStream_t st = reinterpret_cast<hipStream_t>(a->stream);
     char* ws = reinterpret_cast<char*>(a->workspace);
     const int n = a->rows, kn = a->k;
@@ -1377,7 +1377,7 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
         } else if (n <= 64) hipLaunchKernelGGL((hl_merge<1, 256>), dim3(n), dim3(256), 0, st, m);
         else hipLaunchKernelGGL((hl_merge<16, 64>), dim3((n + 15) / 16), dim3(1024), 0, st, m);
     }
-    if (back && (a->dx || a->dhead)) {
+    if (back) {
         uint16_t* dz = reinterpret_cast<uint16_t*>(ws + P.dz);
         const long long panel = 256ll * P.dz_rows;
         for (int v0 = 0; v0 < a->valid; v0 += P.piece) {

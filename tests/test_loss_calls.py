@@ -253,3 +253,17 @@ def test_infinite_weights(device, n, others):
     sign = torch.ones(300, 1, dtype=torch.float64, device=device.torch)
     sign[ids[n // 2]] = -1  # (p - 1 at the row's own token)
     same(f"{n} rows", dhead.double(), math.inf * sign * x[n // 2].double().sign())
+
+
+@pytest.mark.parametrize("n", [5, 40, 300])
+def test_neither_gradient(device, n):
+    """Asked for no gradient, the calls of both give the loss alone."""
+    x, head, w, g = head_inputs(device, n, 900, 800, 6)
+    ids = torch.randint(-100, 900, (n,), generator=g).to(device.torch)
+    ti, tv = teacher(n, 5, 900, g, device)
+    for loss, got in (
+        (head_loss.token_loss(x, head, ids), head_loss.token_loss_grads(x, head, ids, w, x_grad=False, head_grad=False)),
+        (head_loss.distill_loss(x, head, tv, ti), head_loss.distill_loss_grads(x, head, tv, ti, w, x_grad=False, head_grad=False)),
+    ):
+        assert got[1] is None and got[2] is None
+        same("loss", got[0], loss)

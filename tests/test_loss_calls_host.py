@@ -36,6 +36,16 @@ def test_farthest_rows():
             assert (_lib.lib().dr_head_loss_workspace_bytes(ctypes.byref(head(**{name: ld})), 3) > 0) == ok
 
 
+@pytest.mark.parametrize("rows, vals", [(8, None), (100, None), (8192, None), (8192, 4096)])
+def test_no_gradient_asked_for(rows, vals):
+    """Neither dx nor dhead: the workspace is the forward's alone."""
+    both, ask = dict(rows=rows, vocab=128256, valid=128256, vals=vals, ld_vals=1), _lib.lib().dr_head_loss_workspace_bytes
+    forward = ask(ctypes.byref(head(**both)), _lib.DR_LOSS_FORWARD)
+    neither = head(**both, dx=None, dhead=None)
+    assert ask(ctypes.byref(neither), _lib.DR_LOSS_FORWARD | _lib.DR_LOSS_BACKWARD) == forward > 0
+    assert _lib.lib().dr_head_loss_run(ctypes.byref(neither), _lib.DR_LOSS_BACKWARD) == _lib.DR_OK  # (nothing to do)
+
+
 @pytest.mark.parametrize("bad", [
     dict(logits=None), dict(logits=4098), dict(kept=None), dict(kept=4098), dict(dlogits=None), dict(dlogits=4098),
     dict(ld_dlogits=31), dict(rows=0), dict(experts=33), dict(kind=2),

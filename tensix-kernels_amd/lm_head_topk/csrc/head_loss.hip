@@ -394,14 +394,16 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void hl_gemm(const Gemm a) {
                 at[64 * g] = f32x4{acc[0][0][4 * g], acc[0][0][4 * g + 1], acc[0][0][4 * g + 2], acc[0][0][4 * g + 3]};
         }
         step_barrier<0>();
-        if (group) return;
+        if (!group) {
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const f32x4 v = at[64 * g];
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 v = at[64 * g];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[0][0][4 * g + e] += v[e];
+                for (int e = 0; e < 4; ++e) acc[0][0][4 * g + e] += v[e];
+            }
         }
     }
+    const bool second = WK == 2 && group;  // (it has nothing left to do but the statistics' barrier)
 
     // lane: columns n = n0 + wn TN + 32 j + lane % 32, rows m0 + wm TM + 32 i + 8 g + 4 (lane / 32) + 0 .. 3 in words 4 g ..
     const int r = lane & 31, h = lane >> 5;
@@ -431,6 +433,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void hl_gemm(const Gemm a) {
     };
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
+        if (second) continue;
         const int nj = n0 + wn * TN + 32 * j, n = nj + r;
         if constexpr (STATS) {
             const int left = a.m - mw;  // vocabulary rows of this wavefront
@@ -596,7 +599,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void hl_gemm(const Gemm a) {
     }
     if constexpr (STATS) {  // the wavefronts' rows of a column together
         __syncthreads();
-        if (wm == 0 && h == 0) {
+        if (wm == 0 && h == 0 && !second) {
 #pragma unroll
             for (int j = 0; j < NI; ++j) {
                 const int c = wn * TN + 32 * j + r;

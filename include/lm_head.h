@@ -104,6 +104,21 @@ typedef struct dr_head_loss {
  * asked for neither, a backward needs and does nothing), -1 if it is invalid. */
 int64_t dr_head_loss_workspace_bytes(const dr_head_loss* a, int what);
 
+/* What the call launches, without launching it. A tile: rows and columns of the product, and the groups of wavefronts that
+ * split its sum; 0 where the call makes no such product. */
+typedef struct dr_head_loss_info {
+    int32_t z[3];         /* the logits' tile (tokens by rows) for the loss */
+    int32_t dz[3];        /* where they are computed again for their gradient */
+    int32_t dhead[3];     /* (dim by tokens) */
+    int32_t dhead_stages; /* of its K loop */
+    int32_t dx[3];        /* (dim by rows) */
+    int32_t dx_splits;    /* of its sum, where every row counts */
+    int32_t piece, pieces; /* tokens whose dz is in memory at once, and how often */
+    int32_t kept;         /* 1: the logits are kept from the loss to dz */
+    int32_t few;          /* 1: few rows' launch between the products, 2: with what dz's rounding leaves */
+} dr_head_loss_info;
+int dr_head_loss_plan(const dr_head_loss* a, int what, dr_head_loss_info* info);
+
 /* Enqueues the call on the stream: nothing is allocated, kept or waited for, so it can be captured. */
 int dr_head_loss_run(const dr_head_loss* a, int what);
 

@@ -38,6 +38,7 @@ SYMBOLS = (
     "dr_head_pick",
     "dr_head_pick_records",
     "dr_head_loss_workspace_bytes",
+    "dr_head_loss_plan",
     "dr_head_loss_run",
     "dr_moe_workspace_bytes",
     "dr_moe_matmul",
@@ -206,6 +207,21 @@ class HeadLoss(ctypes.Structure):
     ]
 
 
+class HeadLossInfo(ctypes.Structure):
+    _fields_ = [
+        ("z", c_int32 * 3),
+        ("dz", c_int32 * 3),
+        ("dhead", c_int32 * 3),
+        ("dhead_stages", c_int32),
+        ("dx", c_int32 * 3),
+        ("dx_splits", c_int32),
+        ("piece", c_int32),
+        ("pieces", c_int32),
+        ("kept", c_int32),
+        ("few", c_int32),
+    ]
+
+
 class Balance(ctypes.Structure):
     _fields_ = [
         ("logits", c_void_p),
@@ -293,6 +309,8 @@ def lib():
                                            c_void_p, c_int64, c_void_p]
         L.dr_head_loss_workspace_bytes.restype = c_int64
         L.dr_head_loss_workspace_bytes.argtypes = [ctypes.POINTER(HeadLoss), c_int]
+        L.dr_head_loss_plan.restype = c_int
+        L.dr_head_loss_plan.argtypes = [ctypes.POINTER(HeadLoss), c_int, ctypes.POINTER(HeadLossInfo)]
         L.dr_head_loss_run.restype = c_int
         L.dr_head_loss_run.argtypes = [ctypes.POINTER(HeadLoss), c_int]
         L.dr_moe_workspace_bytes.restype = c_int64
@@ -319,6 +337,13 @@ def check(status, what):
     if status in (DR_EINVAL, DR_ERANGE):
         raise ValueError(msg)
     raise RuntimeError(msg)
+
+
+def head_loss_info(A, what):
+    """dr_head_loss_plan's answer, as a dict."""
+    info = HeadLossInfo()
+    check(lib().dr_head_loss_plan(ctypes.byref(A), what, ctypes.byref(info)), "dr_head_loss_plan")
+    return {f: getattr(info, f) if t is c_int32 else tuple(getattr(info, f)) for f, t in HeadLossInfo._fields_}
 
 
 def launch_info(L):

@@ -1170,6 +1170,7 @@ struct Plan {
     int z, y, w, d;  // the tiles of z for the statistics and for dz, of dhead and of dx
     int parts;
     bool gather, raw, own, keep, few, fine;
+    bool one_stage;  // dhead
     int dz_rows;  // the rows of dz and of what is made of it
     long long joined, kept, ids, idc, q, ent, held, idx, pos, live, xc, part, dz, acc, bytes;
 };
@@ -1263,6 +1264,9 @@ bool plan_of(const dr_head_loss* a, int what, Plan& p) {
         p.kept = take(p.keep ? n * p.piece * 4 : 0);
         p.y = choose_z(p.piece, n, a->dim);
         p.w = choose(EPI_DHEAD, a->dim, p.piece, nr, {T256, T128});
+        // (few steps: one stage and five workgroups a CU instead of four and two; 400 rows x 2880 against 50257 tokens, dx
+        // aside, 365 us and 382, 1003 rows 709 and 711, 1500 x 1024 against 8192 98.7 and 94.0)
+        p.one_stage = nr <= KSTEP || (p.w == T128 && n <= 1024);
         if (a->dx) {
             p.d = nr <= 64 ? choose(EPI_DX, a->dim, nr, p.piece, {T256x64, T64K})
                            : choose(EPI_DX, a->dim, nr, p.piece, {T256, T128, T64K});
@@ -1304,6 +1308,28 @@ void launch_z(const Gemm& g, int t, hipStream_t st) {
 extern "C" int64_t dr_head_loss_workspace_bytes(const dr_head_loss* a, int what) {
     Plan p;
     return plan_of(a, what, p) ? p.bytes : -1;
+}
+
+extern "C" int dr_head_loss_plan(const dr_head_loss* a, int what, dr_head_loss_info* info) {
+    Plan p;
+    if (info == nullptr || !plan_of(a, what, p)) return DR_EINVAL;
+    *info = dr_head_loss_info{};
+    const bool fwd = what & DR_LOSS_FORWARD, back = p.piece > 0;
+    auto tile = [](int32_t (&to)[3], int t) { to[0] = SIZE[t].bm, to[1] = SIZE[t].bn, to[2] = SIZE[t].wk; };
+    if (fwd || p.few) tile(info->z, p.z);
+    info->kept = p.keep;
+    info->few = p.few + p.fine;
+    if (!back) return DR_OK;
+    info->piece = p.piece;
+    info->pieces = (a->valid + p.piece - 1) / p.piece;
+    if (!p.keep) tile(info->dz, p.y);
+    if (a->dhead) tile(info->dhead, p.one_stage ? T128 : p.w), info->dhead_stages = p.one_stage ? 1 : 4;
+    if (a->dx) {
+        tile(info->dx, p.d);
+        const Size s = SIZE[p.d];
+        info->dx_splits = dx_splits(pace_of(EPI_DX, p.d), tiles_of(p.d, a->dim, p.dz_rows), p.piece / KSTEP, s.bm * s.bn * 4);
+    }
+    return DR_OK;
 }
 
 extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
@@ -1414,9 +1440,7 @@ extern "C" int dr_head_loss_run(const dr_head_loss* a, int what) {
                 w.out = reinterpret_cast<uint16_t*>(a->dhead) + (long long)v0 * a->ld_dhead;
                 w.ld_out = a->ld_dhead;
                 w.scale = p.top + 1;
-                // (few steps: one stage and five workgroups a CU instead of four and two; 400 rows x 2880 against 50257 tokens, dx
-                // aside, 365 us and 382, 1003 rows 709 and 711, 1500 x 1024 against 8192 98.7 and 94.0)
-                if (P.dz_rows <= KSTEP || (P.w == T128 && n <= 1024)) launch<128, 128, 2, 2, 1, 1, 64, true, true, EPI_DHEAD>(w, st);
+                if (P.one_stage) launch<128, 128, 2, 2, 1, 1, 64, true, true, EPI_DHEAD>(w, st);
                 else if (P.w == T256) launch<256, 256, 2, 4, 1, 4, 32, true, true, EPI_DHEAD>(w, st);
                 else launch<128, 128, 2, 2, 1, 4, 32, true, true, EPI_DHEAD>(w, st);
             }

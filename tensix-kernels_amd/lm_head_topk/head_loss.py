@@ -54,11 +54,11 @@ class _Call:
         assert 1 <= self.valid <= vocab, (valid, rows_t.shape)
         if x.dim() != 2:
             x = x.reshape(-1, dim)
+        n = self.n = x.shape[0]
         # (past MAX_LD the offsets in a tile pass the kernels' 32 bits: a few positions of long sequences, say)
-        if x.stride(-1) != 1 or x.stride(0) % 8 or not dim <= x.stride(0) <= MAX_LD or x.data_ptr() % 16:
+        if x.stride(-1) != 1 or x.data_ptr() % 16 or (n > 1 and (x.stride(0) % 8 or not dim <= x.stride(0) <= MAX_LD)):
             x = x.clone(memory_format=torch.contiguous_format)
         self.x, self.rows_t, self.dim = x, rows_t, dim
-        n = self.n = x.shape[0]
         self.vals = None
         if vals is None:
             assert ids.dtype in (torch.int32, torch.int64), ids.dtype

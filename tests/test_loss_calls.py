@@ -153,6 +153,17 @@ def test_rows_far_apart(device, n, s, d):
     same("backward", leaf.grad, want[1])
 
 
+def test_one_row_is_read_where_it_lies(device):
+    """The last position of one sequence takes no copy, whatever its batch's stride."""
+    x, head, _, g = head_inputs(device, 1, 300, 64, 7)
+    ids = torch.zeros(1, dtype=torch.int64, device=device.torch)
+    want = head_loss.token_loss(x, head, ids)
+    for stride in (1, 12, 1 << 22):
+        view = x.as_strided((1, 64), (stride, 1))
+        assert head_loss._Call(view, head, ids, None, 1.0, None).x.data_ptr() == x.data_ptr(), stride
+        same(f"stride {stride}", head_loss.token_loss(view, head, ids), want)
+
+
 def laid(t, ld, fill):
     """t's rows ld apart, what lies between them filled: (the memory, a check that it still holds that)."""
     wide = torch.full((t.shape[0], ld), fill, dtype=t.dtype, device=t.device)

@@ -47,8 +47,9 @@ int dr_head_pick_records(const void* records, int n_records, int rows, int k, in
                          void* out, void* ids_out, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* The losses. A head [vocab][dim] bf16 (one row a token, as dr_head_pick reads it) against rows x [rows][dim] bf16:
- * z = x . head^T, float32 sums, of which no call has more than 2 GiB in memory. Per row, with lse = log(sum over
- * v < valid of exp(z[v] / T)):
+ * z = x . head^T, float32 sums, of which no call has more than 2 GiB in memory (a call of both directions may keep that
+ * much in its workspace, beside up to 1 GiB of their gradient). Per row, with lse = log(sum over v < valid of
+ * exp(z[v] / T)):
  *   tokens (vals NULL, k 1, T 1): loss = lse - z[id];
  *   a teacher's best k logits (vals): over the entries held, q = softmax(vals / T),
  *     loss = sum q (log q - z[id] / T + lse), the divergence of the row's softmax at temperature T from the teacher's

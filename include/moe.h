@@ -125,7 +125,7 @@ int dr_moe_route_gate_up(const dr_launch* launch, const dr_moe* moe, const dr_ro
 typedef struct dr_balance {
     const float* logits;   /* [batch * rows][ld_logits] */
     int64_t ld_logits;
-    int32_t batch, rows;   /* batch * rows below 2^30, rows * k below 2^31 (the counts) */
+    int32_t batch, rows;   /* batch to 2^16, batch * rows below 2^30, rows * k below 2^31 (the counts) */
     int32_t experts;       /* 1 .. 1024: the logits' columns 0 .. experts - 1 */
     int32_t width;         /* dlogits' columns: zeros from experts on */
     const void* ids;       /* [batch * rows][ld_ids] uint16, or uint32 (ids32) */

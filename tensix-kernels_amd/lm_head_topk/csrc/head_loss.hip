@@ -12,11 +12,12 @@
 // them. One of both directions whose dz is one piece (1 GB) keeps them from the loss to dz where that is faster (KEEP_DIM), and
 // of few rows takes all between the products in one launch (hl_few).
 //
-// What bounds them (8192 rows x 4096 against 128256 tokens, 27.3 ms; a large library product of the same layouts runs at 1200,
-// 985 and 1110 TFLOP/s): z 7.05 ms (1220 TFLOP/s), dz 7.16 (1200), dhead 6.69 (1286), dx 6.85 (1256). With zeros for inputs
-// the same kernels run at 1530 to 1790 TFLOP/s and 2.4 GHz: the power that random values draw, at 1.8 GHz, holds them there.
-// 32 rows: 176 us for the 1.05 GB of the head, 6.0 TB/s. A few rows against a small vocabulary: each launch's start, its first
-// loads and a chain of LDS reads and matrix instructions (48 x 1024 against 8192: 5 launches of 4 to 9 us).
+// What bounds them (8192 rows x 4096 against 128256 tokens, 27.68 ms in one trace; a large library product of the same layouts
+// runs at 1200, 985 and 1110 TFLOP/s): z 6.85 ms (1256 TFLOP/s), dz 7.21 (1195), dhead 6.72 (1281), dx 6.88 (1252), all else
+// 0.03. With zeros for inputs the same kernels run at 1530 to 1790 TFLOP/s and 2.4 GHz: the power that random values draw, at
+// 1.8 GHz, holds them there. 32 rows: 171 us for the 1.05 GB of the head, 6.1 TB/s. A few rows against a small
+// vocabulary: each launch's start, its first loads and a chain of LDS reads and matrix instructions (48 x 1024 against 8192:
+// 5 launches of 4 to 9 us).
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -896,7 +897,7 @@ struct Dz {
 };
 
 // dz from z as the loss left it: a wavefront's rows of one panel, 1 KB read and 512 bytes written each (1842 rows against 128256
-// tokens: 275 us, 5.2 TB/s)
+// tokens: 239 us, 5.9 TB/s)
 constexpr int DZ_ROWS = 8;  // a wavefront, asked for at once
 __global__ __launch_bounds__(256) void hl_dz(const Dz p) {
     const int live = *p.live, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1157,9 +1158,13 @@ constexpr long long DZ_BYTES = 1ll << 30;  // dz a piece at most
 // 1.20, x 64 0.83 and 0.59; 4096 x 2048 6.20 and 7.29.
 constexpr int KEEP_DIM = 768;
 
-// Few rows' sums over them (of one piece) do not average what dz's rounding to bf16 leaves (one row x 552, 5 entries: dhead off by 2.8e-3 of its
-// norm, by its own rounding alone 1.7e-3). Up to 32 rows that rest goes through the products as rows of its own, which a tile
-// of 64 has room for (8 rows x 1024 against 8192 tokens 34 us with it and without, 32 x 4096 against 128256 677 and 659).
+// dz is rounded to bf16 because the matrix instructions take bf16: it is off by half a step, and so is what one value of it
+// dominates, at any number of rows (a token's row of dhead that one row's p - 1 makes, a row's dx that a teacher's best entry
+// does). Over all of dhead or dx that adds 1.6e-3 of the norm at most to the 1.65e-3 of their own rounding (root of the squares:
+// 2.3e-3 with a teacher's 16 entries, 1.7e-3 for 401 rows' tokens). Of one piece and few rows it is the worst (one row x 552,
+// 5 entries: dhead off by 2.8e-3 of its norm, by its own rounding alone 1.7e-3). Up to 32 rows what the rounding
+// leaves goes through the products as rows of its own, which a tile of 64 has room for (8 rows x 1024 against 8192 tokens 34 us
+// with it and without, 32 x 4096 against 128256 677 and 659).
 constexpr int FINE_ROWS = 32;
 constexpr int MOST_TILES = (1 << 23) - 8;  // of 512 lanes: a launch holds fewer than 2^32
 

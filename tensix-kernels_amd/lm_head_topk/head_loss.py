@@ -9,11 +9,14 @@ linear.topk_merge leaves of its top-k records (its dense_reader/linear.py:747-76
   vals, ids = linear.topk_merge(records, nrows, k, k_out=16)    # a teacher's best logits and their ids
   loss, dx, drows = distill_loss_grads(x, student_rows, vals, ids, g, temperature=2.0)
 
-The logits x . rows^T (float32 sums) go by in pieces: no call has more than 2 GiB of them in memory. A row whose target lies
+The logits x . rows^T (float32 sums) go by in pieces, and backward computes them again; a call of both directions whose rows
+times tokens are few enough (the logits 2 GiB, their gradient 1 GiB) keeps them in its workspace instead, which is faster for
+few rows and from 768 values a row on. No call has more of them in memory. A row whose target lies
 outside 0 .. valid - 1 (a padded or ignored position; -100, say), or that holds no teacher entry, is left out: its loss and
 its dx are 0 and it adds nothing to drows, whatever x, the teacher's values or g hold there; it costs next to nothing where
 there are many rows. dx and drows are bf16, summed in float32 from the logits' gradient rounded to bf16 (up to 32 rows, from
-that and what the rounding leaves).
+that and what the rounding leaves): past 32 rows a row of drows or dx that one token's gradient dominates is off by up to half
+a bf16 step twice.
 
 Nothing goes to the host. Memory comes from torch's allocator each call, on the current stream, so calls on several streams,
 threads or captured graphs never share any. In a HIP graph, capture token_loss, distill_loss or the *_grads calls; autograd's

@@ -3,6 +3,7 @@ Most compare two calls that mean the same, bit for bit."""
 
 import ctypes
 import math
+import threading
 
 import pytest
 import torch
@@ -278,3 +279,79 @@ def test_neither_gradient(device, n):
     ):
         assert got[1] is None and got[2] is None
         same("loss", got[0], loss)
+
+
+def test_empty_batches_in_autograd(device):
+    """No rows, and no batches: gradients of the leaves' shapes, zeros where there is anything."""
+    x, head, _, _ = head_inputs(device, 4, 300, 64, 8)
+    leaf, weight = x[:0].clone().requires_grad_(), head.clone().requires_grad_()
+    loss = head_loss.token_loss(leaf, weight, torch.empty(0, dtype=torch.int64, device=device.torch))
+    loss.sum().backward()
+    assert loss.shape == (0,) and leaf.grad.shape == (0, 64) and not weight.grad.any()
+    for shape in ((2, 0, 32), (0, 5, 32)):
+        logits = torch.empty(shape, device=device.torch).requires_grad_()
+        ids = torch.empty(*shape[:2], 4, dtype=torch.int16, device=device.torch)
+        loss, counts = balance.balance_loss(logits, ids, 4)
+        loss.sum().backward()
+        assert loss.shape == shape[:1] and counts.shape == (shape[0], 32) and not counts.any() and logits.grad.shape == shape
+
+
+def test_one_vector(device):
+    """x of rank 1, a target of rank 0, teacher's entries of rank 1."""
+    x, head, _, g = head_inputs(device, 1, 300, 64, 9)
+    ids = torch.randint(0, 300, (1,), generator=g).to(device.torch)
+    ti, tv = teacher(1, 5, 300, g, device)
+    for got, want in ((head_loss.token_loss_grads(x[0], head, ids[0]), head_loss.token_loss_grads(x, head, ids)),
+                      (head_loss.distill_loss_grads(x[0], head, tv[0], ti[0]), head_loss.distill_loss_grads(x, head, tv, ti))):
+        assert got[0].shape == () and got[1].shape == (64,)
+        for part, a, b in zip(("loss", "dx", "dhead"), got, want):
+            same(part, a.reshape(b.shape), b)
+
+
+def test_backward_twice_and_on_another_stream(device):
+    """One graph's backward twice, the second time with the caller on another stream than the forward's."""
+    x, head, w, g = head_inputs(device, 200, 900, 136, 10)
+    ids = torch.randint(-50, 900, (200,), generator=g).to(device.torch)
+    logits, slots, mask, gb = router_inputs(device, 3, 70, 64, 60, 4, 10)
+    want = head_loss.token_loss_grads(x, head, ids, w)
+    more = balance.balance_loss_grads(logits, slots, 4, gb, experts=60, mask=mask[:, :1].expand(3, 70))
+    xl, hl, ll = (t.clone().requires_grad_() for t in (x, head, logits))
+    loss = head_loss.token_loss(xl, hl, ids)
+    bal, _ = balance.balance_loss(ll, slots, 4, experts=60, mask=mask[:, :1].expand(3, 70))
+    total = (loss * w).sum() + (bal * gb).sum()
+    side = torch.cuda.Stream()
+    for stream in (torch.cuda.current_stream(), side):
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            grads = torch.autograd.grad(total, (xl, hl, ll), retain_graph=True)
+        torch.cuda.current_stream().wait_stream(stream)
+        for part, a, b in zip(("dx", "dhead", "dlogits"), grads, (want[1], want[2], more[2])):
+            same(part, a, b)
+
+
+def test_two_threads(device):
+    """Two threads at once, a stream each, of few rows and of many: what one alone gives."""
+    calls = []
+    for n in (40, 500):
+        x, head, w, g = head_inputs(device, n, 2000, 264, n)
+        ids = torch.randint(-50, 2000, (n,), generator=g).to(device.torch)
+        logits, slots, mask, gb = router_inputs(device, 2, n, 64, 64, 4, n)
+        calls.append(lambda x=x, head=head, ids=ids, w=w, logits=logits, slots=slots, gb=gb: (
+            *head_loss.token_loss_grads(x, head, ids, w), *balance.balance_loss_grads(logits, slots, 4, gb)))
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got[i] = [calls[i]() for _ in range(20)]
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for outs, ref in zip(got, want):
+        for out in outs:
+            assert all(torch.equal(a, b) for a, b in zip(out, ref))

@@ -70,7 +70,8 @@ def draw(rng):
                 "act": rng.choice(("swiglu", "geglu")), "mode": rng.choice(("alone", "step", "step", "again"))}
         return case if case["mode"] == "alone" else {**case, "weights": rng.choice((True, True, False))}
     layers = _log(rng, 1, 16 if kind == "norm" else 6)
-    case = {"kind": kind, "layers": layers, "d": _log(rng, 64, 1024), "f": _log(rng, 100, 4096), "v": rng.choice((0, 1000, 8192, 32000)), "type": rng.choice(("float32", "bfloat16", "float16"))}
+    case = {"kind": kind, "layers": layers, "d": _log(rng, 64, 1024), "f": _log(rng, 100, 4096),
+            "v": rng.choice((0, 1000, 8192, 32000)), "type": rng.choice(("float32", "bfloat16", "float16"))}
     return case if kind == "norm" else {**case, "out": rng.choice((case["type"], "float32"))}
 
 

@@ -26,40 +26,13 @@
 
 #include "dense_reader.h"
 #include "lm_head.h"
+#include "mfma_tile.h"
 
 #pragma clang fp contract(off)
 
 namespace {
 
-typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8;
-typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
-typedef __attribute__((__vector_size__(2 * sizeof(float)))) float f32x2;
-typedef __attribute__((__vector_size__(4 * sizeof(float)))) float f32x4;
-typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) void* lds_ptr;
-typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
-
-constexpr int KSTEP = 64;                  // k that plans count in
-constexpr uint32_t PAST = 0x80000000u;     // a buffer offset past every record: the load gives zeros
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-
-__device__ __forceinline__ uint32_t cvt2(float lo, float hi) {  // to bf16, to nearest even
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), bf16x2));
-}
-
-__device__ __forceinline__ f32x16 mfma32(uint4 a, uint4 b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
-// The wavefront's LDS reads done and all but its newest VM loads landed, then the workgroup's barrier.
-template <int VM>
-__device__ __forceinline__ void step_barrier() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt((VM & 15) | (7 << 4) | ((VM >> 4) << 14));  // vmcnt(VM) lgkmcnt(0)
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
+constexpr float LN2 = 0.6931471805599453f;
 
 // two maxima, in the exponent of 2, and sums of what exceeds them
 __device__ __forceinline__ void join(float& m, float& s, float v, float w) {
@@ -108,83 +81,12 @@ struct Gemm {
     const float* scale;     // dhead, dx: the factor taken out of dz
 };
 
-// One operand's tile of ROWS x BK values in LDS: 16-byte chunks, laid out so that neither the loads straight from memory
-// (64 chunks in a row a wavefront) nor the fragments' reads meet in a bank.
-template <int ROWS, bool T, int NT, int BK>
-struct Tile {
-    static constexpr int N = ROWS * BK / 8 / NT;  // chunks a lane loads
-    static constexpr int CK = BK / 8;             // chunks of a row's k
-    uint32_t off[N];
-
-    // row r's chunk c (8 k) turned by row, so that 16 rows' fill all banks; across: k's chunk c (8 rows), in pairs (32 bytes)
-    // turned by k
-    static __device__ __forceinline__ int swz(int r) { return BK == 64 ? (r >> 1) & 7 : (r >> 2) & 3; }
-    static __device__ __forceinline__ int turn(int k) { return ROWS >= 128 ? 2 * (k & 3) : ROWS == 64 ? 2 * ((k >> 1) & 1) : 0; }
-
-    __device__ __forceinline__ void init(int tid, int ld, int rows) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int s = i * NT + tid;
-            if constexpr (T) {
-                constexpr int C = ROWS / 8;
-                const int k = s / C, c = s % C, src = ((((c >> 1) ^ turn(k))) << 1) | (c & 1);
-                off[i] = 8 * src < rows ? (uint32_t)(k * ld * 2) + 16u * src : PAST;
-            } else {
-                const int r = s / CK, c = (s % CK) ^ swz(r);
-                off[i] = (uint32_t)(r * ld * 2) + 16u * c;
-            }
-        }
-    }
-    // The step's loads: at: its first value; ld; rows: the operand's rows in the tile (at least 1); left: its k from this step
-    // on (none left: zeros). Never further than the tile's own run of its last row: what comes after may be rows that are not
-    // to be read.
-    static __device__ __forceinline__ __amdgpu_buffer_rsrc_t source(const uint16_t* at, int ld, int rows, int left) {
-        const int r = T ? min(left, BK) : rows, run = min(T ? (rows + 7) & ~7 : (left + 7) & ~7, T ? ROWS : BK);
-        return __builtin_amdgcn_make_buffer_rsrc((void*)at, (short)0, left > 0 ? ((r - 1) * ld + run) * 2 : 0, 0x00020000);
-    }
-    // the lane's chunk i of it to LDS
-    __device__ __forceinline__ void load(int i, __amdgpu_buffer_rsrc_t from, int left, uint4* lds, int tid) const {
-        uint32_t o = off[i];
-        if constexpr (!T) {
-            if (left < BK) {  // (the last step of a ragged k)
-                const int s = i * NT + tid, c = (s % CK) ^ swz(s / CK);
-                if (8 * c >= left) o = PAST;
-            }
-        }
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_ptr)(lds + i * NT + 64 * __builtin_amdgcn_readfirstlane(tid >> 6)), 16, o,
-                                                 0, 0, 0);
-    }
-    // lane's 8 values of row r0 + lane % 32, k = 16 u + 8 (lane / 32) .., the tile from chunk `from` of the stage on. (One
-    // index from the stage's array: through longer chains the compiler no longer sees which stage a read is of, and has it
-    // wait for the loads to the other.)
-    static __device__ __forceinline__ uint4 frag(const uint4* lds, int from, int r0, int u, int lane) {
-        if constexpr (T) {
-            constexpr int C = ROWS / 8;
-            const int h = lane >> 5, half = (lane >> 4) & 1, i = lane & 15;
-            const int k = 8 * h + (i >> 2), pair = ((r0 >> 4) + half) ^ turn(k);  // (turn: the same 4 and 16 k further)
-            const int at = (from + k * C + 2 * pair) * 8 + 4 * (i & 3) + 16 * u * ROWS;
-            const uint16_t* v = reinterpret_cast<const uint16_t*>(lds);
-            const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(v + at)));
-            const uint2 hi = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(v + (at + 4 * ROWS))));
-            return make_uint4(lo.x, lo.y, hi.x, hi.y);
-        } else {
-            const int r = lane & 31, h = lane >> 5;
-            return lds[from + (r0 + r) * CK + ((2 * u + h) ^ swz(r))];
-        }
-    }
-};
-
 // About the time (us) that a workgroup of each product and tile takes for a step of 64 k (more with more of the CUs at work:
 // the memory and the power are shared) and for its beginning and end, as many workgroups at once as fit the CUs. Fitted to the
 // kernels' times at eight shapes of 73 to 8192 rows, 584 to 4096 values and 2898 to 94639 tokens, most within 15 %; what
 // decides between two tiles is mostly how many rounds they take.
 // (KEEP: the statistics, z kept instead of the entries' taken; DZ1: tokens, their own logit's 1 taken off there)
 enum Epi { EPI_STATS, EPI_KEEP, EPI_DZ, EPI_DZ1, EPI_DHEAD, EPI_DX };
-struct Pace {
-    int at_once;
-    float step, shared, ends;
-};
-constexpr int CUS = 256;
 __host__ __device__ constexpr Pace pace(int epi, int bm, int bn, int wk) {
     const bool dx = epi == EPI_DX, dhead = epi == EPI_DHEAD;
     if (wk == 2) return Pace{CUS, dx ? 0.23f : 0.28f, 0.f, dx ? 4.5f : 2.8f};  // 64 x 64, two groups of wavefronts
@@ -192,45 +94,6 @@ __host__ __device__ constexpr Pace pace(int epi, int bm, int bn, int wk) {
     if (bn == 64) return Pace{2 * CUS, 0.6f, 0.9f, 8.f};
     if (bm == 256) return Pace{CUS, dx ? 1.05f : dhead ? 1.15f : 1.2f, 0.45f, dx ? 13.f : dhead ? 8.f : 12.f};
     return Pace{2 * CUS, dx ? 0.75f : dhead ? 0.6f : 0.62f, dhead ? 0.3f : 0.35f, dx ? 7.f : dhead ? 4.f : 8.f};
-}
-
-__host__ __device__ inline float tiled_us(const Pace& p, int tiles, int steps) {
-    const int rounds = (tiles + p.at_once - 1) / p.at_once;
-    const float full = rounds ? (float)tiles / (float)(rounds * p.at_once) : 0.f;
-    return (float)rounds * ((p.step + p.shared * full) * (float)steps + p.ends);
-}
-
-// dx's splits of its long sum, for one or two rounds of workgroups: their sums' way back through memory costs a launch and
-// about 3.5 TB/s. The rows that count are known on the device alone, so every workgroup finds the splits for itself.
-constexpr int ROUNDS = 2;
-__host__ __device__ inline int dx_splits(const Pace& p, int tiles, int steps, int tile_bytes, float* us = nullptr) {
-    int best = 1;
-    float least = tiled_us(p, tiles, steps);
-    for (int r = 1; r <= ROUNDS; ++r) {
-        int s = r * p.at_once / (tiles > 0 ? tiles : 1);
-        if (s > steps / 4) s = steps / 4;
-        if (s < 2) continue;
-        const float t = tiled_us(p, tiles * s, ((steps + s - 1) / s + 1) & ~1) + 4.f + (float)tiles * (float)s * (float)tile_bytes * 0.28e-6f;
-        if (t < least) least = t, best = s;
-    }
-    if (us) *us = least;
-    return best;
-}
-
-// workgroups go to the XCDs in turn; each XCD takes a run of tiles, in groups of GM row tiles by all column tiles, so that
-// what runs at once on an XCD shares rows and columns in its L2. False past the last.
-__device__ __forceinline__ bool tile_of(int tm, int tn, int splits, int& mt, int& nt, int& split) {
-    const int total = tm * tn * splits, xcd = blockIdx.x & 7, own = (total >> 3) + (xcd < (total & 7));
-    if ((int)(blockIdx.x >> 3) >= own) return false;
-    int w = xcd * (total >> 3) + min(xcd, total & 7) + (blockIdx.x >> 3);
-    split = w / (tm * tn);
-    w -= split * tm * tn;
-    constexpr int GM = 4;
-    const int g = w / (GM * tn), first = g * GM, gm = min(GM, tm - first);
-    w -= g * GM * tn;
-    nt = w / gm;
-    mt = first + w - nt * gm;
-    return true;
 }
 
 // D[m][n] in tiles of BM x BN, a wavefront BM / WM x BN / WN of 32x32x16 matrix instructions; NS stages of BK k in LDS, filled

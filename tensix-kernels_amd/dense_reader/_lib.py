@@ -1,5 +1,5 @@
-"""ctypes binding of libdense_reader.so (the C ABI declared in include/dense_reader.h, include/lm_head.h and
-include/moe.h).
+"""ctypes binding of libdense_reader.so (the C ABI declared in include/dense_reader.h, include/lm_head.h, include/moe.h,
+include/gated.h and include/grads.h).
 
 The library is built in-tree (`python -c "import __graft_entry__; __graft_entry__.build()"` at the repository root,
 or `make -C tensix-kernels_amd/dense_reader/csrc`). There is no fallback: without the library every op raises.
@@ -14,7 +14,7 @@ LIB_PATH = Path(__file__).resolve().parent / LIB_NAME
 
 DR_OK, DR_EINVAL, DR_EHIP, DR_ERANGE = 0, 1, 2, 3
 
-# every symbol include/dense_reader.h, include/lm_head.h and include/moe.h declare
+# every symbol the headers in include/ declare
 SYMBOLS = (
     "dr_codes_bytes",
     "dr_exps_bytes",
@@ -46,11 +46,17 @@ SYMBOLS = (
     "dr_moe_route_gate_up",
     "dr_moe_balance_workspace_bytes",
     "dr_moe_balance",
+    "dr_gated_kept_bytes",
+    "dr_gated_workspace_bytes",
+    "dr_gated_plan",
+    "dr_gated_run",
 )
 
 DR_LOSS_FORWARD, DR_LOSS_BACKWARD = 1, 2
 DR_LOSS_MAX_K = 64
 DR_LOSS_MAX_LD = 1 << 21
+DR_GATED_FORWARD, DR_GATED_BACKWARD = 1, 2
+DR_GATED_MAX_LD = 1 << 21
 DR_BALANCE_LOSS, DR_BALANCE_GRAD, DR_BALANCE_BACKWARD = 1, 2, 8
 
 DR_MOE_GATE_UP, DR_MOE_DOWN, DR_MOE_GATE_UP_ROWS, DR_MOE_DOWN_ROWS = 1, 2, 3, 4
@@ -248,6 +254,45 @@ class Balance(ctypes.Structure):
     ]
 
 
+class Gated(ctypes.Structure):
+    _fields_ = [
+        ("x", c_void_p),
+        ("ldx", c_int64),
+        ("gate", c_void_p),
+        ("ld_gate", c_int64),
+        ("up", c_void_p),
+        ("ld_up", c_int64),
+        ("rows", c_int32),
+        ("dim", c_int32),
+        ("width", c_int32),
+        ("act", c_int32),
+        ("h", c_void_p),
+        ("ld_h", c_int64),
+        ("kept", c_void_p),
+        ("dh", c_void_p),
+        ("ld_dh", c_int64),
+        ("dx", c_void_p),
+        ("ld_dx", c_int64),
+        ("dgate", c_void_p),
+        ("ld_dgate", c_int64),
+        ("dup", c_void_p),
+        ("ld_dup", c_int64),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
+        ("stream", c_void_p),
+    ]
+
+
+class GatedInfo(ctypes.Structure):
+    _fields_ = [
+        ("act", c_int32 * 3),
+        ("dweight", c_int32 * 3),
+        ("dweight_stages", c_int32),
+        ("dx", c_int32 * 3),
+        ("dx_splits", c_int32),
+    ]
+
+
 _lib = None
 
 
@@ -325,6 +370,14 @@ def lib():
         L.dr_moe_balance.argtypes = [ctypes.POINTER(Balance), c_int]
         L.dr_moe_route_gate_up.restype = c_int
         L.dr_moe_route_gate_up.argtypes = [ctypes.POINTER(Launch), ctypes.POINTER(Moe), ctypes.POINTER(Route)]
+        L.dr_gated_kept_bytes.restype = c_int64
+        L.dr_gated_kept_bytes.argtypes = [ctypes.POINTER(Gated)]
+        L.dr_gated_workspace_bytes.restype = c_int64
+        L.dr_gated_workspace_bytes.argtypes = [ctypes.POINTER(Gated), c_int]
+        L.dr_gated_plan.restype = c_int
+        L.dr_gated_plan.argtypes = [ctypes.POINTER(Gated), c_int, ctypes.POINTER(GatedInfo)]
+        L.dr_gated_run.restype = c_int
+        L.dr_gated_run.argtypes = [ctypes.POINTER(Gated), c_int]
         _lib = L
     return _lib
 
@@ -339,11 +392,22 @@ def check(status, what):
     raise RuntimeError(msg)
 
 
+def _fields(info):
+    return {f: getattr(info, f) if t is c_int32 else tuple(getattr(info, f)) for f, t in info._fields_}
+
+
 def head_loss_info(A, what):
     """dr_head_loss_plan's answer, as a dict."""
     info = HeadLossInfo()
     check(lib().dr_head_loss_plan(ctypes.byref(A), what, ctypes.byref(info)), "dr_head_loss_plan")
-    return {f: getattr(info, f) if t is c_int32 else tuple(getattr(info, f)) for f, t in HeadLossInfo._fields_}
+    return _fields(info)
+
+
+def gated_info(A, what):
+    """dr_gated_plan's answer, as a dict."""
+    info = GatedInfo()
+    check(lib().dr_gated_plan(ctypes.byref(A), what, ctypes.byref(info)), "dr_gated_plan")
+    return _fields(info)
 
 
 def launch_info(L):

@@ -1,0 +1,672 @@
+// gated.hip: the gated feed-forward block in training and its gradients for MI355X (gfx950), behind include/gated.h.
+//
+//   g = x . gate^T, u = x . up^T, h = a(g) u              one product of gate's and up's rows together; h is its epilogue
+//   du = dh a(g), dg = dh u a'(g)                         by the value, from what the forward call kept; or the same product
+//                                                         again with this as its epilogue
+//   dgate = dg^T . x, dup = du^T . x                      one product of dg's and du's columns together, summed over rows
+//   dx = dg . gate + du . up                              one product, summed over gate's and then up's outputs
+//
+// All are of one tiled MFMA kernel (gt_gemm) whose operands are read as they lie, along the summed dimension or across it
+// (mfma_tile.h). A tile of the first has as many rows of gate as of up, a wavefront the same outputs of both, so that g and u of
+// an output meet in one lane's registers. dg, du and what is kept lie in panels of 256 outputs ([output / 256][row][256]), which
+// the products that read them take in contiguous blocks.
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <initializer_list>
+
+#include "dense_reader.h"
+#include "gated.h"
+#include "mfma_tile.h"
+
+#pragma clang fp contract(off)
+
+namespace {
+
+// --- the activation -----------------------------------------------------------------------------------------------------
+
+// 1 / (1 + exp(-v))
+__device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-LOG2E * v)); }
+
+// a(g) and a'(g). gelu's tanh form is g p with p = sigmoid(c (g + 0.044715 g^3)), c = 2 sqrt(2 / pi). (Where p is 0 or 1 its slope
+// is 0, and what that is multiplied by stays finite.)
+template <bool GELU>
+__device__ __forceinline__ void act_of(float g, float& a, float& slope) {
+    constexpr float C = 1.5957691216057308f, C3 = 0.044715f * C;
+    if constexpr (GELU) {
+        const float p = sigmoid(g * __builtin_fmaf(C3, g * g, C));
+        const float t = fminf(fmaxf(g, -16.f), 16.f);
+        a = g * p;
+        slope = __builtin_fmaf(t * (p * (1.f - p)), __builtin_fmaf(3.f * C3, t * t, C), p);
+    } else {
+        const float p = sigmoid(g);
+        const float t = fminf(fmaxf(g, -1e30f), 1e30f);
+        a = g * p;
+        slope = p * __builtin_fmaf(t, 1.f - p, 1.f);
+    }
+}
+
+// What a forward call keeps of an output: a(g) and a'(g) u, in 24 bits each (float32's without the last 8 of the mantissa): the upper
+// 16 of both, then a's lower 8 over those of the other. (In bf16 alone dg and du would be rounded twice, and a step's gradients off by
+// 2.9e-3 of their norm instead of 2.35e-3; their own rounding alone makes 1.7e-3. 2 bytes more in 12 of the pass that reads it.)
+__device__ __forceinline__ uint2 upper(const uint32_t (&v)[4]) {
+    return make_uint2((v[0] >> 16) | (v[1] & 0xFFFF0000u), (v[2] >> 16) | (v[3] & 0xFFFF0000u));
+}
+__device__ __forceinline__ uint2 lower(const uint32_t (&a)[4], const uint32_t (&s)[4]) {
+    auto two = [](uint32_t a, uint32_t s) { return (a & 0xFF00u) | (s >> 8 & 0xFFu); };
+    return make_uint2(two(a[0], s[0]) | two(a[1], s[1]) << 16, two(a[2], s[2]) | two(a[3], s[3]) << 16);
+}
+// value e of 4, from its upper part and the lower ones of both
+__device__ __forceinline__ float kept_a(uint2 hi, uint2 lo, int e) {
+    const uint32_t h = e < 2 ? hi.x : hi.y, l = e < 2 ? lo.x : lo.y;
+    return __uint_as_float(e & 1 ? (h & 0xFFFF0000u) | (l >> 16 & 0xFF00u) : h << 16 | (l & 0xFF00u));
+}
+__device__ __forceinline__ float kept_s(uint2 hi, uint2 lo, int e) {
+    const uint32_t h = e < 2 ? hi.x : hi.y, l = e < 2 ? lo.x : lo.y;
+    return __uint_as_float(e & 1 ? (h & 0xFFFF0000u) | (l >> 8 & 0xFF00u) : h << 16 | (l << 8 & 0xFF00u));
+}
+__device__ __forceinline__ float bf16_of(uint2 v, int e) {
+    const uint32_t w = e < 2 ? v.x : v.y;
+    return __uint_as_float(e & 1 ? w & 0xFFFF0000u : w << 16);
+}
+
+// --- the tiled product --------------------------------------------------------------------------------------------------
+
+// ACT, KEEP, AGAIN: D[2 width][rows], A gate and up, B x; DW: D[dim][outputs], A x, B dg and du; DX: D[dim][rows], A gate and up,
+// B dg and du
+enum Epi { EPI_ACT, EPI_KEEP, EPI_AGAIN, EPI_DW, EPI_DX };
+
+struct Prod {
+    const uint16_t *x, *gate, *up;
+    int ldx, ld_gate, ld_up;
+    int rows, dim, width;
+    int panels;             // of 256 outputs, a side
+    long long panel;        // values of one: rows * 256
+    int tm, tn;             // tiles
+    uint16_t* h;
+    long long ld_h;
+    uint16_t* kept;         // [3][panels][rows][256]: see keep_of
+    const uint16_t* dh;
+    long long ld_dh;
+    uint16_t* dz;           // dg, then du, each [panels][rows][256]
+    int side0;              // DW: the first of the sides that are asked for
+    uint16_t *dgate, *dup;
+    long long ld_dgate, ld_dup;
+    uint16_t* dx;           // or NULL: the sums of each split
+    long long ld_dx;
+    float* acc;             // [splits][rows][dim]
+    int splits;
+};
+
+template <int BM, int BN, int WM, int WN, int WK, int NS, int BK, int EPI, bool GELU>
+__global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
+    constexpr bool PAIR = EPI <= EPI_AGAIN, AT = !PAIR, BT = EPI == EPI_DW;
+    constexpr int NW = WM * WN, NT = 64 * NW, TM = BM / WM, TN = BN / WN, MI = TM / 32, NI = TN / 32;
+    constexpr int CA = BM * BK / 8, CH = CA + BN * BK / 8;  // chunks of A, a stage
+    constexpr int NL = CH / NT, NA = CA / NT;               // loads a lane and stage, of A
+    constexpr int FM = PAIR ? BM / 2 : BM, FT = PAIR ? TM / 2 : TM;  // outputs of a tile, of a wavefront
+    static_assert(NS >= 1 && NS <= 4, "one to four stages");
+    static_assert(!PAIR || (MI % 2 == 0 && FT % (NT * 8 / BK) == 0), "a load is of gate or of up, a wavefront has both");
+    constexpr int C1 = NS > 1 ? CH * WK : 1, C2 = NS > 2 ? CH * WK : 1, C3 = NS > 3 ? CH * WK : 1;
+    // (an array each, named where it is used: a read waits for the loads to every array that the compiler cannot rule out)
+    __shared__ uint4 s0[CH * WK], s1[C1], s2[C2], s3[C3];
+    // WK groups of wavefronts, each a share of K in stages of its own, all with the same barriers; tid within the group
+    const int group = WK == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / NT), tid = threadIdx.x - group * NT;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), mine = group * CH;
+    const int wm = wave / WN, wn = wave % WN;
+    int mt, nt, split;
+    if (!tile_of(a.tm, a.tn, EPI == EPI_DX ? a.splits : 1, mt, nt, split)) return;
+    const int m0 = mt * FM, n0 = nt * BN;
+    // DW: the tile's side, and its first output there
+    const int side_n = EPI == EPI_DW ? a.side0 + (n0 >= a.panels * 256) : 0, c0 = EPI == EPI_DW ? n0 - (side_n - a.side0) * a.panels * 256 : n0;
+    const int n_end = EPI == EPI_DW ? a.width : a.rows, m_end = PAIR ? a.width : a.dim;
+    if (c0 >= n_end) return;  // (what a side's last panel has past its last output)
+    // the steps of K: DX sums over gate's outputs, then over up's, each side whole steps
+    const int k_end = PAIR ? a.dim : EPI == EPI_DW ? a.rows : a.width, own = (k_end + BK - 1) / BK;
+    const int all = EPI == EPI_DX ? 2 * own : own;
+    // (a split's steps are whole rounds of the stages: the next split's are not its own)
+    constexpr int ROUND = NS * WK;
+    const int splits = EPI == EPI_DX ? a.splits : 1;
+    const int per = ((all + splits - 1) / splits + ROUND - 1) / ROUND * ROUND, step0 = split * per;
+    const int steps = min(per, all - step0);
+    const int rounds = steps > 0 ? ((steps + WK - 1) / WK + NS - 1) / NS : 0;  // (of the stages)
+
+    Tile<BM, AT, NT, BK> ta;
+    Tile<BN, BT, NT, BK> tb;
+    const int ra = m_end - m0, rb = n_end - c0;  // (rows past the tile's)
+    const int ldb = PAIR ? a.ldx : 256;
+    if constexpr (PAIR) {
+        // row r of the tile: of a wavefront's TM rows the first half gate's outputs, the second up's; a load has rows of one
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+            const int s = i * NT + tid, r = s / ta.CK, c = (s % ta.CK) ^ ta.swz(r);
+            const int ld = (i * NT / ta.CK) % TM >= FT ? a.ld_up : a.ld_gate;
+            ta.off[i] = (uint32_t)((r / TM * FT + r % FT) * ld * 2) + 16u * c;
+        }
+    } else {
+        ta.init(tid, EPI == EPI_DW ? a.ldx : a.ld_gate, ra);
+    }
+    tb.init(tid, ldb, rb);
+    int st = step0 + group * rounds * NS;  // the next step to be loaded
+    __amdgpu_buffer_rsrc_t from_a, from_u, from_b;
+    int left_a, left_b;
+    bool second = false;  // DX: the steps are up's
+    auto next = [&] {
+        const int side = EPI == EPI_DX ? st >= own : 0, k = (st - side * own) * BK;
+        left_a = left_b = k_end - k;
+        if constexpr (PAIR) {
+            const int r = min(FM, ra);
+            from_a = ta.source(a.gate + (long long)m0 * a.ld_gate + k, a.ld_gate, r, left_a);
+            from_u = ta.source(a.up + (long long)m0 * a.ld_up + k, a.ld_up, r, left_a);
+            from_b = tb.source(a.x + (long long)n0 * a.ldx + k, a.ldx, min(BN, rb), left_b);
+        } else if constexpr (EPI == EPI_DW) {
+            from_a = ta.source(a.x + (long long)k * a.ldx + m0, a.ldx, ra, left_a);
+            from_b = tb.source(a.dz + (side_n * a.panels + (c0 >> 8)) * a.panel + (c0 & 255) + (long long)k * 256, 256, rb, left_b);
+        } else {
+            if (side && !second) ta.init(tid, a.ld_up, ra), second = true;  // (up's rows may lie otherwise apart)
+            const int ld = side ? a.ld_up : a.ld_gate;
+            from_a = ta.source((side ? a.up : a.gate) + (long long)k * ld + m0, ld, ra, left_a);
+            from_b = tb.source(a.dz + (side * a.panels + (k >> 8)) * a.panel + (k & 255) + n0 * 256ll, 256, min(BN, rb), left_b);
+        }
+        ++st;
+    };
+    auto load = [&](int i0, int i1, uint4* b) {  // its loads i0 .. i1 - 1 of NL
+#pragma unroll
+        for (int i = i0; i < i1; ++i) {
+            if (i < NA) {
+                if constexpr (PAIR) ta.load(i, (i * NT / ta.CK) % TM >= FT ? from_u : from_a, left_a, b + mine, tid);
+                else ta.load(i, from_a, left_a, b + mine, tid);
+            } else {
+                tb.load(i - NA, from_b, left_b, b + (mine + CA), tid);
+            }
+        }
+    };
+    constexpr int CN = MI * NI > 1 ? 1 : 2;  // sums of one tile: two in turn, which need not wait for each other
+    f32x16 acc[MI][NI], odd;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        odd[e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) acc[i][j][e] = 0.f;
+    }
+    // A step's sums from one stage, the loads of a later step to another; with three stages and more between the sums: a wavefront
+    // that issues all of its loads at once stands still until the memory pipeline has taken them, and all do after the barrier.
+    auto sum = [&](const uint4* b, uint4* to) {
+        constexpr int U = BK / 16;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            uint4 fa[MI], fb[NI];
+#pragma unroll
+            for (int j = 0; j < NI; ++j) fb[j] = Tile<BN, BT, NT, BK>::frag(b, mine + CA, wn * TN + 32 * j, u, lane);
+#pragma unroll
+            for (int i = 0; i < MI; ++i) fa[i] = Tile<BM, AT, NT, BK>::frag(b, mine, wm * TM + 32 * i, u, lane);
+            if constexpr (NS >= 3) load(u * NL / U, (u + 1) * NL / U, to);
+            else if (NS == 2 && u == 0) load(0, NL, to);
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j) {
+                    f32x16& into = CN == 2 && (u & 1) ? odd : acc[i][j];
+                    into = mfma32(fa[i], fb[j], into);
+                }
+            // (one u's fragments at a time: the registers hold no more; a small tile reads them all at once)
+            if constexpr (MI * NI > 2) __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // (whole rounds of the stages: steps past the last are zeros, as are the loads past the end into stages that nothing
+    // reads. A last step of its own behind a branch would have the compiler copy every accumulator.)
+    auto step = [&](uint4* to, const uint4* from) {
+        step_barrier<NS >= 3 ? (NS - 2) * NL : 0>();
+        next();
+        sum(from, to);
+    };
+    auto first = [&](uint4* to) {
+        next();
+        load(0, NL, to);
+    };
+    if (rounds > 0) {
+        first(s0);
+        if constexpr (NS >= 3) first(s1);
+        if constexpr (NS >= 4) first(s2);
+    }
+    for (int s = 0; s < rounds; ++s) {
+        if constexpr (NS == 1) {  // (more workgroups instead)
+            step_barrier<0>();
+            sum(s0, s0);
+            if (s + 1 < rounds) {
+                step_barrier<0>();
+                first(s0);
+            }
+        } else if constexpr (NS == 2) {
+            step(s1, s0);
+            step(s0, s1);
+        } else if constexpr (NS == 3) {
+            step(s2, s0);
+            step(s0, s1);
+            step(s1, s2);
+        } else {
+            step(s3, s0);
+            step(s0, s1);
+            step(s1, s2);
+            step(s2, s3);
+        }
+    }
+    step_barrier<0>();  // (the last loads landed: they write this workgroup's LDS)
+    if constexpr (CN == 2) acc[0][0] += odd;
+    if constexpr (WK > 1) {  // the other groups' sums to the first
+        static_assert(WK == 1 || (WK - 1) * NW * MI * NI * 256 <= C1, "their sums fit a stage");
+        f32x4* const at = reinterpret_cast<f32x4*>(s1) + wave * MI * NI * 256 + lane;
+        if (group) {
+            f32x4* to = at + (group - 1) * NW * MI * NI * 256;
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        to[64 * ((i * NI + j) * 4 + g)] =
+                            f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+        }
+        step_barrier<0>();
+        if (group) return;
+#pragma unroll
+        for (int w = 0; w < WK - 1; ++w)
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const f32x4 v = at[w * NW * MI * NI * 256 + 64 * ((i * NI + j) * 4 + g)];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[i][j][4 * g + e] += v[e];
+                    }
+    }
+
+    // lane: columns n = c0 + wn TN + 32 j + lane % 32, rows mw + 32 i + 8 g + 4 (lane / 32) + 0 .. 3 in words 4 g ..
+    const int r = lane & 31, h = lane >> 5;
+    const int mw = m0 + wm * FT;
+    // the wavefront's own part of the stages: 32 columns of its FT rows in bf16
+    constexpr int FIT = CH * WK / (4 * FT), PER = FIT < NW ? FIT : NW, PARTS = (NW + PER - 1) / PER;
+    static_assert(PARTS <= NS && (WK == 1 || PARTS == 1), "the wavefronts' parts fit the stages that are free");
+    uint4* region = s0 + (wave % PER) * 4 * FT;
+    if constexpr (PARTS > 1) {
+        const int at = wave / PER;
+        region = (at == 0 ? s0 : at == 1 ? s1 : at == 2 ? s2 : s3) + (wave % PER) * 4 * FT;
+    }
+    // 32 columns in bf16, 4 rows of column r at 8-byte unit q: to and from whole runs of a column's rows in memory
+    uint2* const half = reinterpret_cast<uint2*>(region);
+    constexpr int C16 = FT / 8, SWZ = C16 < 16 ? C16 - 1 : 15;  // 16-byte chunks a column; their turn by column
+    constexpr int PC = 64 / C16;                                // columns a turn
+    auto unit = [&](int q) -> uint2& { return half[(r * C16 + ((q >> 1) ^ (r & SWZ))) * 2 + (q & 1)]; };
+    auto store = [&](auto&& at, int cols, int rows) {  // at(c, row): column c's place for 8 of its rows from `row` on
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int t = 0; t < 32 / PC; ++t) {
+            const int c = t * PC + lane / C16, q = lane % C16;
+            if (c < cols && 8 * q < rows) *reinterpret_cast<uint4*>(at(c, 8 * q)) = region[c * C16 + (q ^ (c & SWZ))];
+        }
+        __builtin_amdgcn_wave_barrier();
+    };
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+        const int nj = c0 + wn * TN + 32 * j, n = nj + r;
+        // panels: this wavefront's outputs lie in one
+        const long long at = (mw >> 8) * a.panel + (long long)nj * 256 + (mw & 255);
+        if constexpr (PAIR) {
+            constexpr int HI = MI / 2;
+            const int left = a.width - mw;
+            const long long kept = a.panels * a.panel;
+            uint2 d[HI][4];
+            if constexpr (EPI == EPI_AGAIN) {
+                const uint16_t* from = a.dh + nj * a.ld_dh + mw;
+#pragma unroll
+                for (int t = 0; t < 32 / PC; ++t) {
+                    const int c = t * PC + lane / C16, q = lane % C16;
+                    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                    if (nj + c < n_end && 8 * q < left) v = *reinterpret_cast<const uint4*>(from + c * a.ld_dh + 8 * q);
+                    region[c * C16 + (q ^ (c & SWZ))] = v;
+                }
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int i = 0; i < HI; ++i)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) d[i][g] = unit(8 * i + 2 * g + h);
+                __builtin_amdgcn_wave_barrier();
+            }
+            uint2 one[HI][4], two[HI][4], three[HI][4];
+#pragma unroll
+            for (int i = 0; i < HI; ++i)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    float o[4], p[4];
+                    uint32_t ab[4], sb[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float u = acc[i + HI][j][4 * g + e];
+                        float act, slope;
+                        act_of<GELU>(acc[i][j][4 * g + e], act, slope);
+                        if constexpr (EPI == EPI_AGAIN) {
+                            const float dh = bf16_of(d[i][g], e);
+                            o[e] = dh * (slope * u);
+                            p[e] = dh * act;
+                        } else {
+                            o[e] = act * u;
+                            ab[e] = __float_as_uint(act);
+                            sb[e] = __float_as_uint(slope * u);
+                        }
+                    }
+                    unit(8 * i + 2 * g + h) = make_uint2(cvt2(o[0], o[1]), cvt2(o[2], o[3]));
+                    if constexpr (EPI == EPI_AGAIN) one[i][g] = make_uint2(cvt2(p[0], p[1]), cvt2(p[2], p[3]));
+                    if constexpr (EPI == EPI_KEEP) one[i][g] = upper(ab), two[i][g] = upper(sb), three[i][g] = lower(ab, sb);
+                }
+            auto lay = [&](const uint2 (&v)[HI][4]) {
+#pragma unroll
+                for (int i = 0; i < HI; ++i)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) unit(8 * i + 2 * g + h) = v[i][g];
+            };
+            if constexpr (EPI == EPI_AGAIN) {
+                uint16_t* o = a.dz + at;
+                store([&](int c, int row) { return o + c * 256 + row; }, n_end - nj, left);
+                lay(one);
+                store([&](int c, int row) { return o + kept + c * 256 + row; }, n_end - nj, left);
+            } else {
+                uint16_t* o = a.h + nj * a.ld_h + mw;
+                store([&](int c, int row) { return o + c * a.ld_h + row; }, n_end - nj, left);
+                if constexpr (EPI == EPI_KEEP) {
+                    uint16_t* k = a.kept + at;
+                    lay(one);
+                    store([&](int c, int row) { return k + c * 256 + row; }, n_end - nj, left);
+                    lay(two);
+                    store([&](int c, int row) { return k + kept + c * 256 + row; }, n_end - nj, left);
+                    lay(three);
+                    store([&](int c, int row) { return k + 2 * kept + c * 256 + row; }, n_end - nj, left);
+                }
+            }
+        } else if (EPI == EPI_DW || a.dx != nullptr) {
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    unit(8 * i + 2 * g + h) = make_uint2(cvt2(acc[i][j][4 * g], acc[i][j][4 * g + 1]),
+                                                         cvt2(acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]));
+            const long long ld = EPI == EPI_DX ? a.ld_dx : side_n ? a.ld_dup : a.ld_dgate;
+            uint16_t* o = (EPI == EPI_DX ? a.dx : side_n ? a.dup : a.dgate) + nj * ld + mw;
+            store([&](int c, int row) { return o + c * ld + row; }, n_end - nj, m_end - mw);
+        } else {
+            if (n >= n_end) continue;
+            float* o = a.acc + ((long long)split * a.rows + n) * a.dim + mw;
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int d = 32 * i + 8 * g + 4 * h;
+                    if (mw + d < m_end)
+                        *reinterpret_cast<f32x4*>(o + d) =
+                            f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+                }
+        }
+    }
+}
+
+// --- between and after the products -------------------------------------------------------------------------------------
+
+struct Slope {
+    const uint16_t *kept, *dh;
+    uint16_t* dz;
+    long long ld_dh, panel, side;  // (values of one panel, of one side)
+    int rows, width;
+};
+
+// dg and du from dh and what the forward call kept: a wavefront's rows of one panel
+constexpr int SLOPE_ROWS = 8;  // a wavefront, asked for at once
+__global__ __launch_bounds__(256) void gt_slope(const Slope p) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = (blockIdx.y * 4 + wave) * SLOPE_ROWS, f = blockIdx.x * 256 + 4 * lane;
+    if (n0 >= p.rows || f >= p.width) return;
+    const long long at = blockIdx.x * p.panel + (long long)n0 * 256 + 4 * lane;
+    uint2 dh[SLOPE_ROWS], a[SLOPE_ROWS], s[SLOPE_ROWS], lo[SLOPE_ROWS];
+#pragma unroll
+    for (int i = 0; i < SLOPE_ROWS; ++i) {
+        const int n = min(i, p.rows - 1 - n0);
+        dh[i] = *reinterpret_cast<const uint2*>(p.dh + (n0 + n) * p.ld_dh + f);
+        a[i] = *reinterpret_cast<const uint2*>(p.kept + at + n * 256);
+        s[i] = *reinterpret_cast<const uint2*>(p.kept + p.side + at + n * 256);
+        lo[i] = *reinterpret_cast<const uint2*>(p.kept + 2 * p.side + at + n * 256);
+    }
+#pragma unroll
+    for (int i = 0; i < SLOPE_ROWS; ++i) {
+        if (n0 + i >= p.rows) break;
+        float dg[4], du[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float d = bf16_of(dh[i], e);
+            dg[e] = d * kept_s(s[i], lo[i], e);
+            du[e] = d * kept_a(a[i], lo[i], e);
+        }
+        *reinterpret_cast<uint2*>(p.dz + at + i * 256) = make_uint2(cvt2(dg[0], dg[1]), cvt2(dg[2], dg[3]));
+        *reinterpret_cast<uint2*>(p.dz + p.side + at + i * 256) = make_uint2(cvt2(du[0], du[1]), cvt2(du[2], du[3]));
+    }
+}
+
+struct Join {
+    const float* acc;
+    uint16_t* dx;
+    long long ld_dx;
+    int splits, rows, dim;
+};
+
+// dx from the splits' sums, in their order: 4 values a lane
+__global__ __launch_bounds__(256) void gt_join(const Join p) {
+    const int cols = p.dim / 4;
+    const long long stride = (long long)p.rows * p.dim;
+    for (long long w = blockIdx.x * 256ll + threadIdx.x; w < (long long)p.rows * cols; w += gridDim.x * 256ll) {
+        const int n = (int)(w / cols), d = 4 * (int)(w - (long long)n * cols);
+        const float* at = p.acc + (long long)n * p.dim + d;
+        f32x4 v = *reinterpret_cast<const f32x4*>(at);
+#pragma unroll 4
+        for (int i = 1; i < p.splits; ++i) v += *reinterpret_cast<const f32x4*>(at + i * stride);
+        *reinterpret_cast<uint2*>(p.dx + n * p.ld_dx + d) = make_uint2(cvt2(v[0], v[1]), cvt2(v[2], v[3]));
+    }
+}
+
+// --- the plan -----------------------------------------------------------------------------------------------------------
+
+constexpr int MOST_TILES = (1 << 23) - 8;  // of 512 lanes: a launch holds fewer than 2^32
+
+long long up(long long v, long long to) { return (v + to - 1) / to * to; }
+
+enum Tiles { T256, T128, T64, T64K, T256x64, T128x64 };  // (T64K: two groups of wavefronts split K)
+struct Size {
+    int bm, bn, wk;
+};
+constexpr Size SIZE[] = {{256, 256, 1}, {128, 128, 1}, {64, 64, 1}, {64, 64, 2}, {256, 64, 1}, {128, 64, 1}};
+
+// The times of a workgroup, as head_loss.hip's of the same products.
+Pace pace_of(int epi, int t) {
+    const bool dx = epi == EPI_DX, dw = epi == EPI_DW;
+    switch (t) {
+        case T64K: return Pace{CUS, dx ? 0.23f : 0.28f, 0.f, dx ? 4.5f : 2.8f};
+        case T64: return Pace{2 * CUS, 0.32f, 0.16f, 3.5f};
+        case T256x64:
+        case T128x64: return Pace{2 * CUS, 0.6f, 0.9f, 8.f};
+        case T256: return Pace{CUS, dx ? 1.05f : dw ? 1.15f : 1.2f, 0.45f, dx ? 13.f : dw ? 8.f : 12.f};
+        default: return Pace{2 * CUS, dx ? 0.75f : dw ? 0.6f : 0.62f, dw ? 0.3f : 0.35f, dx ? 7.f : dw ? 4.f : 8.f};
+    }
+}
+
+long long tiles_of(int t, long long m, long long n) { return up(m, SIZE[t].bm) / SIZE[t].bm * (up(n, SIZE[t].bn) / SIZE[t].bn); }
+
+// the tile of `tiles` that takes the least time for a product of m rows by n columns, summed over k
+int choose(int epi, long long m, long long n, long long k, std::initializer_list<int> tiles) {
+    int best = 0;
+    float least = 1e30f;
+    const int steps = (int)(up(k, KSTEP) / KSTEP);
+    for (int t : tiles) {
+        float us;
+        if (epi == EPI_DX) dx_splits(pace_of(epi, t), (int)tiles_of(t, m, n), steps, SIZE[t].bm * SIZE[t].bn * 4, &us);
+        else us = tiled_us(pace_of(epi, t), (int)tiles_of(t, m, n), steps);
+        if (us < least) least = us, best = t;
+    }
+    return best;
+}
+
+struct Plan {
+    int panels, z, w, d, splits;
+    bool one_stage;  // DW
+    long long kept, acc, bytes;  // (the workspace: dg and du, then the sums of dx's splits)
+};
+
+bool ld_ok(long long ld, long long least) { return ld >= least && ld % 8 == 0; }
+
+bool plan_of(const dr_gated* a, int what, Plan& p) {
+    if (a == nullptr || (what != DR_GATED_FORWARD && what != DR_GATED_BACKWARD) || a->rows < 1 || a->rows > (1 << 20) ||
+        a->dim < 8 || a->dim > (1 << 17) || a->dim % 8 || a->width < 8 || a->width > (1 << 20) || a->width % 8 || a->act < 0 ||
+        a->act > 1 || !ld_ok(a->ldx, a->dim) || !ld_ok(a->ld_gate, a->dim) || !ld_ok(a->ld_up, a->dim) ||
+        a->ldx > DR_GATED_MAX_LD || a->ld_gate > DR_GATED_MAX_LD || a->ld_up > DR_GATED_MAX_LD)
+        return false;
+    const long long n = a->rows, f = a->width, d = a->dim;
+    p = Plan{};
+    p.panels = (int)(up(f, 256) / 256);
+    p.kept = 3ll * p.panels * n * 512;
+    const bool back = what == DR_GATED_BACKWARD;
+    if (tiles_of(T64, 2 * f, n) >= MOST_TILES || tiles_of(T64, d, n) >= MOST_TILES || tiles_of(T128, d, 2 * up(f, 256)) >= MOST_TILES)
+        return false;
+    const bool z = !back || (a->kept == nullptr && (a->dx || a->dgate || a->dup));
+    if (z) {
+        if (n <= 64) p.z = tiles_of(T128x64, 2 * f, n) >= 2 * CUS ? T128x64 : T64K;
+        else p.z = choose(EPI_ACT, 2 * f, n, d, {T256, T128, T64K});
+    }
+    if (!back) return true;
+    long long at = 2ll * p.panels * n * 512;
+    if (a->dgate || a->dup) {
+        p.w = choose(EPI_DW, d, up(f, 256) * ((a->dgate != nullptr) + (a->dup != nullptr)), n, {T256, T128});
+        p.one_stage = n <= KSTEP || (p.w == T128 && n <= 1024);
+    }
+    p.acc = at;
+    if (a->dx) {
+        p.d = n <= 64 ? choose(EPI_DX, d, n, 2 * f, {T256x64, T64K}) : choose(EPI_DX, d, n, 2 * f, {T256, T128, T64K});
+        p.splits = dx_splits(pace_of(EPI_DX, p.d), (int)tiles_of(p.d, d, n), (int)(up(2 * f, KSTEP) / KSTEP), SIZE[p.d].bm * SIZE[p.d].bn * 4);
+        if (p.splits > 1) at += up(p.splits * n * d * 4, 256);
+    }
+    p.bytes = a->dx || a->dgate || a->dup ? at : 0;
+    return true;
+}
+
+template <int BM, int BN, int WM, int WN, int WK, int NS, int BK, int EPI, bool GELU>
+void launch(Prod g, int m, int n, hipStream_t st) {
+    g.tm = (m + BM - 1) / BM;
+    g.tn = (n + BN - 1) / BN;
+    const int grid = (g.tm * g.tn * (EPI == EPI_DX ? g.splits : 1) + 7) & ~7;  // (as many for each XCD)
+    hipLaunchKernelGGL((gt_gemm<BM, BN, WM, WN, WK, NS, BK, EPI, GELU>), dim3(grid), dim3(64 * WM * WN * WK), 0, st, g);
+}
+
+template <int EPI, bool GELU>
+void launch_act(const Prod& g, int t, hipStream_t st) {
+    const int m = 2 * g.width, n = g.rows;
+    switch (t) {
+        case T256: return launch<256, 256, 2, 4, 1, 2, 64, EPI, GELU>(g, m, n, st);
+        case T128: return launch<128, 128, 2, 2, 1, 2, 64, EPI, GELU>(g, m, n, st);
+        case T128x64: return launch<128, 64, 2, 2, 1, 3, 64, EPI, GELU>(g, m, n, st);
+        default: return launch<64, 64, 1, 2, 2, 4, 64, EPI, GELU>(g, m, n, st);
+    }
+}
+
+template <int EPI>
+void launch_act(const Prod& g, int act, int t, hipStream_t st) {
+    if (act) launch_act<EPI, true>(g, t, st);
+    else launch_act<EPI, false>(g, t, st);
+}
+
+bool aligned(const void* p, uintptr_t to) { return p != nullptr && reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+}  // namespace
+
+extern "C" int64_t dr_gated_kept_bytes(const dr_gated* a) {
+    Plan p;
+    return plan_of(a, DR_GATED_FORWARD, p) ? p.kept : -1;
+}
+
+extern "C" int64_t dr_gated_workspace_bytes(const dr_gated* a, int what) {
+    Plan p;
+    return plan_of(a, what, p) ? p.bytes : -1;
+}
+
+extern "C" int dr_gated_plan(const dr_gated* a, int what, dr_gated_info* info) {
+    Plan p;
+    if (info == nullptr || !plan_of(a, what, p)) return DR_EINVAL;
+    *info = dr_gated_info{};
+    auto tile = [](int32_t (&to)[3], int t) { to[0] = SIZE[t].bm, to[1] = SIZE[t].bn, to[2] = SIZE[t].wk; };
+    const bool back = what == DR_GATED_BACKWARD;
+    if (!back || (a->kept == nullptr && (a->dx || a->dgate || a->dup))) tile(info->act, p.z);
+    if (!back) return DR_OK;
+    if (a->dgate || a->dup) tile(info->dweight, p.one_stage ? T128 : p.w), info->dweight_stages = p.one_stage ? 1 : 4;
+    if (a->dx) tile(info->dx, p.d), info->dx_splits = p.splits;
+    return DR_OK;
+}
+
+extern "C" int dr_gated_run(const dr_gated* a, int what) {
+    Plan P;
+    if (!plan_of(a, what, P)) return DR_EINVAL;
+    const bool back = what == DR_GATED_BACKWARD;
+    if (!aligned(a->x, 16) || !aligned(a->gate, 16) || !aligned(a->up, 16) || (a->kept && !aligned(a->kept, 16)) ||
+        (!back && (!aligned(a->h, 16) || !ld_ok(a->ld_h, a->width))) ||
+        (back && (!aligned(a->dh, 16) || !ld_ok(a->ld_dh, a->width) || (P.bytes && (!aligned(a->workspace, 256) || a->workspace_bytes < P.bytes)) ||
+                  (a->dx && (!aligned(a->dx, 16) || !ld_ok(a->ld_dx, a->dim))) ||
+                  (a->dgate && (!aligned(a->dgate, 16) || !ld_ok(a->ld_dgate, a->dim))) ||
+                  (a->dup && (!aligned(a->dup, 16) || !ld_ok(a->ld_dup, a->dim))))))
+        return DR_EINVAL;
+    const hipStream_t st = reinterpret_cast<hipStream_t>(a->stream);
+    Prod g{};
+    g.x = reinterpret_cast<const uint16_t*>(a->x), g.ldx = (int)a->ldx;
+    g.gate = reinterpret_cast<const uint16_t*>(a->gate), g.ld_gate = (int)a->ld_gate;
+    g.up = reinterpret_cast<const uint16_t*>(a->up), g.ld_up = (int)a->ld_up;
+    g.rows = a->rows, g.dim = a->dim, g.width = a->width;
+    g.panels = P.panels, g.panel = a->rows * 256ll;
+    if (!back) {
+        g.h = reinterpret_cast<uint16_t*>(a->h), g.ld_h = a->ld_h;
+        g.kept = reinterpret_cast<uint16_t*>(a->kept);
+        if (a->kept) launch_act<EPI_KEEP>(g, a->act, P.z, st);
+        else launch_act<EPI_ACT>(g, a->act, P.z, st);
+        return hipGetLastError() == hipSuccess ? DR_OK : DR_EHIP;
+    }
+    if (!a->dx && !a->dgate && !a->dup) return DR_OK;
+    char* ws = reinterpret_cast<char*>(a->workspace);
+    g.dz = reinterpret_cast<uint16_t*>(ws);
+    g.dh = reinterpret_cast<const uint16_t*>(a->dh), g.ld_dh = a->ld_dh;
+    if (a->kept) {
+        Slope s{reinterpret_cast<const uint16_t*>(a->kept), g.dh, g.dz, a->ld_dh, g.panel, P.panels * g.panel, a->rows, a->width};
+        const int rows = 4 * SLOPE_ROWS;
+        hipLaunchKernelGGL(gt_slope, dim3(P.panels, (a->rows + rows - 1) / rows), dim3(256), 0, st, s);
+    } else {
+        launch_act<EPI_AGAIN>(g, a->act, P.z, st);
+    }
+    if (a->dgate || a->dup) {
+        g.dgate = reinterpret_cast<uint16_t*>(a->dgate), g.ld_dgate = a->ld_dgate;
+        g.dup = reinterpret_cast<uint16_t*>(a->dup), g.ld_dup = a->ld_dup;
+        g.side0 = a->dgate ? 0 : 1;
+        const int outputs = 256 * P.panels * (a->dgate && a->dup ? 2 : 1);
+        if (P.one_stage) launch<128, 128, 2, 2, 1, 1, 64, EPI_DW, false>(g, a->dim, outputs, st);
+        else if (P.w == T256) launch<256, 256, 2, 4, 1, 4, 32, EPI_DW, false>(g, a->dim, outputs, st);
+        else launch<128, 128, 2, 2, 1, 4, 32, EPI_DW, false>(g, a->dim, outputs, st);
+    }
+    if (a->dx) {
+        g.splits = P.splits;
+        g.acc = reinterpret_cast<float*>(ws + P.acc);
+        g.dx = P.splits > 1 ? nullptr : reinterpret_cast<uint16_t*>(a->dx), g.ld_dx = a->ld_dx;
+        if (P.d == T64K) launch<64, 64, 2, 2, 2, 4, 64, EPI_DX, false>(g, a->dim, a->rows, st);
+        else if (P.d == T256x64) launch<256, 64, 2, 2, 1, 4, 32, EPI_DX, false>(g, a->dim, a->rows, st);
+        else if (P.d == T128) launch<128, 128, 2, 2, 1, 4, 32, EPI_DX, false>(g, a->dim, a->rows, st);
+        else launch<256, 256, 2, 4, 1, 4, 32, EPI_DX, false>(g, a->dim, a->rows, st);
+        if (P.splits > 1) {
+            Join j{g.acc, reinterpret_cast<uint16_t*>(a->dx), a->ld_dx, P.splits, a->rows, a->dim};
+            const long long items = ((long long)a->rows * (a->dim / 4) + 255) / 256;
+            hipLaunchKernelGGL(gt_join, dim3((unsigned)(items < 4096 ? items : 4096)), dim3(256), 0, st, j);
+        }
+    }
+    return hipGetLastError() == hipSuccess ? DR_OK : DR_EHIP;
+}

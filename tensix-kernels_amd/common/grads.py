@@ -1,0 +1,141 @@
+"""grads.py: a model's gradients as a whole on MI355X: their global norm, and clipping by it. The reference (XylolabsInc/
+tensix-kernels) has no counterpart; the gradients are those of dense_reader.gated, lm_head_topk.head_loss and moe.balance beside torch's
+own.
+
+  norm = global_norm(p.grad for p in params)                  # float32, on the device
+  norm = clip_((p.grad for p in params), max_norm=1.0)        # in place, by min(1, max_norm / (norm + 1e-6))
+  norm, out = clipped(grads, 1.0, dtype=torch.float32)        # the same into tensors of their own (or out=)
+
+  total = global_norm(mine).square_()                         # gradients that lie on several ranks:
+  dist.all_reduce(total)
+  clip_(mine, 1.0, norm=total.sqrt_())                        # clipped by the norm of all
+
+The tensors are float32, bfloat16 or float16 on one GPU, in any mix and of any shapes (None is passed over). Squares and their sums are
+float64, so that no float32 gradient overflows; a clipped value is the float32 product with the factor, rounded once. A NaN among them
+makes the norm and all that is clipped NaN, an infinity the norm infinite and the clipped values 0 (its own NaN): look at the norm. A
+tensor whose memory is dense in another order of its dims (a transposed gradient) is taken as it lies; any other strided one is read
+from a copy, and refused in place.
+
+Nothing goes to the host and nothing is differentiable. Memory comes from torch's allocator each call, on the current stream, so calls
+on several streams, threads or captured graphs never share any; the addresses are the launches' arguments, so a captured graph goes on
+with the tensors that it saw.
+
+The kernels are dr_grads_norm's and dr_grads_clip's of libdense_reader.so (include/grads.h).
+"""
+
+import ctypes
+import sys
+from pathlib import Path
+
+import torch
+
+sys.path.insert(0, str(Path(__file__).resolve().parents[1]))
+from common import device as dev  # noqa: E402
+from dense_reader import _lib  # noqa: E402
+
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _order(t):
+    """The dims of t by falling stride, if its memory is dense in that order (None otherwise)."""
+    dims = sorted(range(t.dim()), key=lambda d: (t.stride(d), t.shape[d]), reverse=True)
+    return dims if t.permute(dims).is_contiguous() else None
+
+
+def _tensors(grads):
+    """The tensors among them, checked, and their device."""
+    ts = [t for t in grads if t is not None]
+    if not ts:
+        raise ValueError("grads: no gradients")
+    dev.no_tangents("grads", *ts)
+    device, live = ts[0].device, torch.is_grad_enabled()
+    for t in ts:
+        assert t.device == device and t.dtype in TYPES, (t.device, device, t.dtype)
+        assert not (live and t.requires_grad), "grads: no derivative (detach them, or call under torch.no_grad())"
+    assert device.type == "cuda", device
+    return ts, device
+
+
+class _Call:
+    """The tensors' values, and the launch over them."""
+
+    def __init__(self, ts, device):
+        self.device = device
+        self.n = n = len(ts)
+        self.held = ts
+        self.norm = torch.empty((), dtype=torch.float32, device=device)
+        self.A = _lib.Grads(n, (ctypes.c_void_p * n)(*[t.data_ptr() for t in ts]), (ctypes.c_int64 * n)(*[t.numel() for t in ts]),
+                            (ctypes.c_int32 * n)(*[TYPES[t.dtype] for t in ts]))
+
+    def run(self, fn, workspace):
+        A = self.A
+        ref = ctypes.byref(A)
+        if workspace:
+            need = _lib.lib().dr_grads_workspace_bytes(ref)
+            _lib.check(_lib.DR_EINVAL if need < 0 else _lib.DR_OK, "dr_grads_workspace_bytes")
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+            A.workspace, A.workspace_bytes = ws.data_ptr(), need
+        A.norm = self.norm.data_ptr()
+        A.stream = dev.raw_stream(self.device)
+        if self.device.index == torch.cuda.current_device():
+            st = fn(ref)
+        else:  # (a launch goes to the current device)
+            with torch.cuda.device(self.device):
+                st = fn(ref)
+        if st != _lib.DR_OK:
+            _lib.check(st, "dr_grads_norm" if fn is _lib.lib().dr_grads_norm else "dr_grads_clip")
+
+    def clip(self, outs, max_norm, norm):
+        n, A = self.n, self.A
+        A.out = (ctypes.c_void_p * n)(*[t.data_ptr() for t in outs])
+        A.out_types = (ctypes.c_int32 * n)(*[TYPES[t.dtype] for t in outs])
+        A.max_norm = float(max_norm)
+        assert A.max_norm >= 0, f"grads: max_norm {max_norm}"
+        if norm is not None:
+            dev.no_tangents("grads", norm)
+            assert norm.device == self.device and norm.dtype == torch.float32 and norm.numel() == 1, (norm.device, norm.dtype, norm.shape)
+            self.norm, A.given = norm, 1
+        self.run(_lib.lib().dr_grads_clip, norm is None)
+        return self.norm
+
+
+def global_norm(grads):
+    """The 2-norm of all values of the gradients (an iterable of tensors or None): float32 [] on their device."""
+    ts, device = _tensors(grads)
+    c = _Call([t if t.is_contiguous() or _order(t) else t.contiguous() for t in ts], device)
+    c.run(_lib.lib().dr_grads_norm, True)
+    return c.norm
+
+
+def clip_(grads, max_norm, norm=None):
+    """The gradients times min(1, max_norm / (their global norm + 1e-6)), in place; the norm before that, float32 []. norm: take this
+    one instead (float32, one value on their device). Tensors that share memory are refused (ValueError)."""
+    ts, device = _tensors(grads)
+    assert all(t.is_contiguous() or _order(t) for t in ts), "grads: in place, a gradient's memory is dense"
+    norm = _Call(ts, device).clip(ts, max_norm, norm)
+    dev.written(*ts)
+    return norm
+
+
+def clipped(grads, max_norm, out=None, dtype=None, norm=None):
+    """(norm, clipped): clip_'s norm, and the clipped gradients in tensors of their own, of `dtype` (default each one's own), or in `out`,
+    a list of contiguous tensors of their shapes (None where a gradient is). No tensor of out may share memory with another, nor with
+    a gradient but its own as a whole (ValueError)."""
+    grads = list(grads)
+    ts, device = _tensors(grads)
+    if out is None:
+        assert dtype is None or dtype in TYPES, dtype
+        out = [None if t is None else torch.empty(t.shape, dtype=dtype or t.dtype, device=device) for t in grads]
+    else:
+        assert dtype is None, "grads: dtype is out's"
+        out = list(out)
+        assert len(out) == len(grads), (len(out), len(grads))
+        for t, o in zip(grads, out):
+            assert (t is None) == (o is None), "grads: out has a tensor where there is a gradient"
+            if t is not None:
+                assert o.shape == t.shape and o.device == device and o.dtype in TYPES and o.is_contiguous(), (o.shape, t.shape, o.dtype)
+                assert not (torch.is_grad_enabled() and o.requires_grad), "grads: out requires grad"
+    outs = [o for o in out if o is not None]
+    norm = _Call([t.contiguous() for t in ts], device).clip(outs, max_norm, norm)
+    dev.written(*outs)
+    return norm, out

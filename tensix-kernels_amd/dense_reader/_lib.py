@@ -50,6 +50,9 @@ SYMBOLS = (
     "dr_gated_workspace_bytes",
     "dr_gated_plan",
     "dr_gated_run",
+    "dr_grads_workspace_bytes",
+    "dr_grads_norm",
+    "dr_grads_clip",
 )
 
 DR_LOSS_FORWARD, DR_LOSS_BACKWARD = 1, 2
@@ -293,6 +296,23 @@ class GatedInfo(ctypes.Structure):
     ]
 
 
+class Grads(ctypes.Structure):
+    _fields_ = [
+        ("count", c_int32),
+        ("in_", ctypes.POINTER(c_void_p)),
+        ("sizes", ctypes.POINTER(c_int64)),
+        ("types", ctypes.POINTER(c_int32)),
+        ("out", ctypes.POINTER(c_void_p)),
+        ("out_types", ctypes.POINTER(c_int32)),
+        ("max_norm", ctypes.c_double),
+        ("norm", c_void_p),
+        ("given", c_int32),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
+        ("stream", c_void_p),
+    ]
+
+
 _lib = None
 
 
@@ -378,6 +398,12 @@ def lib():
         L.dr_gated_plan.argtypes = [ctypes.POINTER(Gated), c_int, ctypes.POINTER(GatedInfo)]
         L.dr_gated_run.restype = c_int
         L.dr_gated_run.argtypes = [ctypes.POINTER(Gated), c_int]
+        L.dr_grads_workspace_bytes.restype = c_int64
+        L.dr_grads_workspace_bytes.argtypes = [ctypes.POINTER(Grads)]
+        L.dr_grads_norm.restype = c_int
+        L.dr_grads_norm.argtypes = [ctypes.POINTER(Grads)]
+        L.dr_grads_clip.restype = c_int
+        L.dr_grads_clip.argtypes = [ctypes.POINTER(Grads)]
         _lib = L
     return _lib
 

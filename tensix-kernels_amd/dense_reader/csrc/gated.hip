@@ -7,8 +7,8 @@
 //   dx = dg . gate + du . up                              one product, summed over gate's and then up's outputs
 //
 // All are of one tiled MFMA kernel (gt_gemm) whose operands are read as they lie, along the summed dimension or across it
-// (mfma_tile.h). A tile of the first has as many rows of gate as of up, a wavefront the same outputs of both, so that g and u of
-// an output meet in one lane's registers. dg, du and what is kept lie in panels of 256 outputs ([output / 256][row][256]), which
+// (mfma_tile.h). In the first every 32 rows of a tile are 16 of gate and the same 16 of up, so that a fragment of 32 x 32 sums has g
+// and u of an output in one lane. dg, du and what is kept lie in panels of 256 outputs ([output / 256][row][256]), which
 // the products that read them take in contiguous blocks.
 
 #include <hip/hip_runtime.h>
@@ -41,30 +41,29 @@ __device__ __forceinline__ void act_of(float g, float& a, float& slope) {
         slope = __builtin_fmaf(t * (p * (1.f - p)), __builtin_fmaf(3.f * C3, t * t, C), p);
     } else {
         const float p = sigmoid(g);
-        const float t = fminf(fmaxf(g, -1e30f), 1e30f);
         a = g * p;
-        slope = p * __builtin_fmaf(t, 1.f - p, 1.f);
+        slope = __builtin_fmaf(a, 1.f - p, p);
     }
 }
 
-// What a forward call keeps of an output: a(g) and a'(g) u, in 24 bits each (float32's without the last 8 of the mantissa): the upper
-// 16 of both, then a's lower 8 over those of the other. (In bf16 alone dg and du would be rounded twice, and a step's gradients off by
-// 2.9e-3 of their norm instead of 2.35e-3; their own rounding alone makes 1.7e-3. 2 bytes more in 12 of the pass that reads it.)
+// What a forward call keeps of an output: g and u, in 24 bits each (float32's without the last 8 of the mantissa): the upper 16 of
+// g's and of u's, then g's lower 8 over u's. (In bf16 alone a step's gradients would be off by 2.9e-3 of their norm instead of
+// 2.35e-3, of which the rounding of dg and du and their own make 1.7e-3 each. a(g) and a'(g) u in their place would cost the product's
+// epilogue, where nothing else runs, what the pass that reads them has time for.)
+__device__ __forceinline__ uint32_t bytes(uint32_t hi, uint32_t lo, uint32_t pick) { return __builtin_amdgcn_perm(hi, lo, pick); }
 __device__ __forceinline__ uint2 upper(const uint32_t (&v)[4]) {
-    return make_uint2((v[0] >> 16) | (v[1] & 0xFFFF0000u), (v[2] >> 16) | (v[3] & 0xFFFF0000u));
+    return make_uint2(bytes(v[1], v[0], 0x07060302u), bytes(v[3], v[2], 0x07060302u));
 }
-__device__ __forceinline__ uint2 lower(const uint32_t (&a)[4], const uint32_t (&s)[4]) {
-    auto two = [](uint32_t a, uint32_t s) { return (a & 0xFF00u) | (s >> 8 & 0xFFu); };
-    return make_uint2(two(a[0], s[0]) | two(a[1], s[1]) << 16, two(a[2], s[2]) | two(a[3], s[3]) << 16);
+__device__ __forceinline__ uint2 lower(const uint32_t (&g)[4], const uint32_t (&u)[4]) {
+    return make_uint2(bytes(g[0], u[0], 0x0C0C0501u) | bytes(g[1], u[1], 0x05010C0Cu),
+                      bytes(g[2], u[2], 0x0C0C0501u) | bytes(g[3], u[3], 0x05010C0Cu));
 }
 // value e of 4, from its upper part and the lower ones of both
-__device__ __forceinline__ float kept_a(uint2 hi, uint2 lo, int e) {
-    const uint32_t h = e < 2 ? hi.x : hi.y, l = e < 2 ? lo.x : lo.y;
-    return __uint_as_float(e & 1 ? (h & 0xFFFF0000u) | (l >> 16 & 0xFF00u) : h << 16 | (l & 0xFF00u));
+__device__ __forceinline__ float kept_g(uint2 hi, uint2 lo, int e) {
+    return __uint_as_float(bytes(e < 2 ? hi.x : hi.y, e < 2 ? lo.x : lo.y, e & 1 ? 0x0706030Cu : 0x0504010Cu));
 }
-__device__ __forceinline__ float kept_s(uint2 hi, uint2 lo, int e) {
-    const uint32_t h = e < 2 ? hi.x : hi.y, l = e < 2 ? lo.x : lo.y;
-    return __uint_as_float(e & 1 ? (h & 0xFFFF0000u) | (l >> 8 & 0xFF00u) : h << 16 | (l << 8 & 0xFF00u));
+__device__ __forceinline__ float kept_u(uint2 hi, uint2 lo, int e) {
+    return __uint_as_float(bytes(e < 2 ? hi.x : hi.y, e < 2 ? lo.x : lo.y, e & 1 ? 0x0706020Cu : 0x0504000Cu));
 }
 __device__ __forceinline__ float bf16_of(uint2 v, int e) {
     const uint32_t w = e < 2 ? v.x : v.y;
@@ -99,18 +98,21 @@ struct Prod {
     int splits;
 };
 
+// (the K loop's arrays are seen as what they are only where everything is in one function)
+#define INLINE __attribute__((always_inline))
+
 template <int BM, int BN, int WM, int WN, int WK, int NS, int BK, int EPI, bool GELU>
 __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
     constexpr bool PAIR = EPI <= EPI_AGAIN, AT = !PAIR, BT = EPI == EPI_DW;
+    constexpr int AUX = PAIR && BN <= 64 ? 2 : 0;  // (of few rows the weights are read once)
     constexpr int NW = WM * WN, NT = 64 * NW, TM = BM / WM, TN = BN / WN, MI = TM / 32, NI = TN / 32;
     constexpr int CA = BM * BK / 8, CH = CA + BN * BK / 8;  // chunks of A, a stage
     constexpr int NL = CH / NT, NA = CA / NT;               // loads a lane and stage, of A
     constexpr int FM = PAIR ? BM / 2 : BM, FT = PAIR ? TM / 2 : TM;  // outputs of a tile, of a wavefront
-    static_assert(NS >= 1 && NS <= 4, "one to four stages");
-    static_assert(!PAIR || (MI % 2 == 0 && FT % (NT * 8 / BK) == 0), "a load is of gate or of up, a wavefront has both");
-    constexpr int C1 = NS > 1 ? CH * WK : 1, C2 = NS > 2 ? CH * WK : 1, C3 = NS > 3 ? CH * WK : 1;
+    static_assert(NS >= 1 && NS <= 5, "one to five stages");
+    constexpr int C1 = NS > 1 ? CH * WK : 1, C2 = NS > 2 ? CH * WK : 1, C3 = NS > 3 ? CH * WK : 1, C4 = NS > 4 ? CH * WK : 1;
     // (an array each, named where it is used: a read waits for the loads to every array that the compiler cannot rule out)
-    __shared__ uint4 s0[CH * WK], s1[C1], s2[C2], s3[C3];
+    __shared__ uint4 s0[CH * WK], s1[C1], s2[C2], s3[C3], s4[C4];
     // WK groups of wavefronts, each a share of K in stages of its own, all with the same barriers; tid within the group
     const int group = WK == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / NT), tid = threadIdx.x - group * NT;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), mine = group * CH;
@@ -137,28 +139,36 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
     const int ra = m_end - m0, rb = n_end - c0;  // (rows past the tile's)
     const int ldb = PAIR ? a.ldx : 256;
     if constexpr (PAIR) {
-        // row r of the tile: of a wavefront's TM rows the first half gate's outputs, the second up's; a load has rows of one
 #pragma unroll
         for (int i = 0; i < NA; ++i) {
             const int s = i * NT + tid, r = s / ta.CK, c = (s % ta.CK) ^ ta.swz(r);
-            const int ld = (i * NT / ta.CK) % TM >= FT ? a.ld_up : a.ld_gate;
-            ta.off[i] = (uint32_t)((r / TM * FT + r % FT) * ld * 2) + 16u * c;
+            ta.off[i] = (uint32_t)((r / 32 * 16 + r % 16) * (r & 16 ? a.ld_up : a.ld_gate) * 2) + 16u * c;
         }
     } else {
         ta.init(tid, EPI == EPI_DW ? a.ldx : a.ld_gate, ra);
     }
     tb.init(tid, ldb, rb);
     int st = step0 + group * rounds * NS;  // the next step to be loaded
+    // PAIR: a load of a wavefront has 64 / CK rows, all of gate or all of up: by the wavefront, or where it has fewer than 32
+    // rows' loads by the load
+    constexpr int ROWS = NT / Tile<BM, AT, NT, BK>::CK;  // of a load of all wavefronts
+    static_assert(!PAIR || (64 / Tile<BM, AT, NT, BK>::CK <= 16 && (ROWS % 32 == 0 || NT == 64 || NT == 128)), "a load is of gate or of up");
+    const bool up_wave = wave * (64 / Tile<BM, AT, NT, BK>::CK) & 16;
     __amdgpu_buffer_rsrc_t from_a, from_u, from_b;
     int left_a, left_b;
     bool second = false;  // DX: the steps are up's
-    auto next = [&] {
+    auto next = [&] INLINE {
         const int side = EPI == EPI_DX ? st >= own : 0, k = (st - side * own) * BK;
         left_a = left_b = k_end - k;
         if constexpr (PAIR) {
             const int r = min(FM, ra);
-            from_a = ta.source(a.gate + (long long)m0 * a.ld_gate + k, a.ld_gate, r, left_a);
-            from_u = ta.source(a.up + (long long)m0 * a.ld_up + k, a.ld_up, r, left_a);
+            if constexpr (ROWS % 32 == 0) {
+                const int ld = up_wave ? a.ld_up : a.ld_gate;
+                from_a = ta.source((up_wave ? a.up : a.gate) + (long long)m0 * ld + k, ld, r, left_a);
+            } else {
+                from_a = ta.source(a.gate + (long long)m0 * a.ld_gate + k, a.ld_gate, r, left_a);
+                from_u = ta.source(a.up + (long long)m0 * a.ld_up + k, a.ld_up, r, left_a);
+            }
             from_b = tb.source(a.x + (long long)n0 * a.ldx + k, a.ldx, min(BN, rb), left_b);
         } else if constexpr (EPI == EPI_DW) {
             from_a = ta.source(a.x + (long long)k * a.ldx + m0, a.ldx, ra, left_a);
@@ -171,11 +181,11 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
         }
         ++st;
     };
-    auto load = [&](int i0, int i1, uint4* b) {  // its loads i0 .. i1 - 1 of NL
+    auto load = [&](int i0, int i1, uint4* b) INLINE {  // its loads i0 .. i1 - 1 of NL
 #pragma unroll
         for (int i = i0; i < i1; ++i) {
             if (i < NA) {
-                if constexpr (PAIR) ta.load(i, (i * NT / ta.CK) % TM >= FT ? from_u : from_a, left_a, b + mine, tid);
+                if constexpr (PAIR) ta.template load<AUX>(i, ROWS % 32 && (i * ROWS & 16) ? from_u : from_a, left_a, b + mine, tid);
                 else ta.load(i, from_a, left_a, b + mine, tid);
             } else {
                 tb.load(i - NA, from_b, left_b, b + (mine + CA), tid);
@@ -194,7 +204,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
     }
     // A step's sums from one stage, the loads of a later step to another; with three stages and more between the sums: a wavefront
     // that issues all of its loads at once stands still until the memory pipeline has taken them, and all do after the barrier.
-    auto sum = [&](const uint4* b, uint4* to) {
+    auto sum = [&](const uint4* b, uint4* to) INLINE {
         constexpr int U = BK / 16;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -218,12 +228,12 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
     };
     // (whole rounds of the stages: steps past the last are zeros, as are the loads past the end into stages that nothing
     // reads. A last step of its own behind a branch would have the compiler copy every accumulator.)
-    auto step = [&](uint4* to, const uint4* from) {
+    auto step = [&](uint4* to, const uint4* from) INLINE {
         step_barrier<NS >= 3 ? (NS - 2) * NL : 0>();
         next();
         sum(from, to);
     };
-    auto first = [&](uint4* to) {
+    auto first = [&](uint4* to) INLINE {
         next();
         load(0, NL, to);
     };
@@ -231,6 +241,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
         first(s0);
         if constexpr (NS >= 3) first(s1);
         if constexpr (NS >= 4) first(s2);
+        if constexpr (NS >= 5) first(s3);
     }
     for (int s = 0; s < rounds; ++s) {
         if constexpr (NS == 1) {  // (more workgroups instead)
@@ -247,11 +258,17 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
             step(s2, s0);
             step(s0, s1);
             step(s1, s2);
-        } else {
+        } else if constexpr (NS == 4) {
             step(s3, s0);
             step(s0, s1);
             step(s1, s2);
             step(s2, s3);
+        } else {
+            step(s4, s0);
+            step(s0, s1);
+            step(s1, s2);
+            step(s2, s3);
+            step(s3, s4);
         }
     }
     step_barrier<0>();  // (the last loads landed: they write this workgroup's LDS)
@@ -290,102 +307,88 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
     const int r = lane & 31, h = lane >> 5;
     const int mw = m0 + wm * FT;
     // the wavefront's own part of the stages: 32 columns of its FT rows in bf16
-    constexpr int FIT = CH * WK / (4 * FT), PER = FIT < NW ? FIT : NW, PARTS = (NW + PER - 1) / PER;
-    static_assert(PARTS <= NS && (WK == 1 || PARTS == 1), "the wavefronts' parts fit the stages that are free");
-    uint4* region = s0 + (wave % PER) * 4 * FT;
+    constexpr int C16 = FT / 8, CP = C16 == 6 ? 8 : C16, SWZ = CP < 16 ? CP - 1 : 15;  // 16-byte chunks a column, their stride and turn
+    constexpr int PART = 32 * CP, FIT = CH * WK / PART, PER = FIT < NW ? FIT : NW, PARTS = (NW + PER - 1) / PER;
+    static_assert(PARTS <= NS && PARTS <= 4 && (WK == 1 || PARTS == 1), "the wavefronts' parts fit the stages that are free");
+    uint4* region = s0 + (wave % PER) * PART;
     if constexpr (PARTS > 1) {
         const int at = wave / PER;
-        region = (at == 0 ? s0 : at == 1 ? s1 : at == 2 ? s2 : s3) + (wave % PER) * 4 * FT;
+        region = (at == 0 ? s0 : at == 1 ? s1 : at == 2 ? s2 : s3) + (wave % PER) * PART;
     }
     // 32 columns in bf16, 4 rows of column r at 8-byte unit q: to and from whole runs of a column's rows in memory
     uint2* const half = reinterpret_cast<uint2*>(region);
-    constexpr int C16 = FT / 8, SWZ = C16 < 16 ? C16 - 1 : 15;  // 16-byte chunks a column; their turn by column
-    constexpr int PC = 64 / C16;                                // columns a turn
-    auto unit = [&](int q) -> uint2& { return half[(r * C16 + ((q >> 1) ^ (r & SWZ))) * 2 + (q & 1)]; };
-    auto store = [&](auto&& at, int cols, int rows) {  // at(c, row): column c's place for 8 of its rows from `row` on
-        __builtin_amdgcn_wave_barrier();
+    auto unit = [&](int q) -> uint2& { return half[(r * CP + ((q >> 1) ^ (r & SWZ))) * 2 + (q & 1)]; };
+    auto each = [&](auto&& f) INLINE {  // f(column, 8 of its rows, where they lie) over the wavefront's chunks
 #pragma unroll
-        for (int t = 0; t < 32 / PC; ++t) {
-            const int c = t * PC + lane / C16, q = lane % C16;
-            if (c < cols && 8 * q < rows) *reinterpret_cast<uint4*>(at(c, 8 * q)) = region[c * C16 + (q ^ (c & SWZ))];
+        for (int t = 0; t < C16 / 2; ++t) {
+            const int s = t * 64 + lane, c = s / C16, q = s % C16;
+            f(c, 8 * q, region[c * CP + (q ^ (c & SWZ))]);
         }
         __builtin_amdgcn_wave_barrier();
+    };
+    auto store = [&](auto&& at, int cols, int rows) INLINE {  // at(c, row): column c's place for 8 of its rows from `row` on
+        __builtin_amdgcn_wave_barrier();
+        each([&](int c, int row, const uint4& v) INLINE {
+            if (c < cols && row < rows) *reinterpret_cast<uint4*>(at(c, row)) = v;
+        });
     };
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
         const int nj = c0 + wn * TN + 32 * j, n = nj + r;
-        // panels: this wavefront's outputs lie in one
-        const long long at = (mw >> 8) * a.panel + (long long)nj * 256 + (mw & 255);
         if constexpr (PAIR) {
-            constexpr int HI = MI / 2;
+            // output mw + row of row nj + c in the panels
+            auto panel = [&](int c, int row) INLINE { return ((mw + row) >> 8) * a.panel + (long long)(nj + c) * 256 + ((mw + row) & 255); };
             const int left = a.width - mw;
-            const long long kept = a.panels * a.panel;
-            uint2 d[HI][4];
+            const long long side = a.panels * a.panel;
+            uint2 d[MI][2];
             if constexpr (EPI == EPI_AGAIN) {
                 const uint16_t* from = a.dh + nj * a.ld_dh + mw;
+                each([&](int c, int row, uint4& v) INLINE {
+                    v = nj + c < n_end && row < left ? *reinterpret_cast<const uint4*>(from + c * a.ld_dh + row) : make_uint4(0u, 0u, 0u, 0u);
+                });
 #pragma unroll
-                for (int t = 0; t < 32 / PC; ++t) {
-                    const int c = t * PC + lane / C16, q = lane % C16;
-                    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                    if (nj + c < n_end && 8 * q < left) v = *reinterpret_cast<const uint4*>(from + c * a.ld_dh + 8 * q);
-                    region[c * C16 + (q ^ (c & SWZ))] = v;
-                }
-                __builtin_amdgcn_wave_barrier();
+                for (int i = 0; i < MI; ++i)
 #pragma unroll
-                for (int i = 0; i < HI; ++i)
-#pragma unroll
-                    for (int g = 0; g < 4; ++g) d[i][g] = unit(8 * i + 2 * g + h);
+                    for (int g = 0; g < 2; ++g) d[i][g] = unit(4 * i + 2 * g + h);
                 __builtin_amdgcn_wave_barrier();
             }
-            uint2 one[HI][4], two[HI][4], three[HI][4];
+            uint2 more[3][MI][2];  // AGAIN: du; KEEP: what is kept
 #pragma unroll
-            for (int i = 0; i < HI; ++i)
+            for (int i = 0; i < MI; ++i)
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
+                for (int g = 0; g < 2; ++g) {
                     float o[4], p[4];
-                    uint32_t ab[4], sb[4];
+                    uint32_t gb[4], ub[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float u = acc[i + HI][j][4 * g + e];
+                        const float gate = acc[i][j][4 * g + e], u = acc[i][j][8 + 4 * g + e];
                         float act, slope;
-                        act_of<GELU>(acc[i][j][4 * g + e], act, slope);
+                        act_of<GELU>(gate, act, slope);
                         if constexpr (EPI == EPI_AGAIN) {
                             const float dh = bf16_of(d[i][g], e);
                             o[e] = dh * (slope * u);
                             p[e] = dh * act;
                         } else {
                             o[e] = act * u;
-                            ab[e] = __float_as_uint(act);
-                            sb[e] = __float_as_uint(slope * u);
+                            gb[e] = __float_as_uint(gate);
+                            ub[e] = __float_as_uint(u);
                         }
                     }
-                    unit(8 * i + 2 * g + h) = make_uint2(cvt2(o[0], o[1]), cvt2(o[2], o[3]));
-                    if constexpr (EPI == EPI_AGAIN) one[i][g] = make_uint2(cvt2(p[0], p[1]), cvt2(p[2], p[3]));
-                    if constexpr (EPI == EPI_KEEP) one[i][g] = upper(ab), two[i][g] = upper(sb), three[i][g] = lower(ab, sb);
+                    unit(4 * i + 2 * g + h) = make_uint2(cvt2(o[0], o[1]), cvt2(o[2], o[3]));
+                    if constexpr (EPI == EPI_AGAIN) more[0][i][g] = make_uint2(cvt2(p[0], p[1]), cvt2(p[2], p[3]));
+                    if constexpr (EPI == EPI_KEEP) more[0][i][g] = upper(gb), more[1][i][g] = upper(ub), more[2][i][g] = lower(gb, ub);
                 }
-            auto lay = [&](const uint2 (&v)[HI][4]) {
+            if constexpr (EPI == EPI_AGAIN) store([&](int c, int row) INLINE { return a.dz + panel(c, row); }, n_end - nj, left);
+            else store([&](int c, int row) INLINE { return a.h + (nj + c) * a.ld_h + mw + row; }, n_end - nj, left);
+            constexpr int MORE = EPI == EPI_KEEP ? 3 : EPI == EPI_AGAIN ? 1 : 0;
+            uint16_t* const to = EPI == EPI_KEEP ? a.kept : a.dz + side;
 #pragma unroll
-                for (int i = 0; i < HI; ++i)
+            for (int m = 0; m < MORE; ++m) {
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) unit(8 * i + 2 * g + h) = v[i][g];
-            };
-            if constexpr (EPI == EPI_AGAIN) {
-                uint16_t* o = a.dz + at;
-                store([&](int c, int row) { return o + c * 256 + row; }, n_end - nj, left);
-                lay(one);
-                store([&](int c, int row) { return o + kept + c * 256 + row; }, n_end - nj, left);
-            } else {
-                uint16_t* o = a.h + nj * a.ld_h + mw;
-                store([&](int c, int row) { return o + c * a.ld_h + row; }, n_end - nj, left);
-                if constexpr (EPI == EPI_KEEP) {
-                    uint16_t* k = a.kept + at;
-                    lay(one);
-                    store([&](int c, int row) { return k + c * 256 + row; }, n_end - nj, left);
-                    lay(two);
-                    store([&](int c, int row) { return k + kept + c * 256 + row; }, n_end - nj, left);
-                    lay(three);
-                    store([&](int c, int row) { return k + 2 * kept + c * 256 + row; }, n_end - nj, left);
-                }
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) unit(4 * i + 2 * g + h) = more[m][i][g];
+                store([&](int c, int row) INLINE { return to + m * side + panel(c, row); }, n_end - nj, left);
             }
         } else if (EPI == EPI_DW || a.dx != nullptr) {
 #pragma unroll
@@ -396,7 +399,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
                                                          cvt2(acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]));
             const long long ld = EPI == EPI_DX ? a.ld_dx : side_n ? a.ld_dup : a.ld_dgate;
             uint16_t* o = (EPI == EPI_DX ? a.dx : side_n ? a.dup : a.dgate) + nj * ld + mw;
-            store([&](int c, int row) { return o + c * ld + row; }, n_end - nj, m_end - mw);
+            store([&](int c, int row) INLINE { return o + c * ld + row; }, n_end - nj, m_end - mw);
         } else {
             if (n >= n_end) continue;
             float* o = a.acc + ((long long)split * a.rows + n) * a.dim + mw;
@@ -424,18 +427,19 @@ struct Slope {
 
 // dg and du from dh and what the forward call kept: a wavefront's rows of one panel
 constexpr int SLOPE_ROWS = 8;  // a wavefront, asked for at once
+template <bool GELU>
 __global__ __launch_bounds__(256) void gt_slope(const Slope p) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n0 = (blockIdx.y * 4 + wave) * SLOPE_ROWS, f = blockIdx.x * 256 + 4 * lane;
     if (n0 >= p.rows || f >= p.width) return;
     const long long at = blockIdx.x * p.panel + (long long)n0 * 256 + 4 * lane;
-    uint2 dh[SLOPE_ROWS], a[SLOPE_ROWS], s[SLOPE_ROWS], lo[SLOPE_ROWS];
+    uint2 dh[SLOPE_ROWS], g[SLOPE_ROWS], u[SLOPE_ROWS], lo[SLOPE_ROWS];
 #pragma unroll
     for (int i = 0; i < SLOPE_ROWS; ++i) {
         const int n = min(i, p.rows - 1 - n0);
         dh[i] = *reinterpret_cast<const uint2*>(p.dh + (n0 + n) * p.ld_dh + f);
-        a[i] = *reinterpret_cast<const uint2*>(p.kept + at + n * 256);
-        s[i] = *reinterpret_cast<const uint2*>(p.kept + p.side + at + n * 256);
+        g[i] = *reinterpret_cast<const uint2*>(p.kept + at + n * 256);
+        u[i] = *reinterpret_cast<const uint2*>(p.kept + p.side + at + n * 256);
         lo[i] = *reinterpret_cast<const uint2*>(p.kept + 2 * p.side + at + n * 256);
     }
 #pragma unroll
@@ -444,9 +448,11 @@ __global__ __launch_bounds__(256) void gt_slope(const Slope p) {
         float dg[4], du[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
+            float act, slope;
+            act_of<GELU>(kept_g(g[i], lo[i], e), act, slope);
             const float d = bf16_of(dh[i], e);
-            dg[e] = d * kept_s(s[i], lo[i], e);
-            du[e] = d * kept_a(a[i], lo[i], e);
+            dg[e] = d * (slope * kept_u(u[i], lo[i], e));
+            du[e] = d * act;
         }
         *reinterpret_cast<uint2*>(p.dz + at + i * 256) = make_uint2(cvt2(dg[0], dg[1]), cvt2(dg[2], dg[3]));
         *reinterpret_cast<uint2*>(p.dz + p.side + at + i * 256) = make_uint2(cvt2(du[0], du[1]), cvt2(du[2], du[3]));
@@ -480,21 +486,23 @@ constexpr int MOST_TILES = (1 << 23) - 8;  // of 512 lanes: a launch holds fewer
 
 long long up(long long v, long long to) { return (v + to - 1) / to * to; }
 
-enum Tiles { T256, T128, T64, T64K, T256x64, T128x64 };  // (T64K: two groups of wavefronts split K)
+// (K: groups of wavefronts that split the sum)
+enum Tiles { T256, T192x256, T128, T64x128, T64K2, T256x64, T128x64, T32x64K4, T64x32, T64x32K4, T32K4 };
 struct Size {
     int bm, bn, wk;
 };
-constexpr Size SIZE[] = {{256, 256, 1}, {128, 128, 1}, {64, 64, 1}, {64, 64, 2}, {256, 64, 1}, {128, 64, 1}};
+constexpr Size SIZE[] = {{256, 256, 1}, {192, 256, 1}, {128, 128, 1}, {64, 128, 1}, {64, 64, 2}, {256, 64, 1},
+                         {128, 64, 1},  {32, 64, 4},   {64, 32, 1},   {64, 32, 4},  {32, 32, 4}};
 
 // The times of a workgroup, as head_loss.hip's of the same products.
 Pace pace_of(int epi, int t) {
     const bool dx = epi == EPI_DX, dw = epi == EPI_DW;
     switch (t) {
-        case T64K: return Pace{CUS, dx ? 0.23f : 0.28f, 0.f, dx ? 4.5f : 2.8f};
-        case T64: return Pace{2 * CUS, 0.32f, 0.16f, 3.5f};
-        case T256x64:
-        case T128x64: return Pace{2 * CUS, 0.6f, 0.9f, 8.f};
+        case T64K2: return Pace{CUS, dx ? 0.23f : 0.28f, 0.f, dx ? 4.5f : 2.8f};
+        case T64x128: return Pace{2 * CUS, 0.42f, 0.5f, 3.5f};
+        case T256x64: return Pace{2 * CUS, 0.6f, 0.9f, 8.f};
         case T256: return Pace{CUS, dx ? 1.05f : dw ? 1.15f : 1.2f, 0.45f, dx ? 13.f : dw ? 8.f : 12.f};
+        case T192x256: return Pace{CUS, 0.95f, 0.36f, 10.f};
         default: return Pace{2 * CUS, dx ? 0.75f : dw ? 0.6f : 0.62f, dw ? 0.3f : 0.35f, dx ? 7.f : dw ? 4.f : 8.f};
     }
 }
@@ -513,6 +521,16 @@ int choose(int epi, long long m, long long n, long long k, std::initializer_list
         if (us < least) least = us, best = t;
     }
     return best;
+}
+
+// g and u of few rows wait for the weights alone: tiles as narrow as the rows, as many of them and as many groups of wavefronts each as
+// keep the most of them on the way. us, weights from memory, n x dim x width: 8 x 4096 x 4096 13.8 by T32K4 and 17.9 by T64x32K4, 16 x
+// 2048 x 8192 17.6 and 15.1, 32 x 512 x 14336 19.5, 13.5 and 8.5 by T64x32; 33 x 2880 x 2880 13.4 by T32x64K4 and 15.7 by T64K2, 64 x
+// 2048 x 8192 22.4 and 15.5, 64 x 4096 x 14336 67, 51 and 43.8 by T128x64.
+int choose_few(int n, int width) {
+    const int units = (width + 15) / 16;
+    if (n <= 32) return units <= CUS ? T32K4 : units <= 2 * CUS ? T64x32K4 : T64x32;
+    return units <= CUS ? T32x64K4 : units <= 2 * CUS ? T64K2 : T128x64;
 }
 
 struct Plan {
@@ -534,12 +552,11 @@ bool plan_of(const dr_gated* a, int what, Plan& p) {
     p.panels = (int)(up(f, 256) / 256);
     p.kept = 3ll * p.panels * n * 512;
     const bool back = what == DR_GATED_BACKWARD;
-    if (tiles_of(T64, 2 * f, n) >= MOST_TILES || tiles_of(T64, d, n) >= MOST_TILES || tiles_of(T128, d, 2 * up(f, 256)) >= MOST_TILES)
+    if (tiles_of(T64K2, 2 * f, n) >= MOST_TILES || tiles_of(T64K2, d, n) >= MOST_TILES || tiles_of(T128, d, 2 * up(f, 256)) >= MOST_TILES)
         return false;
     const bool z = !back || (a->kept == nullptr && (a->dx || a->dgate || a->dup));
     if (z) {
-        if (n <= 64) p.z = tiles_of(T128x64, 2 * f, n) >= 2 * CUS ? T128x64 : T64K;
-        else p.z = choose(EPI_ACT, 2 * f, n, d, {T256, T128, T64K});
+        p.z = n <= 64 ? choose_few((int)n, a->width) : choose(EPI_ACT, 2 * f, n, d, {T256, T192x256, T128, T64x128, T64K2});
     }
     if (!back) return true;
     long long at = 2ll * p.panels * n * 512;
@@ -549,7 +566,7 @@ bool plan_of(const dr_gated* a, int what, Plan& p) {
     }
     p.acc = at;
     if (a->dx) {
-        p.d = n <= 64 ? choose(EPI_DX, d, n, 2 * f, {T256x64, T64K}) : choose(EPI_DX, d, n, 2 * f, {T256, T128, T64K});
+        p.d = n <= 64 ? choose(EPI_DX, d, n, 2 * f, {T256x64, T64K2}) : choose(EPI_DX, d, n, 2 * f, {T256, T128, T64K2});
         p.splits = dx_splits(pace_of(EPI_DX, p.d), (int)tiles_of(p.d, d, n), (int)(up(2 * f, KSTEP) / KSTEP), SIZE[p.d].bm * SIZE[p.d].bn * 4);
         if (p.splits > 1) at += up(p.splits * n * d * 4, 256);
     }
@@ -570,6 +587,12 @@ void launch_act(const Prod& g, int t, hipStream_t st) {
     const int m = 2 * g.width, n = g.rows;
     switch (t) {
         case T256: return launch<256, 256, 2, 4, 1, 2, 64, EPI, GELU>(g, m, n, st);
+        case T192x256: return launch<192, 256, 2, 4, 1, 2, 64, EPI, GELU>(g, m, n, st);
+        case T64x128: return launch<64, 128, 1, 4, 1, 3, 64, EPI, GELU>(g, m, n, st);
+        case T32K4: return launch<32, 32, 1, 1, 4, 4, 64, EPI, GELU>(g, m, n, st);
+        case T64x32K4: return launch<64, 32, 1, 1, 4, 3, 64, EPI, GELU>(g, m, n, st);
+        case T64x32: return launch<64, 32, 1, 1, 1, 5, 64, EPI, GELU>(g, m, n, st);
+        case T32x64K4: return launch<32, 64, 1, 1, 4, 3, 64, EPI, GELU>(g, m, n, st);
         case T128: return launch<128, 128, 2, 2, 1, 2, 64, EPI, GELU>(g, m, n, st);
         case T128x64: return launch<128, 64, 2, 2, 1, 3, 64, EPI, GELU>(g, m, n, st);
         default: return launch<64, 64, 1, 2, 2, 4, 64, EPI, GELU>(g, m, n, st);
@@ -641,7 +664,9 @@ extern "C" int dr_gated_run(const dr_gated* a, int what) {
     if (a->kept) {
         Slope s{reinterpret_cast<const uint16_t*>(a->kept), g.dh, g.dz, a->ld_dh, g.panel, P.panels * g.panel, a->rows, a->width};
         const int rows = 4 * SLOPE_ROWS;
-        hipLaunchKernelGGL(gt_slope, dim3(P.panels, (a->rows + rows - 1) / rows), dim3(256), 0, st, s);
+        const dim3 grid(P.panels, (a->rows + rows - 1) / rows);
+        if (a->act) hipLaunchKernelGGL(gt_slope<true>, grid, dim3(256), 0, st, s);
+        else hipLaunchKernelGGL(gt_slope<false>, grid, dim3(256), 0, st, s);
     } else {
         launch_act<EPI_AGAIN>(g, a->act, P.z, st);
     }
@@ -658,7 +683,7 @@ extern "C" int dr_gated_run(const dr_gated* a, int what) {
         g.splits = P.splits;
         g.acc = reinterpret_cast<float*>(ws + P.acc);
         g.dx = P.splits > 1 ? nullptr : reinterpret_cast<uint16_t*>(a->dx), g.ld_dx = a->ld_dx;
-        if (P.d == T64K) launch<64, 64, 2, 2, 2, 4, 64, EPI_DX, false>(g, a->dim, a->rows, st);
+        if (P.d == T64K2) launch<64, 64, 2, 2, 2, 4, 64, EPI_DX, false>(g, a->dim, a->rows, st);
         else if (P.d == T256x64) launch<256, 64, 2, 2, 1, 4, 32, EPI_DX, false>(g, a->dim, a->rows, st);
         else if (P.d == T128) launch<128, 128, 2, 2, 1, 4, 32, EPI_DX, false>(g, a->dim, a->rows, st);
         else launch<256, 256, 2, 4, 1, 4, 32, EPI_DX, false>(g, a->dim, a->rows, st);

@@ -75,7 +75,8 @@ struct Tile {
         const int r = T ? min(left, BK) : rows, run = min(T ? (rows + 7) & ~7 : (left + 7) & ~7, T ? ROWS : BK);
         return __builtin_amdgcn_make_buffer_rsrc((void*)at, (short)0, left > 0 ? ((r - 1) * ld + run) * 2 : 0, 0x00020000);
     }
-    // the lane's chunk i of it to LDS
+    // the lane's chunk i of it to LDS (AUX 2: not to be kept in the caches)
+    template <int AUX = 0>
     __device__ __forceinline__ void load(int i, __amdgpu_buffer_rsrc_t from, int left, uint4* lds, int tid) const {
         uint32_t o = off[i];
         if constexpr (!T) {
@@ -85,7 +86,7 @@ struct Tile {
             }
         }
         __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_ptr)(lds + i * NT + 64 * __builtin_amdgcn_readfirstlane(tid >> 6)), 16, o,
-                                                 0, 0, 0);
+                                                 0, 0, AUX);
     }
     // lane's 8 values of row r0 + lane % 32, k = 16 u + 8 (lane / 32) .., the tile from chunk `from` of the stage on. (One
     // index from the stage's array: through longer chains the compiler no longer sees which stage a read is of, and has it

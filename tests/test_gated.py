@@ -6,7 +6,7 @@ Bounds, value by value, u = 2^-24 (float32) and b = 2^-8 (bf16) being a rounding
   the exponent's rounding, the functions' own few units;
 - a = g p: 1.13 |dg| (the largest |a'| of either) and its own roundings; a': 0.8 |dg| (the largest |a''|), its terms' roundings,
   and 1 - p, which is off by u and by p's own error, times what it is multiplied by;
-- what is kept is cut to 24 bits: 2^-15 of itself; dg and du are rounded to bf16; h, dx and the weights' gradients once at the end.
+- what is kept, g and u, is cut to 24 bits: 2^-15 of itself; dg and du are rounded to bf16; h, dx and the weights' gradients once at the end.
 """
 
 import math
@@ -54,11 +54,13 @@ def expected(x, wg, wu, dh, kind, cut):
     a, s, p, v, t = act_of(g, kind)
     r = (8 * v.abs().clamp(max=200) + 16) * U
     ea = 1.13 * eg + a.abs() * (r + 2 * U) + TINY
-    es = 0.8 * eg + (p + t * p * (1 - p)) * (r + 8 * U) + t * p * (p * r + U) + TINY
     h, eh = a * u, u.abs() * ea + a.abs() * eu + ea * eu
     out = {"h": (h, eh + (B + U) * (h.abs() + eh) + TINY)}
+    eg, eu = (e + cut * (m.abs() + e) for e, m in ((eg, g), (eu, u)))
+    ea = 1.13 * eg + a.abs() * (r + 2 * U) + TINY
+    es = 0.8 * eg + (p + t * p * (1 - p)) * (r + 8 * U) + t * p * (p * r + U) + TINY
     su, esu = s * u, es * u.abs() + s.abs() * eu + es * eu
-    esu, ea = esu + (cut + 2 * U) * (su.abs() + esu), ea + cut * (a.abs() + ea)
+    esu += 2 * U * (su.abs() + esu)
     dg, du = dh * su, dh * a
     edg, edu = ((e * dh.abs() + (B + U) * (m.abs() + e * dh.abs())) for e, m in ((esu, dg), (ea, du)))
     for name, val, err, mag, depth in (

@@ -109,7 +109,12 @@ def test_emitted_code(tmp_path):
     wavefront meets the same barriers; no kernel spills."""
     asm = _asm(tmp_path)
     loops = asm.replace("gt_gemm", "hl_gemm")
-    assert len(k_loops(loops)) >= 15 and not extra_waits(loops)
+    # (a workgroup of one wavefront has no barriers left, but as many waits as its loop has stages: five)
+    alone = {name for name, _ in k_loops(loops) if re.search(r"ILi64ELi32ELi1ELi1ELi1ELi5E", name)}
+    assert len(k_loops(loops)) >= 15 and set(extra_waits(loops)) == alone
+    for name, part in k_loops(loops):
+        if name in alone:
+            assert sum(s.startswith("s_waitcnt") and "vmcnt" in s for s in part) <= 5
     found = dict(re.findall(r"^(_Z\S*gt_gemm\S+):(.*?)^\.Lfunc_end", asm, re.M | re.S))
     ways = {name: barriers_left(body) for name, body in found.items()}
     assert len(found) >= 15 and all(len(w) == 1 for w in ways.values()), {n: w for n, w in ways.items() if len(w) != 1}

@@ -32,6 +32,10 @@ __device__ __forceinline__ f32x16 mfma32(uint4 a, uint4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+__device__ __forceinline__ f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
 // The wavefront's LDS reads done and all but its newest VM loads landed, then the workgroup's barrier.
 template <int VM>
 __device__ __forceinline__ void step_barrier() {
@@ -43,7 +47,8 @@ __device__ __forceinline__ void step_barrier() {
 
 // One operand's tile of ROWS x BK values in LDS: 16-byte chunks, laid out so that neither the loads straight from memory
 // (64 chunks in a row a wavefront) nor the fragments' reads meet in a bank.
-template <int ROWS, bool T, int NT, int BK>
+// QUARTERS: for fragments of 16 rows by 32 k (frag16), else of 32 by 16 (frag).
+template <int ROWS, bool T, int NT, int BK, bool QUARTERS = false>
 struct Tile {
     static constexpr int N = ROWS * BK / 8 / NT;  // chunks a lane loads
     static constexpr int CK = BK / 8;             // chunks of a row's k
@@ -52,7 +57,10 @@ struct Tile {
     // row r's chunk c (8 k) turned by row, so that 16 rows' fill all banks; across: k's chunk c (8 rows), in pairs (32 bytes)
     // turned by k
     static __device__ __forceinline__ int swz(int r) { return BK == 64 ? (r >> 1) & 7 : (r >> 2) & 3; }
-    static __device__ __forceinline__ int turn(int k) { return ROWS >= 128 ? 2 * (k & 3) : ROWS == 64 ? 2 * ((k >> 1) & 1) : 0; }
+    static __device__ __forceinline__ int turn(int k) {
+        const int t = ROWS >= 128 ? 2 * (k & 3) : ROWS == 64 ? 2 * ((k >> 1) & 1) : 0;
+        return QUARTERS ? t | ((k >> 3) & 1) : t;  // (32 lanes at a time: 32 rows of the same k, or 16 of k and 8 further)
+    }
 
     __device__ __forceinline__ void init(int tid, int ld, int rows) {
 #pragma unroll
@@ -104,6 +112,22 @@ struct Tile {
         } else {
             const int r = lane & 31, h = lane >> 5;
             return lds[from + (r0 + r) * CK + ((2 * u + h) ^ swz(r))];
+        }
+    }
+    // lane's 8 values of row r0 + lane % 16, k = 32 u + 8 (lane / 16) ..
+    static __device__ __forceinline__ uint4 frag16(const uint4* lds, int from, int r0, int u, int lane) {
+        static_assert(QUARTERS && ROWS % 32 == 0, "a tile laid out for them");
+        const int i = lane & 15, q = lane >> 4;
+        if constexpr (T) {
+            constexpr int C = ROWS / 8;
+            const int k = 8 * q + (i >> 2), pair = (r0 >> 4) ^ turn(k);  // (turn: the same 4 and 32 k further)
+            const int at = (from + k * C + 2 * pair) * 8 + 4 * (i & 3) + 32 * u * ROWS;
+            const uint16_t* v = reinterpret_cast<const uint16_t*>(lds);
+            const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(v + at)));
+            const uint2 hi = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(v + (at + 4 * ROWS))));
+            return make_uint4(lo.x, lo.y, hi.x, hi.y);
+        } else {
+            return lds[from + (r0 + i) * CK + ((4 * u + q) ^ swz(r0 + i))];
         }
     }
 };

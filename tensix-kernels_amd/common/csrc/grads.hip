@@ -23,12 +23,7 @@
 
 namespace {
 
-typedef __attribute__((__vector_size__(4 * sizeof(float)))) float f32x4;
-typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8;
-typedef __attribute__((__vector_size__(8 * sizeof(_Float16)))) _Float16 f16x8;
-typedef __attribute__((__vector_size__(8 * sizeof(float)))) float f32x8;
-
-constexpr int CHUNK = 8192, LANES = 256, VECS = CHUNK / (8 * LANES);  // values, of a lane 8 at a time
+constexpr int CHUNK = 8192, LANES = 256;  // values
 constexpr int MOST = 128;                                             // tensors a launch: its arguments fit 4 KB
 constexpr int GRID = 2048;                                            // 8 workgroups a CU
 
@@ -61,19 +56,36 @@ __device__ __forceinline__ float one(const void* p, long long i) {
     else return (float)reinterpret_cast<const _Float16*>(p)[i];
 }
 
-// 8 values in memory's form
-template <int TYPE>
-struct Eight {
-    f32x4 v[TYPE == DR_GRADS_F32 ? 2 : 1];
+// N values of a lane: 16 bytes of the wider type, so that the lanes' lie one after another, loads and stores
+template <int TYPE, int N>
+struct Some {
+    typedef __attribute__((__vector_size__(N * (TYPE == DR_GRADS_F32 ? 4 : 2)))) uint8_t raw;
+    typedef __attribute__((__vector_size__(N * sizeof(float)))) float floats;
+    raw v;
     __device__ __forceinline__ void load(const void* p, long long i) {
-        const f32x4* at = reinterpret_cast<const f32x4*>(reinterpret_cast<const char*>(p) + i * (TYPE == DR_GRADS_F32 ? 4 : 2));
-        v[0] = at[0];
-        if constexpr (TYPE == DR_GRADS_F32) v[1] = at[1];
+        v = *reinterpret_cast<const raw*>(reinterpret_cast<const char*>(p) + i * (TYPE == DR_GRADS_F32 ? 4 : 2));
     }
-    __device__ __forceinline__ f32x8 get() const {
-        if constexpr (TYPE == DR_GRADS_F32) return f32x8{v[0][0], v[0][1], v[0][2], v[0][3], v[1][0], v[1][1], v[1][2], v[1][3]};
-        else if constexpr (TYPE == DR_GRADS_BF16) return __builtin_convertvector(__builtin_bit_cast(bf16x8, v[0]), f32x8);
-        else return __builtin_convertvector(__builtin_bit_cast(f16x8, v[0]), f32x8);
+    __device__ __forceinline__ floats get() const {
+        if constexpr (TYPE == DR_GRADS_F32) return __builtin_bit_cast(floats, v);
+        else if constexpr (TYPE == DR_GRADS_BF16) {
+            typedef __attribute__((__vector_size__(N * sizeof(__bf16)))) __bf16 halves;
+            return __builtin_convertvector(__builtin_bit_cast(halves, v), floats);
+        } else {
+            typedef __attribute__((__vector_size__(N * sizeof(_Float16)))) _Float16 halves;
+            return __builtin_convertvector(__builtin_bit_cast(halves, v), floats);
+        }
+    }
+    // (past the caches: what is read again by this call should stay there)
+    static __device__ __forceinline__ void store(void* p, long long i, floats v) {
+        raw* o = reinterpret_cast<raw*>(reinterpret_cast<char*>(p) + i * (TYPE == DR_GRADS_F32 ? 4 : 2));
+        if constexpr (TYPE == DR_GRADS_F32) __builtin_nontemporal_store(__builtin_bit_cast(raw, v), o);
+        else if constexpr (TYPE == DR_GRADS_BF16) {
+            typedef __attribute__((__vector_size__(N * sizeof(__bf16)))) __bf16 halves;
+            __builtin_nontemporal_store(__builtin_bit_cast(raw, __builtin_convertvector(v, halves)), o);
+        } else {
+            typedef __attribute__((__vector_size__(N * sizeof(_Float16)))) _Float16 halves;
+            __builtin_nontemporal_store(__builtin_bit_cast(raw, __builtin_convertvector(v, halves)), o);
+        }
     }
 };
 
@@ -82,20 +94,6 @@ __device__ __forceinline__ void put(void* p, long long i, float v) {
     if constexpr (TYPE == DR_GRADS_F32) reinterpret_cast<float*>(p)[i] = v;
     else if constexpr (TYPE == DR_GRADS_BF16) reinterpret_cast<__bf16*>(p)[i] = (__bf16)v;
     else reinterpret_cast<_Float16*>(p)[i] = (_Float16)v;
-}
-
-template <int TYPE>
-__device__ __forceinline__ void put8(void* p, long long i, f32x8 v) {
-    if constexpr (TYPE == DR_GRADS_F32) {
-        f32x4* at = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p) + i);
-        __builtin_nontemporal_store(f32x4{v[0], v[1], v[2], v[3]}, at);
-        __builtin_nontemporal_store(f32x4{v[4], v[5], v[6], v[7]}, at + 1);
-    } else {
-        f32x4 w;
-        if constexpr (TYPE == DR_GRADS_BF16) w = __builtin_bit_cast(f32x4, __builtin_convertvector(v, bf16x8));
-        else w = __builtin_bit_cast(f32x4, __builtin_convertvector(v, f16x8));
-        __builtin_nontemporal_store(w, reinterpret_cast<f32x4*>(reinterpret_cast<uint16_t*>(p) + i));
-    }
 }
 
 // The sum of the workgroup's lanes, to all of them, in one order.
@@ -111,29 +109,32 @@ __device__ __forceinline__ double block_sum(double s) {
 template <int TYPE>
 __device__ __forceinline__ double squares(const void* p, int n, bool vec) {
     const int tid = threadIdx.x;
+    constexpr int N = TYPE == DR_GRADS_F32 ? 4 : 8, VECS = CHUNK / (N * LANES);
+    typedef Some<TYPE, N> Values;
     double s = 0., t = 0.;
-    auto add = [&](f32x8 v) {
+    auto add = [&](const Values& x) {
+        const auto v = x.get();
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
+        for (int e = 0; e < N; e += 2) {
             s = __builtin_fma((double)v[e], (double)v[e], s);
             t = __builtin_fma((double)v[e + 1], (double)v[e + 1], t);
         }
     };
     int from = 0;
     if (vec && n == CHUNK) {
-        Eight<TYPE> v[VECS];
+        Values v[VECS];
 #pragma unroll
-        for (int j = 0; j < VECS; ++j) v[j].load(p, 8 * (j * LANES + tid));
+        for (int j = 0; j < VECS; ++j) v[j].load(p, N * (j * LANES + tid));
 #pragma unroll
-        for (int j = 0; j < VECS; ++j) add(v[j].get());
+        for (int j = 0; j < VECS; ++j) add(v[j]);
         from = n;
     } else if (vec) {
-        for (int i = tid; i < n / 8; i += LANES) {
-            Eight<TYPE> v;
-            v.load(p, 8 * i);
-            add(v.get());
+        for (int i = tid; i < n / N; i += LANES) {
+            Values v;
+            v.load(p, N * i);
+            add(v);
         }
-        from = n & ~7;
+        from = n / N * N;
     }
 #pragma unroll 8
     for (int i = from + tid; i < n; i += LANES) {
@@ -179,23 +180,24 @@ __global__ __launch_bounds__(LANES) void gr_norm(const double* sums, int count, 
 
 template <int TYPE, int OUT>
 __device__ __forceinline__ void scale(const void* p, void* o, int n, bool vec, float f) {
+    constexpr int N = TYPE == DR_GRADS_F32 || OUT == DR_GRADS_F32 ? 4 : 8, VECS = CHUNK / (N * LANES);
     const int tid = threadIdx.x;
     int from = 0;
     if (vec && n == CHUNK) {
-        Eight<TYPE> v[VECS];
+        Some<TYPE, N> v[VECS];
 #pragma unroll
-        for (int j = 0; j < VECS; ++j) v[j].load(p, 8 * (j * LANES + tid));
+        for (int j = 0; j < VECS; ++j) v[j].load(p, N * (j * LANES + tid));
 #pragma unroll
-        for (int j = 0; j < VECS; ++j) put8<OUT>(o, 8 * (j * LANES + tid), v[j].get() * f);
+        for (int j = 0; j < VECS; ++j) Some<OUT, N>::store(o, N * (j * LANES + tid), v[j].get() * f);
         return;
     }
     if (vec) {
-        for (int i = tid; i < n / 8; i += LANES) {
-            Eight<TYPE> v;
-            v.load(p, 8 * i);
-            put8<OUT>(o, 8 * i, v.get() * f);
+        for (int i = tid; i < n / N; i += LANES) {
+            Some<TYPE, N> v;
+            v.load(p, N * i);
+            Some<OUT, N>::store(o, N * i, v.get() * f);
         }
-        from = n & ~7;
+        from = n / N * N;
     }
 #pragma unroll 8
     for (int i = from + tid; i < n; i += LANES) put<OUT>(o, i, one<TYPE>(p, i) * f);

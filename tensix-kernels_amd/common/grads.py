@@ -25,6 +25,7 @@ The kernels are dr_grads_norm's and dr_grads_clip's of libdense_reader.so (inclu
 
 import ctypes
 import sys
+from array import array
 from pathlib import Path
 
 import torch
@@ -48,24 +49,29 @@ def _tensors(grads):
     if not ts:
         raise ValueError("grads: no gradients")
     dev.no_tangents("grads", *ts)
-    device, live = ts[0].device, torch.is_grad_enabled()
-    for t in ts:
-        assert t.device == device and t.dtype in TYPES, (t.device, device, t.dtype)
-        assert not (live and t.requires_grad), "grads: no derivative (detach them, or call under torch.no_grad())"
+    device = ts[0].device
     assert device.type == "cuda", device
+    assert set(map(torch.Tensor.get_device, ts)) == {device.index}, f"grads: not all on {device}"
+    assert not (torch.is_grad_enabled() and any(t.requires_grad for t in ts)), (
+        "grads: no derivative (detach them, or call under torch.no_grad())")
     return ts, device
 
 
+def _types(ts):
+    kinds = [TYPES.get(t.dtype) for t in ts]
+    assert None not in kinds, {t.dtype for t in ts}
+    return array("i", kinds)
+
+
 class _Call:
-    """The tensors' values, and the launch over them."""
+    """The tensors' values, and the launch over them. (The lists are arrays of the standard library: what the call's host time goes
+    by is how often each tensor is asked for something.)"""
 
     def __init__(self, ts, device):
-        self.device = device
-        self.n = n = len(ts)
-        self.held = ts
+        self.device, self.held = device, ts
         self.norm = torch.empty((), dtype=torch.float32, device=device)
-        self.A = _lib.Grads(n, (ctypes.c_void_p * n)(*[t.data_ptr() for t in ts]), (ctypes.c_int64 * n)(*[t.numel() for t in ts]),
-                            (ctypes.c_int32 * n)(*[TYPES[t.dtype] for t in ts]))
+        self.ins, self.sizes, self.types = array("Q", map(torch.Tensor.data_ptr, ts)), array("q", map(torch.Tensor.numel, ts)), _types(ts)
+        self.A = _lib.Grads(len(ts), *(a.buffer_info()[0] for a in (self.ins, self.sizes, self.types)))
 
     def run(self, fn, workspace):
         A = self.A
@@ -86,9 +92,9 @@ class _Call:
             _lib.check(st, "dr_grads_norm" if fn is _lib.lib().dr_grads_norm else "dr_grads_clip")
 
     def clip(self, outs, max_norm, norm):
-        n, A = self.n, self.A
-        A.out = (ctypes.c_void_p * n)(*[t.data_ptr() for t in outs])
-        A.out_types = (ctypes.c_int32 * n)(*[TYPES[t.dtype] for t in outs])
+        A = self.A
+        at, types = (self.ins, self.types) if outs is self.held else (array("Q", map(torch.Tensor.data_ptr, outs)), _types(outs))
+        A.out, A.out_types = at.buffer_info()[0], types.buffer_info()[0]
         A.max_norm = float(max_norm)
         assert A.max_norm >= 0, f"grads: max_norm {max_norm}"
         if norm is not None:
@@ -133,9 +139,12 @@ def clipped(grads, max_norm, out=None, dtype=None, norm=None):
         for t, o in zip(grads, out):
             assert (t is None) == (o is None), "grads: out has a tensor where there is a gradient"
             if t is not None:
-                assert o.shape == t.shape and o.device == device and o.dtype in TYPES and o.is_contiguous(), (o.shape, t.shape, o.dtype)
-                assert not (torch.is_grad_enabled() and o.requires_grad), "grads: out requires grad"
+                assert o.shape == t.shape, (o.shape, t.shape)
+        outs = _tensors(out)
+        assert outs[1] == device and all(map(torch.Tensor.is_contiguous, outs[0])), "grads: out is contiguous, on the gradients' device"
     outs = [o for o in out if o is not None]
-    norm = _Call([t.contiguous() for t in ts], device).clip(outs, max_norm, norm)
+    if not all(map(torch.Tensor.is_contiguous, ts)):
+        ts = [t.contiguous() for t in ts]
+    norm = _Call(ts, device).clip(outs, max_norm, norm)
     dev.written(*outs)
     return norm, out

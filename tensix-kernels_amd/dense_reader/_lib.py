@@ -299,11 +299,11 @@ class GatedInfo(ctypes.Structure):
 class Grads(ctypes.Structure):
     _fields_ = [
         ("count", c_int32),
-        ("in_", ctypes.POINTER(c_void_p)),
-        ("sizes", ctypes.POINTER(c_int64)),
-        ("types", ctypes.POINTER(c_int32)),
-        ("out", ctypes.POINTER(c_void_p)),
-        ("out_types", ctypes.POINTER(c_int32)),
+        ("in_", c_void_p),
+        ("sizes", c_void_p),
+        ("types", c_void_p),
+        ("out", c_void_p),
+        ("out_types", c_void_p),
         ("max_norm", ctypes.c_double),
         ("norm", c_void_p),
         ("given", c_int32),

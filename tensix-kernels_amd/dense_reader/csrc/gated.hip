@@ -70,11 +70,15 @@ __device__ __forceinline__ float bf16_of(uint2 v, int e) {
     return __uint_as_float(e & 1 ? w & 0xFFFF0000u : w << 16);
 }
 
+// (the K loop's arrays are seen as what they are only where everything is in one function)
+#define INLINE __attribute__((always_inline))
+
 // --- the tiled product --------------------------------------------------------------------------------------------------
 
 // ACT, KEEP, AGAIN: D[2 width][rows], A gate and up, B x; DW: D[dim][outputs], A x, B dg and du; DX: D[dim][rows], A gate and up,
-// B dg and du
-enum Epi { EPI_ACT, EPI_KEEP, EPI_AGAIN, EPI_DW, EPI_DX };
+// B dg and du. DWF: DW of one step, which makes its dg and du from what was kept for itself (the first row of tiles leaves them in memory).
+// DXJ: DX whose splits' sums the last workgroup of a tile adds up.
+enum Epi { EPI_ACT, EPI_KEEP, EPI_AGAIN, EPI_DW, EPI_DWF, EPI_DX, EPI_DXJ };
 
 struct Prod {
     const uint16_t *x, *gate, *up;
@@ -97,14 +101,47 @@ struct Prod {
     float* acc;             // [splits][rows][dim]
     int splits;
     int past;               // ACT, KEEP: the outputs pass the caches by
+    uint32_t* arrived;      // DXJ: of each tile the splits that are done; AGAIN, DWF: to be cleared for it
+    int counters;
 };
 
-// (the K loop's arrays are seen as what they are only where everything is in one function)
-#define INLINE __attribute__((always_inline))
+// The tile of dg or du that a DWF workgroup multiplies by, from dh and what was kept: rows (its k) by BN outputs from c0 on, in the
+// places of its operand's loads; to memory too (leave).
+template <typename T, int BN, int NT, bool GELU>
+__device__ __forceinline__ void dz_tile(const Prod& a, uint4* to, int tid, int side, int c0, bool leave) {
+#pragma unroll
+    for (int i = 0; i < T::N; ++i) {
+        constexpr int C = BN / 8;
+        const int s = i * NT + tid, k = s / C, c = s % C, f = 8 * ((((c >> 1) ^ T::turn(k)) << 1) | (c & 1)), left = a.width - c0 - f;
+        uint4 out = make_uint4(0u, 0u, 0u, 0u);
+        if (k < a.rows && left > 0) {
+            const long long one = a.panels * a.panel, at = (long long)(c0 >> 8) * a.panel + (long long)k * 256 + (c0 & 255) + f;
+            const uint4 dh = *reinterpret_cast<const uint4*>(a.dh + k * a.ld_dh + c0 + f);
+            const uint4 g = *reinterpret_cast<const uint4*>(a.kept + at), u = *reinterpret_cast<const uint4*>(a.kept + one + at),
+                        lo = *reinterpret_cast<const uint4*>(a.kept + 2 * one + at);
+            auto four = [&](uint2 d, uint2 g, uint2 u, uint2 lo) INLINE {
+                float o[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float act, slope;
+                    act_of<GELU>(kept_g(g, lo, e), act, slope);
+                    o[e] = bf16_of(d, e) * (side ? act : slope * kept_u(u, lo, e));
+                }
+                return make_uint2(cvt2(o[0], o[1]), cvt2(o[2], o[3]));
+            };
+            const uint2 x = four(make_uint2(dh.x, dh.y), make_uint2(g.x, g.y), make_uint2(u.x, u.y), make_uint2(lo.x, lo.y));
+            const uint2 y = four(make_uint2(dh.z, dh.w), make_uint2(g.z, g.w), make_uint2(u.z, u.w), make_uint2(lo.z, lo.w));
+            out = make_uint4(x.x, x.y, y.x, y.y);
+            if (leave) *reinterpret_cast<uint4*>(a.dz + side * one + at) = out;
+        }
+        to[s] = out;
+    }
+}
 
 template <int BM, int BN, int WM, int WN, int WK, int NS, int BK, int EPI, bool GELU>
 __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
-    constexpr bool PAIR = EPI <= EPI_AGAIN, AT = !PAIR, BT = EPI == EPI_DW;
+    constexpr bool PAIR = EPI <= EPI_AGAIN, DW = EPI == EPI_DW || EPI == EPI_DWF, DX = EPI == EPI_DX || EPI == EPI_DXJ;
+    constexpr bool AT = !PAIR, BT = DW;
     constexpr int AUX = PAIR && BN <= 64 ? 2 : 0;  // (of few rows the weights are read once)
     constexpr int NW = WM * WN, NT = 64 * NW, TM = BM / WM, TN = BN / WN, MI = TM / 16, NI = TN / 16;
     constexpr int CA = BM * BK / 8, CH = CA + BN * BK / 8;  // chunks of A, a stage
@@ -120,19 +157,23 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
     const int group = WK == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / NT), tid = threadIdx.x - group * NT;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), mine = group * CH;
     const int wm = wave / WN, wn = wave % WN;
+    if constexpr (EPI == EPI_AGAIN || EPI == EPI_DWF) {
+        if (blockIdx.x == 0)
+            for (int i = threadIdx.x; i < a.counters; i += 64 * WM * WN * WK) a.arrived[i] = 0;
+    }
     int mt, nt, split;
-    if (!tile_of(a.tm, a.tn, EPI == EPI_DX ? a.splits : 1, mt, nt, split)) return;
+    if (!tile_of(a.tm, a.tn, DX ? a.splits : 1, mt, nt, split)) return;
     const int m0 = mt * FM, n0 = nt * BN;
     // DW: the tile's side, and its first output there
-    const int side_n = EPI == EPI_DW ? a.side0 + (n0 >= a.panels * 256) : 0, c0 = EPI == EPI_DW ? n0 - (side_n - a.side0) * a.panels * 256 : n0;
-    const int n_end = EPI == EPI_DW ? a.width : a.rows, m_end = PAIR ? a.width : a.dim;
+    const int side_n = DW ? a.side0 + (n0 >= a.panels * 256) : 0, c0 = DW ? n0 - (side_n - a.side0) * a.panels * 256 : n0;
+    const int n_end = DW ? a.width : a.rows, m_end = PAIR ? a.width : a.dim;
     if (c0 >= n_end) return;  // (what a side's last panel has past its last output)
     // the steps of K: DX sums over gate's outputs, then over up's, each side whole steps
-    const int k_end = PAIR ? a.dim : EPI == EPI_DW ? a.rows : a.width, own = (k_end + BK - 1) / BK;
-    const int all = EPI == EPI_DX ? 2 * own : own;
+    const int k_end = PAIR ? a.dim : DW ? a.rows : a.width, own = (k_end + BK - 1) / BK;
+    const int all = DX ? 2 * own : own;
     // (a split's steps are whole rounds of the stages: the next split's are not its own)
     constexpr int ROUND = NS * WK;
-    const int splits = EPI == EPI_DX ? a.splits : 1;
+    const int splits = DX ? a.splits : 1;
     const int per = ((all + splits - 1) / splits + ROUND - 1) / ROUND * ROUND, step0 = split * per;
     const int steps = min(per, all - step0);
     const int rounds = steps > 0 ? ((steps + WK - 1) / WK + NS - 1) / NS : 0;  // (of the stages)
@@ -148,7 +189,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
             ta.off[i] = (uint32_t)((r / 32 * 16 + r % 16) * (r & 16 ? a.ld_up : a.ld_gate) * 2) + 16u * c;
         }
     } else {
-        ta.init(tid, EPI == EPI_DW ? a.ldx : a.ld_gate, ra);
+        ta.init(tid, DW ? a.ldx : a.ld_gate, ra);
     }
     tb.init(tid, ldb, rb);
     int st = step0 + group * rounds * NS;  // the next step to be loaded
@@ -161,7 +202,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
     int left_a, left_b;
     bool second = false;  // DX: the steps are up's
     auto next = [&] INLINE {
-        const int side = EPI == EPI_DX ? st >= own : 0, k = (st - side * own) * BK;
+        const int side = DX ? st >= own : 0, k = (st - side * own) * BK;
         left_a = left_b = k_end - k;
         if constexpr (PAIR) {
             const int r = min(FM, ra);
@@ -173,7 +214,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
                 from_u = ta.source(a.up + (long long)m0 * a.ld_up + k, a.ld_up, r, left_a);
             }
             from_b = tb.source(a.x + (long long)n0 * a.ldx + k, a.ldx, min(BN, rb), left_b);
-        } else if constexpr (EPI == EPI_DW) {
+        } else if constexpr (DW) {
             from_a = ta.source(a.x + (long long)k * a.ldx + m0, a.ldx, ra, left_a);
             from_b = tb.source(a.dz + (side_n * a.panels + (c0 >> 8)) * a.panel + (c0 & 255) + (long long)k * 256, 256, rb, left_b);
         } else {
@@ -235,7 +276,12 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
         next();
         load(0, NL, to);
     };
-    if (rounds > 0) {
+    if constexpr (EPI == EPI_DWF) {
+        static_assert(EPI != EPI_DWF || (NS == 1 && WK == 1), "one stage");
+        next();
+        load(0, NA, s0);
+        dz_tile<TileB, BN, NT, GELU>(a, s0 + CA, tid, side_n, c0, mt == 0);
+    } else if (rounds > 0) {
         first(s0);
         if constexpr (NS >= 3) first(s1);
         if constexpr (NS >= 4) first(s2);
@@ -281,13 +327,53 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
                 for (int j = 0; j < NI; ++j) to[64 * (i * NI + j)] = acc[i][j];
         }
         step_barrier<0>();
-        if (group) return;
+        if (EPI != EPI_DXJ && group) return;
 #pragma unroll
-        for (int w = 0; w < WK - 1; ++w)
+        for (int w = 0; w < WK - 1 && group == 0; ++w)
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
                 for (int j = 0; j < NI; ++j) acc[i][j] += at[w * NW * MI * NI * 64 + 64 * (i * NI + j)];
+    }
+
+    if constexpr (EPI == EPI_DXJ) {
+        // The L2s of the XCDs are not coherent with each other: device-scope accesses, each lane's own places, in the splits' order.
+        __shared__ uint32_t before;
+        if (splits > 1) {
+            const int tile = mt * a.tn + nt;
+            float* const sums = a.acc + (long long)tile * splits * (BM * BN) + tid;
+            if (!group) {
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int j = 0; j < NI; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            __hip_atomic_store(sums + split * (BM * BN) + ((i * NI + j) * 4 + e) * NT, acc[i][j][e], __ATOMIC_RELAXED,
+                                               __HIP_MEMORY_SCOPE_AGENT);
+            }
+            step_barrier<0>();  // (they have landed)
+            if (threadIdx.x == 0) before = __hip_atomic_fetch_add(a.arrived + tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            step_barrier<0>();
+            if (before != (uint32_t)(splits - 1)) return;
+            if (!group) {
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+                for (int w = 0; w < splits; ++w)
+#pragma unroll
+                    for (int i = 0; i < MI; ++i)
+#pragma unroll
+                        for (int j = 0; j < NI; ++j)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                acc[i][j][e] += __hip_atomic_load(sums + w * (BM * BN) + ((i * NI + j) * 4 + e) * NT, __ATOMIC_RELAXED,
+                                                                  __HIP_MEMORY_SCOPE_AGENT);
+            }
+        }
+        if (group) return;
     }
 
     // lane: columns n = c0 + wn TN + 16 j + lane % 16, rows mw + 16 i + 4 (lane / 16) + 0 .. 3; two j's columns at a time
@@ -319,8 +405,13 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
             if (c >= cols || row >= rows) return;
             f32x4* o = reinterpret_cast<f32x4*>(at(c, row));
             const f32x4 w = __builtin_bit_cast(f32x4, v);
-            if (PAIR && a.past) __builtin_nontemporal_store(w, o);
-            else *o = w;
+            if (PAIR && a.past) {
+                asm volatile("" ::: "memory");  // (around it: else the compiler makes one plain store of both)
+                __builtin_nontemporal_store(w, o);
+                asm volatile("" ::: "memory");
+            } else {
+                *o = w;
+            }
         });
     };
 #pragma unroll
@@ -382,7 +473,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
                     for (int i = 0; i < HI; ++i) unit(jj, 4 * i + q4) = more[m][jj][i];
                 store([&](int c, int row) INLINE { return to + m * side + panel(c, row); }, n_end - nj, left);
             }
-        } else if (EPI == EPI_DW || a.dx != nullptr) {
+        } else if (DW || EPI == EPI_DXJ || a.dx != nullptr) {
 #pragma unroll
             for (int jj = 0; jj < 2; ++jj)
 #pragma unroll
@@ -390,8 +481,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
                     const f32x4 v = acc[i][j + jj];
                     unit(jj, 4 * i + q4) = make_uint2(cvt2(v[0], v[1]), cvt2(v[2], v[3]));
                 }
-            const long long ld = EPI == EPI_DX ? a.ld_dx : side_n ? a.ld_dup : a.ld_dgate;
-            uint16_t* o = (EPI == EPI_DX ? a.dx : side_n ? a.dup : a.dgate) + nj * ld + mw;
+            const long long ld = DX ? a.ld_dx : side_n ? a.ld_dup : a.ld_dgate;
+            uint16_t* o = (DX ? a.dx : side_n ? a.dup : a.dgate) + nj * ld + mw;
             store([&](int c, int row) INLINE { return o + c * ld + row; }, n_end - nj, m_end - mw);
         } else {
 #pragma unroll
@@ -414,6 +505,8 @@ struct Slope {
     uint16_t* dz;
     long long ld_dh, panel, side;  // (values of one panel, of one side)
     int rows, width;
+    uint32_t* arrived;  // cleared
+    int counters;
 };
 
 __device__ __forceinline__ uint2 passing(const uint16_t* at) {  // read once
@@ -428,6 +521,8 @@ template <bool GELU, bool PAST>
 __global__ __launch_bounds__(256) void gt_slope(const Slope p) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n0 = (blockIdx.y * 4 + wave) * SLOPE_ROWS, f = blockIdx.x * 256 + 4 * lane;
+    if (blockIdx.x == 0 && blockIdx.y == 0)
+        for (int i = threadIdx.x; i < p.counters; i += 256) p.arrived[i] = 0;
     if (n0 >= p.rows || f >= p.width) return;
     const long long at = blockIdx.x * p.panel + (long long)n0 * 256 + 4 * lane;
     uint2 dh[SLOPE_ROWS], g[SLOPE_ROWS], u[SLOPE_ROWS], lo[SLOPE_ROWS];
@@ -532,7 +627,9 @@ int choose_few(int n, int width) {
 struct Plan {
     int panels, z, w, d, splits;
     bool one_stage;  // DW
-    long long kept, acc, bytes;  // (the workspace: dg and du, then the sums of dx's splits)
+    bool fused;      // DWF
+    int counters;    // DXJ
+    long long kept, acc, arrived, bytes;  // (the workspace: dg and du, then the sums of dx's splits, then the counters)
 };
 
 bool ld_ok(long long ld, long long least) { return ld >= least && ld % 8 == 0; }
@@ -564,8 +661,15 @@ bool plan_of(const dr_gated* a, int what, Plan& p) {
     if (a->dx) {
         p.d = n <= 64 ? choose(EPI_DX, d, n, 2 * f, {T256x64, T64K2}) : choose(EPI_DX, d, n, 2 * f, {T256, T128, T64K2});
         p.splits = dx_splits(pace_of(EPI_DX, p.d), (int)tiles_of(p.d, d, n), (int)(up(2 * f, KSTEP) / KSTEP), SIZE[p.d].bm * SIZE[p.d].bn * 4);
-        if (p.splits > 1) at += up(p.splits * n * d * 4, 256);
+        if (p.splits > 1 && p.d == T64K2) {
+            p.counters = (int)tiles_of(T64K2, d, n);
+            at += (long long)p.splits * p.counters * (64 * 64 * 4);
+            p.arrived = at;
+            at += up(p.counters * 4, 256);
+        } else if (p.splits > 1) at += up(p.splits * n * d * 4, 256);
     }
+    // of both sides, so that dx finds them; and where the pass that makes them costs more than making them in every row of tiles
+    p.fused = p.one_stage && a->kept && a->dgate && a->dup && n <= KSTEP;
     p.bytes = a->dx || a->dgate || a->dup ? at : 0;
     return true;
 }
@@ -574,7 +678,7 @@ template <int BM, int BN, int WM, int WN, int WK, int NS, int BK, int EPI, bool 
 void launch(Prod g, int m, int n, hipStream_t st) {
     g.tm = (m + BM - 1) / BM;
     g.tn = (n + BN - 1) / BN;
-    const int grid = (g.tm * g.tn * (EPI == EPI_DX ? g.splits : 1) + 7) & ~7;  // (as many for each XCD)
+    const int grid = (g.tm * g.tn * (EPI == EPI_DX || EPI == EPI_DXJ ? g.splits : 1) + 7) & ~7;  // (as many for each XCD)
     hipLaunchKernelGGL((gt_gemm<BM, BN, WM, WN, WK, NS, BK, EPI, GELU>), dim3(grid), dim3(64 * WM * WN * WK), 0, st, g);
 }
 
@@ -663,13 +767,16 @@ extern "C" int dr_gated_run(const dr_gated* a, int what) {
     char* ws = reinterpret_cast<char*>(a->workspace);
     g.dz = reinterpret_cast<uint16_t*>(ws);
     g.dh = reinterpret_cast<const uint16_t*>(a->dh), g.ld_dh = a->ld_dh;
-    if (a->kept) {
-        Slope s{reinterpret_cast<const uint16_t*>(a->kept), g.dh, g.dz, a->ld_dh, g.panel, P.panels * g.panel, a->rows, a->width};
+    g.kept = reinterpret_cast<uint16_t*>(a->kept);
+    g.arrived = reinterpret_cast<uint32_t*>(ws + P.arrived), g.counters = P.counters;
+    if (a->kept && !P.fused) {
+        Slope s{reinterpret_cast<const uint16_t*>(a->kept), g.dh, g.dz, a->ld_dh, g.panel, P.panels * g.panel, a->rows, a->width,
+                g.arrived, g.counters};
         const int rows = 4 * SLOPE_ROWS;
         const dim3 grid(P.panels, (a->rows + rows - 1) / rows);
         auto slope = a->act ? past ? gt_slope<true, true> : gt_slope<true, false> : past ? gt_slope<false, true> : gt_slope<false, false>;
         hipLaunchKernelGGL(slope, grid, dim3(256), 0, st, s);
-    } else {
+    } else if (!a->kept) {
         launch_act<EPI_AGAIN>(g, a->act, P.z, st);
     }
     if (a->dgate || a->dup) {
@@ -677,7 +784,9 @@ extern "C" int dr_gated_run(const dr_gated* a, int what) {
         g.dup = reinterpret_cast<uint16_t*>(a->dup), g.ld_dup = a->ld_dup;
         g.side0 = a->dgate ? 0 : 1;
         const int outputs = 256 * P.panels * (a->dgate && a->dup ? 2 : 1);
-        if (P.one_stage) launch<128, 128, 2, 2, 1, 1, 64, EPI_DW, false>(g, a->dim, outputs, st);
+        if (P.fused && a->act) launch<128, 128, 2, 2, 1, 1, 64, EPI_DWF, true>(g, a->dim, outputs, st);
+        else if (P.fused) launch<128, 128, 2, 2, 1, 1, 64, EPI_DWF, false>(g, a->dim, outputs, st);
+        else if (P.one_stage) launch<128, 128, 2, 2, 1, 1, 64, EPI_DW, false>(g, a->dim, outputs, st);
         else if (P.w == T256) launch<256, 256, 2, 4, 1, 4, 32, EPI_DW, false>(g, a->dim, outputs, st);
         else launch<128, 128, 2, 2, 1, 4, 32, EPI_DW, false>(g, a->dim, outputs, st);
     }
@@ -685,11 +794,14 @@ extern "C" int dr_gated_run(const dr_gated* a, int what) {
         g.splits = P.splits;
         g.acc = reinterpret_cast<float*>(ws + P.acc);
         g.dx = P.splits > 1 ? nullptr : reinterpret_cast<uint16_t*>(a->dx), g.ld_dx = a->ld_dx;
-        if (P.d == T64K2) launch<64, 64, 2, 2, 2, 4, 64, EPI_DX, false>(g, a->dim, a->rows, st);
+        if (P.d == T64K2) {
+            g.dx = reinterpret_cast<uint16_t*>(a->dx);
+            launch<64, 64, 2, 2, 2, 4, 64, EPI_DXJ, false>(g, a->dim, a->rows, st);
+        }
         else if (P.d == T256x64) launch<256, 64, 2, 2, 1, 4, 32, EPI_DX, false>(g, a->dim, a->rows, st);
         else if (P.d == T128) launch<128, 128, 2, 2, 1, 4, 32, EPI_DX, false>(g, a->dim, a->rows, st);
         else launch<256, 256, 2, 4, 1, 4, 32, EPI_DX, false>(g, a->dim, a->rows, st);
-        if (P.splits > 1) {
+        if (P.splits > 1 && P.d != T64K2) {
             Join j{g.acc, reinterpret_cast<uint16_t*>(a->dx), a->ld_dx, P.splits, a->rows, a->dim};
             const long long items = ((long long)a->rows * (a->dim / 4) + 255) / 256;
             hipLaunchKernelGGL(gt_join, dim3((unsigned)(items < 4096 ? items : 4096)), dim3(256), 0, st, j);

@@ -117,5 +117,9 @@ def test_emitted_code(tmp_path):
             assert sum(s.startswith("s_waitcnt") and "vmcnt" in s for s in part) <= 5
     found = dict(re.findall(r"^(_Z\S*gt_gemm\S+):(.*?)^\.Lfunc_end", asm, re.M | re.S))
     ways = {name: barriers_left(body) for name, body in found.items()}
+    # (EPI_DXJ: two barriers more where a launch's sums are split, all of its workgroups alike)
+    joined = [w for name, w in ways.items() if re.search(r"ELi6ELb0E", name)]
+    assert joined and all(len(w) == 2 and max(w) == min(w) + 2 for w in joined), joined
+    ways = {name: w for name, w in ways.items() if w not in joined}
     assert len(found) >= 15 and all(len(w) == 1 for w in ways.values()), {n: w for n, w in ways.items() if len(w) != 1}
     assert set(re.findall(r"\.private_segment_fixed_size: (\d+)", asm)) == {"0"}

@@ -32,10 +32,16 @@ def test_struct_matches_c(tmp_path):
 
 def call(ins, sizes, types, outs=None, out_types=None, **kw):
     """A dr_grads whose pointers are never read on a device."""
-    n = len(sizes)
-    A = _lib.Grads(n, (ctypes.c_void_p * n)(*ins), (ctypes.c_int64 * n)(*sizes), (ctypes.c_int32 * n)(*types))
+    n, held = len(sizes), []
+
+    def at(kind, values):
+        held.append((kind * n)(*values))
+        return ctypes.addressof(held[-1])
+
+    A = _lib.Grads(n, at(ctypes.c_void_p, ins), at(ctypes.c_int64, sizes), at(ctypes.c_int32, types))
     if outs is not None:
-        A.out, A.out_types = (ctypes.c_void_p * n)(*outs), (ctypes.c_int32 * n)(*(types if out_types is None else out_types))
+        A.out, A.out_types = at(ctypes.c_void_p, outs), at(ctypes.c_int32, types if out_types is None else out_types)
+    A.held = held  # (as long as the call's struct)
     A.max_norm, A.norm, A.workspace, A.workspace_bytes = 1.0, 4096, 4096, 1 << 40
     for name, v in kw.items():
         setattr(A, name, v)

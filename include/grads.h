@@ -37,7 +37,10 @@ typedef struct dr_grads {
     void* stream;
 } dr_grads;
 
-/* Bytes of workspace that a call over these tensors needs, -1 if it is invalid. */
+/* Bytes of workspace that a call over these tensors needs, -1 if it is invalid: at most DR_GRADS_LIST_BYTES for every DR_GRADS_LIST
+ * tensors begun. */
+#define DR_GRADS_LIST 128
+#define DR_GRADS_LIST_BYTES 16384
 int64_t dr_grads_workspace_bytes(const dr_grads* a);
 
 /* Enqueue the norm, or the norm (unless given) and the clip, on the stream: nothing is allocated on the device, kept or waited for,

@@ -24,8 +24,9 @@
 namespace {
 
 constexpr int CHUNK = 8192, LANES = 256;  // values
-constexpr int MOST = 128;                                             // tensors a launch: its arguments fit 4 KB
-constexpr int GRID = 2048;                                            // 8 workgroups a CU
+constexpr int MOST = DR_GRADS_LIST;        // tensors a launch: its arguments fit 4 KB
+constexpr int GRID = 2048;                 // 8 workgroups a CU
+static_assert(GRID * 8 == DR_GRADS_LIST_BYTES, "the header's bytes");
 
 struct List {
     const void* in[MOST];

@@ -74,20 +74,17 @@ class _Call:
         self.A = _lib.Grads(len(ts), *(a.buffer_info()[0] for a in (self.ins, self.sizes, self.types)))
 
     def run(self, fn, workspace):
-        A = self.A
-        ref = ctypes.byref(A)
+        A, device = self.A, self.device
         if workspace:
-            need = _lib.lib().dr_grads_workspace_bytes(ref)
-            _lib.check(_lib.DR_EINVAL if need < 0 else _lib.DR_OK, "dr_grads_workspace_bytes")
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-            A.workspace, A.workspace_bytes = ws.data_ptr(), need
+            ws = torch.empty(-(-A.count // _lib.DR_GRADS_LIST) * _lib.DR_GRADS_LIST_BYTES, dtype=torch.uint8, device=device)
+            A.workspace, A.workspace_bytes = ws.data_ptr(), ws.numel()
         A.norm = self.norm.data_ptr()
-        A.stream = dev.raw_stream(self.device)
-        if self.device.index == torch.cuda.current_device():
-            st = fn(ref)
+        A.stream = dev.raw_stream(device)
+        if device.index == torch.cuda.current_device():
+            st = fn(ctypes.byref(A))
         else:  # (a launch goes to the current device)
-            with torch.cuda.device(self.device):
-                st = fn(ref)
+            with torch.cuda.device(device):
+                st = fn(ctypes.byref(A))
         if st != _lib.DR_OK:
             _lib.check(st, "dr_grads_norm" if fn is _lib.lib().dr_grads_norm else "dr_grads_clip")
 
@@ -125,24 +122,22 @@ def clip_(grads, max_norm, norm=None):
 
 def clipped(grads, max_norm, out=None, dtype=None, norm=None):
     """(norm, clipped): clip_'s norm, and the clipped gradients in tensors of their own, of `dtype` (default each one's own), or in `out`,
-    a list of contiguous tensors of their shapes (None where a gradient is). No tensor of out may share memory with another, nor with
+    a list of contiguous tensors of as many values (None where a gradient is). No tensor of out may share memory with another, nor with
     a gradient but its own as a whole (ValueError)."""
     grads = list(grads)
     ts, device = _tensors(grads)
     if out is None:
         assert dtype is None or dtype in TYPES, dtype
         out = [None if t is None else torch.empty(t.shape, dtype=dtype or t.dtype, device=device) for t in grads]
+        outs = [o for o in out if o is not None]
     else:
         assert dtype is None, "grads: dtype is out's"
         out = list(out)
-        assert len(out) == len(grads), (len(out), len(grads))
-        for t, o in zip(grads, out):
-            assert (t is None) == (o is None), "grads: out has a tensor where there is a gradient"
-            if t is not None:
-                assert o.shape == t.shape, (o.shape, t.shape)
-        outs = _tensors(out)
-        assert outs[1] == device and all(map(torch.Tensor.is_contiguous, outs[0])), "grads: out is contiguous, on the gradients' device"
-    outs = [o for o in out if o is not None]
+        outs, where = _tensors(out)
+        assert where == device and all(map(torch.Tensor.is_contiguous, outs)), "grads: out is contiguous, on the gradients' device"
+        if len(ts) < len(grads):
+            assert [t is None for t in grads] == [o is None for o in out], "grads: out has a tensor where there is a gradient"
+        assert list(map(torch.Tensor.numel, outs)) == list(map(torch.Tensor.numel, ts)), "grads: out has as many values of each"
     if not all(map(torch.Tensor.is_contiguous, ts)):
         ts = [t.contiguous() for t in ts]
     norm = _Call(ts, device).clip(outs, max_norm, norm)

@@ -380,7 +380,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
     const int r = lane & 15, q4 = lane >> 4;
     const int mw = m0 + wm * FT;
     // the wavefront's own part of the stages: 32 columns of its FT rows in bf16
-    constexpr int C16 = FT / 8, CP = C16 == 6 ? 8 : C16, SWZ = CP < 16 ? CP - 1 : 15;  // 16-byte chunks a column, their stride and turn
+    constexpr int C16 = FT / 8, CP = C16 == 6 ? 8 : C16 == 12 ? 16 : C16, SWZ = CP < 16 ? CP - 1 : 15;  // 16-byte chunks a column, their stride and turn
+    static_assert((CP & (CP - 1)) == 0, "chunks turn within a power of two");
     constexpr int PART = 32 * CP, FIT = CH * WK / PART, PER = FIT < NW ? FIT : NW, PARTS = (NW + PER - 1) / PER;
     static_assert(PARTS <= NS && PARTS <= 4 && (WK == 1 || PARTS == 1), "the wavefronts' parts fit the stages that are free");
     uint4* region = s0 + (wave % PER) * PART;
@@ -585,34 +586,60 @@ struct Size {
 constexpr Size SIZE[] = {{256, 256, 1}, {192, 256, 1}, {128, 128, 1}, {64, 128, 1}, {64, 64, 2}, {256, 64, 1},
                          {128, 64, 1},  {32, 64, 4},   {64, 32, 1},   {64, 32, 4},  {32, 32, 4}};
 
-// The times of a workgroup, as head_loss.hip's of the same products.
+// The times of a workgroup, fitted to the kernels' at 35 to 60 shapes of 72 to 4096 rows, 512 to 4096 values and 1408 to 14336 outputs,
+// most within 6 % (dx 12 %); what they choose is the fastest of these tiles or within 2 % of it at all of them (dx: within 8 %).
 Pace pace_of(int epi, int t) {
     const bool dx = epi == EPI_DX, dw = epi == EPI_DW;
     switch (t) {
-        case T64K2: return Pace{CUS, dx ? 0.23f : 0.28f, 0.f, dx ? 4.5f : 2.8f};
-        case T64x128: return Pace{2 * CUS, 0.42f, 0.5f, 3.5f};
-        case T256x64: return Pace{2 * CUS, 0.6f, 0.9f, 8.f};
-        case T256: return Pace{CUS, dx ? 1.05f : dw ? 1.15f : 1.2f, 0.45f, dx ? 13.f : dw ? 8.f : 12.f};
-        case T192x256: return Pace{CUS, 0.95f, 0.36f, 10.f};
-        default: return Pace{2 * CUS, dx ? 0.75f : dw ? 0.6f : 0.62f, dw ? 0.3f : 0.35f, dx ? 7.f : dw ? 4.f : 8.f};
+        case T256: return dx ? Pace{CUS, 1.45f, 0.05f, 1.5f} : dw ? Pace{CUS, 0.66f, 0.77f, 7.9f} : Pace{CUS, 1.07f, 0.435f, 3.f};
+        case T192x256: return dw ? Pace{CUS, 0.73f, 0.33f, 6.2f} : Pace{CUS, 0.875f, 0.313f, 3.1f};
+        case T128: return dx ? Pace{2 * CUS, 0.63f, 0.55f, 0.5f} : dw ? Pace{2 * CUS, 0.23f, 0.62f, 4.2f} : Pace{2 * CUS, 0.557f, 0.351f, 2.f};
+        case T64x128: return Pace{2 * CUS, 0.244f, 0.327f, 1.9f};
+        case T256x64: return Pace{CUS, 1.05f, 0.3f, 8.f};
+        default: return dx ? Pace{CUS, 0.19f, 0.05f, 2.f} : Pace{CUS, 0.25f, 0.03f, 2.1f};
     }
 }
 
 long long tiles_of(int t, long long m, long long n) { return up(m, SIZE[t].bm) / SIZE[t].bm * (up(n, SIZE[t].bn) / SIZE[t].bn); }
 
+// dx's splits of its long sum, for half a round of workgroups to two: their sums' way back through memory costs a launch and about 3.5
+// TB/s, or (T64K2) the last workgroup of a tile half a us for each.
+int splits_of(int t, int tiles, int steps, float* us) {
+    const Pace p = pace_of(EPI_DX, t);
+    int best = 1;
+    *us = tiled_us(p, tiles, steps);
+    for (int h = 1; h <= 4; ++h) {
+        int s = h * p.at_once / (2 * tiles);
+        if (s > steps / 4) s = steps / 4;
+        if (s < 2) continue;
+        const float join = t == T64K2 ? 0.55f * s : 4.f + (float)tiles * s * SIZE[t].bm * SIZE[t].bn * 4 * 0.28e-6f;
+        const float here = tiled_us(p, tiles * s, ((steps + s - 1) / s + 1) & ~1) + join;
+        if (here < *us) *us = here, best = s;
+    }
+    return best;
+}
+
 // the tile of `tiles` that takes the least time for a product of m rows by n columns, summed over k
-int choose(int epi, long long m, long long n, long long k, std::initializer_list<int> tiles) {
+int choose(int epi, long long m, long long n, long long k, std::initializer_list<int> tiles, int* splits = nullptr) {
     int best = 0;
     float least = 1e30f;
     const int steps = (int)(up(k, KSTEP) / KSTEP);
     for (int t : tiles) {
         float us;
-        if (epi == EPI_DX) dx_splits(pace_of(epi, t), (int)tiles_of(t, m, n), steps, SIZE[t].bm * SIZE[t].bn * 4, &us);
+        int s = 1;
+        if (epi == EPI_DX) s = splits_of(t, (int)tiles_of(t, m, n), steps, &us);
         else us = tiled_us(pace_of(epi, t), (int)tiles_of(t, m, n), steps);
-        if (us < least) least = us, best = t;
+        if (us < least) {
+            least = us, best = t;
+            if (splits) *splits = s;
+        }
     }
     return best;
 }
+
+// dx of few rows waits for the weights: past what the caches hold by tall tiles (64 x 4096 x 14336 57 us, by T64K2 63; 8 rows 48 and 54; 64
+// x 4096 x 4096 28 and 27)
+constexpr long long HELD = 96ll << 20;
 
 // g and u of few rows wait for the weights alone: tiles as narrow as the rows, as many of them and as many groups of wavefronts each as
 // keep the most of them on the way. us, weights from memory, n x dim x width: 8 x 4096 x 4096 13.8 by T32K4 and 17.9 by T64x32K4, 16 x
@@ -654,13 +681,14 @@ bool plan_of(const dr_gated* a, int what, Plan& p) {
     if (!back) return true;
     long long at = 2ll * p.panels * n * 512;
     if (a->dgate || a->dup) {
-        p.w = choose(EPI_DW, d, up(f, 256) * ((a->dgate != nullptr) + (a->dup != nullptr)), n, {T256, T128});
+        p.w = choose(EPI_DW, d, up(f, 256) * ((a->dgate != nullptr) + (a->dup != nullptr)), n, {T256, T192x256, T128});
         p.one_stage = n <= KSTEP || (p.w == T128 && n <= 1024);
     }
     p.acc = at;
     if (a->dx) {
-        p.d = n <= 64 ? choose(EPI_DX, d, n, 2 * f, {T256x64, T64K2}) : choose(EPI_DX, d, n, 2 * f, {T256, T128, T64K2});
-        p.splits = dx_splits(pace_of(EPI_DX, p.d), (int)tiles_of(p.d, d, n), (int)(up(2 * f, KSTEP) / KSTEP), SIZE[p.d].bm * SIZE[p.d].bn * 4);
+        if (n > 64) p.d = choose(EPI_DX, d, n, 2 * f, {T256, T128, T64K2}, &p.splits);
+        else if (4 * f * d > HELD) p.d = choose(EPI_DX, d, n, 2 * f, {T256x64}, &p.splits);
+        else p.d = choose(EPI_DX, d, n, 2 * f, {T64K2}, &p.splits);
         if (p.splits > 1 && p.d == T64K2) {
             p.counters = (int)tiles_of(T64K2, d, n);
             at += (long long)p.splits * p.counters * (64 * 64 * 4);
@@ -668,8 +696,9 @@ bool plan_of(const dr_gated* a, int what, Plan& p) {
             at += up(p.counters * 4, 256);
         } else if (p.splits > 1) at += up(p.splits * n * d * 4, 256);
     }
-    // of both sides, so that dx finds them; and where the pass that makes them costs more than making them in every row of tiles
-    p.fused = p.one_stage && a->kept && a->dgate && a->dup && n <= KSTEP;
+    // of both sides, so that dx finds them; and few tiles, each row of which makes them again (16 x 4096 x 1408, 768 tiles, 22 us and 24 by a
+    // pass of its own; 33 x 2880 x 2880, 1104 tiles, 29.6 and 28.8; 64 x 4096 x 14336 154 and 126)
+    p.fused = p.one_stage && a->kept && a->dgate && a->dup && n <= KSTEP && tiles_of(T128, d, 2 * up(f, 256)) <= 4 * CUS;
     p.bytes = a->dx || a->dgate || a->dup ? at : 0;
     return true;
 }
@@ -731,7 +760,7 @@ extern "C" int dr_gated_plan(const dr_gated* a, int what, dr_gated_info* info) {
     const bool back = what == DR_GATED_BACKWARD;
     if (!back || (a->kept == nullptr && (a->dx || a->dgate || a->dup))) tile(info->act, p.z);
     if (!back) return DR_OK;
-    if (a->dgate || a->dup) tile(info->dweight, p.one_stage ? T128 : p.w), info->dweight_stages = p.one_stage ? 1 : 4;
+    if (a->dgate || a->dup) tile(info->dweight, p.one_stage ? T128 : p.w), info->dweight_stages = p.one_stage ? 1 : p.w == T192x256 ? 2 : 4;
     if (a->dx) tile(info->dx, p.d), info->dx_splits = p.splits;
     return DR_OK;
 }
@@ -788,6 +817,7 @@ extern "C" int dr_gated_run(const dr_gated* a, int what) {
         else if (P.fused) launch<128, 128, 2, 2, 1, 1, 64, EPI_DWF, false>(g, a->dim, outputs, st);
         else if (P.one_stage) launch<128, 128, 2, 2, 1, 1, 64, EPI_DW, false>(g, a->dim, outputs, st);
         else if (P.w == T256) launch<256, 256, 2, 4, 1, 4, 32, EPI_DW, false>(g, a->dim, outputs, st);
+        else if (P.w == T192x256) launch<192, 256, 2, 4, 1, 2, 64, EPI_DW, false>(g, a->dim, outputs, st);
         else launch<128, 128, 2, 2, 1, 4, 32, EPI_DW, false>(g, a->dim, outputs, st);
     }
     if (a->dx) {

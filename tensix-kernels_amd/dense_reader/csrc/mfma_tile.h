@@ -58,7 +58,7 @@ struct Tile {
     // turned by k
     static __device__ __forceinline__ int swz(int r) { return BK == 64 ? (r >> 1) & 7 : (r >> 2) & 3; }
     static __device__ __forceinline__ int turn(int k) {
-        const int t = ROWS >= 128 ? 2 * (k & 3) : ROWS == 64 ? 2 * ((k >> 1) & 1) : 0;
+        const int t = ROWS % 128 == 0 ? 2 * (k & 3) : ROWS % 64 == 0 ? 2 * ((k >> 1) & 1) : 0;  // (a row of k is 0 or 128 bytes mod 256)
         return QUARTERS ? t | ((k >> 3) & 1) : t;  // (32 lanes at a time: 32 rows of the same k, or 16 of k and 8 further)
     }
 

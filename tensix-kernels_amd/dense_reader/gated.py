@@ -36,7 +36,9 @@ PANEL = 256  # outputs of a panel of what is kept
 
 
 def _rows(t, dim):
-    """t [..., dim] as rows the kernels read where they lie (itself, or a copy)."""
+    """t [..., dim] as rows the kernels read where they lie (itself, or a copy), and the values from one to the next."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t, dim
     if t.dim() != 2:
         t = t.reshape(-1, dim)
     if t.stride(-1) != 1 or t.data_ptr() % 16 or (t.shape[0] > 1 and (t.stride(0) % 8 or not dim <= t.stride(0) <= MAX_LD)):
@@ -50,40 +52,38 @@ class _Call:
     def __init__(self, x, w_gate, w_up, activation):
         dev.no_tangents("gated", x, w_gate, w_up)
         assert activation in ACTIVATIONS, f"gated: activation {activation!r}"
-        device = self.device = x.device
-        assert x.is_cuda and x.dtype == torch.bfloat16 and x.dim() >= 1, (x.device, x.dtype, x.shape)
-        assert w_gate.dim() == 2 and w_gate.shape == w_up.shape, (w_gate.shape, w_up.shape)
-        self.width, self.dim = width, dim = w_gate.shape
-        assert x.shape[-1] == dim, (x.shape, w_gate.shape)
+        device, bf16 = x.device, torch.bfloat16
+        assert x.is_cuda and x.dtype is bf16 and x.dim() >= 1, (device, x.dtype, x.shape)
+        assert w_gate.dtype is bf16 and w_up.dtype is bf16, (w_gate.dtype, w_up.dtype)
+        assert w_gate.device == device and w_up.device == device, (w_gate.device, w_up.device, device)
+        shape = w_gate.shape
+        assert len(shape) == 2 and shape == w_up.shape, (shape, w_up.shape)
+        self.width, self.dim = width, dim = shape
+        self.device, self.shape = device, x.shape
+        assert self.shape[-1] == dim, (x.shape, shape)
         assert dim % 8 == 0 and width % 8 == 0 and dim and width, f"gated: [{width}, {dim}] weights: not multiples of 8"
-        for w in (w_gate, w_up):
-            assert w.device == device and w.dtype == torch.bfloat16, (w.device, w.dtype)
-        self.shape = x.shape
+        n = self.n = x.numel() // dim
         x, ldx = _rows(x, dim)
         gate, ld_gate = _rows(w_gate, dim)
         up, ld_up = _rows(w_up, dim)
-        n = self.n = x.shape[0]
         self.held = x, gate, up
         self.A = _lib.Gated(x.data_ptr(), ldx, gate.data_ptr(), ld_gate, up.data_ptr(), ld_up, n, dim, width,
                             ACTIVATIONS[activation])
 
-    def empty(self, *shape):
-        return torch.empty(shape, dtype=torch.bfloat16, device=self.device)
-
     def run(self, what):
-        A = self.A
+        A, device = self.A, self.device
         ref = ctypes.byref(A)
         lib = _lib.lib()
         if what == _lib.DR_GATED_BACKWARD:
             need = lib.dr_gated_workspace_bytes(ref, what)
             _lib.check(_lib.DR_EINVAL if need < 0 else _lib.DR_OK, "dr_gated_workspace_bytes")
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+            ws = torch.empty(need, dtype=torch.uint8, device=device)
             A.workspace, A.workspace_bytes = ws.data_ptr(), need
-        A.stream = dev.raw_stream(self.device)
-        if self.device.index == torch.cuda.current_device():
+        A.stream = dev.raw_stream(device)
+        if device.index == torch.cuda.current_device():
             st = lib.dr_gated_run(ref, what)
         else:  # (a launch goes to the current device)
-            with torch.cuda.device(self.device):
+            with torch.cuda.device(device):
                 st = lib.dr_gated_run(ref, what)
         if st != _lib.DR_OK:
             _lib.check(st, "dr_gated_run")
@@ -92,36 +92,38 @@ class _Call:
         return 3, -(-self.width // PANEL), self.n, PANEL
 
     def forward(self, keep):
-        n, width, A = self.n, self.width, self.A
-        h = self.empty(*self.shape[:-1], width)
-        kept = torch.empty(self.kept_shape(), dtype=torch.int16, device=self.device) if keep else None
-        if n:
-            A.h, A.ld_h = h.data_ptr(), width
-            A.kept = None if kept is None else kept.data_ptr()
+        A, x = self.A, self.held[0]
+        h = x.new_empty((*self.shape[:-1], self.width))
+        kept = x.new_empty(self.kept_shape(), dtype=torch.int16) if keep else None
+        if self.n:
+            A.h, A.ld_h = h.data_ptr(), self.width
+            if keep:
+                A.kept = kept.data_ptr()
             self.run(_lib.DR_GATED_FORWARD)
         return h, kept
 
     def backward(self, dh, kept, x_grad, gate_grad, up_grad):
-        n, width, dim, A = self.n, self.width, self.dim, self.A
-        dx = self.empty(*self.shape) if x_grad else None
-        dgate, dup = (self.empty(width, dim) if asked else None for asked in (gate_grad, up_grad))
-        if n == 0:
+        width, dim, A = self.width, self.dim, self.A
+        x, gate, _ = self.held
+        dx = x.new_empty(self.shape) if x_grad else None
+        dgate, dup = (gate.new_empty((width, dim)) if asked else None for asked in (gate_grad, up_grad))
+        if self.n == 0:
             for t in (dgate, dup):
                 if t is not None:
                     t.zero_()
             return dx, dgate, dup
         dh, A.ld_dh = _rows(dh, width)
         A.dh, A.ld_dx, A.ld_dgate, A.ld_dup = dh.data_ptr(), dim, dim, dim
-        A.kept, A.dx, A.dgate, A.dup = (None if t is None else t.data_ptr() for t in (kept, dx, dgate, dup))
+        A.kept, A.dx, A.dgate, A.dup = [None if t is None else t.data_ptr() for t in (kept, dx, dgate, dup)]
         self.run(_lib.DR_GATED_BACKWARD)
         return dx, dgate, dup
 
     def check_grads(self, dh, kept):
         dev.no_tangents("gated", dh, kept)
-        assert dh.device == self.device and dh.dtype == torch.bfloat16, (dh.device, dh.dtype)
+        assert dh.device == self.device and dh.dtype is torch.bfloat16, (dh.device, dh.dtype)
         assert dh.shape == (*self.shape[:-1], self.width), (dh.shape, self.shape, self.width)
         if kept is not None:
-            assert kept.device == self.device and kept.dtype == torch.int16, (kept.device, kept.dtype)
+            assert kept.device == self.device and kept.dtype is torch.int16, (kept.device, kept.dtype)
             assert kept.shape == self.kept_shape(), (kept.shape, self.kept_shape())
             assert kept.is_contiguous() and kept.data_ptr() % 16 == 0, "gated: kept as gated_keep gave it"
 

@@ -26,7 +26,9 @@ def test_struct_matches_c(tmp_path):
     got = [int(v) for v in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
     assert got == [ctypes.sizeof(_lib.Grads)] + [getattr(_lib.Grads, n).offset for n in names]
     text = (ROOT / "include" / "grads.h").read_text()
-    types = {k: int(v) for k, v in re.findall(r"^#define DR_GRADS_(\w+) (\d)", text, re.M)}
+    for name in ("DR_GRADS_LIST", "DR_GRADS_LIST_BYTES"):
+        assert int(re.search(rf"^#define {name} (\d+)", text, re.M).group(1)) == getattr(_lib, name)
+    types = {k: int(v) for k, v in re.findall(r"^#define DR_GRADS_(F32|BF16|F16) (\d)", text, re.M)}
     assert types == {"F32": grads.TYPES[torch.float32], "BF16": grads.TYPES[torch.bfloat16], "F16": grads.TYPES[torch.float16]}
 
 

@@ -27,7 +27,7 @@ typedef struct dr_grads {
     const void* const* in;    /* each one's values, at a multiple of their size (fastest at one of 16) */
     const int64_t* sizes;     /* values of each, 0 or more, to 2^40 in all */
     const int32_t* types;
-    void* const* out;         /* clip: where each one's values go, its own in (of the same type) or memory apart from every other */
+    void* const* out;         /* clip: where each one's values go, its own in (of the same type) or memory apart from every other's and the norm's */
     const int32_t* out_types;
     double max_norm;          /* clip: 0 or more */
     float* norm;              /* written; a clip with `given` reads it */

@@ -261,11 +261,14 @@ struct Span {
     bool out;
 };
 
-// Whether no out shares memory with any other tensor's in or out, nor with its own in but all of it (swept by address). -1: no memory.
+// Whether no out shares memory with any other tensor's in or out or with the norm, nor with its own in but all of it (swept by
+// address). -1: no memory.
 int apart(const dr_grads* a) {
-    Span* s = new (std::nothrow) Span[2 * (size_t)a->count];
+    Span* s = new (std::nothrow) Span[2 * (size_t)a->count + 1];
     if (!s) return -1;
     int n = 0;
+    const uintptr_t norm = reinterpret_cast<uintptr_t>(a->norm);  // (read or written while the others are)
+    s[n++] = Span{norm, norm + 4, -1, !a->given};
     for (int i = 0; i < a->count; ++i) {
         if (!a->sizes[i]) continue;
         const uintptr_t in = reinterpret_cast<uintptr_t>(a->in[i]), out = reinterpret_cast<uintptr_t>(a->out[i]);

@@ -18,6 +18,7 @@ from torch.autograd import forward_ad
 
 from common.testing import raises, same, within
 from dense_reader import _lib, gated
+from test_gated_host import TILES
 
 pytestmark = pytest.mark.gpu
 
@@ -79,7 +80,7 @@ SIZES = [(1, 8, 8), (1, 64, 4096), (2, 1024, 264), (5, 72, 1000), (31, 520, 96),
          (1000, 128, 5000), (1003, 2056, 1288), (2100, 512, 2048), (5000, 64, 40), (4100, 1032, 2056)]
 
 
-@pytest.mark.parametrize("n, d, f", SIZES)
+@pytest.mark.parametrize("n, d, f", SIZES + [sizes for sizes, _ in TILES])
 @pytest.mark.parametrize("kind", ["swiglu", "geglu"])
 def test_step(device, n, d, f, kind):
     x, wg, wu, dh = inputs(device, n, d, f, n + d + f)
@@ -252,6 +253,18 @@ def test_autograd(device, n, keep):
     same("a broadcast dh", w.grad, ones[1])
     with torch.no_grad():
         assert not gated.gated(a, w, v, "geglu").requires_grad
+
+
+@pytest.mark.parametrize("n, d, f", [(60, 128, 264), (70, 400, 12128), (69, 280, 11016), (1100, 72, 520)])
+def test_one_weight(device, n, d, f):
+    """Either weight's gradient alone, in each kind of tile."""
+    x, wg, wu, dh = inputs(device, n, d, f, 25)
+    want = gated.gated_grads(x, wg, wu, dh, kept=gated.gated_keep(x, wg, wu)[1])
+    for i in (0, 1):
+        ts = [wg.clone().requires_grad_(i == 0), wu.clone().requires_grad_(i == 1)]
+        gated.gated(x, *ts).backward(dh)
+        same(f"weight {i}", ts[i].grad, want[1 + i])
+        assert ts[1 - i].grad is None
 
 
 def test_inputs_written_in_between(device):

@@ -91,6 +91,42 @@ def test_workspaces():
     assert L.dr_gated_run(call(workspace_bytes=need - 1, dx=None), BACKWARD) == _lib.DR_EINVAL
 
 
+# Calls whose products take each of the tiles, and what of their plan they are there for: (rows, dim, width), {field of dr_gated_info: value};
+# the GPU's tests run them
+T256, T192, T128 = (256, 256, 1), (192, 256, 1), (128, 128, 1)
+TILES = [
+    ((1, 64, 64), dict(act=(32, 32, 4), dweight=T128, dweight_stages=1, dx=(64, 64, 2), dx_splits=1)),
+    ((2, 64, 4128), dict(act=(64, 32, 4), dx_splits=32)),
+    ((1, 64, 8256), dict(act=(64, 32, 1))),
+    ((39, 72, 64), dict(act=(32, 64, 4))),
+    ((40, 64, 4408), dict(act=(64, 64, 2))),
+    ((40, 64, 8368), dict(act=(128, 64, 1))),
+    ((77, 64, 72), dict(act=(64, 128, 1), dx=T128, dx_splits=1)),
+    ((134, 144, 2584), dict(act=(64, 64, 2))),
+    ((419, 64, 4104), dict(act=T128)),
+    ((279, 64, 11024), dict(act=T192)),
+    ((341, 64, 13240), dict(act=T256)),
+    ((2, 560, 13248), dict(dweight=T128, dweight_stages=1)),
+    ((1093, 72, 72), dict(dweight=T128, dweight_stages=4)),
+    ((69, 280, 11016), dict(dweight=T192, dweight_stages=2)),
+    ((70, 400, 12128), dict(dweight=T256, dweight_stages=4)),
+    ((3, 3264, 7808), dict(dx=(256, 64, 1), dx_splits=19)),
+    ((7223, 1128, 64), dict(dx=T256, dx_splits=1)),
+    ((3739, 136, 6416), dict(dx=T256)),
+]
+
+
+@pytest.mark.parametrize("sizes, want", TILES, ids=[str(s) for s, _ in TILES])
+def test_plans(sizes, want):
+    A = call(*sizes)._obj
+    info = {**_lib.gated_info(A, BACKWARD), "act": _lib.gated_info(A, FORWARD)["act"]}
+    assert {k: info[k] for k in want} == want, info
+    A.kept = None
+    assert _lib.gated_info(A, BACKWARD)["act"] == info["act"]
+    if want.get("dx") == T256 and "dx_splits" not in want:
+        assert info["dx_splits"] > 1
+
+
 def _asm(tmp_path):
     import __graft_entry__ as G
 

@@ -88,6 +88,13 @@ def test_refused_memory(ins, sizes, types, outs, out_types):
     assert _lib.lib().dr_grads_clip(call(ins, sizes, types, outs, out_types)) == _lib.DR_EINVAL
 
 
+@pytest.mark.parametrize("given", [0, 1])
+def test_norm_within_the_outs(given):
+    L = _lib.lib()
+    assert L.dr_grads_clip(call([8192], [8], [0], [8192], norm=8192 + 28, given=given)) == _lib.DR_EINVAL
+    assert L.dr_grads_clip(call([8192], [8], [0], [16384], norm=16384, given=given)) == _lib.DR_EINVAL
+
+
 def test_workspaces():
     L = _lib.lib()
     assert L.dr_grads_workspace_bytes(call([], [], [])) == 0

@@ -92,6 +92,7 @@ class _Call:
         A = self.A
         at, types = (self.ins, self.types) if outs is self.held else (array("Q", map(torch.Tensor.data_ptr, outs)), _types(outs))
         A.out, A.out_types = at.buffer_info()[0], types.buffer_info()[0]
+        assert not isinstance(max_norm, torch.Tensor), "grads: max_norm is a number of the host's"
         A.max_norm = float(max_norm)
         assert A.max_norm >= 0, f"grads: max_norm {max_norm}"
         if norm is not None:

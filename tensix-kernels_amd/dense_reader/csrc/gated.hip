@@ -1,7 +1,7 @@
 // gated.hip: the gated feed-forward block in training and its gradients for MI355X (gfx950), behind include/gated.h.
 //
 //   g = x . gate^T, u = x . up^T, h = a(g) u              one product of gate's and up's rows together; h is its epilogue
-//   du = dh a(g), dg = dh u a'(g)                         by the value, from what the forward call kept; or the same product
+//   du = dh a(g), dg = dh u a'(g)                         value by value, from what the forward call kept; or the same product
 //                                                         again with this as its epilogue
 //   dgate = dg^T . x, dup = du^T . x                      one product of dg's and du's columns together, summed over rows
 //   dx = dg . gate + du . up                              one product, summed over gate's and then up's outputs
@@ -9,7 +9,14 @@
 // All are of one tiled MFMA kernel (gt_gemm) whose operands are read as they lie, along the summed dimension or across it
 // (mfma_tile.h). In the first every 32 rows of a tile are 16 of gate and the same 16 of up, so that two neighbouring fragments of 16 x
 // 16 sums have g and u of an output in one lane. dg, du and what is kept lie in panels of 256 outputs ([output / 256][row][256]), which
-// the products that read them take in contiguous blocks.
+// the products that read them take in contiguous blocks. No atomics but counters: every sum has one order.
+//
+// What bounds them. 8192 rows x 4096 x 14336, a step in 4.73 to 4.83 ms (one machine and another): 1504 us for h and what is kept (1280
+// TFLOP/s; h alone 1410), 216 for dg and du (1.41 GB, 6.5 TB/s), 1410 for both weights' gradients (1365), 1560 for dx (1235): the matrix
+// cores, busy 57 to 64 % of the clocks, and the power that random values draw, which holds the clock at 1.7 to 1.9 GHz (a large
+// library product of the three layouts, the card as warm: 1220, 1580, 1370 us). 32 rows x 4096 x 14336: the weights' 235 MB in
+// 38.4 us, 6.1 TB/s. A few rows by a small layer: each launch's start, its first loads and the way of a few sums (48 x 1024 x
+// 4096: 3 launches of 10 to 13 us for a step).
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -138,6 +145,17 @@ __device__ __forceinline__ void dz_tile(const Prod& a, uint4* to, int tid, int s
     }
 }
 
+// D[m][n] in tiles of BM x BN, a wavefront BM / WM x BN / WN of 16 x 16 x 32 matrix instructions (from registers alone 2090 TFLOP/s on
+// random bf16 values, 32 x 32 x 16 ones 1830; here 1502 us fell to 1410, h alone of 8192 x 4096 x 14336); NS stages of BK k in LDS, filled
+// straight from memory.
+// - 256 x 256 by 8 wavefronts, along k (h) in two stages of 64, a whole 128-byte line of a row; across (dx, the weights' gradients) in four
+//   of 32. 4 wavefronts of 128 x 128 that read their fragments a step ahead, accumulators pinned, took 1474 us for h and 3 % off the
+//   others, with matrix instructions that the compiler cannot see the waits of; h in four stages of 32 1490 to 1600; fragments read
+//   ahead by 8 wavefronts 1500 to 1640.
+// - 192 x 256 where 256 x 256 leaves CUs idle in its last round (2047 x 2880 x 2880: 253 tiles for 184, h 68 to 62 us).
+// - 128 x 128, 64 x 128 twice a CU, 64 x 64 by two groups of wavefronts that split K: fewer tiles than CUs (choose).
+// - few rows: choose_few.
+// The epilogues' bf16 leave through LDS in whole runs of a row.
 template <int BM, int BN, int WM, int WN, int WK, int NS, int BK, int EPI, bool GELU>
 __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
     constexpr bool PAIR = EPI <= EPI_AGAIN, DW = EPI == EPI_DW || EPI == EPI_DWF, DX = EPI == EPI_DX || EPI == EPI_DXJ;
@@ -516,7 +534,8 @@ __device__ __forceinline__ uint2 passing(const uint16_t* at) {  // read once
     return make_uint2(v[0], v[1]);
 }
 
-// dg and du from dh and what the forward call kept: a wavefront's rows of one panel. PAST: the caches hold none of it.
+// dg and du from dh and what the forward call kept: a wavefront's rows of one panel. PAST: the caches hold none of it (8192 x 14336: 1.41
+// GB in 216 us, 6.5 TB/s; 224 to 268 without).
 constexpr int SLOPE_ROWS = 8;  // a wavefront, asked for at once
 template <bool GELU, bool PAST>
 __global__ __launch_bounds__(256) void gt_slope(const Slope p) {

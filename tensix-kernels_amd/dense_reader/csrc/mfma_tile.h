@@ -56,7 +56,12 @@ struct Tile {
 
     // row r's chunk c (8 k) turned by row, so that 16 rows' fill all banks; across: k's chunk c (8 rows), in pairs (32 bytes)
     // turned by k
-    static __device__ __forceinline__ int swz(int r) { return BK == 64 ? (r >> 1) & 7 : (r >> 2) & 3; }
+    // (QUARTERS, 64 bytes a row: lanes 0-3, 12-15 and 20-27 read together, 8 rows of one chunk and 8 of the next)
+    static __device__ __forceinline__ int swz(int r) {
+        if constexpr (BK == 64) return (r >> 1) & 7;
+        const int v = (r >> 2) & 3;
+        return QUARTERS ? ((v << 1) & 3) ^ (3 * (v >> 1)) : v;
+    }
     static __device__ __forceinline__ int turn(int k) {
         const int t = ROWS % 128 == 0 ? 2 * (k & 3) : ROWS % 64 == 0 ? 2 * ((k >> 1) & 1) : 0;  // (a row of k is 0 or 128 bytes mod 256)
         return QUARTERS ? t | ((k >> 3) & 1) : t;  // (32 lanes at a time: 32 rows of the same k, or 16 of k and 8 further)
@@ -144,23 +149,6 @@ __host__ __device__ inline float tiled_us(const Pace& p, int tiles, int steps) {
     const int rounds = (tiles + p.at_once - 1) / p.at_once;
     const float full = rounds ? (float)tiles / (float)(rounds * p.at_once) : 0.f;
     return (float)rounds * ((p.step + p.shared * full) * (float)steps + p.ends);
-}
-
-// dx's splits of its long sum, for one or two rounds of workgroups: their sums' way back through memory costs a launch and
-// about 3.5 TB/s. The rows that count are known on the device alone, so every workgroup finds the splits for itself.
-constexpr int ROUNDS = 2;
-__host__ __device__ inline int dx_splits(const Pace& p, int tiles, int steps, int tile_bytes, float* us = nullptr) {
-    int best = 1;
-    float least = tiled_us(p, tiles, steps);
-    for (int r = 1; r <= ROUNDS; ++r) {
-        int s = r * p.at_once / (tiles > 0 ? tiles : 1);
-        if (s > steps / 4) s = steps / 4;
-        if (s < 2) continue;
-        const float t = tiled_us(p, tiles * s, ((steps + s - 1) / s + 1) & ~1) + 4.f + (float)tiles * (float)s * (float)tile_bytes * 0.28e-6f;
-        if (t < least) least = t, best = s;
-    }
-    if (us) *us = least;
-    return best;
 }
 
 // workgroups go to the XCDs in turn; each XCD takes a run of tiles, in groups of GM row tiles by all column tiles, so that

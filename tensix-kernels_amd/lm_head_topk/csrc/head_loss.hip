@@ -96,6 +96,23 @@ __host__ __device__ constexpr Pace pace(int epi, int bm, int bn, int wk) {
     return Pace{2 * CUS, dx ? 0.75f : dhead ? 0.6f : 0.62f, dhead ? 0.3f : 0.35f, dx ? 7.f : dhead ? 4.f : 8.f};
 }
 
+// dx's splits of its long sum, for one or two rounds of workgroups: their sums' way back through memory costs a launch and
+// about 3.5 TB/s. The rows that count are known on the device alone, so every workgroup finds the splits for itself.
+constexpr int ROUNDS = 2;
+__host__ __device__ inline int dx_splits(const Pace& p, int tiles, int steps, int tile_bytes, float* us = nullptr) {
+    int best = 1;
+    float least = tiled_us(p, tiles, steps);
+    for (int r = 1; r <= ROUNDS; ++r) {
+        int s = r * p.at_once / (tiles > 0 ? tiles : 1);
+        if (s > steps / 4) s = steps / 4;
+        if (s < 2) continue;
+        const float t = tiled_us(p, tiles * s, ((steps + s - 1) / s + 1) & ~1) + 4.f + (float)tiles * (float)s * (float)tile_bytes * 0.28e-6f;
+        if (t < least) least = t, best = s;
+    }
+    if (us) *us = least;
+    return best;
+}
+
 // D[m][n] in tiles of BM x BN, a wavefront BM / WM x BN / WN of 32x32x16 matrix instructions; NS stages of BK k in LDS, filled
 // straight from memory.
 // - 256 x 256 by 8 wavefronts: the largest that the registers hold, so the fewest bytes into a CU for each operation. Its

@@ -256,6 +256,7 @@ def test_refusals(device):
         ("integers", bad, lambda: grads.global_norm([a.int()])),
         ("requires grad", bad, lambda: grads.global_norm([leaf])),
         ("max_norm < 0", bad, lambda: grads.clip_([a], -1.0)),
+        ("max_norm on the device", bad, lambda: grads.clip_([a], torch.ones((), device=device.torch))),
         ("max_norm NaN", bad, lambda: grads.clip_([a], math.nan)),
         ("one tensor twice", ValueError, lambda: grads.clip_([a, a], 1.0)),
         ("shared memory", ValueError, lambda: grads.clip_([pool[:100], pool[99:]], 1.0)),

@@ -113,35 +113,46 @@ struct Prod {
 };
 
 // The tile of dg or du that a DWF workgroup multiplies by, from dh and what was kept: rows (its k) by BN outputs from c0 on, in the
-// places of its operand's loads; to memory too (leave).
+// places of its operand's loads; to memory too (leave). All loads first: they would wait for each other's values else.
 template <typename T, int BN, int NT, bool GELU>
 __device__ __forceinline__ void dz_tile(const Prod& a, uint4* to, int tid, int side, int c0, bool leave) {
+    constexpr int C = BN / 8;
+    const long long one = a.panels * a.panel, panel = (long long)(c0 >> 8) * a.panel + (c0 & 255);
+    uint4 dh[T::N], g[T::N], u[T::N], lo[T::N];
+    auto place = [&](int i, int& k, int& f) INLINE {  // chunk i's row and first output; false past the last
+        const int s = i * NT + tid, c = s % C;
+        k = s / C, f = 8 * ((((c >> 1) ^ T::turn(k)) << 1) | (c & 1));
+        return k < a.rows && f < a.width - c0;
+    };
 #pragma unroll
     for (int i = 0; i < T::N; ++i) {
-        constexpr int C = BN / 8;
-        const int s = i * NT + tid, k = s / C, c = s % C, f = 8 * ((((c >> 1) ^ T::turn(k)) << 1) | (c & 1)), left = a.width - c0 - f;
-        uint4 out = make_uint4(0u, 0u, 0u, 0u);
-        if (k < a.rows && left > 0) {
-            const long long one = a.panels * a.panel, at = (long long)(c0 >> 8) * a.panel + (long long)k * 256 + (c0 & 255) + f;
-            const uint4 dh = *reinterpret_cast<const uint4*>(a.dh + k * a.ld_dh + c0 + f);
-            const uint4 g = *reinterpret_cast<const uint4*>(a.kept + at), u = *reinterpret_cast<const uint4*>(a.kept + one + at),
-                        lo = *reinterpret_cast<const uint4*>(a.kept + 2 * one + at);
-            auto four = [&](uint2 d, uint2 g, uint2 u, uint2 lo) INLINE {
-                float o[4];
+        int k, f;
+        if (!place(i, k, f)) k = f = 0;  // (there is one)
+        const long long at = panel + (long long)k * 256 + f;
+        dh[i] = *reinterpret_cast<const uint4*>(a.dh + k * a.ld_dh + c0 + f);
+        g[i] = *reinterpret_cast<const uint4*>(a.kept + at);
+        u[i] = *reinterpret_cast<const uint4*>(a.kept + one + at);
+        lo[i] = *reinterpret_cast<const uint4*>(a.kept + 2 * one + at);
+    }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float act, slope;
-                    act_of<GELU>(kept_g(g, lo, e), act, slope);
-                    o[e] = bf16_of(d, e) * (side ? act : slope * kept_u(u, lo, e));
-                }
-                return make_uint2(cvt2(o[0], o[1]), cvt2(o[2], o[3]));
-            };
-            const uint2 x = four(make_uint2(dh.x, dh.y), make_uint2(g.x, g.y), make_uint2(u.x, u.y), make_uint2(lo.x, lo.y));
-            const uint2 y = four(make_uint2(dh.z, dh.w), make_uint2(g.z, g.w), make_uint2(u.z, u.w), make_uint2(lo.z, lo.w));
-            out = make_uint4(x.x, x.y, y.x, y.y);
-            if (leave) *reinterpret_cast<uint4*>(a.dz + side * one + at) = out;
-        }
-        to[s] = out;
+    for (int i = 0; i < T::N; ++i) {
+        auto four = [&](uint2 d, uint2 g, uint2 u, uint2 lo) INLINE {
+            float o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float act, slope;
+                act_of<GELU>(kept_g(g, lo, e), act, slope);
+                o[e] = bf16_of(d, e) * (side ? act : slope * kept_u(u, lo, e));
+            }
+            return make_uint2(cvt2(o[0], o[1]), cvt2(o[2], o[3]));
+        };
+        const uint2 x = four(make_uint2(dh[i].x, dh[i].y), make_uint2(g[i].x, g[i].y), make_uint2(u[i].x, u[i].y), make_uint2(lo[i].x, lo[i].y));
+        const uint2 y = four(make_uint2(dh[i].z, dh[i].w), make_uint2(g[i].z, g[i].w), make_uint2(u[i].z, u[i].w), make_uint2(lo[i].z, lo[i].w));
+        int k, f;
+        const bool in = place(i, k, f);
+        const uint4 out = in ? make_uint4(x.x, x.y, y.x, y.y) : make_uint4(0u, 0u, 0u, 0u);
+        if (leave && in) *reinterpret_cast<uint4*>(a.dz + side * one + panel + (long long)k * 256 + f) = out;
+        to[i * NT + tid] = out;
     }
 }
 
@@ -359,15 +370,17 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
         __shared__ uint32_t before;
         if (splits > 1) {
             const int tile = mt * a.tn + nt;
-            float* const sums = a.acc + (long long)tile * splits * (BM * BN) + tid;
+            // (two at a time)
+            uint64_t* const sums = reinterpret_cast<uint64_t*>(a.acc) + (long long)tile * splits * (BM * BN / 2) + tid;
             if (!group) {
 #pragma unroll
                 for (int i = 0; i < MI; ++i)
 #pragma unroll
                     for (int j = 0; j < NI; ++j)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            __hip_atomic_store(sums + split * (BM * BN) + ((i * NI + j) * 4 + e) * NT, acc[i][j][e], __ATOMIC_RELAXED,
+                        for (int e = 0; e < 2; ++e)
+                            __hip_atomic_store(sums + split * (BM * BN / 2) + ((i * NI + j) * 2 + e) * NT,
+                                               __builtin_bit_cast(uint64_t, (f32x2{acc[i][j][2 * e], acc[i][j][2 * e + 1]})), __ATOMIC_RELAXED,
                                                __HIP_MEMORY_SCOPE_AGENT);
             }
             step_barrier<0>();  // (they have landed)
@@ -386,9 +399,11 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
 #pragma unroll
                         for (int j = 0; j < NI; ++j)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                acc[i][j][e] += __hip_atomic_load(sums + w * (BM * BN) + ((i * NI + j) * 4 + e) * NT, __ATOMIC_RELAXED,
-                                                                  __HIP_MEMORY_SCOPE_AGENT);
+                            for (int e = 0; e < 2; ++e) {
+                                const f32x2 v = __builtin_bit_cast(f32x2, __hip_atomic_load(sums + w * (BM * BN / 2) + ((i * NI + j) * 2 + e) * NT,
+                                                                                            __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+                                acc[i][j][2 * e] += v[0], acc[i][j][2 * e + 1] += v[1];
+                            }
             }
         }
         if (group) return;

@@ -253,6 +253,9 @@ def test_autograd(device, n, keep):
     same("a broadcast dh", w.grad, ones[1])
     with torch.no_grad():
         assert not gated.gated(a, w, v, "geglu").requires_grad
+    (fused,) = leaves(torch.cat([wg, wu]))  # both halves of one parameter
+    gated.gated(x, fused[:264], fused[264:], "geglu", keep=keep).backward(dh)
+    same("a fused parameter", fused.grad, torch.cat(want[1:]))
 
 
 @pytest.mark.parametrize("n, d, f", [(60, 128, 264), (70, 400, 12128), (69, 280, 11016), (1100, 72, 520)])

@@ -96,7 +96,7 @@ struct Prod {
     int tm, tn;             // tiles
     uint16_t* h;
     long long ld_h;
-    uint16_t* kept;         // [3][panels][rows][256]: see keep_of
+    uint16_t* kept;         // [3][panels][rows][256]: g's upper parts, u's, the lower ones of both
     const uint16_t* dh;
     long long ld_dh;
     uint16_t* dz;           // dg, then du, each [panels][rows][256]
@@ -221,7 +221,6 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
         ta.init(tid, DW ? a.ldx : a.ld_gate, ra);
     }
     tb.init(tid, ldb, rb);
-    int st = step0 + group * rounds * NS;  // the next step to be loaded
     // PAIR: a load of a wavefront has 64 / CK rows, all of gate or all of up: by the wavefront, or where it has fewer than 32
     // rows' loads by the load
     constexpr int ROWS = NT / TileA::CK;  // of a load of all wavefronts
@@ -229,30 +228,48 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
     const bool up_wave = wave * (64 / TileA::CK) & 16;
     __amdgpu_buffer_rsrc_t from_a, from_u, from_b;
     int left_a, left_b;
-    bool second = false;  // DX: the steps are up's
+    // where the next step to be loaded lies, and its k (DX: within its side)
+    const int st = step0 + group * rounds * NS;
+    bool second = DX && st >= own;  // DX: up's steps
+    int k = (st - (second ? own : 0)) * BK, la = DW ? a.ldx : second || (PAIR && up_wave) ? a.ld_up : a.ld_gate;
+    const uint16_t *pa, *pu = nullptr, *pb;
+    if constexpr (PAIR) {
+        pa = (ROWS % 32 == 0 && up_wave ? a.up : a.gate) + (long long)m0 * (ROWS % 32 == 0 ? la : a.ld_gate) + k;
+        pu = a.up + (long long)m0 * a.ld_up + k;
+        pb = a.x + (long long)n0 * a.ldx + k;
+    } else if constexpr (DW) {
+        pa = a.x + (long long)k * a.ldx + m0;
+        pb = a.dz + (side_n * a.panels + (c0 >> 8)) * a.panel + (c0 & 255) + (long long)k * 256;
+    } else {
+        pa = (second ? a.up : a.gate) + (long long)k * la + m0;
+        pb = a.dz + ((second ? a.panels : 0) + (k >> 8)) * a.panel + (k & 255) + n0 * 256ll;
+    }
+    if (DX && second) ta.init(tid, a.ld_up, ra);
     auto next = [&] INLINE {
-        const int side = DX ? st >= own : 0, k = (st - side * own) * BK;
+        if (DX && k == own * BK && !second) {  // on to up's, whose rows may lie otherwise apart
+            second = true, k = 0, la = a.ld_up;
+            pa = a.up + m0;
+            pb = a.dz + a.panels * a.panel + n0 * 256ll;
+            ta.init(tid, la, ra);
+        }
         left_a = left_b = k_end - k;
         if constexpr (PAIR) {
             const int r = min(FM, ra);
-            if constexpr (ROWS % 32 == 0) {
-                const int ld = up_wave ? a.ld_up : a.ld_gate;
-                from_a = ta.source((up_wave ? a.up : a.gate) + (long long)m0 * ld + k, ld, r, left_a);
-            } else {
-                from_a = ta.source(a.gate + (long long)m0 * a.ld_gate + k, a.ld_gate, r, left_a);
-                from_u = ta.source(a.up + (long long)m0 * a.ld_up + k, a.ld_up, r, left_a);
-            }
-            from_b = tb.source(a.x + (long long)n0 * a.ldx + k, a.ldx, min(BN, rb), left_b);
+            from_a = ta.source(pa, ROWS % 32 == 0 ? la : a.ld_gate, r, left_a);
+            if constexpr (ROWS % 32) from_u = ta.source(pu, a.ld_up, r, left_a);
+            from_b = tb.source(pb, a.ldx, min(BN, rb), left_b);
+            pa += BK, pu += BK, pb += BK, k += BK;
         } else if constexpr (DW) {
-            from_a = ta.source(a.x + (long long)k * a.ldx + m0, a.ldx, ra, left_a);
-            from_b = tb.source(a.dz + (side_n * a.panels + (c0 >> 8)) * a.panel + (c0 & 255) + (long long)k * 256, 256, rb, left_b);
+            from_a = ta.source(pa, a.ldx, ra, left_a);
+            from_b = tb.source(pb, 256, rb, left_b);
+            pa += (long long)BK * a.ldx, pb += BK * 256, k += BK;
         } else {
-            if (side && !second) ta.init(tid, a.ld_up, ra), second = true;  // (up's rows may lie otherwise apart)
-            const int ld = side ? a.ld_up : a.ld_gate;
-            from_a = ta.source((side ? a.up : a.gate) + (long long)k * ld + m0, ld, ra, left_a);
-            from_b = tb.source(a.dz + (side * a.panels + (k >> 8)) * a.panel + (k & 255) + n0 * 256ll, 256, min(BN, rb), left_b);
+            from_a = ta.source(pa, la, ra, left_a);
+            from_b = tb.source(pb, 256, min(BN, rb), left_b);
+            pa += (long long)BK * la;
+            pb += (k & 255) == 256 - BK ? a.panel - 256 + BK : BK;
+            k += BK;
         }
-        ++st;
     };
     auto load = [&](int i0, int i1, uint4* b) INLINE {  // its loads i0 .. i1 - 1 of NL
 #pragma unroll

@@ -289,6 +289,9 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
         for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     // A step's sums from one stage, the loads of a later step to another; with three stages and more between the sums: a wavefront
     // that issues all of its loads at once stands still until the memory pipeline has taken them, and all do after the barrier.
+    // (LATE: the next step's addresses behind the fragments' reads: 2047 x 2880 x 2880 in 192 x 256 73.8 to 72.2 us; 8192 x 4096 x 14336 in
+    // 256 x 256 takes 1 % longer with it)
+    constexpr bool LATE = NS == 2 && MI * NI < 32;
     auto sum = [&](const uint4* b, uint4* to) INLINE {
         constexpr int U = BK / 32, H = NS >= 3 && MI >= 4 ? 2 : 1;  // (parts of the sums between which the loads lie)
 #pragma unroll
@@ -298,6 +301,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
             for (int j = 0; j < NI; ++j) fb[j] = TileB::frag16(b, mine + CA, wn * TN + 16 * j, u, lane);
 #pragma unroll
             for (int i = 0; i < MI; ++i) fa[i] = TileA::frag16(b, mine, wm * TM + 16 * i, u, lane);
+            if (LATE && u == 0) next();
 #pragma unroll
             for (int p = 0; p < H; ++p) {
                 if constexpr (NS >= 3) load((u * H + p) * NL / (U * H), (u * H + p + 1) * NL / (U * H), to);
@@ -315,7 +319,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
     // reads. A last step of its own behind a branch would have the compiler copy every accumulator.)
     auto step = [&](uint4* to, const uint4* from) INLINE {
         step_barrier<NS >= 3 ? (NS - 2) * NL : 0>();
-        next();
+        if constexpr (!LATE) next();
         sum(from, to);
     };
     auto first = [&](uint4* to) INLINE {

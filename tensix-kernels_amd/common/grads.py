@@ -136,7 +136,7 @@ def clipped(grads, max_norm, out=None, dtype=None, norm=None):
         out = list(out)
         outs, where = _tensors(out)
         assert where == device and all(map(torch.Tensor.is_contiguous, outs)), "grads: out is contiguous, on the gradients' device"
-        if len(ts) < len(grads):
+        if len(ts) < len(grads) or len(outs) < len(out):
             assert [t is None for t in grads] == [o is None for o in out], "grads: out has a tensor where there is a gradient"
         assert list(map(torch.Tensor.numel, outs)) == list(map(torch.Tensor.numel, ts)), "grads: out has as many values of each"
     if not all(map(torch.Tensor.is_contiguous, ts)):

@@ -268,6 +268,8 @@ def test_refusals(device):
         ("out strided", bad, lambda: grads.clipped([a], 1.0, out=[pool[:128:2]])),
         ("outs' number", bad, lambda: grads.clipped([a, b], 1.0, out=[b])),
         ("out for None", bad, lambda: grads.clipped([a, None], 1.0, out=[pool[:64], b])),
+        ("None for a gradient", bad, lambda: grads.clipped([a, b], 1.0, out=[pool[:64], None, pool[64:128]])),
+        ("a None too many", bad, lambda: grads.clipped([a], 1.0, out=[b, None])),
         ("out and dtype", bad, lambda: grads.clipped([a], 1.0, out=[b], dtype=F32)),
         ("dtype", bad, lambda: grads.clipped([a], 1.0, dtype=torch.float64)),
         ("a norm of the host", bad, lambda: grads.clip_([a], 1.0, norm=torch.ones(()))),

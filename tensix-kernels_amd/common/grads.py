@@ -26,6 +26,7 @@ The kernels are dr_grads_norm's and dr_grads_clip's of libdense_reader.so (inclu
 import ctypes
 import sys
 from array import array
+from operator import attrgetter
 from pathlib import Path
 
 import torch
@@ -34,6 +35,8 @@ sys.path.insert(0, str(Path(__file__).resolve().parents[1]))
 from common import device as dev  # noqa: E402
 from dense_reader import _lib  # noqa: E402
 
+_data_ptr, _numel, _contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
+_dtype, _requires_grad = attrgetter("dtype"), attrgetter("requires_grad")
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -52,25 +55,25 @@ def _tensors(grads):
     device = ts[0].device
     assert device.type == "cuda", device
     assert set(map(torch.Tensor.get_device, ts)) == {device.index}, f"grads: not all on {device}"
-    assert not (torch.is_grad_enabled() and any(t.requires_grad for t in ts)), (
+    assert not (torch.is_grad_enabled() and any(map(_requires_grad, ts))), (
         "grads: no derivative (detach them, or call under torch.no_grad())")
     return ts, device
 
 
 def _types(ts):
-    kinds = [TYPES.get(t.dtype) for t in ts]
-    assert None not in kinds, {t.dtype for t in ts}
+    kinds = list(map(TYPES.get, map(_dtype, ts)))
+    assert None not in kinds, set(map(_dtype, ts))
     return array("i", kinds)
 
 
 class _Call:
-    """The tensors' values, and the launch over them. (The lists are arrays of the standard library: what the call's host time goes
-    by is how often each tensor is asked for something.)"""
+    """The tensors' values, and the launch over them. (The lists are arrays of the standard library, each made of a list, which is
+    faster than of an iterator: what the call's host time goes by is how often each tensor is asked for something.)"""
 
-    def __init__(self, ts, device):
+    def __init__(self, ts, device, sizes=None):
         self.device, self.held = device, ts
         self.norm = torch.empty((), dtype=torch.float32, device=device)
-        self.ins, self.sizes, self.types = array("Q", map(torch.Tensor.data_ptr, ts)), array("q", map(torch.Tensor.numel, ts)), _types(ts)
+        self.ins, self.sizes, self.types = array("Q", list(map(_data_ptr, ts))), array("q", sizes or list(map(_numel, ts))), _types(ts)
         self.A = _lib.Grads(len(ts), *(a.buffer_info()[0] for a in (self.ins, self.sizes, self.types)))
 
     def run(self, fn, workspace):
@@ -90,7 +93,7 @@ class _Call:
 
     def clip(self, outs, max_norm, norm):
         A = self.A
-        at, types = (self.ins, self.types) if outs is self.held else (array("Q", map(torch.Tensor.data_ptr, outs)), _types(outs))
+        at, types = (self.ins, self.types) if outs is self.held else (array("Q", list(map(_data_ptr, outs))), _types(outs))
         A.out, A.out_types = at.buffer_info()[0], types.buffer_info()[0]
         assert not isinstance(max_norm, torch.Tensor), "grads: max_norm is a number of the host's"
         A.max_norm = float(max_norm)
@@ -127,6 +130,7 @@ def clipped(grads, max_norm, out=None, dtype=None, norm=None):
     a gradient but its own as a whole (ValueError)."""
     grads = list(grads)
     ts, device = _tensors(grads)
+    sizes = None
     if out is None:
         assert dtype is None or dtype in TYPES, dtype
         out = [None if t is None else torch.empty(t.shape, dtype=dtype or t.dtype, device=device) for t in grads]
@@ -135,12 +139,13 @@ def clipped(grads, max_norm, out=None, dtype=None, norm=None):
         assert dtype is None, "grads: dtype is out's"
         out = list(out)
         outs, where = _tensors(out)
-        assert where == device and all(map(torch.Tensor.is_contiguous, outs)), "grads: out is contiguous, on the gradients' device"
+        assert where == device and all(map(_contiguous, outs)), "grads: out is contiguous, on the gradients' device"
         if len(ts) < len(grads) or len(outs) < len(out):
             assert [t is None for t in grads] == [o is None for o in out], "grads: out has a tensor where there is a gradient"
-        assert list(map(torch.Tensor.numel, outs)) == list(map(torch.Tensor.numel, ts)), "grads: out has as many values of each"
-    if not all(map(torch.Tensor.is_contiguous, ts)):
+        sizes = list(map(_numel, ts))
+        assert list(map(_numel, outs)) == sizes, "grads: out has as many values of each"
+    if not all(map(_contiguous, ts)):
         ts = [t.contiguous() for t in ts]
-    norm = _Call(ts, device).clip(outs, max_norm, norm)
+    norm = _Call(ts, device, sizes).clip(outs, max_norm, norm)
     dev.written(*outs)
     return norm, out

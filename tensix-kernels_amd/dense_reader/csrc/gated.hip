@@ -11,9 +11,9 @@
 // 16 sums have g and u of an output in one lane. dg, du and what is kept lie in panels of 256 outputs ([output / 256][row][256]), which
 // the products that read them take in contiguous blocks. No atomics but counters: every sum has one order.
 //
-// What bounds them. 8192 rows x 4096 x 14336, a step in 4.73 to 4.83 ms (one machine and another): 1504 us for h and what is kept (1280
-// TFLOP/s; h alone 1410), 216 for dg and du (1.41 GB, 6.5 TB/s), 1410 for both weights' gradients (1365), 1560 for dx (1235): the matrix
-// cores, busy 57 to 64 % of the clocks, and the power that random values draw, which holds the clock at 1.7 to 1.9 GHz (a large
+// What bounds them. 8192 rows x 4096 x 14336, a step in 4.50 to 4.59 ms (one machine and another): 1500 us for h and what is kept (1283
+// TFLOP/s; h alone 1395), 216 for dg and du (1.41 GB, 6.5 TB/s), 1390 for both weights' gradients (1384), 1480 for dx (1300): the matrix
+// cores, busy 65 to 70 % of the clocks, and the power that random values draw, which holds the clock at 1.6 to 1.8 GHz (a large
 // library product of the three layouts, the card as warm: 1220, 1580, 1370 us). 32 rows x 4096 x 14336: the weights' 235 MB in
 // 38.4 us, 6.1 TB/s. A few rows by a small layer: each launch's start, its first loads and the way of a few sums (48 x 1024 x
 // 4096: 3 launches of 10 to 13 us for a step).
@@ -163,7 +163,7 @@ __device__ __forceinline__ void dz_tile(const Prod& a, uint4* to, int tid, int s
 //   of 32. 4 wavefronts of 128 x 128 that read their fragments a step ahead, accumulators pinned, took 1474 us for h and 3 % off the
 //   others, with matrix instructions that the compiler cannot see the waits of; h in four stages of 32 1490 to 1600; fragments read
 //   ahead by 8 wavefronts 1500 to 1640.
-// - 192 x 256 where 256 x 256 leaves CUs idle in its last round (2047 x 2880 x 2880: 253 tiles for 184, h 68 to 62 us).
+// - 192 x 256 where 256 x 256 leaves CUs idle in its last round (2047 x 2880 x 2880: 253 tiles for 184, h 68 to 62 us; 57 since).
 // - 128 x 128, 64 x 128 twice a CU, 64 x 64 by two groups of wavefronts that split K: fewer tiles than CUs (choose).
 // - few rows: choose_few.
 // The epilogues' bf16 leave through LDS in whole runs of a row.

@@ -393,39 +393,46 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
             const int tile = mt * a.tn + nt;
             // (two at a time)
             uint64_t* const sums = reinterpret_cast<uint64_t*>(a.acc) + (long long)tile * splits * (BM * BN / 2) + tid;
+            // (the fragments with rows: both gradients of 8 x 1024 x 4096 23.2 to 21.8 us, of 48 rows 24.9 to 24.6)
+            const int live = (rb - wn * TN + 15) / 16;
             if (!group) {
 #pragma unroll
-                for (int i = 0; i < MI; ++i)
+                for (int j = 0; j < NI; ++j) {
+                    if (j >= live) break;
 #pragma unroll
-                    for (int j = 0; j < NI; ++j)
+                    for (int i = 0; i < MI; ++i)
 #pragma unroll
                         for (int e = 0; e < 2; ++e)
                             __hip_atomic_store(sums + split * (BM * BN / 2) + ((i * NI + j) * 2 + e) * NT,
                                                __builtin_bit_cast(uint64_t, (f32x2{acc[i][j][2 * e], acc[i][j][2 * e + 1]})), __ATOMIC_RELAXED,
                                                __HIP_MEMORY_SCOPE_AGENT);
+                }
             }
             step_barrier<0>();  // (they have landed)
             if (threadIdx.x == 0) before = __hip_atomic_fetch_add(a.arrived + tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             step_barrier<0>();
             if (before != (uint32_t)(splits - 1)) return;
-            if (!group) {
+            auto join = [&](int fragments) INLINE {
 #pragma unroll
                 for (int i = 0; i < MI; ++i)
 #pragma unroll
-                    for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    for (int j = 0; j < fragments; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
                 for (int w = 0; w < splits; ++w)
 #pragma unroll
                     for (int i = 0; i < MI; ++i)
 #pragma unroll
-                        for (int j = 0; j < NI; ++j)
+                        for (int j = 0; j < fragments; ++j)
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
                                 const f32x2 v = __builtin_bit_cast(f32x2, __hip_atomic_load(sums + w * (BM * BN / 2) + ((i * NI + j) * 2 + e) * NT,
                                                                                             __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
                                 acc[i][j][2 * e] += v[0], acc[i][j][2 * e + 1] += v[1];
                             }
-            }
+            };
+            static_assert(EPI != EPI_DXJ || NI == 2, "one fragment or both");
+            if (!group && live >= 2) join(2);
+            else if (!group && live == 1) join(1);
         }
         if (group) return;
     }

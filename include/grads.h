@@ -4,7 +4,8 @@
  *   norm = sqrt(sum over all values of all tensors of v^2); factor = min(1, max_norm / (norm + 1e-6)); out = v factor
  *
  * Squares and their sums are float64 (no float32 overflows or is lost), each out is rounded once from the float32 product. A NaN
- * among the values makes the norm and every out NaN; an infinity makes the norm infinite, the factor 0 and its own out NaN.
+ * among the values makes the norm and every out NaN; an infinity makes the norm infinite, the factor 0 and its own out NaN. An infinite
+ * max_norm is no limit: the factor is 1 unless the norm is NaN.
  *
  * No counterpart in the reference, which has no training.
  */
@@ -29,7 +30,7 @@ typedef struct dr_grads {
     const int32_t* types;
     void* const* out;         /* clip: where each one's values go, its own in (of the same type) or memory apart from every other's and the norm's */
     const int32_t* out_types;
-    double max_norm;          /* clip: 0 or more */
+    double max_norm;          /* clip: 0 or more, an infinity too */
     float* norm;              /* written; a clip with `given` reads it */
     int32_t given;            /* clip: norm holds the norm (of more gradients than these, say) */
     void* workspace;          /* dr_grads_workspace_bytes, 8-byte aligned; its contents mean nothing between calls */

@@ -218,7 +218,8 @@ __global__ __launch_bounds__(LANES) void gr_clip(const List a, const double* sum
     const double v = sums ? norm_of(sums, count) : (double)*norm;
     if (sums && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)v;
     const double q = max_norm / (v + 1e-6);
-    const float f = q >= 1. ? 1.f : (float)q;  // (a NaN stays one)
+    // (a NaN of the norm stays one; no limit clips nothing, whatever else the norm is)
+    const float f = q >= 1. || (max_norm == __builtin_inf() && v == v) ? 1.f : (float)q;
     for (uint32_t i = blockIdx.x; i < a.chunks; i += gridDim.x) {
         uint32_t within;
         const int t = tensor_of(a, a.chunks - 1 - i, within), kind = a.kind[t], type = kind & 3, out = kind >> 2 & 3;

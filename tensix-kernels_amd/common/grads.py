@@ -12,9 +12,9 @@ own.
 
 The tensors are float32, bfloat16 or float16 on one GPU, in any mix and of any shapes (None is passed over). Squares and their sums are
 float64, so that no float32 gradient overflows; a clipped value is the float32 product with the factor, rounded once. A NaN among them
-makes the norm and all that is clipped NaN, an infinity the norm infinite and the clipped values 0 (its own NaN): look at the norm. A
-tensor whose memory is dense in another order of its dims (a transposed gradient) is taken as it lies; any other strided one is read
-from a copy, and refused in place.
+makes the norm and all that is clipped NaN, an infinity the norm infinite and the clipped values 0 (its own NaN): look at the norm. An
+infinite max_norm is no limit: all stays as it is, infinities too, but for a NaN's. A tensor whose memory is dense in another order of
+its dims (a transposed gradient) is taken as it lies; any other strided one is read from a copy, and refused in place.
 
 Nothing goes to the host and nothing is differentiable. Memory comes from torch's allocator each call, on the current stream, so calls
 on several streams, threads or captured graphs never share any; the addresses are the launches' arguments, so a captured graph goes on

@@ -285,3 +285,28 @@ def test_refusals(device):
         grads.clip_([leaf], 1.0)
     raises("written before its backward", RuntimeError, y.backward)
     same("gradients beside each other", grads.clipped([a], 1.0, out=[a])[1][0], a)
+
+
+@pytest.mark.parametrize("lists", [1, 3])
+def test_no_limit(device, lists):
+    """max_norm infinite: the norm alone is asked for. Nothing is clipped whatever the norm is, but for a NaN, which makes all NaN."""
+    ts = make(device, [9000, 50, 8192] + [3] * (128 * (lists - 1)), [F32, BF16, F16], 4)
+    for what, value, want in [("finite", 1.0, None), ("infinite", -math.inf, math.inf), ("past float32", None, math.inf), ("NaN", math.nan, math.nan)]:
+        mine = [t.clone() for t in ts]
+        if value is None:
+            mine[0][:] = 3e38
+        else:
+            mine[0][8500] = value
+        norm = grads.global_norm(mine)
+        for given in (None, norm):
+            n, outs = grads.clipped(mine, math.inf, norm=given)
+            wide = grads.clipped(mine, math.inf, dtype=F32, norm=given)[1]
+            there = [t.clone() for t in mine]
+            same_norm = grads.clip_(there, math.inf, norm=given)
+            for v in (n, same_norm):
+                assert v.isnan() if want is math.nan else v.item() == (norm.item() if want is None else want), (what, v)
+            for t, o, w, p in zip(mine, outs, wide, there):
+                if want is math.nan:
+                    assert bool(o.isnan().all()) and bool(w.isnan().all()) and bool(p.isnan().all()), what
+                else:
+                    same(f"{what}: as it was", o, t), same("float32", w, t.float()), same("in place", p, t)

@@ -5,7 +5,7 @@
 // turn; each leaves one sum of squares. The next launch adds those up in every workgroup for itself (16 KB at most a launch of
 // them, which the caches hold), in one order, and is the clip itself, or one workgroup for the norm alone: no atomics, two launches
 // for 128 tensors. The clip takes the chunks the other way round, the last ones read first, which the 256 MB cache behind the
-// L2s still holds.
+// L2s still holds. Of many launches' sums one workgroup adds up all first (gr_total).
 //
 // Bound by memory: one read, and for a clip a second and one write. 252 M bf16 values in 146 tensors 73 us (6.9 TB/s); 283 M float32
 // values clipped 189 us for the squares (6.0 TB/s) and 416 for the rest (5.5; a large copy reaches 4.9). 18 tensors of 190 k values:
@@ -168,17 +168,28 @@ __global__ __launch_bounds__(LANES) void gr_squares(const List a, double* sums) 
     if (threadIdx.x == 0) sums[blockIdx.x] = s;
 }
 
-// sqrt of the sums' sum, the same in every workgroup
-__device__ __forceinline__ double norm_of(const double* sums, int count) {
+// the sums' sum, the same in every workgroup, and its square root
+__device__ __forceinline__ double sum_of(const double* sums, int count) {
     double s = 0.;
 #pragma unroll 8
     for (int i = threadIdx.x; i < count; i += LANES) s += sums[i];
-    return sqrt(block_sum(s));
+    return block_sum(s);
 }
+
+__device__ __forceinline__ double norm_of(const double* sums, int count) { return sqrt(sum_of(sums, count)); }
 
 __global__ __launch_bounds__(LANES) void gr_norm(const double* sums, int count, float* norm) {
     const double v = norm_of(sums, count);
     if (threadIdx.x == 0) *norm = (float)v;
+}
+
+// Of several launches the sums' sum, in the place of the first: the clip's launches, as many, would each add up all of them in every
+// workgroup. From ADDED (launches times sums) on: 384 tensors of 16 chunks 72 us with it and 76 without, 1024 193 and
+// 255, 8192 1.7 and 8.3 ms; but 384 of 3 chunks 37.4 and 36.4, 256 of one 20.4 and 19.1 us.
+constexpr long long ADDED = 8192;
+__global__ __launch_bounds__(LANES) void gr_total(double* sums, int count) {
+    const double s = sum_of(sums, count);
+    if (threadIdx.x == 0) *sums = s;  // (all have read theirs: block_sum's barrier)
 }
 
 template <int TYPE, int OUT>
@@ -312,11 +323,12 @@ bool fill(const dr_grads* a, bool clip, int& i, int to, List& l) {
 
 int groups(uint32_t chunks) { return (int)std::min<uint32_t>(chunks, GRID); }
 
-// the sums' launches; how many sums there are
-int squares_of(const dr_grads* a, hipStream_t st) {
+// the sums' launches, how many; how many sums there are
+int squares_of(const dr_grads* a, hipStream_t st, int& lists) {
     List l;
     int count = 0;
-    for (int i = 0; fill(a, false, i, a->count, l);) {
+    lists = 0;
+    for (int i = 0; fill(a, false, i, a->count, l); ++lists) {
         const int g = groups(l.chunks);
         hipLaunchKernelGGL(gr_squares, dim3(g), dim3(LANES), 0, st, l, reinterpret_cast<double*>(a->workspace) + count);
         count += g;
@@ -342,7 +354,8 @@ extern "C" int64_t dr_grads_workspace_bytes(const dr_grads* a) {
 extern "C" int dr_grads_norm(const dr_grads* a) {
     if (!list_ok(a, false) || !call_ok(a)) return DR_EINVAL;
     const hipStream_t st = reinterpret_cast<hipStream_t>(a->stream);
-    const int count = squares_of(a, st);
+    int lists;
+    const int count = squares_of(a, st, lists);
     hipLaunchKernelGGL(gr_norm, dim3(1), dim3(LANES), 0, st, reinterpret_cast<const double*>(a->workspace), count, a->norm);
     return hipGetLastError() == hipSuccess ? DR_OK : DR_EHIP;
 }
@@ -353,8 +366,12 @@ extern "C" int dr_grads_clip(const dr_grads* a) {
     const int ok = apart(a);
     if (ok <= 0) return ok < 0 ? DR_EHIP : DR_EINVAL;
     const hipStream_t st = reinterpret_cast<hipStream_t>(a->stream);
-    const double* sums = reinterpret_cast<const double*>(a->workspace);
-    const int count = a->given ? 0 : squares_of(a, st);
+    double* sums = reinterpret_cast<double*>(a->workspace);
+    int lists = 0, count = a->given ? 0 : squares_of(a, st, lists);
+    if (lists > 1 && (long long)lists * count >= ADDED) {
+        hipLaunchKernelGGL(gr_total, dim3(1), dim3(LANES), 0, st, sums, count);
+        count = 1;
+    }
     bool any = false;
     for (int to = a->count; to > 0;) {  // (the last tensors first: they were read last)
         int from = to;

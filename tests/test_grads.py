@@ -310,3 +310,42 @@ def test_no_limit(device, lists):
                     assert bool(o.isnan().all()) and bool(w.isnan().all()) and bool(p.isnan().all()), what
                 else:
                     same(f"{what}: as it was", o, t), same("float32", w, t.float()), same("in place", p, t)
+
+
+def test_many_lists(device):
+    """8192 tensors, 64 launches' worth: right, and a clip takes about the time of its norm and of a clip by a given norm (each
+    launch of it would add up all 131072 sums again otherwise, several times as long)."""
+    count, each = 8192, 16 * 8192
+    g = torch.Generator(device.torch).manual_seed(3)
+    pool = torch.randn(count, each, generator=g, device=device.torch, dtype=BF16)
+    out = torch.empty_like(pool)
+    ts, outs = list(pool.unbind()), list(out.unbind())
+    want = torch.stack([t.double().square().sum() for t in pool.split(512)]).sum().sqrt()
+    norm = grads.global_norm(ts)
+    within("norm", norm[None], want[None], (want * U * 1.01)[None])
+    given = norm.clone()
+    calls = {"clip": lambda: grads.clipped(ts, 1.0, out=outs)[0], "norm": lambda: grads.global_norm(ts),
+             "given": lambda: grads.clipped(ts, 1.0, out=outs, norm=given)[0]}
+    us = {}
+    for name, call in calls.items():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = call()
+        out.fill_(7)
+        for _ in range(3):
+            graph.replay()
+        ends = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+        ends[0].record()
+        for _ in range(5):
+            graph.replay()
+        ends[1].record()
+        torch.cuda.synchronize()
+        us[name] = ends[0].elapsed_time(ends[1]) * 200
+        same(name, got, norm)
+        if name == "norm":
+            continue
+        for i in (0, 127, 128, 5000, 8191):
+            r = ts[i].double() * (1.0 / (want + 1e-6))
+            within(f"{name}: {i}", outs[i], r, (2.0**-8 + 2.1 * U) * r.abs() + 2.0**-133)
+    print(us, flush=True)
+    assert us["clip"] < 1.5 * (us["norm"] + us["given"]), us

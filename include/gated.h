@@ -67,6 +67,7 @@ typedef struct dr_gated_info {
     int32_t dweight_stages; /* of its K loop */
     int32_t dx[3];     /* (dim by rows) */
     int32_t dx_splits; /* of its sum */
+    int32_t act_once;  /* 1: act reads each weight once, past the caches */
 } dr_gated_info;
 int dr_gated_plan(const dr_gated* a, int what, dr_gated_info* info);
 

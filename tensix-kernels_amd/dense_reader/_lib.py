@@ -294,6 +294,7 @@ class GatedInfo(ctypes.Structure):
         ("dweight_stages", c_int32),
         ("dx", c_int32 * 3),
         ("dx_splits", c_int32),
+        ("act_once", c_int32),
     ]
 
 

@@ -167,11 +167,13 @@ __device__ __forceinline__ void dz_tile(const Prod& a, uint4* to, int tid, int s
 // - 128 x 128, 64 x 128 twice a CU, 64 x 64 by two groups of wavefronts that split K: fewer tiles than CUs (choose).
 // - few rows: choose_few.
 // The epilogues' bf16 leave through LDS in whole runs of a row.
-template <int BM, int BN, int WM, int WN, int WK, int NS, int BK, int EPI, bool GELU>
+// ONCE: of one column tile each weight's row is read once, past the caches (choose_few).
+template <int BM, int BN, int WM, int WN, int WK, int NS, int BK, int EPI, bool GELU, bool ONCE>
 __global__ __launch_bounds__(64 * WM * WN * WK) void gt_gemm(const Prod a) {
     constexpr bool PAIR = EPI <= EPI_AGAIN, DW = EPI == EPI_DW || EPI == EPI_DWF, DX = EPI == EPI_DX || EPI == EPI_DXJ;
     constexpr bool AT = !PAIR, BT = DW;
-    constexpr int AUX = PAIR && BN <= 64 ? 2 : 0;  // (of few rows the weights are read once)
+    constexpr int AUX = ONCE ? 2 : 0;
+    static_assert(!ONCE || (PAIR && BN <= 64), "one column tile of few rows");
     constexpr int NW = WM * WN, NT = 64 * NW, TM = BM / WM, TN = BN / WN, MI = TM / 16, NI = TN / 16;
     constexpr int CA = BM * BK / 8, CH = CA + BN * BK / 8;  // chunks of A, a stage
     constexpr int NL = CH / NT, NA = CA / NT;               // loads a lane and stage, of A
@@ -707,6 +709,12 @@ constexpr long long HELD = 96ll << 20;
 // keep the most of them on the way. us, weights from memory, n x dim x width: 8 x 4096 x 4096 13.8 by T32K4 and 17.9 by T64x32K4, 16 x
 // 2048 x 8192 17.6 and 15.1, 32 x 512 x 14336 19.5, 13.5 and 8.5 by T64x32; 33 x 2880 x 2880 13.4 by T32x64K4 and 15.7 by T64K2, 64 x
 // 2048 x 8192 22.4 and 15.5, 64 x 4096 x 14336 67, 51 and 43.8 by T128x64.
+// One tile has all rows (FEW), so a product reads each weight once, past the caches: 8 x 4096 x 4096 13.8 and 15.2 through them, 64 x 2048
+// x 8192 15.8 and 17.7, 16 x 1024 x 4096 6.9 and 7.1, 32 x 4096 x 14336 42 and 47. (What reads them after it then finds none there: both
+// gradients computed again, 48 x 1024 x 4096 31.5 and 29.1, 8 x 4096 x 4096 55 and 55, 32 x 4096 x 14336 154 and 164.) T64K2 of more rows
+// has several tiles read each weight and leaves them in the caches: 128 x 2880 x 2880 18.4 and 19.4 past them, a step 55 and 62; 256 x
+// 512 x 1408 5.8 and 6.9; 100 x 1024 x 4096 8.9 and 8.7, a step 35.2 and 38.6.
+constexpr int FEW = 64;
 int choose_few(int n, int width) {
     const int units = (width + 15) / 16;
     if (n <= 32) return units <= CUS ? T32K4 : units <= 2 * CUS ? T64x32K4 : T64x32;
@@ -715,6 +723,7 @@ int choose_few(int n, int width) {
 
 struct Plan {
     int panels, z, w, d, splits;
+    bool once;       // z's loads of the weights pass the caches
     bool one_stage;  // DW
     bool fused;      // DWF
     int counters;    // DXJ
@@ -738,7 +747,8 @@ bool plan_of(const dr_gated* a, int what, Plan& p) {
         return false;
     const bool z = !back || (a->kept == nullptr && (a->dx || a->dgate || a->dup));
     if (z) {
-        p.z = n <= 64 ? choose_few((int)n, a->width) : choose(EPI_ACT, 2 * f, n, d, {T256, T192x256, T128, T64x128, T64K2});
+        p.z = n <= FEW ? choose_few((int)n, a->width) : choose(EPI_ACT, 2 * f, n, d, {T256, T192x256, T128, T64x128, T64K2});
+        p.once = n <= FEW;
     }
     if (!back) return true;
     long long at = 2ll * p.panels * n * 512;
@@ -765,35 +775,35 @@ bool plan_of(const dr_gated* a, int what, Plan& p) {
     return true;
 }
 
-template <int BM, int BN, int WM, int WN, int WK, int NS, int BK, int EPI, bool GELU>
+template <int BM, int BN, int WM, int WN, int WK, int NS, int BK, int EPI, bool GELU, bool ONCE = false>
 void launch(Prod g, int m, int n, hipStream_t st) {
     g.tm = (m + BM - 1) / BM;
     g.tn = (n + BN - 1) / BN;
     const int grid = (g.tm * g.tn * (EPI == EPI_DX || EPI == EPI_DXJ ? g.splits : 1) + 7) & ~7;  // (as many for each XCD)
-    hipLaunchKernelGGL((gt_gemm<BM, BN, WM, WN, WK, NS, BK, EPI, GELU>), dim3(grid), dim3(64 * WM * WN * WK), 0, st, g);
+    hipLaunchKernelGGL((gt_gemm<BM, BN, WM, WN, WK, NS, BK, EPI, GELU, ONCE>), dim3(grid), dim3(64 * WM * WN * WK), 0, st, g);
 }
 
 template <int EPI, bool GELU>
-void launch_act(const Prod& g, int t, hipStream_t st) {
+void launch_act(const Prod& g, int t, bool once, hipStream_t st) {
     const int m = 2 * g.width, n = g.rows;
     switch (t) {
         case T256: return launch<256, 256, 2, 4, 1, 2, 64, EPI, GELU>(g, m, n, st);
         case T192x256: return launch<192, 256, 2, 4, 1, 2, 64, EPI, GELU>(g, m, n, st);
         case T64x128: return launch<64, 128, 1, 4, 1, 3, 64, EPI, GELU>(g, m, n, st);
-        case T32K4: return launch<32, 32, 1, 1, 4, 4, 64, EPI, GELU>(g, m, n, st);
-        case T64x32K4: return launch<64, 32, 1, 1, 4, 3, 64, EPI, GELU>(g, m, n, st);
-        case T64x32: return launch<64, 32, 1, 1, 1, 5, 64, EPI, GELU>(g, m, n, st);
-        case T32x64K4: return launch<32, 64, 1, 1, 4, 3, 64, EPI, GELU>(g, m, n, st);
+        case T32K4: return launch<32, 32, 1, 1, 4, 4, 64, EPI, GELU, true>(g, m, n, st);
+        case T64x32K4: return launch<64, 32, 1, 1, 4, 3, 64, EPI, GELU, true>(g, m, n, st);
+        case T64x32: return launch<64, 32, 1, 1, 1, 5, 64, EPI, GELU, true>(g, m, n, st);
+        case T32x64K4: return launch<32, 64, 1, 1, 4, 3, 64, EPI, GELU, true>(g, m, n, st);
         case T128: return launch<128, 128, 2, 2, 1, 2, 64, EPI, GELU>(g, m, n, st);
-        case T128x64: return launch<128, 64, 2, 2, 1, 3, 64, EPI, GELU>(g, m, n, st);
-        default: return launch<64, 64, 1, 2, 2, 4, 64, EPI, GELU>(g, m, n, st);
+        case T128x64: return launch<128, 64, 2, 2, 1, 3, 64, EPI, GELU, true>(g, m, n, st);
+        default: return once ? launch<64, 64, 1, 2, 2, 4, 64, EPI, GELU, true>(g, m, n, st) : launch<64, 64, 1, 2, 2, 4, 64, EPI, GELU>(g, m, n, st);
     }
 }
 
 template <int EPI>
-void launch_act(const Prod& g, int act, int t, hipStream_t st) {
-    if (act) launch_act<EPI, true>(g, t, st);
-    else launch_act<EPI, false>(g, t, st);
+void launch_act(const Prod& g, int act, const Plan& p, hipStream_t st) {
+    if (act) launch_act<EPI, true>(g, p.z, p.once, st);
+    else launch_act<EPI, false>(g, p.z, p.once, st);
 }
 
 // What a forward call leaves passes the caches by where they (256 MB) could not hold it until it is read: 8192 x 4096 x 14336 1604 to
@@ -820,7 +830,7 @@ extern "C" int dr_gated_plan(const dr_gated* a, int what, dr_gated_info* info) {
     *info = dr_gated_info{};
     auto tile = [](int32_t (&to)[3], int t) { to[0] = SIZE[t].bm, to[1] = SIZE[t].bn, to[2] = SIZE[t].wk; };
     const bool back = what == DR_GATED_BACKWARD;
-    if (!back || (a->kept == nullptr && (a->dx || a->dgate || a->dup))) tile(info->act, p.z);
+    if (!back || (a->kept == nullptr && (a->dx || a->dgate || a->dup))) tile(info->act, p.z), info->act_once = p.once;
     if (!back) return DR_OK;
     if (a->dgate || a->dup) tile(info->dweight, p.one_stage ? T128 : p.w), info->dweight_stages = p.one_stage ? 1 : p.w == T192x256 ? 2 : 4;
     if (a->dx) tile(info->dx, p.d), info->dx_splits = p.splits;
@@ -850,8 +860,8 @@ extern "C" int dr_gated_run(const dr_gated* a, int what) {
         g.h = reinterpret_cast<uint16_t*>(a->h), g.ld_h = a->ld_h;
         g.kept = reinterpret_cast<uint16_t*>(a->kept);
         g.past = past;
-        if (a->kept) launch_act<EPI_KEEP>(g, a->act, P.z, st);
-        else launch_act<EPI_ACT>(g, a->act, P.z, st);
+        if (a->kept) launch_act<EPI_KEEP>(g, a->act, P, st);
+        else launch_act<EPI_ACT>(g, a->act, P, st);
         return hipGetLastError() == hipSuccess ? DR_OK : DR_EHIP;
     }
     if (!a->dx && !a->dgate && !a->dup) return DR_OK;
@@ -868,7 +878,7 @@ extern "C" int dr_gated_run(const dr_gated* a, int what) {
         auto slope = a->act ? past ? gt_slope<true, true> : gt_slope<true, false> : past ? gt_slope<false, true> : gt_slope<false, false>;
         hipLaunchKernelGGL(slope, grid, dim3(256), 0, st, s);
     } else if (!a->kept) {
-        launch_act<EPI_AGAIN>(g, a->act, P.z, st);
+        launch_act<EPI_AGAIN>(g, a->act, P, st);
     }
     if (a->dgate || a->dup) {
         g.dgate = reinterpret_cast<uint16_t*>(a->dgate), g.ld_dgate = a->ld_dgate;

@@ -159,3 +159,20 @@ def test_emitted_code(tmp_path):
     ways = {name: w for name, w in ways.items() if w not in joined}
     assert len(found) >= 15 and all(len(w) == 1 for w in ways.values()), {n: w for n, w in ways.items() if len(w) != 1}
     assert set(re.findall(r"\.private_segment_fixed_size: (\d+)", asm)) == {"0"}
+
+
+@pytest.mark.parametrize("rows, dim, width", [(1, 64, 64), (32, 4096, 14336), (33, 2048, 8192), (64, 1024, 4352), (65, 1024, 4096), (128, 2880, 2880),
+                                              (256, 512, 1408), (300, 4096, 14336)])
+@pytest.mark.parametrize("what, kept", [(FORWARD, 4096), (FORWARD, None), (BACKWARD, None)])
+def test_weights_past_the_caches(rows, dim, width, what, kept):
+    """Only where one tile has all rows, so that no other reads the weights again."""
+    info = _lib.gated_info(call(rows, dim, width, kept=kept)._obj, what)
+    assert info["act_once"] == (rows <= 64) and (not info["act_once"] or rows <= info["act"][1])
+
+
+def test_loads_past_the_caches(tmp_path):
+    """The kernels of one column tile alone load anything past the caches: the weights (64 x 64 in both kinds: of many rows too)."""
+    found = dict(re.findall(r"^(_Z\S*gt_gemm\S+):(.*?)^\.Lfunc_end", _asm(tmp_path), re.M | re.S))
+    past = {name: bool(re.search(r"buffer_load_dwordx4 .* lds.* nt|buffer_load_dwordx4 .* nt .*lds", body)) for name, body in found.items()}
+    assert past and all(p == name.split("EEEv")[0].endswith("Lb1") for name, p in past.items()), past
+    assert {p for name, p in past.items() if "ILi64ELi64ELi1ELi2ELi2E" in name} == {False, True}

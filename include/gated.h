@@ -35,7 +35,7 @@ typedef struct dr_gated {
     int64_t ld_gate;
     const void* up;   /* [width][ld_up] bf16 */
     int64_t ld_up;
-    int32_t rows, dim, width; /* rows to 2^20, dim to 2^17, width to 2^20; dim and width multiples of 8 */
+    int32_t rows, dim, width; /* rows to 2^20, dim to 2^17, width to 2^20, multiples of 8 but the rows; rows * width below 2^38 */
     int32_t act;      /* 0 silu, 1 gelu_tanh (dense_reader.h's) */
     void* h;          /* [rows][ld_h] bf16 */
     int64_t ld_h;

@@ -683,12 +683,13 @@ int splits_of(int t, int tiles, int steps, float* us) {
     return best;
 }
 
-// the tile of `tiles` that takes the least time for a product of m rows by n columns, summed over k
+// the tile of `tiles` that takes the least time for a product of m rows by n columns, summed over k; -1: more of each than a launch holds
 int choose(int epi, long long m, long long n, long long k, std::initializer_list<int> tiles, int* splits = nullptr) {
-    int best = 0;
+    int best = -1;
     float least = 1e30f;
     const int steps = (int)(up(k, KSTEP) / KSTEP);
     for (int t : tiles) {
+        if (tiles_of(t, m, n) >= MOST_TILES) continue;
         float us;
         int s = 1;
         if (epi == EPI_DX) s = splits_of(t, (int)tiles_of(t, m, n), steps, &us);
@@ -743,24 +744,23 @@ bool plan_of(const dr_gated* a, int what, Plan& p) {
     p.panels = (int)(up(f, 256) / 256);
     p.kept = 3ll * p.panels * n * 512;
     const bool back = what == DR_GATED_BACKWARD;
-    if (tiles_of(T64K2, 2 * f, n) >= MOST_TILES || tiles_of(T64K2, d, n) >= MOST_TILES || tiles_of(T128, d, 2 * up(f, 256)) >= MOST_TILES)
-        return false;
-    const bool z = !back || (a->kept == nullptr && (a->dx || a->dgate || a->dup));
-    if (z) {
-        p.z = n <= FEW ? choose_few((int)n, a->width) : choose(EPI_ACT, 2 * f, n, d, {T256, T192x256, T128, T64x128, T64K2});
-        p.once = n <= FEW;
-    }
+    // (a backward call's sizes are those of a forward call)
+    p.z = n <= FEW ? choose_few((int)n, a->width) : choose(EPI_ACT, 2 * f, n, d, {T256, T192x256, T128, T64x128, T64K2});
+    p.once = n <= FEW;
+    if (p.z < 0) return false;
     if (!back) return true;
     long long at = 2ll * p.panels * n * 512;
     if (a->dgate || a->dup) {
         p.w = choose(EPI_DW, d, up(f, 256) * ((a->dgate != nullptr) + (a->dup != nullptr)), n, {T256, T192x256, T128});
         p.one_stage = n <= KSTEP || (p.w == T128 && n <= 1024);
+        if (p.w < 0 || (p.one_stage && tiles_of(T128, d, 2 * up(f, 256)) >= MOST_TILES)) return false;
     }
     p.acc = at;
     if (a->dx) {
         if (n > 64) p.d = choose(EPI_DX, d, n, 2 * f, {T256, T128, T64K2}, &p.splits);
         else if (4 * f * d > HELD) p.d = choose(EPI_DX, d, n, 2 * f, {T256x64}, &p.splits);
         else p.d = choose(EPI_DX, d, n, 2 * f, {T64K2}, &p.splits);
+        if (p.d < 0) return false;
         if (p.splits > 1 && p.d == T64K2) {
             p.counters = (int)tiles_of(T64K2, d, n);
             at += (long long)p.splits * p.counters * (64 * 64 * 4);

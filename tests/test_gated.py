@@ -406,3 +406,15 @@ def test_refusals(device):
     }.items():
         raises(what, bad, fn)
     assert _lib.DR_GATED_BACKWARD == 2
+
+
+def test_most_rows(device):
+    """2^20 rows by 16384 outputs, more tiles of 64 x 64 than a launch holds: the large tiles'."""
+    n, d, f = 1 << 20, 8, 16384
+    g = torch.Generator(device.torch).manual_seed(5)
+    bf16 = lambda *s: torch.randn(*s, generator=g, device=device.torch).to(torch.bfloat16)
+    x, wg, wu = bf16(n, d), bf16(f, d), bf16(f, d)
+    h = gated.gated(x, wg, wu)
+    rows = torch.tensor([0, 1, 255, 256, 524287, 1 << 19, n - 257, n - 1], device=device.torch)
+    part = expected(x[rows], wg, wu, torch.zeros(len(rows), f, device=device.torch), "swiglu", 0.0)
+    within("h of rows", h[rows], *part["h"])

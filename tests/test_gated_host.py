@@ -176,3 +176,15 @@ def test_loads_past_the_caches(tmp_path):
     past = {name: bool(re.search(r"buffer_load_dwordx4 .* lds.* nt|buffer_load_dwordx4 .* nt .*lds", body)) for name, body in found.items()}
     assert past and all(p == name.split("EEEv")[0].endswith("Lb1") for name, p in past.items()), past
     assert {p for name, p in past.items() if "ILi64ELi64ELi1ELi2ELi2E" in name} == {False, True}
+
+
+@pytest.mark.parametrize("rows, dim, width", [(1 << 20, 8, 16384), (1 << 20, 64, 65536), (1 << 18, 1 << 17, 64), (1 << 20, 4096, 14336)])
+def test_sizes_past_small_tiles(rows, dim, width):
+    """Sizes within the header's of which a launch could not hold the smaller tiles: they go by large ones."""
+    L = _lib.lib()
+    A = call(rows, dim, width)._obj
+    assert L.dr_gated_kept_bytes(ctypes.byref(A)) == 3 * -(-width // 256) * rows * 512
+    assert L.dr_gated_workspace_bytes(ctypes.byref(A), BACKWARD) >= 2 * -(-width // 256) * rows * 512
+    info = {**_lib.gated_info(A, BACKWARD), "act": _lib.gated_info(A, FORWARD)["act"]}
+    for (bm, bn, _), m, n in ((info["act"], 2 * width, rows), (info["dx"], dim, rows), (info["dweight"], dim, 2 * width)):
+        assert -(-m // bm) * -(-n // bn) < 1 << 23

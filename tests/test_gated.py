@@ -418,3 +418,32 @@ def test_most_rows(device):
     rows = torch.tensor([0, 1, 255, 256, 524287, 1 << 19, n - 257, n - 1], device=device.torch)
     part = expected(x[rows], wg, wu, torch.zeros(len(rows), f, device=device.torch), "swiglu", 0.0)
     within("h of rows", h[rows], *part["h"])
+
+
+@pytest.mark.parametrize("kind", ["swiglu", "geglu"])
+@pytest.mark.parametrize("n", [5, 64, 65, 700])
+def test_saturated_gradients(device, n, kind):
+    """Gates to 2^70, where a is g or 0 and a' 1 or 0: every gradient against those, by what was kept (few rows and many) and again."""
+    x, wg, wu, dh = inputs(device, n, 64, 96, 6)
+    wg = wg * 2.0**70
+    gx, gw, gu, gd = (t.double() for t in (x, wg, wu, dh))
+    g, u = gx @ gw.T, gx @ gu.T
+    eg, eu = (66 * U * (gx.abs() @ w.abs().T) for w in (gw, gu))
+    sure = (g.abs() > 4 * eg) & (g.abs() > 1e4)  # (the sign is the kernel's too, and the sigmoid 0 or 1 in 64 bits)
+    dh = torch.where(sure, dh, torch.zeros_like(dh))  # (the others count for nothing)
+    gd = dh.double()
+    on = ((g > 0) & sure).double()
+    dg, du = gd * u * on, gd * g * on
+    h, kept = gated.gated_keep(x, wg, wu, kind)
+    for what, k, cut in (("kept", kept, CUT), ("again", None, 0.0)):
+        edg = gd.abs() * (eu + cut * (u.abs() + eu) + 4 * U * u.abs()) * on
+        edu = gd.abs() * (eg + cut * (g.abs() + eg) + 4 * U * g.abs()) * on
+        edg, edu = edg + (B + U) * (dg.abs() + edg), edu + (B + U) * (du.abs() + edu)
+        got = gated.gated_grads(x, wg, wu, dh, kind, kept=k)
+        for name, t, val, err, mag, depth in (
+            ("dx", got[0], dg @ gw + du @ gu, edg @ gw.abs() + edu @ gu.abs(), dg.abs() @ gw.abs() + du.abs() @ gu.abs(), 2 * 96),
+            ("dgate", got[1], dg.T @ gx, edg.T @ gx.abs(), dg.abs().T @ gx.abs(), n),
+            ("dup", got[2], du.T @ gx, edu.T @ gx.abs(), du.abs().T @ gx.abs(), n),
+        ):
+            e = err + (depth + 64) * U * 1.02 * mag
+            within(f"{kind} {n} {what}: {name}", t, val, e + (B + U) * (val.abs() + e) + TINY)

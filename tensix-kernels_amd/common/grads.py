@@ -101,6 +101,7 @@ class _Call:
         if norm is not None:
             dev.no_tangents("grads", norm)
             assert norm.device == self.device and norm.dtype == torch.float32 and norm.numel() == 1, (norm.device, norm.dtype, norm.shape)
+            assert not (torch.is_grad_enabled() and norm.requires_grad), "grads: no derivative by the norm (detach it)"
             self.norm, A.given = norm, 1
         self.run(_lib.lib().dr_grads_clip, norm is None)
         return self.norm

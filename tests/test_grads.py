@@ -349,3 +349,16 @@ def test_many_lists(device):
             within(f"{name}: {i}", outs[i], r, (2.0**-8 + 2.1 * U) * r.abs() + 2.0**-133)
     print(us, flush=True)
     assert us["clip"] < 1.5 * (us["norm"] + us["given"]), us
+
+
+def test_norm_that_requires_grad(device):
+    """A given norm in a graph: its derivative would be dropped, so it is refused as gradients in a graph are."""
+    (a,) = make(device, [64], [F32], 1)
+    leaf = torch.full((), 0.5, device=device.torch, requires_grad=True)
+    for norm in (leaf, leaf * 2):
+        raises("in place", AssertionError, lambda: grads.clip_([a.clone()], 1.0, norm=norm))
+        raises("copies", AssertionError, lambda: grads.clipped([a], 1.0, norm=norm))
+        want = grads.clipped([a], 1.0, norm=torch.full((), norm.item(), device=device.torch))[1][0]
+        with torch.no_grad():
+            same("without a graph", grads.clipped([a], 1.0, norm=norm)[1][0], want)
+        same("detached", grads.clipped([a], 1.0, norm=norm.detach())[1][0], want)

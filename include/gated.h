@@ -7,8 +7,8 @@
  *   dg = dh u a'(g), du = dh a(g); dx = dg . gate + du . up, dgate = dg^T . x, dup = du^T . x.
  *
  * dg and du are rounded to bf16, which the matrix instructions take; sums are float32, h, dx, dgate and dup rounded once. What a
- * forward call keeps for its gradients is a(g) and a'(g) u in 24 bits each; a backward call that is given none computes g and u
- * again (two products more).
+ * forward call keeps for its gradients is g and u in 24 bits each (float32 without the last 8 of the mantissa, cut off), which a
+ * backward call of the same act makes a(g) and a'(g) of; one that is given none computes g and u again (two products more).
  *
  * No counterpart in the reference, which has no training: the block is its fused GLU stage (dense_reader/linear.py:568-744,
  * glu and glu_act) with weights as a training program holds them.
@@ -36,7 +36,7 @@ typedef struct dr_gated {
     const void* up;   /* [width][ld_up] bf16 */
     int64_t ld_up;
     int32_t rows, dim, width; /* rows to 2^20, dim to 2^17, width to 2^20, multiples of 8 but the rows; rows * width below 2^38 */
-    int32_t act;      /* 0 silu, 1 gelu_tanh (dense_reader.h's) */
+    int32_t act;      /* 0 silu, 1 gelu_tanh (dense_reader.h's); of a backward call that of the call that kept */
     void* h;          /* [rows][ld_h] bf16 */
     int64_t ld_h;
     void* kept;       /* dr_gated_kept_bytes, or NULL */

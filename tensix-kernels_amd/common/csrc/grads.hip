@@ -1,15 +1,16 @@
 // grads.hip: the global norm of a model's gradients and clipping by it for MI355X (gfx950), behind include/grads.h.
 //
 // A launch takes up to 128 tensors of any sizes and types, whose addresses and sizes are its arguments, so that nothing about them
-// goes through memory first. They are cut into chunks of 8192 values, which a grid of as many workgroups as the card holds takes in
-// turn; each leaves one sum of squares. The next launch adds those up in every workgroup for itself (16 KB at most a launch of
-// them, which the caches hold), in one order, and is the clip itself, or one workgroup for the norm alone: no atomics, two launches
-// for 128 tensors. The clip takes the chunks the other way round, the last ones read first, which the 256 MB cache behind the
-// L2s still holds. Of many launches' sums one workgroup adds up all first (gr_total).
+// goes through memory first. They are cut into chunks of 8192 values, which a grid of at most 2048 workgroups takes in turn (of
+// gr_squares all are on the card at once, of gr_clip, whose lanes hold more registers, 1280); each leaves one sum of squares. The next
+// launch adds those up in every workgroup for itself (16 KB at most a launch of them, which the caches hold), in one order, and is the
+// clip itself, or one workgroup for the norm alone: no atomics, two launches for 128 tensors. Of many launches' sums one workgroup adds
+// up all first (gr_total). The clip takes the chunks the other way round, the last ones read first, which the 256 MB cache behind the L2s
+// still holds.
 //
-// Bound by memory: one read, and for a clip a second and one write. 252 M bf16 values in 146 tensors 73 us (6.9 TB/s); 283 M float32
-// values clipped 189 us for the squares (6.0 TB/s) and 416 for the rest (5.5; a large copy reaches 4.9). 18 tensors of 190 k values:
-// two launches, 5.5 and 1.7 us, less than the host's 19.
+// Bound by memory: one read, and for a clip a second and one write. 252 M bf16 values in 145 tensors, two launches of 70 and 16 us (5.9
+// TB/s) and 4 for the norm; 283 M float32 values clipped 189 us for the squares (6.0 TB/s) and 416 for the rest (5.5; a large copy
+// reaches 4.9). 18 tensors of 190 k values: two launches, 5.5 and 1.7 us, less than the host's 19.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -27,7 +28,7 @@ namespace {
 
 constexpr int CHUNK = 8192, LANES = 256;  // values
 constexpr int MOST = DR_GRADS_LIST;        // tensors a launch: its arguments fit 4 KB
-constexpr int GRID = 2048;                 // 8 workgroups a CU
+constexpr int GRID = 2048;                 // 8 workgroups a CU of gr_squares (60 registers a lane), 5 of gr_clip (92) at once
 static_assert(GRID * 8 == DR_GRADS_LIST_BYTES, "the header's bytes");
 
 struct List {

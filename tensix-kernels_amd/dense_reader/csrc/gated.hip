@@ -163,7 +163,7 @@ __device__ __forceinline__ void dz_tile(const Prod& a, uint4* to, int tid, int s
 //   of 32. 4 wavefronts of 128 x 128 that read their fragments a step ahead, accumulators pinned, took 1474 us for h and 3 % off the
 //   others, with matrix instructions that the compiler cannot see the waits of; h in four stages of 32 1490 to 1600; fragments read
 //   ahead by 8 wavefronts 1500 to 1640.
-// - 192 x 256 where 256 x 256 leaves CUs idle in its last round (2047 x 2880 x 2880: 253 tiles for 184, h 68 to 62 us; 57 since).
+// - 192 x 256 where 256 x 256 leaves CUs idle in its last round (2047 x 2880 x 2880: 240 tiles for 184, h 68 to 62 us; 57 since).
 // - 128 x 128, 64 x 128 twice a CU, 64 x 64 by two groups of wavefronts that split K: fewer tiles than CUs (choose).
 // - few rows: choose_few.
 // The epilogues' bf16 leave through LDS in whole runs of a row.

@@ -10,8 +10,8 @@ counterpart.
 
 Sums are float32; h and the gradients bf16, rounded once. The gradients' products take dg and du, the gradients of both
 projections' outputs, rounded to bf16: a value of dx or of a weight's gradient that one of theirs dominates is off by up to half a
-bf16 step twice. What the forward pass keeps is a(g) and a'(g) u, 24 bits each, 6 bytes an output and row; with keep=False, or
-kept=None, g and u are computed again instead.
+bf16 step twice. What the forward pass keeps is both projections' outputs, g and u, in 24 bits each (float32 without the last 8 of
+the mantissa), 6 bytes an output and row; with keep=False, or kept=None, they are computed again instead.
 
 Nothing goes to the host. Memory comes from torch's allocator each call, on the current stream, so calls on several streams, threads
 or captured graphs never share any. In a HIP graph, capture gated, gated_keep and gated_grads; autograd's backward refuses to be
@@ -149,7 +149,7 @@ class _Gated(torch.autograd.Function):
 
 def gated(x, w_gate, w_up, activation="swiglu", keep=True):
     """h = a(x . w_gate^T) * (x . w_up^T): x [..., dim] bf16 on the GPU, w_gate and w_up [width, dim] bf16, dim and width multiples
-    of 8; h [..., width] bf16, differentiable in all three. activation: "swiglu" (a silu) or "geglu" (gelu's tanh form). keep: hold
+    of 8 (to 2^17 and 2^20, to 2^20 rows); h [..., width] bf16, differentiable in all three. activation: "swiglu" (a silu) or "geglu" (gelu's tanh form). keep: hold
     6 bytes an output and row for backward, which otherwise computes both projections again from x."""
     if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad):
         return _Gated.apply(x, w_gate, w_up, activation, keep)
@@ -158,7 +158,7 @@ def gated(x, w_gate, w_up, activation="swiglu", keep=True):
 
 def gated_keep(x, w_gate, w_up, activation="swiglu"):
     """(h, kept): gated's h, and what gated_grads of the same x, weights and activation takes ([3, ceil(width / 256), rows, 256]
-    int16: the library's own layout of a(g) and a'(g) u)."""
+    int16: the library's own layout of both projections' outputs)."""
     return _Call(x, w_gate, w_up, activation).forward(True)
 
 

@@ -101,6 +101,7 @@ class _Call:
         if norm is not None:
             dev.no_tangents("grads", norm)
             assert norm.device == self.device and norm.dtype == torch.float32 and norm.numel() == 1, (norm.device, norm.dtype, norm.shape)
+            assert not norm.is_neg(), "grads: a norm is no negative view"
             assert not (torch.is_grad_enabled() and norm.requires_grad), "grads: no derivative by the norm (detach it)"
             self.norm, A.given = norm, 1
         self.run(_lib.lib().dr_grads_clip, norm is None)
@@ -131,7 +132,7 @@ def clipped(grads, max_norm, out=None, dtype=None, norm=None):
     a gradient but its own as a whole (ValueError)."""
     grads = list(grads)
     ts, device = _tensors(grads)
-    sizes = None
+    sizes = list(map(_numel, ts))
     if out is None:
         assert dtype is None or dtype in TYPES, dtype
         out = [None if t is None else torch.empty(t.shape, dtype=dtype or t.dtype, device=device) for t in grads]
@@ -143,10 +144,12 @@ def clipped(grads, max_norm, out=None, dtype=None, norm=None):
         assert where == device and all(map(_contiguous, outs)), "grads: out is contiguous, on the gradients' device"
         if len(ts) < len(grads) or len(outs) < len(out):
             assert [t is None for t in grads] == [o is None for o in out], "grads: out has a tensor where there is a gradient"
-        sizes = list(map(_numel, ts))
         assert list(map(_numel, outs)) == sizes, "grads: out has as many values of each"
     if not all(map(_contiguous, ts)):
         ts = [t.contiguous() for t in ts]
+    if 1 in sizes:  # (the only contiguous memory that can stand for its negative: a value of a conjugate's imaginary part)
+        assert not any(o.is_neg() for o in outs), "grads: out is a negative view"
+        ts = [t.resolve_neg() for t in ts]
     norm = _Call(ts, device, sizes).clip(outs, max_norm, norm)
     dev.written(*outs)
     return norm, out

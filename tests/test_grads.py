@@ -362,3 +362,23 @@ def test_norm_that_requires_grad(device):
         with torch.no_grad():
             same("without a graph", grads.clipped([a], 1.0, norm=norm)[1][0], want)
         same("detached", grads.clipped([a], 1.0, norm=norm.detach())[1][0], want)
+
+
+def test_negative_views(device):
+    """The imaginary part of a conjugate is a view of memory with the other sign: one value of it is contiguous."""
+    for n in (1, 5):
+        z = torch.randn(n, dtype=torch.complex64, generator=torch.Generator().manual_seed(n)).to(device.torch)
+        view, plain = z.conj().imag, -z.imag.clone()
+        assert view.is_neg() and view.is_contiguous() == (n == 1)
+        for max_norm in (0.1, 1e3):
+            norm, (got,) = grads.clipped([view], max_norm)
+            same("clipped", got, grads.clipped([plain], max_norm)[1][0]), same("norm", norm, grads.global_norm([view]))
+            into = torch.empty_like(plain)
+            same("into out", grads.clipped([view], max_norm, out=[into])[1][0], got)
+            if n == 1:
+                there = z.clone()
+                grads.clip_([there.conj().imag], max_norm)
+                same("in place", -there.imag, got)
+    one = torch.ones(1, dtype=torch.complex64, device=device.torch).conj().imag
+    raises("a negative out", AssertionError, lambda: grads.clipped([torch.ones(1, device=device.torch)], 1.0, out=[one]))
+    raises("a negative norm", AssertionError, lambda: grads.clipped([torch.ones(1, device=device.torch)], 1.0, norm=one))
